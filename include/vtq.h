@@ -33,6 +33,10 @@
  *                          tokens past seq_len, inference.rs:301-311)
  * No entry point aborts or panics.
  *
+ * The operators of a batched serving step (the last part of this header) have
+ * no counterpart in the reference, which serves one sequence with f32
+ * activations; they use the same context, codes and error texts.
+ *
  * Threading: a context is used by one host thread at a time (the reference's
  * Accelerator takes &mut self, src/accel/mod.rs:82).  Contexts on different
  * threads are independent.
@@ -66,6 +70,7 @@ extern "C" {
 #define VTQ_TYPE_Q8_0 8
 #define VTQ_TYPE_Q4_K 12
 #define VTQ_TYPE_Q6_K 14
+#define VTQ_TYPE_BF16 30 /* activations and caches of the serving operators only */
 
 /* Numerical regime of the Q4_K arm, chosen by a Cargo feature in the
  * reference (src/model/forward_quantized.rs:704-725):
@@ -88,7 +93,7 @@ const char *vtq_last_error(const vtq_ctx *ctx);
  * the ABI of this header and of vtq_runtime.h together; 0.2.0 added the
  * trailing digest_v1 argument of vtqrt_run (a caller built against 0.1.0
  * headers must not load this library); 0.3.0 added vtqrt_set_prompt_mode
- * (no existing signature changed). */
+ * (no existing signature changed); 0.3.1 added the serving operators. */
 const char *vtq_version(void);
 
 /* ---- host-pointer entry points (synchronous; y is complete on return) ----
@@ -168,6 +173,148 @@ int vtq_linear_device(vtq_ctx *ctx, int ggml_type, int regime, const float *d_x,
 int vtq_linear_device_noalloc(vtq_ctx *ctx, int ggml_type, int regime, const float *d_x,
                               const uint8_t *d_w, size_t w_len, float *d_y, size_t batch,
                               size_t in_feat, size_t out_feat, void *stream);
+
+/* ---- operators of a batched serving step (device pointers, asynchronous) ----
+ * Between the linears of a step that serves several sequences: an int8 linear
+ * with scales per token and channel, rotary positions, appending to a paged
+ * KV cache, and attention over it for a batch whose sequences share a prefix.
+ * All pointers but the structs' own are device memory on the context's device;
+ * the work is enqueued on `stream` (a hipStream_t of that device, NULL for the
+ * null stream) without synchronising, whichever device is current, which stays
+ * current.  Nothing is allocated, so every call may be captured into a graph,
+ * and calls on different streams share no memory but the caller's.
+ * `type` arguments take VTQ_TYPE_F32, VTQ_TYPE_F16 or VTQ_TYPE_BF16.  Leading
+ * dimensions and strides count elements; the last dimension is contiguous.
+ * Results do not change from run to run: no sums of a changing order.
+ * Refusals: VTQ_E_INVALID_ARGUMENT (null or unaligned pointer, value out of its
+ * range), VTQ_E_INVALID_SHAPE (sizes or strides that do not fit together) and
+ * VTQ_E_NOT_IMPLEMENTED (type combinations and sizes beyond the kernels), with
+ * a text, before anything is launched. */
+
+/* Rows to 8 bits: scale[m] = max_k |x[m][k]| / 127 (f32, rounded once) and
+ * q[m][k] = x[m][k] / scale[m] to the nearest whole number (the exact quotient;
+ * ties to even; at most 127 in magnitude), 0 where the scale is 0.  A row that holds an infinity or a NaN
+ * gets that as its scale and zeros, so its products are NaN.  x has rows ld_x
+ * apart, q rows ld_q bytes apart (a multiple of 16, at least n; q itself 16-byte
+ * aligned); the bytes from n to ld_q are set to 0.  n <= 131071.  Weights take
+ * the same call, one row per output channel. */
+int vtq_quantize_i8_device(vtq_ctx *ctx, int x_type, const void *d_x, size_t ld_x, int8_t *d_q, size_t ld_q,
+                           float *d_scale, size_t rows, size_t n, void *stream);
+
+/* y[m][o] = x_scale[m] * w_scale[o] * sum_k xq[m][k] * wq[o][k] + bias[o]; the sum
+ * is exact (32 bits: in_feat <= 131071), the rest f32, rounded once to y_type.
+ * bias may be NULL.  xq and wq rows are ld_x and ld_w bytes apart (multiples of
+ * 16, at least in_feat; 16-byte aligned), readable up to the next multiple of 16
+ * past in_feat; in xq those bytes past in_feat must be 0, as the call above
+ * leaves them.  y rows are ld_y apart.  in_feat 0 gives the bias alone. */
+int vtq_linear_i8_device(vtq_ctx *ctx, const int8_t *d_xq, size_t ld_x, const float *d_x_scale, const int8_t *d_wq,
+                         size_t ld_w, const float *d_w_scale, const float *d_bias, int y_type, void *d_y, size_t ld_y,
+                         size_t batch, size_t in_feat, size_t out_feat, void *stream);
+
+/* Rotary positions.  The first rot_dim elements of a head (even, 2 to 256) form
+ * rot_dim / 2 pairs, (2i, 2i + 1) interleaved or (i, i + rot_dim / 2) by halves;
+ * at position p pair i turns by the angle p * f_i:
+ *   (a, b) -> magnitude * (a cos - b sin, a sin + b cos),  f_i = theta^(-2i / rot_dim) / factors[i].
+ * scaling stretches f_i for contexts longer than the trained original_context:
+ *   LINEAR  f_i / factor;
+ *   BANDS   with t = original_context * f_i / 2 pi turns in the original context and
+ *           k = (t - low) / (high - low) clamped to 0..1:  k f_i + (1 - k) f_i / factor
+ *           (low, high: 1 and 4 where 0 is given);
+ *   YARN    a ramp over the pair index between the pairs that make `high` and `low`
+ *           turns (32 and 1 where 0 is given), rounded outwards to whole indices, and
+ *           magnitude 0.1 ln(factor) + 1.
+ * magnitude, where it is not 0, replaces the rule's own.  A plan is plain memory:
+ * it may be copied, and holds f_i as fractions of a turn in 64 bits, so that
+ * p * f_i modulo a turn is exact for every 32-bit position. */
+#define VTQ_ROPE_INTERLEAVED 0
+#define VTQ_ROPE_HALF 1
+#define VTQ_ROPE_SCALE_NONE 0
+#define VTQ_ROPE_SCALE_LINEAR 1
+#define VTQ_ROPE_SCALE_BANDS 2
+#define VTQ_ROPE_SCALE_YARN 3
+typedef struct {
+    int layout, scaling, rot_dim;
+    int original_context;
+    double theta, factor, low, high, magnitude;
+    const float *factors; /* host, rot_dim / 2 values, or NULL: all 1 */
+} vtq_rope_params;
+typedef struct {
+    int layout, rot_dim;
+    float magnitude;
+    int reserved;
+    uint64_t turns[128];
+} vtq_rope;
+/* Fills *out on the host; ctx only takes the error text and may be NULL. */
+int vtq_rope_plan(vtq_ctx *ctx, const vtq_rope_params *params, vtq_rope *out);
+
+/* y[t][h] = x[t][h] rotated to position pos[t] (int32, negative ones turn
+ * backwards); elements past rot_dim are copied.  x and y are tokens x heads x
+ * head_dim with their own token and head strides; y may be x itself (the same
+ * pointer and strides), and must not overlap it otherwise. */
+int vtq_rope_device(vtq_ctx *ctx, const vtq_rope *rope, int type, const void *d_x, size_t x_token_stride,
+                    size_t x_head_stride, void *d_y, size_t y_token_stride, size_t y_head_stride,
+                    const int32_t *d_pos, size_t tokens, size_t heads, size_t head_dim, void *stream);
+
+/* A paged KV cache: slot s of page p of KV head h is head_dim contiguous elements
+ * at p * page_stride + h * head_stride + s * slot_stride, in k and v alike.
+ * page_size is a power of two, 8 to 4096; head_dim a multiple of 8 up to 256; the
+ * strides are multiples of 8 with slots and heads apart (at least head_dim), and k
+ * and v 16-byte aligned. */
+typedef struct {
+    int type, page_size, kv_heads, head_dim;
+    size_t n_pages;
+    void *k, *v;
+    size_t page_stride, head_stride, slot_stride;
+} vtq_kv_cache;
+
+/* A ragged batch.  Tokens q_start[b] to q_start[b + 1] of the call are the newest
+ * of sequence b, which holds len[b] tokens of its own (these included) in the
+ * slots of pages[b * max_pages + j], j = 0, 1, ..., behind a prefix of prefix_len
+ * tokens that all sequences share in prefix_pages.  So token i of the n of a
+ * sequence stands at position prefix_len + len[b] - n + i.
+ * q_start (batch + 1, not decreasing, from 0), len and the page lists are device
+ * memory, read when the work runs: a captured graph takes their new contents.
+ * max_q is the host's idea of the longest sequence of tokens and max_len of the
+ * longest own part (0: max_pages * page_size); they only choose how the work is
+ * split.  Tokens of the call from q_start[batch] on are left alone, in every
+ * output.  Page numbers outside the cache, and own tokens past max_pages pages,
+ * are never read or written (see each call). */
+typedef struct {
+    int batch, max_pages, max_q, max_len, prefix_len;
+    const int32_t *q_start, *len, *pages, *prefix_pages;
+} vtq_kv_batch;
+
+/* Writes the tokens' keys, rotated to their positions (rope NULL: as they are),
+ * and values to their slots, rounded once to the cache's type, and, where d_q is
+ * not NULL, the tokens' queries rotated to d_q_out (which may be d_q itself with
+ * the same strides).  k and v are tokens x kv_heads x head_dim, q tokens x
+ * heads x head_dim.  A token whose slot does not exist (a page number outside the
+ * cache, a place below 0 or past max_pages pages) is not written.  Two tokens
+ * must not share a slot: a page belongs to one sequence, or to the prefix. */
+int vtq_kv_append_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_batch *batch, const vtq_rope *rope,
+                         int type, size_t tokens, const void *d_k, size_t k_token_stride, size_t k_head_stride,
+                         const void *d_v, size_t v_token_stride, size_t v_head_stride, size_t heads, const void *d_q,
+                         size_t q_token_stride, size_t q_head_stride, void *d_q_out, size_t q_out_token_stride,
+                         size_t q_out_head_stride, void *stream);
+
+/* Attention of the batch's tokens over the prefix, which all of them see whole, and
+ * the sequence's own tokens up to and including themselves:
+ *   y[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j,  lse[t][h] = ln sum_j exp(scale * q . k_j),
+ * query head h reading KV head h / (heads / kv_heads); heads is a multiple of
+ * kv_heads.  The prefix is read once for all sequences.  A row that sees no key
+ * gives zeros and an lse of -infinity; what stands in slots that a row does not
+ * see never reaches it.  Keys in pages outside the cache count as zeros.  type is
+ * the queries' and y's: the cache's own, or VTQ_TYPE_F32 with any cache.  lse
+ * (f32, tokens x heads, or NULL) is in natural logarithms.  scale is positive.
+ * d_ws is at least vtq_attention_workspace bytes, 256-byte aligned, for this call
+ * alone until its work is done (calls that may overlap need one each); the size
+ * depends on the host's numbers only, not on the lengths in device memory. */
+size_t vtq_attention_workspace(const vtq_kv_cache *cache, const vtq_kv_batch *batch, int type, size_t tokens,
+                               size_t heads);
+int vtq_attention_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_batch *batch, int type, size_t tokens,
+                         size_t heads, const void *d_q, size_t q_token_stride, size_t q_head_stride, void *d_y,
+                         size_t y_token_stride, size_t y_head_stride, float *d_lse, float scale, void *d_ws,
+                         size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

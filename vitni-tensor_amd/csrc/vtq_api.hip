@@ -15,6 +15,7 @@
 
 #include "../../include/vtq.h"
 #include "vtq_kernels.h"
+#include "vtq_serve.h"
 
 namespace {
 
@@ -437,6 +438,24 @@ int linear_host(vtq_ctx* c, int type, int regime, const float* x, size_t x_len, 
 
 namespace vtq {
 
+int ctx_error(vtq_ctx* c, int code, const char* text) noexcept {
+    try {
+        return set_err(c, code, text);
+    } catch (...) {  // no memory for the text
+        return code;
+    }
+}
+
+int ctx_hip_error(vtq_ctx* c, hipError_t e, const char* where) noexcept {
+    try {
+        return hip_fail(c, e, where);
+    } catch (...) {
+        return VTQ_E_GPU;
+    }
+}
+
+int ctx_device(const vtq_ctx* c) { return c->device; }
+
 hipError_t allow_dynamic_lds(const void* kernel, size_t bytes) {
     if (bytes <= 65536) return hipSuccess;
     // (device, kernel) -> limit set; a fixed table (no heap: the no-alloc
@@ -466,7 +485,7 @@ hipError_t allow_dynamic_lds(const void* kernel, size_t bytes) {
 
 extern "C" {
 
-const char* vtq_version(void) { return "vtq 0.3.0 (gfx950)"; }
+const char* vtq_version(void) { return "vtq 0.3.1 (gfx950)"; }
 
 int vtq_create(int device, vtq_ctx** out) {
     if (!out) return VTQ_E_INVALID_ARGUMENT;

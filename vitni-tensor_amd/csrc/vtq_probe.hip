@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "vtq_rules.h"
+#include "vtq_serve.h"
 
 namespace {
 
@@ -28,6 +29,11 @@ __global__ __launch_bounds__(256) void stream_read_kernel(const uint4* __restric
         acc ^= v.x ^ v.y ^ v.z ^ v.w;
     }
     if (acc == 0x9E3779B9u) sink[blockIdx.x] = acc;
+}
+
+int told(const vtq::Refusal& r, const char** text) {
+    if (text) *text = r.text;
+    return r.code;
 }
 
 }  // namespace
@@ -71,6 +77,45 @@ int vtqp_kquant_form(int type, int batch, int in_feat, int out_feat) {
     if (!vtq::q4k_gemm_faster(batch, in_feat, out_feat)) return 0;
     const int form = vtq::gemm_form(R, out_feat, M, Mt);
     return form == 3 ? 300 + vtq::sk_piece(R, NR * Mt) : form == 2 ? 2 : 1;
+}
+
+// What the serving operators refuse: the status that a call with these arguments
+// gets before anything is launched, and its text.
+int vtqp_check_quantize_i8(const char** text, int x_type, const void* d_x, size_t ld_x, int8_t* d_q, size_t ld_q,
+                           float* d_scale, size_t rows, size_t n) {
+    return told(vtq::check_quantize_i8(x_type, d_x, ld_x, d_q, ld_q, d_scale, rows, n), text);
+}
+int vtqp_check_linear_i8(const char** text, const int8_t* d_xq, size_t ld_x, const float* d_x_scale,
+                         const int8_t* d_wq, size_t ld_w, const float* d_w_scale, const float* d_bias, int y_type,
+                                 void* d_y, size_t ld_y, size_t batch, size_t in_feat, size_t out_feat) {
+    return told(vtq::check_linear_i8(d_xq, ld_x, d_x_scale, d_wq, ld_w, d_w_scale, d_bias, y_type, d_y, ld_y, batch,
+                                     in_feat, out_feat), text);
+}
+int vtqp_check_rope_call(const char** text, const vtq_rope* rope, int type, const void* d_x, size_t x_token_stride,
+                         size_t x_head_stride, void* d_y, size_t y_token_stride, size_t y_head_stride,
+                                 const int32_t* d_pos, size_t tokens, size_t heads, size_t head_dim) {
+    return told(vtq::check_rope_call(rope, type, d_x, x_token_stride, x_head_stride, d_y, y_token_stride,
+                                     y_head_stride, d_pos, tokens, heads, head_dim), text);
+}
+int vtqp_check_append(const char** text, const vtq_kv_cache* cache, const vtq_kv_batch* batch, const vtq_rope* rope,
+                      int type, size_t tokens, const void* d_k, size_t k_token_stride, size_t k_head_stride,
+                              const void* d_v, size_t v_token_stride, size_t v_head_stride, size_t heads,
+                                      const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_q_out,
+                                              size_t q_out_token_stride, size_t q_out_head_stride) {
+    return told(vtq::check_append(cache, batch, rope, type, tokens, d_k, k_token_stride, k_head_stride, d_v,
+                                  v_token_stride, v_head_stride, heads, d_q, q_token_stride, q_head_stride, d_q_out,
+                                          q_out_token_stride, q_out_head_stride), text);
+}
+int vtqp_check_attention(const char** text, const vtq_kv_cache* cache, const vtq_kv_batch* batch, int type,
+                         size_t tokens, size_t heads, const void* d_q, size_t q_token_stride, size_t q_head_stride,
+                                 void* d_y, size_t y_token_stride, size_t y_head_stride, float* d_lse, float scale) {
+    return told(vtq::check_attention(cache, batch, type, tokens, heads, d_q, q_token_stride, q_head_stride, d_y,
+                                     y_token_stride, y_head_stride, d_lse, scale), text);
+}
+
+// Where a place of a sequence begins in the cache (vtq_serve.h).
+int64_t vtqp_slot_of(const vtq_kv_cache* cache, const int32_t* pages, int max_pages, int64_t place) {
+    return vtq::slot_of(*cache, pages, max_pages, place);
 }
 
 }  // extern "C"

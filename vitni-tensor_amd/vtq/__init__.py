@@ -24,11 +24,17 @@ LIB_PATH = os.path.join(LIB_DIR, "libvtq.so")
 
 # GGUF tensor type tags (src/model/gguf.rs:127-139)
 F32, F16, Q4_0, Q5_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 6, 8, 12, 14
-TYPE_NAMES = {F32: "F32", F16: "F16", Q4_0: "Q4_0", Q5_0: "Q5_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q6_K: "Q6_K"}
+BF16 = 30  # activations and caches of the serving operators only
+TYPE_NAMES = {F32: "F32", F16: "F16", Q4_0: "Q4_0", Q5_0: "Q5_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q6_K: "Q6_K",
+              BF16: "BF16"}
 BLOCK = {Q4_0: (32, 18), Q5_0: (32, 22), Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210)}
 
 REGIME_INTEGER = 0       # std-parallel build: integer Q4_K
 REGIME_FLOAT_FUSED = 1   # default build: float-fused Q4_K
+
+# rotary layouts and scalings of long contexts (include/vtq.h)
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BANDS, ROPE_SCALE_YARN = 0, 1, 2, 3
 
 OK, E_INTERNAL, E_GPU, E_NOT_IMPLEMENTED, E_INVALID_ARGUMENT = 0, 1, 2, 3, 4
 E_MALFORMED, E_TRUNCATED, E_OVERFLOW, E_SHAPE_MISMATCH, E_INVALID_SHAPE = 5, 6, 7, 8, 9
@@ -146,6 +152,20 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.vtq_release_weights.restype = i
     lib.vtq_linear_device.argtypes = [vp, i, i, vp, vp, sz, vp, sz, sz, sz, vp]
     lib.vtq_linear_device.restype = i
+    lib.vtq_quantize_i8_device.argtypes = [vp, i, vp, sz, vp, sz, vp, sz, sz, vp]
+    lib.vtq_quantize_i8_device.restype = i
+    lib.vtq_linear_i8_device.argtypes = [vp, vp, sz, vp, vp, sz, vp, vp, i, vp, sz, sz, sz, sz, vp]
+    lib.vtq_linear_i8_device.restype = i
+    lib.vtq_rope_plan.argtypes = [vp, vp, vp]
+    lib.vtq_rope_plan.restype = i
+    lib.vtq_rope_device.argtypes = [vp, vp, i, vp, sz, sz, vp, sz, sz, vp, sz, sz, sz, vp]
+    lib.vtq_rope_device.restype = i
+    lib.vtq_kv_append_device.argtypes = [vp, vp, vp, vp, i, sz, vp, sz, sz, vp, sz, sz, sz, vp, sz, sz, vp, sz, sz, vp]
+    lib.vtq_kv_append_device.restype = i
+    lib.vtq_attention_workspace.argtypes = [vp, vp, i, sz, sz]
+    lib.vtq_attention_workspace.restype = sz
+    lib.vtq_attention_device.argtypes = [vp, vp, vp, i, sz, sz, vp, sz, sz, vp, sz, sz, vp, ctypes.c_float, vp, sz, vp]
+    lib.vtq_attention_device.restype = i
     _lib = lib
     return lib
 
@@ -154,7 +174,76 @@ EXPORTED = (
     "vtq_create", "vtq_destroy", "vtq_last_error", "vtq_version", "vtq_linear",
     "vtq_linear_q4_k_integer", "vtq_linear_q6_k_integer", "vtq_linear_q4_k_fused",
     "vtq_linear_q4_0", "vtq_release_weights", "vtq_linear_device", "vtq_linear_device_noalloc",
+    "vtq_quantize_i8_device", "vtq_linear_i8_device", "vtq_rope_plan", "vtq_rope_device", "vtq_kv_append_device",
+    "vtq_attention_workspace", "vtq_attention_device",
 )
+
+
+class _RopeParams(ctypes.Structure):
+    _fields_ = [("layout", ctypes.c_int), ("scaling", ctypes.c_int), ("rot_dim", ctypes.c_int),
+                ("original_context", ctypes.c_int), ("theta", ctypes.c_double), ("factor", ctypes.c_double),
+                ("low", ctypes.c_double), ("high", ctypes.c_double), ("magnitude", ctypes.c_double),
+                ("factors", ctypes.c_void_p)]
+
+
+class _RopePlan(ctypes.Structure):
+    _fields_ = [("layout", ctypes.c_int), ("rot_dim", ctypes.c_int), ("magnitude", ctypes.c_float),
+                ("reserved", ctypes.c_int), ("turns", ctypes.c_uint64 * 128)]
+
+
+class _KvCache(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int), ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("n_pages", ctypes.c_size_t), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("page_stride", ctypes.c_size_t), ("head_stride", ctypes.c_size_t),
+                ("slot_stride", ctypes.c_size_t)]
+
+
+class _KvBatch(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int), ("max_pages", ctypes.c_int), ("max_q", ctypes.c_int),
+                ("max_len", ctypes.c_int), ("prefix_len", ctypes.c_int), ("q_start", ctypes.c_void_p),
+                ("len", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("prefix_pages", ctypes.c_void_p)]
+
+
+class Rope:
+    """A rotary plan (vtq_rope_plan): the rot_dim / 2 frequencies and the magnitude.  Host memory, made
+    without a device; any context may use it."""
+
+    def __init__(self, rot_dim, layout=ROPE_HALF, theta=10000.0, scaling=ROPE_SCALE_NONE, factor=1.0,
+                 original_context=0, low=0.0, high=0.0, magnitude=0.0, factors=None):
+        lib = load_library()
+        f = None if factors is None else np.ascontiguousarray(factors, dtype=np.float32)
+        if f is not None and f.size != int(rot_dim) // 2:
+            raise InvalidShape("vtq: one rope factor a pair")
+        params = _RopeParams(layout, scaling, rot_dim, original_context, theta, factor, low, high, magnitude,
+                             None if f is None else f.ctypes.data)
+        self.plan = _RopePlan()
+        rc = lib.vtq_rope_plan(None, ctypes.byref(params), ctypes.byref(self.plan))
+        if rc != OK:
+            raise _ERRORS.get(rc, VtqError)("vtq: invalid rope parameters")
+        self.ref = ctypes.byref(self.plan)
+
+
+class KvCache:
+    """A paged KV cache on the device (vtq_kv_cache): pages x kv_heads x page_size x head_dim, or the
+    given strides in elements.  Holds addresses, not the memory."""
+
+    def __init__(self, ggml_type, k_ptr, v_ptr, n_pages, page_size, kv_heads, head_dim, page_stride=None,
+                 head_stride=None, slot_stride=None):
+        slot = head_dim if slot_stride is None else slot_stride
+        head = page_size * slot if head_stride is None else head_stride
+        page = kv_heads * head if page_stride is None else page_stride
+        self.desc = _KvCache(int(ggml_type), page_size, kv_heads, head_dim, n_pages, k_ptr, v_ptr, page, head, slot)
+        self.ref = ctypes.byref(self.desc)
+
+
+class KvBatch:
+    """A ragged batch over a paged cache (vtq_kv_batch); the pointers are int32 lists on the device."""
+
+    def __init__(self, batch, q_start_ptr, len_ptr, pages_ptr, max_pages, max_q=1, max_len=0, prefix_len=0,
+                 prefix_pages=None):
+        self.desc = _KvBatch(batch, max_pages, max_q, max_len, prefix_len, q_start_ptr, len_ptr, pages_ptr,
+                             prefix_pages)
+        self.ref = ctypes.byref(self.desc)
 
 
 class Context:
@@ -266,6 +355,54 @@ class Context:
         rc = self.lib.vtq_linear_device(self.handle, int(ggml_type), int(regime), x_ptr, w_ptr, w_len, y_ptr,
                                         batch, in_feat, out_feat, stream)
         self._check(rc)
+
+    # -- operators of a batched serving step (device pointers) ---------------
+
+    def quantize_i8_device(self, x_type, x_ptr, ld_x, q_ptr, ld_q, scale_ptr, rows, n, stream=None):
+        """vtq_quantize_i8_device: rows of x to 8 bits with a scale each."""
+        rc = self.lib.vtq_quantize_i8_device(self.handle, x_type, x_ptr, ld_x, q_ptr, ld_q, scale_ptr, rows, n, stream)
+        if rc:
+            self._check(rc)
+
+    def linear_i8_device(self, xq_ptr, ld_x, x_scale_ptr, wq_ptr, ld_w, w_scale_ptr, bias_ptr, y_type, y_ptr, ld_y,
+                         batch, in_feat, out_feat, stream=None):
+        """vtq_linear_i8_device: the int8 product with scales per token and channel."""
+        rc = self.lib.vtq_linear_i8_device(self.handle, xq_ptr, ld_x, x_scale_ptr, wq_ptr, ld_w, w_scale_ptr, bias_ptr,
+                                           y_type, y_ptr, ld_y, batch, in_feat, out_feat, stream)
+        if rc:
+            self._check(rc)
+
+    def rope_device(self, rope, ggml_type, x_ptr, x_token_stride, x_head_stride, y_ptr, y_token_stride, y_head_stride,
+                    pos_ptr, tokens, heads, head_dim, stream=None):
+        """vtq_rope_device: x rotated to its positions, into y (or in place)."""
+        rc = self.lib.vtq_rope_device(self.handle, rope.ref, ggml_type, x_ptr, x_token_stride, x_head_stride, y_ptr,
+                                      y_token_stride, y_head_stride, pos_ptr, tokens, heads, head_dim, stream)
+        if rc:
+            self._check(rc)
+
+    def kv_append_device(self, cache, batch, rope, ggml_type, tokens, k_ptr, k_token_stride, k_head_stride, v_ptr,
+                         v_token_stride, v_head_stride, stream=None, heads=0, q_ptr=None, q_token_stride=0,
+                         q_head_stride=0, q_out_ptr=None, q_out_token_stride=0, q_out_head_stride=0):
+        """vtq_kv_append_device: rotated keys and plain values to their slots, rotated queries to q_out."""
+        rc = self.lib.vtq_kv_append_device(self.handle, cache.ref, batch.ref, None if rope is None else rope.ref,
+                                           ggml_type, tokens, k_ptr, k_token_stride, k_head_stride, v_ptr,
+                                           v_token_stride, v_head_stride, heads, q_ptr, q_token_stride, q_head_stride,
+                                           q_out_ptr, q_out_token_stride, q_out_head_stride, stream)
+        if rc:
+            self._check(rc)
+
+    def attention_workspace(self, cache, batch, ggml_type, tokens, heads):
+        """vtq_attention_workspace: bytes that attention_device needs for these numbers."""
+        return self.lib.vtq_attention_workspace(cache.ref, batch.ref, ggml_type, tokens, heads)
+
+    def attention_device(self, cache, batch, ggml_type, tokens, heads, q_ptr, q_token_stride, q_head_stride, y_ptr,
+                         y_token_stride, y_head_stride, scale, ws_ptr, ws_bytes, stream=None, lse_ptr=None):
+        """vtq_attention_device: attention over the shared prefix and the sequences' own pages."""
+        rc = self.lib.vtq_attention_device(self.handle, cache.ref, batch.ref, ggml_type, tokens, heads, q_ptr,
+                                           q_token_stride, q_head_stride, y_ptr, y_token_stride, y_head_stride, lse_ptr,
+                                           scale, ws_ptr, ws_bytes, stream)
+        if rc:
+            self._check(rc)
 
 
 def row_bytes(ggml_type: int, in_feat: int) -> int:

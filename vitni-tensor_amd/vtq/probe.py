@@ -25,8 +25,24 @@ def lib() -> ctypes.CDLL:
         for f in (L.vtqp_canon_form, L.vtqp_kquant_form):
             f.argtypes = [ctypes.c_int] * 4
             f.restype = ctypes.c_int
+        vp, sz, i, f = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float
+        L.vtqp_check_quantize_i8.argtypes = [vp, i, vp, sz, vp, sz, vp, sz, sz]
+        L.vtqp_check_linear_i8.argtypes = [vp, vp, sz, vp, vp, sz, vp, vp, i, vp, sz, sz, sz, sz]
+        L.vtqp_check_rope_call.argtypes = [vp, vp, i, vp, sz, sz, vp, sz, sz, vp, sz, sz, sz]
+        L.vtqp_check_append.argtypes = [vp, vp, vp, vp, i, sz, vp, sz, sz, vp, sz, sz, sz, vp, sz, sz, vp, sz, sz]
+        L.vtqp_check_attention.argtypes = [vp, vp, vp, i, sz, sz, vp, sz, sz, vp, sz, sz, vp, f]
+        L.vtqp_slot_of.argtypes = [vp, vp, i, ctypes.c_int64]
+        L.vtqp_slot_of.restype = ctypes.c_int64
         _lib = L
     return _lib
+
+
+def refusal(operator: str, *args):
+    """(status, text) that a serving operator's call with these arguments (without context, workspace and
+    stream) gets before anything is launched; no GPU is needed."""
+    text = ctypes.c_char_p()
+    rc = getattr(lib(), "vtqp_check_" + operator)(ctypes.byref(text), *args)
+    return rc, (text.value or b"").decode()
 
 
 def stream_read(ptr: int, nbytes: int, workgroups: int, sink_ptr: int, stream: int) -> None:
