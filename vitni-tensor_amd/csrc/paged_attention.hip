@@ -3,82 +3,697 @@
 //
 //   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - m),  m = max_j scale q.k_j
 //
-// in one pass over the keys, with the running maximum and sum of each row in f32.
+// One pass over the keys, with the running maximum and sum of each row in f32.
+// The prefix is one matrix of keys for the rows of every sequence (tokens x the
+// query heads of a KV head): workgroups take 32 rows a wave against tiles that the
+// waves share.  A sequence's own keys meet few rows (the query heads of its one
+// token): there the waves of a workgroup take different tiles against the same 32
+// rows, and merge at the end.  Both kinds of workgroup are one launch, mixed, so
+// that the prefix's matrix work runs beside the other's memory traffic.  Key ranges
+// are split to fill the chip; a second launch joins the parts of a row by their
+// maxima and sums.  The order of every sum goes by sizes alone.
+//
+// Per 32 keys and 32 rows, S^T = K Q^T and O^T += V^T P^T on 32x32 MFMAs.  Lane l
+// then holds row l & 31 and keys 8i + 4(l >> 5) + e of a tile, a maximum or sum over
+// keys stays within a lane and its partner, and the registers of P^T are the second
+// product's operand as they are: the order of keys inside an MFMA is free, so V is
+// read in the order that P has.  V's transpose comes from the LDS transposing read.
+// f32 queries multiply in f32 (32x32x2 MFMAs; 16-bit keys and values widen exactly).
 #include <type_traits>
 
 #include "vtq_device.h"
+#include "vtq_kernels.h"
+#include "vtq_lds_load.h"
 #include "vtq_serve.h"
 
 namespace vtq {
 namespace {
 
-// One wave a row: lane j scores key j of a chunk of 64, then the lanes share out the
-// elements of the values.
-template <class Q, class C>
-__global__ __launch_bounds__(64) void attention_rows_kernel(Attention a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t t = (int64_t)blockIdx.x;
-    const int h = (int)blockIdx.y, hd = a.cache.head_dim;
-    int seq = 0;
-    for (int b = 0; b < a.batch.batch; b += 64)
-        seq += __popcll(__ballot(b + lane < a.batch.batch && a.batch.q_start[b + lane + 1] <= t));
-    if (seq >= a.batch.batch) return;
-    const int64_t place = (int64_t)a.batch.len[seq] - (a.batch.q_start[seq + 1] - t);
-    const int64_t limit = min((int64_t)a.batch.max_pages * a.cache.page_size, place + 1);
-    const int64_t keys = a.batch.prefix_len + max((int64_t)0, limit);
-    const int64_t head_at = (int64_t)(h / (a.heads / a.cache.kv_heads)) * a.cache.head_stride;
-    const Q* q = static_cast<const Q*>(a.q.p) + t * a.q.token_stride + h * a.q.head_stride;
-    float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
-    for (int64_t j0 = 0; j0 < keys; j0 += 64) {
-        const int64_t j = j0 + lane;
-        int64_t at = -1;
-        float s = -INFINITY;
-        if (j < keys) {
-            const bool own = j >= a.batch.prefix_len;
-            const int64_t i = own ? j - a.batch.prefix_len : j;
-            const int64_t page = own ? a.batch.pages[(int64_t)seq * a.batch.max_pages + i / a.cache.page_size]
-                                     : a.batch.prefix_pages[i / a.cache.page_size];
-            s = 0.0f;
-            if (page >= 0 && page < (int64_t)a.cache.n_pages) {
-                at = page * (int64_t)a.cache.page_stride + (i % a.cache.page_size) * (int64_t)a.cache.slot_stride + head_at;
-                for (int d = 0; d < hd; d++) s = fmaf((float)q[d], (float)static_cast<const C*>(a.cache.k)[at + d], s);
-            }
-            s *= a.scale;
-        }
-        float top = s;
-        for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
-        const float m1 = fmaxf(m, top), base = m1 == -INFINITY ? 0.0f : m1;
-        const float shrink = expf(m - base), p = expf(s - base);
-        float sum = p;
-        for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x, 64);
-        l = l * shrink + sum;
-        m = m1;
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr int kWord3 = 0x00020000;  // raw buffer, stride 0
+
+struct Job {
+    Attention a;
+    int group;        // query heads of a KV head
+    int page_shift;
+    int prefix_rows;  // row tiles of the prefix
+    int prefix_splits, prefix_chunk;  // key ranges, and keys to one (a multiple of 128)
+    int own_rows, own_splits;         // row tiles of a sequence (a workgroup may take several), key ranges
+    int shared_prefix, shared_own;    // whether the waves share tiles (else they share rows)
+    int prefix_blocks, own_blocks;
+    float c;          // scale * log2(e)
+    float* part_o;    // [splits][tokens * heads][head_dim]
+    float2* part_ml;  // [splits][tokens * heads]: maximum (log2) and sum
+};
+
+// What a wave has of a 32-row tile.
+template <int D>
+struct State {
+    v16f o[D / 32];
+    float m, l;  // maximum of q.k; sum of this lane's weights (the partner lane has the other keys')
+};
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float swap_halves(float x) { return __shfl_xor(x, 32, 64); }
+
+template <class C, int D>
+struct Tile {
+    static constexpr int kRow = D * (int)sizeof(C);    // bytes of a key in LDS
+    static constexpr int kChunks = kRow / 16;
+    static constexpr int kLoadRows = 1024 / kRow;      // rows of one wave load
+    static constexpr int kBytes = 32 * kRow;           // 32 keys
+    static constexpr int kLoads = 32 / kLoadRows;
+    // The 16-byte chunks of a row are permuted so that no read meets its neighbours
+    // in the same bank: K is read 32 rows at one column, V (16 bits) 4 rows x 32
+    // bytes, V (f32) two rows x 128 bytes.
+    __device__ static int k_chunk(int row, int c) {
+        return kChunks == 8 ? c ^ ((row ^ (row >> 3)) & 7) : c ^ (row & 15);
+    }
+    __device__ static int v_chunk(int row, int c) {
+        if (sizeof(C) == 4) return c ^ (((row >> 2) & 1) << 3);
+        return kChunks == 8 ? c ^ ((row & 3) << 1) : c ^ ((row & 7) << 1);
+    }
+};
+
+// Where keys come from: a page list with its length in keys.  The page numbers of up
+// to 64 pages are held a lane each.
+struct Pages {
+    const int32_t* list;
+    int keys;     // keys that exist: later ones read as zeros
+    int shift;
+    int first;    // page that lane 0 holds
+    int held;
+};
+
+__device__ __forceinline__ void hold_pages(Pages& p, int key) {
+    const int lane = threadIdx.x & 63, last = (p.keys - 1) >> p.shift;
+    p.first = key >> p.shift;
+    p.held = p.list[min(p.first + lane, last)];
+}
+
+// Loads of a wave: 1 KiB of consecutive keys of K or V to LDS.
+template <class C, int D>
+struct Loader {
+    using T = Tile<C, D>;
+    const char *k, *v;         // of this KV head
+    int64_t page_bytes;
+    uint32_t slot_bytes;
+    int n_pages, page_mask;
+
+    __device__ __forceinline__ void init(const vtq_kv_cache& c, int head) {
+        const int64_t at = (int64_t)head * (int64_t)c.head_stride * (int64_t)sizeof(C);
+        k = static_cast<const char*>(c.k) + at;
+        v = static_cast<const char*>(c.v) + at;
+        page_bytes = (int64_t)c.page_stride * (int64_t)sizeof(C);
+        slot_bytes = (uint32_t)(c.slot_stride * sizeof(C));
+        n_pages = (int)c.n_pages;
+        page_mask = c.page_size - 1;
+    }
+    // byte offset of this lane's 16 bytes in load l of a tile, from the load's first row
+    template <bool V>
+    __device__ __forceinline__ uint32_t offset(int l, int head_dim) const {
+        const int lane = threadIdx.x & 63;
+        const int r = lane / T::kChunks, row = l * T::kLoadRows + r;
+        const int c = V ? T::v_chunk(row, lane % T::kChunks) : T::k_chunk(row, lane % T::kChunks);
+        // chunks past head_dim read past the end: zeros
+        return c * 16 < head_dim * (int)sizeof(C) ? (uint32_t)r * slot_bytes + (uint32_t)c * 16 : 0x7FFFFFF0u;
+    }
+    // Load l of the tile that starts at `key` into lds (the tile's first byte).
+    template <bool V>
+    __device__ __forceinline__ void load(const Pages& p, int key, int l, uint32_t lds, int head_dim) const {
+        const int row = key + l * T::kLoadRows;
+        const int rows = min(T::kLoadRows, p.keys - row);
+        const int page = __builtin_amdgcn_readlane(p.held, ((row >> p.shift) - p.first) & 63);
+        const bool ok = rows > 0 && (uint32_t)page < (uint32_t)n_pages;
+        const int64_t at = ok ? (int64_t)page * page_bytes + (int64_t)(row & page_mask) * slot_bytes : 0;
+        const int bytes = ok ? (rows - 1) * (int)slot_bytes + head_dim * (int)sizeof(C) : 0;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>((V ? v : k) + at), (short)0, bytes, kWord3);
+        load_to_lds<16>(rs, offset<V>(l, head_dim), lds + (uint32_t)l * 1024u);
+    }
+};
+
+// ------------------------------------------------ one tile of 32 keys
+
+template <class Q, class C, int D>
+struct Compute {
+    using T = Tile<C, D>;
+    static constexpr bool kWide = std::is_same_v<Q, float>;  // f32 products
+    static constexpr int kStep = sizeof(C) == 4 ? 8 : 16;     // elements of a head that both half-waves read at once
+    typedef Q v8q __attribute__((ext_vector_type(8)));
+    typedef C v8c __attribute__((ext_vector_type(8)));
+    typedef C v4c __attribute__((ext_vector_type(4)));
+    // q of row lane & 31: per step, this half-wave's elements
+    struct Query {
+        std::conditional_t<kWide, float, v8q> v[kWide ? D / 2 : D / 16];
+    };
+
+    __device__ static void load_query(Query& q, const Q* p, bool valid, int head_dim) {
+        const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] *= shrink;
-        const int n = (int)min((int64_t)64, keys - j0);
-        for (int k = 0; k < n; k++) {
-            const float pk = __shfl(p, k, 64);
-            const int64_t vk = __shfl(at, k, 64);
+        for (int s = 0; s < D / kStep; s++) {
+            const int d = s * kStep + h * (kStep / 2);
+            const bool in = valid && d < head_dim;
+            if constexpr (!kWide) {
+                v8q z;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int d = lane + 64 * e;
-                if (d < hd && vk >= 0) o[e] = fmaf(pk, (float)static_cast<const C*>(a.cache.v)[vk + d], o[e]);
+                for (int j = 0; j < 8; j++) z[j] = (Q)0.0f;
+                q.v[s] = in ? *reinterpret_cast<const v8q*>(p + d) : z;
+            } else {
+#pragma unroll
+                for (int j = 0; j < kStep / 2; j += 4) {
+                    const float4 f = in ? *reinterpret_cast<const float4*>(p + d + j) : make_float4(0, 0, 0, 0);
+                    q.v[s * (kStep / 2) + j] = f.x, q.v[s * (kStep / 2) + j + 1] = f.y;
+                    q.v[s * (kStep / 2) + j + 2] = f.z, q.v[s * (kStep / 2) + j + 3] = f.w;
+                }
             }
         }
     }
-    Q* y = static_cast<Q*>(a.y) + t * a.y_token_stride + h * a.y_head_stride;
+
+    __device__ static v16f mma(v8q a, v8q b, v16f c) {
+        if constexpr (std::is_same_v<Q, __bf16>) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+        else if constexpr (std::is_same_v<Q, _Float16>) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+        else return c;
+    }
+
+    // scores of 32 keys: register 4i + e is key 8i + 4h + e, row lane & 31
+    __device__ static v16f scores(const uint8_t* k, const Query& q) {
+        const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+        v16f s = {};
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (lane + 64 * e < hd) y[lane + 64 * e] = (Q)(keys > 0 ? o[e] / l : 0.0f);
-    if (a.lse && lane == 0) a.lse[t * a.heads + h] = keys > 0 ? m + logf(l) : -INFINITY;
+        for (int i = 0; i < D / kStep; i++) {
+            const uint8_t* at = k + row * T::kRow + T::k_chunk(row, 2 * i + h) * 16;
+            if constexpr (!kWide) {
+                s = mma(*reinterpret_cast<const v8q*>(at), q.v[i], s);
+            } else if constexpr (sizeof(C) == 4) {
+                const float4 f = *reinterpret_cast<const float4*>(at);
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.x, q.v[4 * i], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.y, q.v[4 * i + 1], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.z, q.v[4 * i + 2], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.w, q.v[4 * i + 3], s, 0, 0, 0);
+            } else {
+                const v8c f = *reinterpret_cast<const v8c*>(at);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32((float)f[j], q.v[8 * i + j], s, 0, 0, 0);
+            }
+        }
+        return s;
+    }
+
+    // elements 32 db + (lane & 31) of keys 8i + 4h + 0..3
+    __device__ static v4c values4(const uint8_t* v, int db, int i) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        if constexpr (sizeof(C) == 4) {
+            v4c x;
+            const int d = 32 * db + (lane & 31);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int row = 8 * i + 4 * h + e;
+                x[e] = *reinterpret_cast<const float*>(v + row * T::kRow + T::v_chunk(row, d / 4) * 16 + (d & 3) * 4);
+            }
+            return x;
+        } else {
+            const int n = lane & 15, row = 8 * i + 4 * h + n / 4;
+            const int c = 4 * db + 2 * ((lane >> 4) & 1) + ((n & 3) >> 1);
+            const uint8_t* at = v + row * T::kRow + T::v_chunk(row, c) * 16 + (n & 1) * 8;
+            return __builtin_bit_cast(v4c, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at)));
+        }
+    }
+
+    // What the second product takes of a value: itself; itself where it is finite, else 0;
+    // 1 where it is infinite with this sign or no number, else 0.
+    enum Part { kAll, kFinite, kPlusInfinite, kMinusInfinite };
+    template <Part P>
+    __device__ static v4c part_of(v4c x) {
+        if constexpr (P != kAll) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float f = (float)x[e];
+                if constexpr (P == kFinite) x[e] = fabsf(f) < INFINITY ? x[e] : (C)0.0f;
+                if constexpr (P == kPlusInfinite) x[e] = !(f < INFINITY) ? (C)1.0f : (C)0.0f;
+                if constexpr (P == kMinusInfinite) x[e] = !(f > -INFINITY) ? (C)1.0f : (C)0.0f;
+            }
+        }
+        return x;
+    }
+
+    struct Weights {
+        std::conditional_t<kWide, v16f, v8q> v[kWide ? 1 : 2];
+    };
+    __device__ static Weights weights(v16f p) {
+        Weights w;
+        if constexpr (kWide) {
+            w.v[0] = p;
+        } else {  // rounded to the values' type: a relative 2^-9 (bf16) or 2^-12 (f16) of each, the sum stays f32
+#pragma unroll
+            for (int j = 0; j < 8; j++) w.v[0][j] = (Q)p[j], w.v[1][j] = (Q)p[8 + j];
+        }
+        return w;
+    }
+
+    // o + V^T P^T for elements 32 db .. of a head
+    template <Part P>
+    __device__ static v16f add_values(const uint8_t* v, const Weights& w, int db, v16f o) {
+#pragma unroll
+        for (int i = 0; i < 4; i += kWide ? 1 : 2) {
+            const v4c a = part_of<P>(values4(v, db, i));
+            if constexpr (kWide) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    o = __builtin_amdgcn_mfma_f32_32x32x2f32((float)a[e], w.v[0][4 * i + e], o, 0, 0, 0);
+            } else {
+                const v4c b = part_of<P>(values4(v, db, i + 1));
+                v8q x;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = a[e], x[4 + e] = b[e];
+                o = mma(x, w.v[i / 2], o);
+            }
+        }
+        return o;
+    }
+
+    // Keys key .. key + 31 of the tile at k, v.  limit: keys that this lane's row sees;
+    // low: the least of them over the wave's rows; there: keys that exist (later ones
+    // are zeros in LDS).
+    template <class Between>
+    __device__ static void tile(State<D>& st, const Query& q, const uint8_t* k, const uint8_t* v, int key, int limit,
+                                int low, int there, float c, Between between) {
+        const int h = (threadIdx.x & 63) >> 5;
+        v16f s = scores(k, q);
+        between();  // K is read; V's loads may still be on their way
+        const bool edge = key + 32 > low;  // uniform: some row does not see all of the tile
+        if (edge) {
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (key + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[r] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+        top = fmaxf(top, swap_halves(top));
+        if (__ballot(top > st.m)) {
+            const float m = fmaxf(st.m, top), base = m == -INFINITY ? 0.0f : m * c;
+            const float shrink = __builtin_amdgcn_exp2f(fmaf(st.m, c, -base));
+            st.m = m;
+            st.l *= shrink;
+#pragma unroll
+            for (int b = 0; b < D / 32; b++) st.o[b] *= shrink;
+        }
+        const float base = st.m == -INFINITY ? 0.0f : st.m * c;
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -base));
+            sum += s[r];
+        }
+        st.l += sum;
+        const Weights w = weights(s);
+        if (!edge || low >= there) {
+#pragma unroll
+            for (int b = 0; b < D / 32; b++) st.o[b] = add_values<kAll>(v, w, b, st.o[b]);
+            return;
+        }
+        // Some row sees less than what is there.  A weight of 0 does not silence a value that is not finite: such values count as
+        // zeros here, and the rows that see one get its infinity (or NaN, the sum of
+        // both) on top.
+        v16f sees;
+#pragma unroll
+        for (int r = 0; r < 16; r++) sees[r] = key + 8 * (r / 4) + 4 * h + r % 4 < limit ? 1.0f : 0.0f;
+        const Weights seen = weights(sees);
+#pragma unroll
+        for (int b = 0; b < D / 32; b++) {
+            st.o[b] = add_values<kFinite>(v, w, b, st.o[b]);
+            const v16f up = add_values<kPlusInfinite>(v, seen, b, v16f{});
+            const v16f down = add_values<kMinusInfinite>(v, seen, b, v16f{});
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                st.o[b][r] += (up[r] > 0.0f ? INFINITY : 0.0f) + (down[r] > 0.0f ? -INFINITY : 0.0f);
+        }
+    }
+};
+
+// ------------------------------------------------ workgroups
+
+template <class Q, class C, int D>
+struct Config {
+    static constexpr int kTile = Tile<C, D>::kBytes;         // 32 keys of K or V
+    static constexpr int kWaves = kTile > 16384 ? 2 : 4;
+    static constexpr int kLds = kWaves * 2 * kTile;           // a tile of K and V a wave, or two stages shared
+    static constexpr int kPerCu = kLds <= 80 * 1024 ? 2 : 1;  // workgroups of a CU
+};
+
+// Finishes a row: y and lse, or a part.  o0..o3 are elements d..d+3 of the row.
+template <class Q>
+__device__ __forceinline__ void put_row(const Job& j, int split, int64_t token, int head, int d, float4 o, float m,
+                                        float l) {
+    const Attention& a = j.a;
+    const int64_t row = token * a.heads + head;
+    if (j.prefix_splits + j.own_splits > 1) {
+        const int64_t at = (int64_t)split * a.tokens * a.heads + row;
+        *reinterpret_cast<float4*>(j.part_o + at * a.cache.head_dim + d) = o;
+        if (d == 0) j.part_ml[at] = make_float2(m, l);
+        return;
+    }
+    const bool none = l == 0.0f && m == -INFINITY;
+    const float inv = none ? 0.0f : 1.0f / l;
+    Q* y = static_cast<Q*>(a.y) + token * a.y_token_stride + head * a.y_head_stride + d;
+    typedef Q v4q __attribute__((ext_vector_type(4)));
+    v4q r;
+    r[0] = (Q)(o.x * inv), r[1] = (Q)(o.y * inv), r[2] = (Q)(o.z * inv), r[3] = (Q)(o.w * inv);
+    *reinterpret_cast<v4q*>(y) = r;
+    if (d == 0 && a.lse) a.lse[row] = none ? -INFINITY : (m + __log2f(l)) * kLn2;
+}
+
+template <class Q, class C, int D>
+__global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::kPerCu)) void attention_kernel(Job j) {
+    using Cfg = Config<Q, C, D>;
+    using T = Tile<C, D>;
+    using X = Compute<Q, C, D>;
+    constexpr int W = Cfg::kWaves;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ float2 wave_ml[W][32];
+    const Attention& a = j.a;
+    const int lane = threadIdx.x & 63, wave = wave_id(), h = lane >> 5;
+    const int hd = a.cache.head_dim, G = j.group, kv_heads = a.cache.kv_heads;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
+
+    // which part of the work: prefix and own workgroups evenly mixed
+    const int64_t blocks = j.prefix_blocks + j.own_blocks, b = blockIdx.x;
+    const int p_before = (int)(b * j.prefix_blocks / blocks), p_after = (int)((b + 1) * j.prefix_blocks / blocks);
+    const bool prefix = p_after > p_before;
+    int unit = prefix ? p_before : (int)b - p_before;
+    const int row_tiles = prefix ? j.prefix_rows : j.own_rows;
+    const int splits = prefix ? j.prefix_splits : j.own_splits;
+    const bool shared = prefix ? j.shared_prefix : j.shared_own;
+    int row_tile = unit % row_tiles;
+    unit /= row_tiles;
+    const int kv_head = unit % kv_heads;
+    unit /= kv_heads;
+    const int split = unit % splits, seq = unit / splits;
+
+    // tokens, keys and the key range
+    const int64_t all = min((int64_t)max(uniform(a.batch.q_start[a.batch.batch]), 0), a.tokens);
+    int64_t t0 = 0, t1 = all;
+    Pages pages;
+    pages.shift = j.page_shift;
+    int k0, k1, unseen = 0;  // row of token t sees keys below  t - t0 + 1 + unseen  (own keys)
+    if (prefix) {
+        pages.list = a.batch.prefix_pages;
+        pages.keys = a.batch.prefix_len;
+        k0 = split * j.prefix_chunk;
+        k1 = min(pages.keys, k0 + j.prefix_chunk);
+    } else {
+        t0 = min(max((int64_t)uniform(a.batch.q_start[seq]), (int64_t)0), all);
+        t1 = min(max((int64_t)uniform(a.batch.q_start[seq + 1]), t0), all);
+        pages.list = a.batch.pages + (int64_t)seq * a.batch.max_pages;
+        const int len = uniform(min(max(a.batch.len[seq], -(1 << 29)), 1 << 30));
+        pages.keys = min(max(len, 0), a.batch.max_pages << j.page_shift);
+        unseen = len - (int)(t1 - t0);
+        const int chunk = ((pages.keys + splits - 1) / splits + 127) & ~127;
+        k0 = (int)min((int64_t)split * chunk, (int64_t)pages.keys);
+        k1 = min(pages.keys, k0 + chunk);
+    }
+    const int n_rows = (int)min((t1 - t0) * G, (int64_t)INT32_MAX);
+    const int tile_rows = shared ? W * 32 : 32;
+    Loader<C, D> from;
+    from.init(a.cache, kv_head);
+
+    // own workgroups take every row_tiles-th tile of a sequence's rows
+    for (int r0 = row_tile * tile_rows; r0 < n_rows; r0 += row_tiles * tile_rows) {
+        const int r = r0 + (shared ? wave * 32 : 0) + (lane & 31);
+        const bool valid = r < n_rows;
+        const int64_t token = t0 + r / G;
+        const int head = kv_head * G + r % G;
+        // keys that a row sees; rows that do not exist see all
+        const int limit = !valid || prefix ? k1 : min(max(unseen + 1 + r / G, 0), k1);
+        int low = limit, high = valid ? limit : 0;
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2) low = min(low, __shfl_xor(low, x, 64)), high = max(high, __shfl_xor(high, x, 64));
+        low = uniform(low);
+        high = uniform(high);
+        // the last row of the tile sees the most
+        const int last_row = min(n_rows, r0 + tile_rows) - 1;
+        const int end = prefix ? k1 : min(max(unseen + 1 + last_row / G, 0), k1);
+        const int tiles = end > k0 ? (end - k0 + 31) / 32 : 0;  // of 32 keys
+        typename X::Query q;
+        X::load_query(q, static_cast<const Q*>(a.q.p) + token * a.q.token_stride + head * a.q.head_stride, valid, hd);
+        State<D> st;
+        st.m = -INFINITY;
+        st.l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) st.o[i] = v16f{};
+        if (tiles > 0) {
+            hold_pages(pages, k0);
+            auto holds = [&](int key) {
+                if (((min(key + 31, pages.keys - 1)) >> pages.shift) - pages.first >= 64) hold_pages(pages, key);
+            };
+            if (shared) {
+                // stages of W / 2 tiles; wave w loads rows 16w .. 16w + 15 of a stage's
+                constexpr int kStageKeys = 16 * W, kHalf = T::kLoads / 2;
+                constexpr uint32_t kStage = W * T::kBytes;  // K then V
+                const int stages = (end - k0 + kStageKeys - 1) / kStageKeys;
+                auto load_stage = [&](int n) {
+                    const int key = k0 + n * kStageKeys + (wave / 2) * 32, l0 = (wave & 1) * kHalf;
+                    const uint32_t at = lds0 + (n & 1) * kStage + (wave / 2) * T::kBytes;
+                    holds(key);
+#pragma unroll
+                    for (int l = 0; l < kHalf; l++) from.template load<false>(pages, key, l0 + l, at, hd);
+#pragma unroll
+                    for (int l = 0; l < kHalf; l++) from.template load<true>(pages, key, l0 + l, at + kStage / 2, hd);
+                };
+                load_stage(0);
+                for (int n = 0; n < stages; n++) {
+                    wait_vmcnt<0>();
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                    if (n + 1 < stages) load_stage(n + 1);
+                    const uint8_t* kt = lds + (n & 1) * kStage;
+#pragma unroll 1
+                    for (int i = 0; i < W / 2; i++) {
+                        const int key = k0 + n * kStageKeys + 32 * i;
+                        if (key < high)
+                            X::tile(st, q, kt + i * T::kBytes, kt + kStage / 2 + i * T::kBytes, key, limit, low,
+                                    pages.keys, j.c, [] {});
+                    }
+                }
+                // the next row tile's loads overwrite what other waves may still read
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            } else {
+                uint8_t* kt = lds + wave * 2 * T::kBytes;
+                const uint32_t at = lds0 + (uint32_t)wave * 2 * T::kBytes;
+                auto load_k = [&](int n) {
+                    holds(k0 + 32 * n);
+#pragma unroll
+                    for (int l = 0; l < T::kLoads; l++) from.template load<false>(pages, k0 + 32 * n, l, at, hd);
+                };
+                auto load_v = [&](int n) {
+                    holds(k0 + 32 * n);
+                    if constexpr (2 * T::kLoads > 63) wait_vmcnt<63 - T::kLoads>();  // the counter's range
+#pragma unroll
+                    for (int l = 0; l < T::kLoads; l++)
+                        from.template load<true>(pages, k0 + 32 * n, l, at + T::kBytes, hd);
+                };
+                if (wave < tiles) {
+                    load_k(wave);
+                    load_v(wave);
+                }
+                for (int n = wave; n < tiles; n += W) {
+                    const bool more = n + W < tiles;
+                    wait_vmcnt<T::kLoads>();
+                    asm volatile("" ::: "memory");
+                    X::tile(st, q, kt, kt + T::kBytes, k0 + 32 * n, limit, low, pages.keys, j.c, [&] {
+                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                        if (more) {
+                            load_k(n + W);
+                            wait_vmcnt<T::kLoads>();
+                        } else {
+                            wait_vmcnt<0>();
+                        }
+                        asm volatile("" ::: "memory");
+                    });
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (more) load_v(n + W);
+                }
+            }
+        }
+        st.l += swap_halves(st.l);
+        const float m2 = st.m == -INFINITY ? -INFINITY : st.m * j.c;
+        const int out_split = prefix ? split : j.prefix_splits + split;
+        if (shared) {
+            if (valid) {
+#pragma unroll
+                for (int db = 0; db < D / 32; db++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int d = 32 * db + 8 * i + 4 * h;
+                        const v16f& o = st.o[db];
+                        if (d < hd)
+                            put_row<Q>(j, out_split, token, head, d,
+                                       make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]), m2, st.l);
+                    }
+            }
+        } else {
+            // merge the waves' parts of the same rows, each in its own part of LDS
+            float* mine = reinterpret_cast<float*>(lds + wave * 2 * T::kBytes);
+            const int row = lane & 31;
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int db = 0; db < D / 32; db++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int c = (8 * db + 2 * i + h) ^ (row & 15);
+                    const v16f& o = st.o[db];
+                    *reinterpret_cast<float4*>(mine + row * D + 4 * c) =
+                        make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+            if (h == 0) wave_ml[wave][row] = make_float2(m2, st.l);
+            __syncthreads();
+            const int rows = min(32, n_rows - r0);
+            for (int e = threadIdx.x; e < rows * (D / 4); e += W * 64) {
+                const int rr = e / (D / 4), c = e % (D / 4);
+                if (4 * c >= hd) continue;
+                float m = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < W; w++) m = fmaxf(m, wave_ml[w][rr].x);
+                const float base = m == -INFINITY ? 0.0f : m;
+                float l = 0.0f;
+                float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const float2 ml = wave_ml[w][rr];
+                    const float f = __builtin_amdgcn_exp2f(ml.x - base);
+                    const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(
+                                                                          lds + w * 2 * T::kBytes) +
+                                                                      rr * D + 4 * (c ^ (rr & 15)));
+                    l = fmaf(ml.y, f, l);
+                    o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+                }
+                put_row<Q>(j, out_split, t0 + (r0 + rr) / G, kv_head * G + (r0 + rr) % G, 4 * c, o, m, l);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// Joins the parts of a row: one wave a row, lanes over its elements.
+template <class Q>
+__global__ __launch_bounds__(256) void join_kernel(Job j) {
+    const Attention& a = j.a;
+    const int lane = threadIdx.x & 63, splits = j.prefix_splits + j.own_splits, hd = a.cache.head_dim;
+    const int64_t rows = a.tokens * a.heads, row = (int64_t)blockIdx.x * 4 + wave_id();
+    const int64_t token = row / a.heads;
+    if (row >= rows || token >= a.batch.q_start[a.batch.batch]) return;
+    float m = -INFINITY;
+    for (int s = lane; s < splits; s += 64) m = fmaxf(m, j.part_ml[s * rows + row].x);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 64));
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    const bool in = 4 * lane < hd;
+    for (int s = 0; s < splits; s++) {
+        const float2 ml = j.part_ml[s * rows + row];
+        const float f = __builtin_amdgcn_exp2f(ml.x - base);
+        l = fmaf(ml.y, f, l);
+        if (in && ml.y != 0.0f) {
+            const float4 x = *reinterpret_cast<const float4*>(j.part_o + (s * rows + row) * hd + 4 * lane);
+            o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+        }
+    }
+    const bool none = m == -INFINITY && l == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / l;
+    typedef Q v4q __attribute__((ext_vector_type(4)));
+    if (in) {
+        v4q r;
+        r[0] = (Q)(o.x * inv), r[1] = (Q)(o.y * inv), r[2] = (Q)(o.z * inv), r[3] = (Q)(o.w * inv);
+        *reinterpret_cast<v4q*>(static_cast<Q*>(a.y) + token * a.y_token_stride + (row % a.heads) * a.y_head_stride +
+                                4 * lane) = r;
+    }
+    if (a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (m + __log2f(l)) * kLn2;
+}
+
+// ------------------------------------------------ how the work is split
+
+int waves_of(int cache_type, int head_dim) {
+    const int d = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    return 32 * d * (int)type_bytes(cache_type) > 16384 ? 2 : 4;
+}
+
+void split_work(Job& j) {
+    const Attention& a = j.a;
+    const int W = waves_of(a.cache.type, a.cache.head_dim);
+    auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    const int64_t slots = 512;
+    j.group = a.heads / a.cache.kv_heads;
+    j.page_shift = __builtin_ctz((unsigned)a.cache.page_size);
+    const int64_t prefix_rows = a.tokens * j.group;
+    const int64_t own_rows = std::min<int64_t>(std::max(1, a.batch.max_q), a.tokens) * j.group;
+    j.shared_prefix = prefix_rows > 32;
+    j.shared_own = own_rows > 32;
+    j.prefix_rows = j.prefix_splits = 0;
+    j.prefix_chunk = 128;
+    if (a.batch.prefix_len) {
+        j.prefix_rows = (int)up(prefix_rows, j.shared_prefix ? 32 * W : 32);
+        const int64_t units = (int64_t)a.cache.kv_heads * j.prefix_rows;
+        int64_t splits = std::min<int64_t>({up(slots, units), up(a.batch.prefix_len, 256), 64});
+        j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), 128) * 128);
+        j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
+    }
+    const int64_t most = (int64_t)a.batch.max_pages << j.page_shift;
+    const int64_t len = a.batch.max_len ? std::min<int64_t>(a.batch.max_len, most) : most;
+    j.own_rows = (int)up(own_rows, j.shared_own ? 32 * W : 32);
+    const int64_t units = (int64_t)a.cache.kv_heads * j.own_rows * a.batch.batch;
+    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({up(slots, units), up(len, 256), 64}));
+    j.prefix_blocks = a.cache.kv_heads * j.prefix_rows * j.prefix_splits;
+    j.own_blocks = (int)(units * j.own_splits);
 }
 
 }  // namespace
 
-size_t attention_workspace(const vtq_kv_cache&, const vtq_kv_batch&, int, int64_t, int) { return 0; }
+size_t attention_workspace(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int, int64_t tokens, int heads) {
+    Job j{};
+    j.a.cache = cache;
+    j.a.batch = batch;
+    j.a.tokens = tokens;
+    j.a.heads = heads;
+    split_work(j);
+    const size_t splits = j.prefix_splits + j.own_splits;
+    return splits > 1 ? splits * tokens * heads * (cache.head_dim * sizeof(float) + sizeof(float2)) + 256 : 0;
+}
+
+template <class Q, class C, int D>
+hipError_t launch_attention_of(const Job& j, hipStream_t stream) {
+    using Cfg = Config<Q, C, D>;
+    const void* f = reinterpret_cast<const void*>(&attention_kernel<Q, C, D>);
+    if (hipError_t e = allow_dynamic_lds(f, Cfg::kLds + 2048)) return e;
+    hipLaunchKernelGGL((attention_kernel<Q, C, D>), dim3((unsigned)(j.prefix_blocks + j.own_blocks)),
+                       dim3(Cfg::kWaves * 64), Cfg::kLds, stream, j);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (j.prefix_splits + j.own_splits > 1) {
+        hipLaunchKernelGGL((join_kernel<Q>), dim3((unsigned)((j.a.tokens * j.a.heads + 3) / 4)), dim3(256), 0, stream, j);
+        return hipGetLastError();
+    }
+    return hipSuccess;
+}
 
 hipError_t launch_attention(const Attention& a, int type, hipStream_t stream) {
-    const dim3 grid((unsigned)a.tokens, (unsigned)a.heads);
+    Job j{};
+    j.a = a;
+    split_work(j);
+    j.c = a.scale * kLog2E;
+    const size_t rows = (size_t)(j.prefix_splits + j.own_splits) * a.tokens * a.heads;
+    j.part_o = static_cast<float*>(a.ws);
+    j.part_ml = reinterpret_cast<float2*>(static_cast<char*>(a.ws) +
+                                          (rows * a.cache.head_dim * sizeof(float) + 255) / 256 * 256);
     return with_type(type, [&](auto q) {
         using Q = decltype(q);
         return with_type(a.cache.type, [&](auto c) {
@@ -86,8 +701,9 @@ hipError_t launch_attention(const Attention& a, int type, hipStream_t stream) {
             if constexpr (!std::is_same_v<Q, C> && !std::is_same_v<Q, float>) {
                 return hipErrorInvalidValue;
             } else {
-                hipLaunchKernelGGL((attention_rows_kernel<Q, C>), grid, dim3(64), 0, stream, a);
-                return hipGetLastError();
+                if (a.cache.head_dim <= 64) return launch_attention_of<Q, C, 64>(j, stream);
+                if (a.cache.head_dim <= 128) return launch_attention_of<Q, C, 128>(j, stream);
+                return launch_attention_of<Q, C, 256>(j, stream);
             }
         });
     });

@@ -122,6 +122,7 @@ size_t vtq_attention_workspace(const vtq_kv_cache* cache, const vtq_kv_batch* ba
                                size_t heads) {
     if (!cache || !batch || check_cache(cache) || check_batch(batch, cache, false)) return 0;
     if (type_bytes(type) == 0 || tokens > kMostTokens || heads > 65535 || heads % cache->kv_heads) return 0;
+    if (!attention_fits(cache, batch, tokens, heads)) return 0;
     if (tokens == 0 || heads == 0 || batch->batch == 0) return 0;
     return attention_workspace(*cache, *batch, type, (int64_t)tokens, (int)heads);
 }

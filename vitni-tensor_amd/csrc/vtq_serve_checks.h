@@ -52,6 +52,7 @@ inline Refusal check_cache(const vtq_kv_cache* c) {
     VTQ_REFUSE(c->slot_stride >= (size_t)1 << 24 || c->head_stride >= kMostStride / 65536 ||
                    c->page_stride >= kMostStride / 4,
                VTQ_E_NOT_IMPLEMENTED, "vtq: cache stride too large");
+    VTQ_REFUSE(c->n_pages * (c->page_stride / 8) > (size_t)1 << 43, VTQ_E_NOT_IMPLEMENTED, "vtq: cache too large");
     VTQ_REFUSE(c->n_pages && (!c->k || !c->v), VTQ_E_INVALID_ARGUMENT, "vtq: null cache");
     VTQ_REFUSE(!aligned(c->k, 16) || !aligned(c->v, 16), VTQ_E_INVALID_ARGUMENT,
                "vtq: the cache must be 16-byte aligned");
@@ -79,6 +80,14 @@ inline Refusal check_rows(const void* p, size_t token_stride, size_t head_stride
     VTQ_REFUSE(token_stride >= kMostStride / 4 || head_stride >= kMostStride / 4, VTQ_E_NOT_IMPLEMENTED,
                "vtq: stride too large");
     return {};
+}
+
+// Whether the launches stay below 2^32 threads: 256 of them to 4 rows of queries, and
+// to a sequence, KV head and 32 rows.
+inline bool attention_fits(const vtq_kv_cache* c, const vtq_kv_batch* b, size_t tokens, size_t heads) {
+    const size_t max_q = (size_t)b->max_q < tokens ? (size_t)b->max_q : tokens;
+    return tokens * heads <= (size_t)1 << 25 &&
+           (size_t)b->batch * (size_t)c->kv_heads * (max_q * (heads / (size_t)c->kv_heads) / 32 + 1) <= (size_t)1 << 22;
 }
 
 // A plan from its parameters.
@@ -231,6 +240,7 @@ inline Refusal check_attention(const vtq_kv_cache* cache, const vtq_kv_batch* ba
                "vtq: activations are F32 or of the cache's type");
     VTQ_REFUSE(tokens > kMostTokens || heads > 65535, VTQ_E_NOT_IMPLEMENTED, "vtq: too many tokens or heads");
     VTQ_REFUSE(heads % cache->kv_heads, VTQ_E_INVALID_SHAPE, "vtq: heads must be a multiple of kv_heads");
+    VTQ_REFUSE(!attention_fits(cache, batch, tokens, heads), VTQ_E_NOT_IMPLEMENTED, "vtq: more than 2^25 rows of queries");
     VTQ_REFUSE(!std::isfinite(scale) || scale <= 0.0f, VTQ_E_INVALID_ARGUMENT, "vtq: scale must be positive");
     if (tokens == 0 || heads == 0 || batch->batch == 0) return {};
     const size_t hd = cache->head_dim, es = type_bytes(type);
