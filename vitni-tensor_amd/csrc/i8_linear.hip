@@ -121,14 +121,17 @@ __global__ __launch_bounds__(W * 64) void i8_rows_kernel(I8Linear a) {
 // ------------------------------------------------ product, many tokens
 
 // A workgroup owns BM tokens x BN channels, a wave 32 TM x 32 TN of them on 32x32x32
-// MFMAs.  Tiles of both operands go from memory straight to LDS, two stages of 128
+// MFMAs.  Tiles of both operands go from memory straight to LDS, S stages of 128
 // bytes of K; the 16-byte chunks of a row are permuted so that the 16 rows that a
-// read takes at one column lie in different banks.
+// read takes at one column lie in different banks.  Operands are read one MFMA group
+// ahead, across the stages' barrier too; loads past the last stage read zeros from
+// nowhere, so that the count of those in flight stays the same.
 typedef int v16i __attribute__((ext_vector_type(16)));
 
-template <int TM_, int TN_, int WM_, int WN_>
+template <int TM_, int TN_, int WM_, int WN_, int S_, int PER_CU_>
 struct Tiles {
-    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, W = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, S = S_, PER_CU = PER_CU_;
+    static constexpr int W = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
     static constexpr int kStage = (BM + BN) * 128;
     static constexpr int kLoadsA = BM / 8 / W, kLoadsB = BN / 8 / W;  // 1 KiB (8 rows) each, a wave
 };
@@ -136,8 +139,9 @@ struct Tiles {
 __device__ __forceinline__ int chunk_of(int row, int c) { return c ^ ((row ^ ((row >> 3) & 1)) & 7); }
 
 template <class O, class T>
-__global__ __launch_bounds__(T::W * 64, T::W / 4 == 2 ? 2 : 1) void i8_tiles_kernel(I8Linear a, int m_tiles, int n_tiles) {
+__global__ __launch_bounds__(T::W * 64, T::PER_CU * T::W / 4) void i8_tiles_kernel(I8Linear a, int m_tiles, int n_tiles) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ __attribute__((aligned(16))) float x_scale[T::BM], w_scale[T::BN], w_bias[T::BN];
     const int lane = threadIdx.x & 63, wave = wave_id(), row = lane & 31, h = lane >> 5;
     // Workgroups go to the 8 XCDs in turn: each XCD takes one run of tiles, 8 token
     // tiles deep before the next channels, so that what it loads meets its own L2.
@@ -161,9 +165,9 @@ __global__ __launch_bounds__(T::W * 64, T::W / 4 == 2 ? 2 : 1) void i8_tiles_ker
     for (int i = 0; i < T::kLoadsB; i++) off_b[i] = at((wave * T::kLoadsB + i) * 8 + lane / 8, a.ld_w);
     auto load = [&](int k, int stage) {
         const __amdgpu_buffer_rsrc_t rx =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp + k), (short)0, x_bytes - k, kWord3);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp + k), (short)0, k < k_end ? x_bytes - k : 0, kWord3);
         const __amdgpu_buffer_rsrc_t rw =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp + k), (short)0, w_bytes - k, kWord3);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp + k), (short)0, k < k_end ? w_bytes - k : 0, kWord3);
         const uint32_t to = lds0 + (uint32_t)stage * T::kStage;
         // chunks past the row's end, in the last step, read as zeros
         const auto cut = [&](uint32_t off, int r) {
@@ -186,57 +190,122 @@ __global__ __launch_bounds__(T::W * 64, T::W / 4 == 2 ? 2 : 1) void i8_tiles_ker
 #pragma unroll
         for (int j = 0; j < T::TN; j++) acc[i][j] = v16i{};
     const int wm = wave / T::WN * T::TM * 32, wn = wave % T::WN * T::TN * 32;
-    load(0, 0);
-    for (int k = 0, stage = 0; k < k_end; k += 128, stage ^= 1) {
-        wait_vmcnt<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (k + 128 < k_end) load(k + 128, stage ^ 1);
-        const uint8_t* la = lds + stage * T::kStage + (wm + row) * 128;
-        const uint8_t* lb = lds + stage * T::kStage + (T::BM + wn + row) * 128;
+    // operands of 32 inputs: step s of the stage at `from`
+    struct Operands {
+        v4i a[T::TM], b[T::TN];
+    };
+    auto read = [&](Operands& o, const uint8_t* from, int s) {
+        const int c = 16 * chunk_of(row, 2 * s + h);  // rows 16 apart have the same permutation
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-            // rows 16 apart have the same permutation
-            const int c = 16 * chunk_of(row, 2 * s + h);
-            v4i av[T::TM], bv[T::TN];
+        for (int i = 0; i < T::TM; i++) o.a[i] = *reinterpret_cast<const v4i*>(from + (wm + row + 32 * i) * 128 + c);
 #pragma unroll
-            for (int i = 0; i < T::TM; i++) av[i] = *reinterpret_cast<const v4i*>(la + i * 32 * 128 + c);
-#pragma unroll
-            for (int j = 0; j < T::TN; j++) bv[j] = *reinterpret_cast<const v4i*>(lb + j * 32 * 128 + c);
-#pragma unroll
-            for (int i = 0; i < T::TM; i++)
-#pragma unroll
-                for (int j = 0; j < T::TN; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], bv[j], acc[i][j], 0, 0, 0);
-        }
-    }
-    // acc: channel lane & 31, tokens 8 (r / 4) + 4 h + r % 4
-#pragma unroll
-    for (int j = 0; j < T::TN; j++) {
-        const int n = wn + 32 * j + row;
-        if (n >= n_rows) continue;
+        for (int j = 0; j < T::TN; j++)
+            o.b[j] = *reinterpret_cast<const v4i*>(from + (T::BM + wn + row + 32 * j) * 128 + c);
+    };
+    auto multiply = [&](const Operands& o) {
 #pragma unroll
         for (int i = 0; i < T::TM; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int m = wm + 32 * i + 8 * (r / 4) + 4 * h + r % 4;
-                if (m < m_rows) store<O>(a, m0 + m, n0 + n, acc[i][j][r]);
+            for (int j = 0; j < T::TN; j++)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(o.b[j], o.a[i], acc[i][j], 0, 0, 0);
+    };
+    for (int m = threadIdx.x; m < T::BM; m += T::W * 64) x_scale[m] = m < m_rows && a.in_feat ? a.xs[m0 + m] : 0.0f;
+    for (int n = threadIdx.x; n < T::BN; n += T::W * 64) {
+        w_scale[n] = n < n_rows && a.in_feat ? a.ws[n0 + n] : 0.0f;
+        w_bias[n] = n < n_rows && a.bias ? a.bias[n0 + n] : 0.0f;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // seen by all after the loop's barriers
+    constexpr int kLoads = T::kLoadsA + T::kLoadsB;
+#pragma unroll
+    for (int i = 0; i < T::S; i++) load(128 * i, i);
+    wait_vmcnt<(T::S - 1) * kLoads>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Operands x[2];
+    read(x[0], lds, 0);
+    int stage = 0;
+    for (int k = 0; k < k_end; k += 128) {
+        const uint8_t* here = lds + stage * T::kStage;
+#pragma unroll
+        for (int s = 0; s < 3; s++) {
+            read(x[(s + 1) & 1], here, s + 1);
+            multiply(x[s & 1]);
+        }
+        // The stage's last operands are in registers: once every wave is here it is free
+        // for the loads of S steps on, and the next one has landed.
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_vmcnt<(T::S - 2) * kLoads>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int next = stage + 1 == T::S ? 0 : stage + 1;
+        read(x[0], lds + next * T::kStage, 0);
+        load(k + 128 * T::S, stage);
+        multiply(x[1]);
+        stage = next;
+    }
+    // The tile's outputs go through the wave's own part of LDS, 32 tokens at a time, so
+    // that rows of 16-byte pieces leave (written as the MFMAs hold them, 256 x 256 of
+    // bf16 took a workgroup 27 us).  acc: token lane & 31, channels 8 g + 4 h + e.
+    wait_vmcnt<0>();  // the loads of zeros
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    typedef O o4 __attribute__((ext_vector_type(4)));
+    constexpr int kRow = T::TN * 32 * (int)sizeof(O), kPitch = kRow + 16, kPieces = kRow / 16, kEach = 16 / (int)sizeof(O);
+    static_assert(32 * kPitch * T::W <= T::S * T::kStage, "LDS of the epilogue");
+    uint8_t* out = lds + wave * 32 * kPitch;
+    O* y = static_cast<O*>(a.y) + (size_t)(m0 + wm) * a.ld_y + n0 + wn;
+    const bool whole = reinterpret_cast<uintptr_t>(y) % 16 == 0 && a.ld_y * sizeof(O) % 16 == 0;
+#pragma unroll
+    for (int i = 0; i < T::TM; i++) {
+        const float xs = x_scale[wm + 32 * i + row];
+#pragma unroll
+        for (int j = 0; j < T::TN; j++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int n = 32 * j + 8 * g + 4 * h;
+                const float4 ws = *reinterpret_cast<const float4*>(&w_scale[wn + n]);
+                const float4 bias = *reinterpret_cast<const float4*>(&w_bias[wn + n]);
+                o4 v;
+                v[0] = (O)((float)acc[i][j][4 * g] * xs * ws.x + bias.x);
+                v[1] = (O)((float)acc[i][j][4 * g + 1] * xs * ws.y + bias.y);
+                v[2] = (O)((float)acc[i][j][4 * g + 2] * xs * ws.z + bias.z);
+                v[3] = (O)((float)acc[i][j][4 * g + 3] * xs * ws.w + bias.w);
+                *reinterpret_cast<o4*>(out + row * kPitch + n * (int)sizeof(O)) = v;
             }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's LDS accesses are in order
+#pragma unroll
+        for (int p = 0; p < 32 * kPieces / 64; p++) {
+            const int m = (p * 64 + lane) / kPieces, c = (p * 64 + lane) % kPieces;
+            if (wm + 32 * i + m >= m_rows) continue;
+            const uint8_t* from = out + m * kPitch + c * 16;
+            O* to = y + (size_t)(32 * i + m) * a.ld_y + c * kEach;
+            if (whole && wn + (c + 1) * kEach <= n_rows) {
+                *reinterpret_cast<v4i*>(to) = *reinterpret_cast<const v4i*>(from);
+            } else {
+                for (int e = 0; e < kEach; e++)
+                    if (wn + c * kEach + e < n_rows) to[e] = reinterpret_cast<const O*>(from)[e];
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
-using Tiles256 = Tiles<4, 2, 2, 4>;     // 256 x 256, 8 waves
-using Tiles128 = Tiles<2, 2, 2, 2>;     // 128 x 128, 4 waves
-using Tiles256x128 = Tiles<4, 2, 2, 2>;  // 4 waves
+using Tiles128 = Tiles<2, 2, 2, 2, 2, 2>;
+using Tiles128x256 = Tiles<2, 4, 2, 2, 3, 1>;
+using Tiles256 = Tiles<4, 2, 2, 4, 2, 1>;
+using TF9 = Tiles<2, 2, 2, 4, 3, 1>;
+using TF10 = Tiles<2, 1, 2, 4, 4, 1>;
+using TF11 = Tiles<2, 1, 2, 4, 2, 2>;
+using TF7 = Tiles<2, 2, 2, 2, 4, 1>;
+using TF12 = Tiles<4, 1, 2, 4, 3, 1>;
 
 template <class O, class T>
 hipError_t launch_tiles(const I8Linear& a, hipStream_t stream) {
     const int m_tiles = (a.batch + T::BM - 1) / T::BM, n_tiles = (a.out_feat + T::BN - 1) / T::BN;
     const void* f = reinterpret_cast<const void*>(&i8_tiles_kernel<O, T>);
-    if (hipError_t e = allow_dynamic_lds(f, 2 * T::kStage)) return e;
+    if (hipError_t e = allow_dynamic_lds(f, T::S * T::kStage + 4096)) return e;
     const int per = (m_tiles * n_tiles + 7) / 8;
-    hipLaunchKernelGGL((i8_tiles_kernel<O, T>), dim3((unsigned)per * 8), dim3(T::W * 64), 2 * T::kStage, stream, a, m_tiles,
+    hipLaunchKernelGGL((i8_tiles_kernel<O, T>), dim3((unsigned)per * 8), dim3(T::W * 64), T::S * T::kStage, stream, a, m_tiles,
                        n_tiles);
     return hipGetLastError();
 }
@@ -256,8 +325,13 @@ hipError_t launch_form(const I8Linear& a, int form, hipStream_t stream) {
     case 2: return launch_rows<O, 4, 2>(a, stream);
     case 3: return launch_rows<O, 4, 4>(a, stream);
     case 4: return launch_tiles<O, Tiles128>(a, stream);
-    case 5: return launch_tiles<O, Tiles256x128>(a, stream);
-    default: return launch_tiles<O, Tiles256>(a, stream);
+    case 5: return launch_tiles<O, Tiles128x256>(a, stream);
+    case 6: return launch_tiles<O, Tiles256>(a, stream);
+    case 7: return launch_tiles<O, TF7>(a, stream);
+    case 9: return launch_tiles<O, TF9>(a, stream);
+    case 10: return launch_tiles<O, TF10>(a, stream);
+    case 11: return launch_tiles<O, TF11>(a, stream);
+    default: return launch_tiles<O, TF12>(a, stream);
     }
 }
 
