@@ -19,38 +19,92 @@ constexpr int kWord3 = 0x00020000;  // raw buffer, stride 0
 
 // ------------------------------------------------ quantization
 
-// x / s to the nearest whole number, ties to even, of the exact quotient: the f32
-// quotient may round onto a half, so the remainder decides.  x - q s is exact in one
-// fma (a multiple of the smaller unit in the last place, below s in magnitude).
-__device__ __forceinline__ int quotient(float x, float s) {
-    float q = rintf(x / s);
+// x / s to the nearest whole number, ties to even, of the exact quotient.  x times
+// the reciprocal is off by two units in its last place at most, so it rounds to a
+// neighbour of the answer; the remainder, exact in one fma (a multiple of the smaller
+// unit in the last place, below 2 s in magnitude), decides.
+__device__ __forceinline__ int quotient(float x, float s, float inv) {
+    float q = rintf(x * inv);
     const float r = fmaf(-q, s, x), twice = 2.0f * fabsf(r);
     if (twice > s || (twice == s && ((int)q & 1))) q += (r < 0.0f) ? -1.0f : 1.0f;
     return (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
-constexpr int kQuantThreads = 256;
+// A thread takes 16 elements at a time, whole 16-byte pieces of the output; rows of up
+// to 16384 stay in registers between the maximum and the rounding.  Rows of up to 1024
+// elements take one wave of a workgroup's four, longer ones a workgroup.  One row of
+// 4096 bf16: 3.3 us, a launch's own time; 11.1 with an element at a time, twice read.
+constexpr int kQuantMost = 1024;  // threads
 
 template <class T>
-__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T* x, size_t ld_x, int8_t* q, size_t ld_q,
-                                                                 float* scale, int rows, int n) {
-    __shared__ uint32_t top[kQuantThreads / 64];
-    for (int m = (int)blockIdx.x; m < rows; m += (int)gridDim.x) {
-        const T* xr = x + (size_t)m * ld_x;
-        // the largest magnitude by its bits: a NaN is above an infinity above every number
-        uint32_t a = 0;
-        for (int k = threadIdx.x; k < n; k += kQuantThreads)
-            a = max(a, __float_as_uint((float)xr[k]) & 0x7FFFFFFFu);
+__device__ __forceinline__ void load16(float (&f)[16], const T* p, int left, bool whole) {
+    if (whole && left >= 16) {
+        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+        constexpr int N = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 16 / N; i++) {
+            const vec v = reinterpret_cast<const vec*>(p)[i];
+#pragma unroll
+            for (int e = 0; e < N; e++) f[i * N + e] = (float)v[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) f[e] = e < left ? (float)p[e] : 0.0f;
+    }
+}
+
+__device__ __forceinline__ uint32_t top_bits(const float (&f)[16]) {
+    uint32_t a = 0;  // magnitudes by their bits: a NaN is above an infinity above every number
+#pragma unroll
+    for (int e = 0; e < 16; e++) a = max(a, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+    return a;
+}
+
+// tpr: threads of a row, 64 (the workgroup's waves have a row each) or the whole workgroup
+template <class T>
+__global__ __launch_bounds__(kQuantMost) void quantize_kernel(const T* x, size_t ld_x, int8_t* q, size_t ld_q,
+                                                              float* scale, int rows, int n, int tpr, bool whole) {
+    __shared__ uint32_t top[kQuantMost / 64];
+    const int per = (int)blockDim.x / tpr, t = (int)threadIdx.x % tpr;
+    for (int64_t m0 = (int64_t)blockIdx.x * per; m0 < rows; m0 += (int64_t)gridDim.x * per) {
+        const int64_t m = m0 + (int)threadIdx.x / tpr;
+        const bool row = m < rows;
+        const T* xr = x + (row ? m : 0) * ld_x;
+        const int last = row ? n : 0;
+        float f[16];
+        load16(f, xr + 16 * t, last - 16 * t, whole);
+        uint32_t a = top_bits(f);
+        for (int k = 16 * (t + tpr); k < last; k += 16 * tpr) {
+            float g[16];
+            load16(g, xr + k, last - k, whole);
+            a = max(a, top_bits(g));
+        }
+#pragma unroll
         for (int d = 1; d < 64; d *= 2) a = max(a, (uint32_t)__shfl_xor((int)a, d, 64));
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = a;
-        __syncthreads();
-        for (int w = 0; w < kQuantThreads / 64; w++) a = max(a, top[w]);
-        const bool finite = a < 0x7F800000u;
-        const float s = finite ? __uint_as_float(a) / 127.0f : __uint_as_float(a);
-        if (threadIdx.x == 0) scale[m] = s;
-        for (size_t k = threadIdx.x; k < ld_q; k += kQuantThreads)
-            q[(size_t)m * ld_q + k] = (int8_t)(k < (size_t)n && finite && s > 0.0f ? quotient((float)xr[k], s) : 0);
+        if (tpr > 64) {
+            if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = a;
+            __syncthreads();
+            for (int w = 0; w < tpr / 64; w++) a = max(a, top[w]);
+            __syncthreads();
+        }
+        if (!row) continue;
+        const float s = a < 0x7F800000u ? __uint_as_float(a) / 127.0f : __uint_as_float(a);
+        const bool some = a < 0x7F800000u && s > 0.0f;
+        // where the reciprocal would overflow, both are scaled: exact powers of two
+        const float up = s < 0x1p-100f ? 0x1p100f : 1.0f, su = s * up, inv = some ? 1.0f / su : 0.0f;
+        if (t == 0) scale[m] = s;
+        for (size_t k = 16 * (size_t)t; k < ld_q; k += 16 * (size_t)tpr) {
+            if (k != 16 * (size_t)t) load16(f, xr + k, n > (int64_t)k ? n - (int)k : 0, whole);
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                o[i] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    o[i] |= (uint32_t)((some ? quotient(f[4 * i + e] * up, su, inv) : 0) & 255) << (8 * e);
+            }
+            *reinterpret_cast<uint4*>(q + m * ld_q + k) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
     }
 }
 
@@ -67,7 +121,13 @@ __device__ __forceinline__ void store(const I8Linear& a, int m, int n, int sum) 
 
 // A workgroup owns 16 output channels x 16 MT tokens, its waves every W-th 256 bytes
 // of K; lane (r, g) of a wave takes the 64 bytes g of row r, channel and token alike
-// (the order of K inside an MFMA is free as long as both operands share it).
+// (the order of K inside an MFMA is free as long as both operands share it).  The next
+// 256 bytes load while these multiply.
+template <int MT>
+struct RowOperands {
+    v4i w[4], x[MT][4];
+};
+
 template <class O, int W, int MT>
 __global__ __launch_bounds__(W * 64) void i8_rows_kernel(I8Linear a) {
     __shared__ int part[W][16 * MT][17];
@@ -82,25 +142,35 @@ __global__ __launch_bounds__(W * 64) void i8_rows_kernel(I8Linear a) {
     v4i acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) acc[t] = v4i{0, 0, 0, 0};
-    for (int k = wave * 256; k < k_end; k += W * 256) {
-        v4i wv[4], xv[MT][4];
+    auto load = [&](RowOperands<MT>& o, int k) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int at = k + g * 64 + i * 16;
             // rows past the last one and bytes past the row give zeros
-            const int ow = at < k_end && r < n_rows ? (int)(r * a.ld_w) + at : -1;
-            wv[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, ow, 0, 0));
+            const int ow = at < k_end && r < n_rows ? (int)(r * a.ld_w) + at : -16;
+            o.w[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, ow, 0, 0));
 #pragma unroll
             for (int t = 0; t < MT; t++) {
-                const int ox = at < k_end && 16 * t + r < m_rows ? (int)((16 * t + r) * a.ld_x) + at : -1;
-                xv[t][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, ox, 0, 0));
+                const int ox = at < k_end && 16 * t + r < m_rows ? (int)((16 * t + r) * a.ld_x) + at : -16;
+                o.x[t][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, ox, 0, 0));
             }
         }
+    };
+    auto multiply = [&](const RowOperands<MT>& o) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int t = 0; t < MT; t++)
-                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[t][i], wv[i], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.x[t][i], o.w[i], acc[t], 0, 0, 0);
+    };
+    RowOperands<MT> u, v;
+    int k = wave * 256;
+    load(u, k);
+    for (; k < k_end; k += 2 * W * 256) {
+        load(v, k + W * 256);
+        multiply(u);
+        load(u, k + 2 * W * 256);
+        multiply(v);
     }
     // acc: channel lane & 15, tokens 4 (lane >> 4) + 0..3
 #pragma unroll
@@ -299,6 +369,111 @@ using TF11 = Tiles<2, 1, 2, 4, 2, 2>;
 using TF7 = Tiles<2, 2, 2, 2, 4, 1>;
 using TF12 = Tiles<4, 1, 2, 4, 3, 1>;
 
+// ------------------------------------------------ product, some tens of tokens
+
+// A workgroup owns 32 TM tokens x 32 channels, its 4 waves every fourth 128 bytes of K,
+// each with tiles of its own in LDS, S deep: nothing waits for another wave until the
+// sums are joined.
+template <class O, int TM, int S>
+__global__ __launch_bounds__(256, 1) void i8_slices_kernel(I8Linear a) {
+    constexpr int kStage = (TM + 1) * 4096, kLoads = (TM + 1) * 4, BM = 32 * TM;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = wave_id(), row = lane & 31, h = lane >> 5;
+    const int n0 = (int)blockIdx.x * 32, m0 = (int)blockIdx.y * BM;
+    const int k_end = (a.in_feat + 15) & ~15;
+    const int m_rows = min(BM, a.batch - m0), n_rows = min(32, a.out_feat - n0);
+    const int8_t* xp = a.x + (size_t)m0 * a.ld_x;
+    const int8_t* wp = a.w + (size_t)n0 * a.ld_w;
+    const int x_bytes = (int)((m_rows - 1) * a.ld_x) + k_end, w_bytes = (int)((n_rows - 1) * a.ld_w) + k_end;
+    uint8_t* mine = lds + wave * S * kStage;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)mine;
+    auto load = [&](int k, int stage) {
+        const __amdgpu_buffer_rsrc_t rx =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp + k), (short)0, k < k_end ? x_bytes - k : 0, kWord3);
+        const __amdgpu_buffer_rsrc_t rw =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp + k), (short)0, k < k_end ? w_bytes - k : 0, kWord3);
+        const uint32_t to = lds0 + (uint32_t)stage * kStage;
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const bool is_w = i < 4;
+            const int r = (is_w ? i : i - 4) * 8 + lane / 8, c = 16 * chunk_of(r, lane & 7);
+            // chunks past the row's end, in the last step, read as zeros
+            const uint32_t off =
+                k + 128 > k_end && k + c >= k_end ? 0x7FFFFFF0u : (uint32_t)(r * (is_w ? a.ld_w : a.ld_x)) + (uint32_t)c;
+            load_to_lds<16>(is_w ? rw : rx, off, to + 1024u * i);
+        }
+    };
+    v16i acc[TM];
+#pragma unroll
+    for (int i = 0; i < TM; i++) acc[i] = v16i{};
+    const int k0 = wave * 128;
+#pragma unroll
+    for (int i = 0; i < S; i++) load(k0 + 512 * i, i);
+    int stage = 0;
+    for (int k = k0; k < k_end; k += 512) {
+        wait_vmcnt<(S - 1) * kLoads>();
+        asm volatile("" ::: "memory");
+        const uint8_t* from = mine + stage * kStage + row * 128;
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const int c = 16 * chunk_of(row, 2 * s + h);
+            const v4i w = *reinterpret_cast<const v4i*>(from + c);
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+                acc[i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+                    w, *reinterpret_cast<const v4i*>(from + (i + 1) * 4096 + c), acc[i], 0, 0, 0);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: free for the loads of S steps on
+        load(k + 512 * S, stage);
+        stage = stage + 1 == S ? 0 : stage + 1;
+    }
+    wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    // acc: token lane & 31, channels 8 g + 4 h + e.  Sums of a token: 32 channels and a pad.
+    static_assert(BM * 36 * 4 <= S * kStage, "LDS of the sums");
+    int* sums = reinterpret_cast<int*>(mine);
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<v4i*>(sums + (32 * i + row) * 36 + 8 * g + 4 * h) =
+                v4i{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+    __syncthreads();
+    for (int e = threadIdx.x; e < BM * 8; e += 256) {
+        const int m = e / 8, n = e % 8 * 4;
+        if (m >= m_rows || n >= n_rows) continue;
+        v4i sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            sum += *reinterpret_cast<const v4i*>(reinterpret_cast<const int*>(lds + w * S * kStage) + m * 36 + n);
+        const float xs = a.in_feat ? a.xs[m0 + m] : 0.0f;
+        O* y = static_cast<O*>(a.y) + (size_t)(m0 + m) * a.ld_y + n0 + n;
+        typedef O o4 __attribute__((ext_vector_type(4)));
+        o4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const bool in = n + i < n_rows;
+            v[i] = (O)((float)sum[i] * xs * (in && a.in_feat ? a.ws[n0 + n + i] : 0.0f) + (in && a.bias ? a.bias[n0 + n + i] : 0.0f));
+        }
+        if (n + 4 <= n_rows && reinterpret_cast<uintptr_t>(y) % sizeof(o4) == 0) {
+            *reinterpret_cast<o4*>(y) = v;
+        } else {
+            for (int i = 0; i < 4 && n + i < n_rows; i++) y[i] = v[i];
+        }
+    }
+}
+
+template <class O, int TM, int S>
+hipError_t launch_slices(const I8Linear& a, hipStream_t stream) {
+    const void* f = reinterpret_cast<const void*>(&i8_slices_kernel<O, TM, S>);
+    constexpr int bytes = 4 * S * (TM + 1) * 4096;
+    if (hipError_t e = allow_dynamic_lds(f, bytes)) return e;
+    hipLaunchKernelGGL((i8_slices_kernel<O, TM, S>),
+                       dim3((unsigned)((a.out_feat + 31) / 32), (unsigned)((a.batch + 32 * TM - 1) / (32 * TM))), dim3(256),
+                       bytes, stream, a);
+    return hipGetLastError();
+}
+
 template <class O, class T>
 hipError_t launch_tiles(const I8Linear& a, hipStream_t stream) {
     const int m_tiles = (a.batch + T::BM - 1) / T::BM, n_tiles = (a.out_feat + T::BN - 1) / T::BN;
@@ -321,6 +496,15 @@ template <class O>
 hipError_t launch_form(const I8Linear& a, int form, hipStream_t stream) {
     switch (form) {
     case 0: return launch_rows<O, 4, 1>(a, stream);
+    case 30: return launch_slices<O, 1, 4>(a, stream);
+    case 31: return launch_slices<O, 1, 2>(a, stream);
+    case 32: return launch_slices<O, 2, 3>(a, stream);
+    case 33: return launch_slices<O, 2, 2>(a, stream);
+    case 34: return launch_slices<O, 4, 2>(a, stream);
+    case 35: return launch_slices<O, 3, 2>(a, stream);
+    case 20: return launch_rows<O, 8, 2>(a, stream);
+    case 21: return launch_rows<O, 8, 4>(a, stream);
+    case 22: return launch_rows<O, 16, 1>(a, stream);
     case 1: return launch_rows<O, 8, 1>(a, stream);
     case 2: return launch_rows<O, 4, 2>(a, stream);
     case 3: return launch_rows<O, 4, 4>(a, stream);
@@ -339,17 +523,21 @@ hipError_t launch_form(const I8Linear& a, int form, hipStream_t stream) {
 
 hipError_t launch_quantize_i8(int type, const void* x, size_t ld_x, int8_t* q, size_t ld_q, float* scale, size_t rows,
                               int n, hipStream_t stream) {
-    const unsigned grid = (unsigned)(rows < 65536 ? rows : 65536);
+    const size_t es = type_bytes(type);
+    const bool whole = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || ld_x * es % 16 == 0);
+    const int tpr = n <= 1024 ? 64 : std::min(kQuantMost, (n + 1023) / 1024 * 64);
+    const int threads = tpr == 64 ? 256 : tpr, per = threads / tpr;
+    const unsigned grid = (unsigned)std::min<size_t>((rows + per - 1) / per, 1 << 20);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((quantize_kernel<T>), dim3(grid), dim3(kQuantThreads), 0, stream, static_cast<const T*>(x),
-                           ld_x, q, ld_q, scale, (int)rows, n);
+        hipLaunchKernelGGL((quantize_kernel<T>), dim3(grid), dim3(threads), 0, stream, static_cast<const T*>(x), ld_x, q,
+                           ld_q, scale, (int)rows, n, tpr, whole);
         return hipGetLastError();
     });
 }
 
 hipError_t launch_linear_i8(const I8Linear& a, int y_type, hipStream_t stream) {
-    const int form = a.batch <= 16 ? 1 : a.batch <= 32 ? 2 : a.batch <= 64 ? 3 : a.batch <= 1024 ? 4 : 6;
+    const int form = a.batch <= 16 ? 0 : a.batch <= 32 ? 30 : a.batch <= 64 ? 32 : a.batch <= 128 ? 34 : a.batch <= 1024 ? 9 : 6;
     // a launch takes a part of the tokens, so that its grid stays in range
     const int64_t most = ((int64_t)1 << 28) / (a.out_feat + 255) * 256;
     const int step = (int)std::max<int64_t>(256, std::min<int64_t>(most, 65535 * 16));
