@@ -100,9 +100,16 @@ def _product(ctx, m, k, n, out, bias, seed, garbage=True, ld_y=None):
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 16, 16), (1, 4096, 4096), (2, 100, 33), (3, 256, 1000), (16, 2048, 5632),
                                    (17, 4096, 256), (19, 11008, 512), (33, 1001, 777), (64, 4096, 4096), (65, 640, 129),
                                    (100, 5000, 2000), (128, 14336, 300), (200, 64, 4100), (255, 4112, 257),
-                                   (512, 4096, 1000), (700, 130, 2049), (1025, 896, 4864)])
+                                   (512, 4096, 1000), (700, 130, 2049), (1025, 896, 4864),
+                                   (190, 4100, 11001), (250, 11000, 4090), (1001, 4112, 11003)])
 def test_product(ctx, m, k, n, out):
     _product(ctx, m, k, n, out, bias=(m + n) % 2 == 0, seed=m * 7 + k * 3 + n)
+
+
+def test_product_over_more_channels_and_tokens_than_a_launch(ctx):
+    _product(ctx, 1, 40, (1 << 20) + 300, "bf16", True, 11)
+    _product(ctx, 70, 33, (1 << 20) + 17, "f32", False, 12)
+    _product(ctx, 1048560 + 100, 16, 19, "f16", True, 13)
 
 
 def test_product_at_the_largest_sums(ctx):

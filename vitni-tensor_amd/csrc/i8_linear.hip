@@ -3,10 +3,13 @@
 //
 //   s_m = max_k |x_mk| / 127,  q_mk = x_mk / s_m rounded,  y_mn = s_m t_n sum_k q_mk w_nk + b_n
 //
-// Integer sums are exact in any order, so how K is split never shows.
+// Integer sums are exact in any order, so how K is split never shows.  Few tokens are
+// bound by the weights' bytes, many by the matrix cores: vtq_i8_rules.h says which form
+// takes a call.
 #include <algorithm>
 
 #include "vtq_device.h"
+#include "vtq_i8_rules.h"
 #include "vtq_kernels.h"
 #include "vtq_lds_load.h"
 #include "vtq_serve.h"
@@ -108,83 +111,71 @@ __global__ __launch_bounds__(kQuantMost) void quantize_kernel(const T* x, size_t
     }
 }
 
-// One output: the sum to f32, its two scales and the bias, each rounded once, then the
-// output's type.
-template <class O>
-__device__ __forceinline__ void store(const I8Linear& a, int m, int n, int sum) {
-    float y = a.in_feat ? (float)sum * a.xs[m] * a.ws[n] : 0.0f;
-    if (a.bias) y += a.bias[n];
-    static_cast<O*>(a.y)[(size_t)m * a.ld_y + n] = (O)y;
-}
+// One output before its type: the sum to f32, its two scales and the bias, each rounded
+// once.  (No inputs: scales that are not there count as 0.)
+__device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) { return (float)sum * xs * ws + bias; }
 
 // ------------------------------------------------ product, few tokens
 
-// A workgroup owns 16 output channels x 16 MT tokens, its waves every W-th 256 bytes
-// of K; lane (r, g) of a wave takes the 64 bytes g of row r, channel and token alike
-// (the order of K inside an MFMA is free as long as both operands share it).  The next
-// 256 bytes load while these multiply.
-template <int MT>
+// A workgroup owns 16 output channels x 16 tokens, its waves every fourth 256 bytes of
+// K; lane (r, g) of a wave takes the 64 bytes g of row r, channel and token alike (the
+// order of K inside an MFMA is free as long as both operands share it).  The next
+// 256 bytes load while these multiply.  Bound by the weights: 1 x 11008 -> 4096 10.3 us,
+// 4.4 TB/s (8 waves 11.6, 16 waves 12.4).
+constexpr int kRowWaves = 4;
 struct RowOperands {
-    v4i w[4], x[MT][4];
+    v4i w[4], x[4];
 };
 
-template <class O, int W, int MT>
-__global__ __launch_bounds__(W * 64) void i8_rows_kernel(I8Linear a) {
-    __shared__ int part[W][16 * MT][17];
+template <class O>
+__global__ __launch_bounds__(kRowWaves * 64) void i8_rows_kernel(I8Linear a) {
+    __shared__ int part[kRowWaves][16][17];
     const int lane = threadIdx.x & 63, wave = wave_id(), r = lane & 15, g = lane >> 4;
-    const int n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16 * MT;
+    const int n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16;
     const int k_end = (a.in_feat + 15) & ~15;
-    const int n_rows = min(16, a.out_feat - n0), m_rows = min(16 * MT, a.batch - m0);
+    const int n_rows = min(16, a.out_feat - n0), m_rows = min(16, a.batch - m0);
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<int8_t*>(a.w + (size_t)n0 * a.ld_w), (short)0, (int)((n_rows - 1) * a.ld_w + k_end), kWord3);
     const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<int8_t*>(a.x + (size_t)m0 * a.ld_x), (short)0, (int)((m_rows - 1) * a.ld_x + k_end), kWord3);
-    v4i acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; t++) acc[t] = v4i{0, 0, 0, 0};
-    auto load = [&](RowOperands<MT>& o, int k) {
+    v4i acc = {0, 0, 0, 0};
+    auto load = [&](RowOperands& o, int k) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int at = k + g * 64 + i * 16;
             // rows past the last one and bytes past the row give zeros
             const int ow = at < k_end && r < n_rows ? (int)(r * a.ld_w) + at : -16;
+            const int ox = at < k_end && r < m_rows ? (int)(r * a.ld_x) + at : -16;
             o.w[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, ow, 0, 0));
-#pragma unroll
-            for (int t = 0; t < MT; t++) {
-                const int ox = at < k_end && 16 * t + r < m_rows ? (int)((16 * t + r) * a.ld_x) + at : -16;
-                o.x[t][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, ox, 0, 0));
-            }
+            o.x[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, ox, 0, 0));
         }
     };
-    auto multiply = [&](const RowOperands<MT>& o) {
+    auto multiply = [&](const RowOperands& o) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int t = 0; t < MT; t++)
-                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.x[t][i], o.w[i], acc[t], 0, 0, 0);
+        for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.x[i], o.w[i], acc, 0, 0, 0);
     };
-    RowOperands<MT> u, v;
+    RowOperands u, v;
     int k = wave * 256;
     load(u, k);
-    for (; k < k_end; k += 2 * W * 256) {
-        load(v, k + W * 256);
+    for (; k < k_end; k += 2 * kRowWaves * 256) {
+        load(v, k + kRowWaves * 256);
         multiply(u);
-        load(u, k + 2 * W * 256);
+        load(u, k + 2 * kRowWaves * 256);
         multiply(v);
     }
     // acc: channel lane & 15, tokens 4 (lane >> 4) + 0..3
 #pragma unroll
-    for (int t = 0; t < MT; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) part[wave][16 * t + 4 * g + i][r] = acc[t][i];
+    for (int i = 0; i < 4; i++) part[wave][4 * g + i][r] = acc[i];
     __syncthreads();
-    for (int e = threadIdx.x; e < 256 * MT; e += W * 64) {
+    for (int e = threadIdx.x; e < 256; e += kRowWaves * 64) {
         const int m = e >> 4, n = e & 15;
         if (m >= m_rows || n >= n_rows) continue;
         int sum = 0;
 #pragma unroll
-        for (int w = 0; w < W; w++) sum += part[w][m][n];
-        store<O>(a, m0 + m, n0 + n, sum);
+        for (int w = 0; w < kRowWaves; w++) sum += part[w][m][n];
+        static_cast<O*>(a.y)[(size_t)(m0 + m) * a.ld_y + n0 + n] =
+            (O)scaled(sum, a.in_feat ? a.xs[m0 + m] : 0.0f, a.in_feat ? a.ws[n0 + n] : 0.0f,
+                      a.bias ? a.bias[n0 + n] : 0.0f);
     }
 }
 
@@ -209,7 +200,8 @@ struct Tiles {
 __device__ __forceinline__ int chunk_of(int row, int c) { return c ^ ((row ^ ((row >> 3) & 1)) & 7); }
 
 template <class O, class T>
-__global__ __launch_bounds__(T::W * 64, T::PER_CU * T::W / 4) void i8_tiles_kernel(I8Linear a, int m_tiles, int n_tiles) {
+__global__ __launch_bounds__(T::W * 64, T::PER_CU * T::W / 4) void i8_tiles_kernel(I8Linear a, int m_tiles,
+        int n_tiles) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ __attribute__((aligned(16))) float x_scale[T::BM], w_scale[T::BN], w_bias[T::BN];
     const int lane = threadIdx.x & 63, wave = wave_id(), row = lane & 31, h = lane >> 5;
@@ -235,9 +227,11 @@ __global__ __launch_bounds__(T::W * 64, T::PER_CU * T::W / 4) void i8_tiles_kern
     for (int i = 0; i < T::kLoadsB; i++) off_b[i] = at((wave * T::kLoadsB + i) * 8 + lane / 8, a.ld_w);
     auto load = [&](int k, int stage) {
         const __amdgpu_buffer_rsrc_t rx =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp + k), (short)0, k < k_end ? x_bytes - k : 0, kWord3);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp + k), (short)0, k < k_end ? x_bytes - k : 0,
+                                              kWord3);
         const __amdgpu_buffer_rsrc_t rw =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp + k), (short)0, k < k_end ? w_bytes - k : 0, kWord3);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp + k), (short)0, k < k_end ? w_bytes - k : 0,
+                                              kWord3);
         const uint32_t to = lds0 + (uint32_t)stage * T::kStage;
         // chunks past the row's end, in the last step, read as zeros
         const auto cut = [&](uint32_t off, int r) {
@@ -320,7 +314,8 @@ __global__ __launch_bounds__(T::W * 64, T::PER_CU * T::W / 4) void i8_tiles_kern
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     typedef O o4 __attribute__((ext_vector_type(4)));
-    constexpr int kRow = T::TN * 32 * (int)sizeof(O), kPitch = kRow + 16, kPieces = kRow / 16, kEach = 16 / (int)sizeof(O);
+    constexpr int kRow = T::TN * 32 * (int)sizeof(O), kPitch = kRow + 16, kPieces = kRow / 16,
+            kEach = 16 / (int)sizeof(O);
     static_assert(32 * kPitch * T::W <= T::S * T::kStage, "LDS of the epilogue");
     uint8_t* out = lds + wave * 32 * kPitch;
     O* y = static_cast<O*>(a.y) + (size_t)(m0 + wm) * a.ld_y + n0 + wn;
@@ -336,10 +331,10 @@ __global__ __launch_bounds__(T::W * 64, T::PER_CU * T::W / 4) void i8_tiles_kern
                 const float4 ws = *reinterpret_cast<const float4*>(&w_scale[wn + n]);
                 const float4 bias = *reinterpret_cast<const float4*>(&w_bias[wn + n]);
                 o4 v;
-                v[0] = (O)((float)acc[i][j][4 * g] * xs * ws.x + bias.x);
-                v[1] = (O)((float)acc[i][j][4 * g + 1] * xs * ws.y + bias.y);
-                v[2] = (O)((float)acc[i][j][4 * g + 2] * xs * ws.z + bias.z);
-                v[3] = (O)((float)acc[i][j][4 * g + 3] * xs * ws.w + bias.w);
+                v[0] = (O)scaled(acc[i][j][4 * g], xs, ws.x, bias.x);
+                v[1] = (O)scaled(acc[i][j][4 * g + 1], xs, ws.y, bias.y);
+                v[2] = (O)scaled(acc[i][j][4 * g + 2], xs, ws.z, bias.z);
+                v[3] = (O)scaled(acc[i][j][4 * g + 3], xs, ws.w, bias.w);
                 *reinterpret_cast<o4*>(out + row * kPitch + n * (int)sizeof(O)) = v;
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's LDS accesses are in order
@@ -360,14 +355,10 @@ __global__ __launch_bounds__(T::W * 64, T::PER_CU * T::W / 4) void i8_tiles_kern
     }
 }
 
-using Tiles128 = Tiles<2, 2, 2, 2, 2, 2>;
-using Tiles128x256 = Tiles<2, 4, 2, 2, 3, 1>;
+using Tiles128 = Tiles<2, 2, 2, 2, 4, 1>;     // 128 x 128, deep: grids that leave a CU one workgroup
+using Pair128 = Tiles<2, 1, 2, 4, 2, 2>;      // 128 x 128, two workgroups a CU
+using Tiles128x256 = Tiles<2, 2, 2, 4, 3, 1>;
 using Tiles256 = Tiles<4, 2, 2, 4, 2, 1>;
-using TF9 = Tiles<2, 2, 2, 4, 3, 1>;
-using TF10 = Tiles<2, 1, 2, 4, 4, 1>;
-using TF11 = Tiles<2, 1, 2, 4, 2, 2>;
-using TF7 = Tiles<2, 2, 2, 2, 4, 1>;
-using TF12 = Tiles<4, 1, 2, 4, 3, 1>;
 
 // ------------------------------------------------ product, some tens of tokens
 
@@ -389,17 +380,19 @@ __global__ __launch_bounds__(256, 1) void i8_slices_kernel(I8Linear a) {
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)mine;
     auto load = [&](int k, int stage) {
         const __amdgpu_buffer_rsrc_t rx =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp + k), (short)0, k < k_end ? x_bytes - k : 0, kWord3);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp + k), (short)0, k < k_end ? x_bytes - k : 0,
+                                              kWord3);
         const __amdgpu_buffer_rsrc_t rw =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp + k), (short)0, k < k_end ? w_bytes - k : 0, kWord3);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp + k), (short)0, k < k_end ? w_bytes - k : 0,
+                                              kWord3);
         const uint32_t to = lds0 + (uint32_t)stage * kStage;
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
             const bool is_w = i < 4;
             const int r = (is_w ? i : i - 4) * 8 + lane / 8, c = 16 * chunk_of(r, lane & 7);
             // chunks past the row's end, in the last step, read as zeros
-            const uint32_t off =
-                k + 128 > k_end && k + c >= k_end ? 0x7FFFFFF0u : (uint32_t)(r * (is_w ? a.ld_w : a.ld_x)) + (uint32_t)c;
+            const uint32_t at = (uint32_t)(r * (is_w ? a.ld_w : a.ld_x)) + (uint32_t)c;
+            const uint32_t off = k + 128 > k_end && k + c >= k_end ? 0x7FFFFFF0u : at;
             load_to_lds<16>(is_w ? rw : rx, off, to + 1024u * i);
         }
     };
@@ -453,7 +446,8 @@ __global__ __launch_bounds__(256, 1) void i8_slices_kernel(I8Linear a) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const bool in = n + i < n_rows;
-            v[i] = (O)((float)sum[i] * xs * (in && a.in_feat ? a.ws[n0 + n + i] : 0.0f) + (in && a.bias ? a.bias[n0 + n + i] : 0.0f));
+            v[i] = (O)scaled(sum[i], xs, in && a.in_feat ? a.ws[n0 + n + i] : 0.0f,
+                             in && a.bias ? a.bias[n0 + n + i] : 0.0f);
         }
         if (n + 4 <= n_rows && reinterpret_cast<uintptr_t>(y) % sizeof(o4) == 0) {
             *reinterpret_cast<o4*>(y) = v;
@@ -469,7 +463,8 @@ hipError_t launch_slices(const I8Linear& a, hipStream_t stream) {
     constexpr int bytes = 4 * S * (TM + 1) * 4096;
     if (hipError_t e = allow_dynamic_lds(f, bytes)) return e;
     hipLaunchKernelGGL((i8_slices_kernel<O, TM, S>),
-                       dim3((unsigned)((a.out_feat + 31) / 32), (unsigned)((a.batch + 32 * TM - 1) / (32 * TM))), dim3(256),
+                       dim3((unsigned)((a.out_feat + 31) / 32), (unsigned)((a.batch + 32 * TM - 1) / (32 * TM))),
+                               dim3(256),
                        bytes, stream, a);
     return hipGetLastError();
 }
@@ -480,43 +475,32 @@ hipError_t launch_tiles(const I8Linear& a, hipStream_t stream) {
     const void* f = reinterpret_cast<const void*>(&i8_tiles_kernel<O, T>);
     if (hipError_t e = allow_dynamic_lds(f, T::S * T::kStage + 4096)) return e;
     const int per = (m_tiles * n_tiles + 7) / 8;
-    hipLaunchKernelGGL((i8_tiles_kernel<O, T>), dim3((unsigned)per * 8), dim3(T::W * 64), T::S * T::kStage, stream, a, m_tiles,
+    hipLaunchKernelGGL((i8_tiles_kernel<O, T>), dim3((unsigned)per * 8), dim3(T::W * 64), T::S * T::kStage, stream,
+                       a, m_tiles,
                        n_tiles);
     return hipGetLastError();
 }
 
-template <class O, int W, int MT>
+template <class O>
 hipError_t launch_rows(const I8Linear& a, hipStream_t stream) {
-    hipLaunchKernelGGL((i8_rows_kernel<O, W, MT>), dim3((unsigned)((a.out_feat + 15) / 16), (unsigned)((a.batch + 16 * MT - 1) / (16 * MT))),
-                       dim3(W * 64), 0, stream, a);
+    const dim3 grid((unsigned)((a.out_feat + 15) / 16), (unsigned)((a.batch + 15) / 16));
+    hipLaunchKernelGGL((i8_rows_kernel<O>), grid, dim3(kRowWaves * 64), 0, stream, a);
     return hipGetLastError();
 }
 
 template <class O>
-hipError_t launch_form(const I8Linear& a, int form, hipStream_t stream) {
+hipError_t launch_form(const I8Linear& a, I8Form form, hipStream_t stream) {
     switch (form) {
-    case 0: return launch_rows<O, 4, 1>(a, stream);
-    case 30: return launch_slices<O, 1, 4>(a, stream);
-    case 31: return launch_slices<O, 1, 2>(a, stream);
-    case 32: return launch_slices<O, 2, 3>(a, stream);
-    case 33: return launch_slices<O, 2, 2>(a, stream);
-    case 34: return launch_slices<O, 4, 2>(a, stream);
-    case 35: return launch_slices<O, 3, 2>(a, stream);
-    case 20: return launch_rows<O, 8, 2>(a, stream);
-    case 21: return launch_rows<O, 8, 4>(a, stream);
-    case 22: return launch_rows<O, 16, 1>(a, stream);
-    case 1: return launch_rows<O, 8, 1>(a, stream);
-    case 2: return launch_rows<O, 4, 2>(a, stream);
-    case 3: return launch_rows<O, 4, 4>(a, stream);
-    case 4: return launch_tiles<O, Tiles128>(a, stream);
-    case 5: return launch_tiles<O, Tiles128x256>(a, stream);
-    case 6: return launch_tiles<O, Tiles256>(a, stream);
-    case 7: return launch_tiles<O, TF7>(a, stream);
-    case 9: return launch_tiles<O, TF9>(a, stream);
-    case 10: return launch_tiles<O, TF10>(a, stream);
-    case 11: return launch_tiles<O, TF11>(a, stream);
-    default: return launch_tiles<O, TF12>(a, stream);
+    case kI8Rows: return launch_rows<O>(a, stream);
+    case kI8Slices32: return launch_slices<O, 1, 2>(a, stream);
+    case kI8Slices64: return launch_slices<O, 2, 2>(a, stream);
+    case kI8Slices128: return launch_slices<O, 4, 2>(a, stream);
+    case kI8Tiles128: return launch_tiles<O, Tiles128>(a, stream);
+    case kI8Pair128: return launch_tiles<O, Pair128>(a, stream);
+    case kI8Tiles128x256: return launch_tiles<O, Tiles128x256>(a, stream);
+    case kI8Tiles256: return launch_tiles<O, Tiles256>(a, stream);
     }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
@@ -530,25 +514,33 @@ hipError_t launch_quantize_i8(int type, const void* x, size_t ld_x, int8_t* q, s
     const unsigned grid = (unsigned)std::min<size_t>((rows + per - 1) / per, 1 << 20);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((quantize_kernel<T>), dim3(grid), dim3(threads), 0, stream, static_cast<const T*>(x), ld_x, q,
+        hipLaunchKernelGGL((quantize_kernel<T>), dim3(grid), dim3(threads), 0, stream, static_cast<const T*>(x),
+                           ld_x, q,
                            ld_q, scale, (int)rows, n, tpr, whole);
         return hipGetLastError();
     });
 }
 
 hipError_t launch_linear_i8(const I8Linear& a, int y_type, hipStream_t stream) {
-    const int form = a.batch <= 16 ? 0 : a.batch <= 32 ? 30 : a.batch <= 64 ? 32 : a.batch <= 128 ? 34 : a.batch <= 1024 ? 9 : 6;
-    // a launch takes a part of the tokens, so that its grid stays in range
-    const int64_t most = ((int64_t)1 << 28) / (a.out_feat + 255) * 256;
-    const int step = (int)std::max<int64_t>(256, std::min<int64_t>(most, 65535 * 16));
-    for (int m0 = 0; m0 < a.batch; m0 += step) {
+    // a launch takes a part of the channels and tokens, so that its grid stays in range
+    // (at most a thread per output of the smallest tiles, 2^31, and 65535 in y)
+    const int n_step = 1 << 20;
+    for (int n0 = 0; n0 < a.out_feat; n0 += std::min(n_step, a.out_feat - n0)) {
         I8Linear b = a;
-        b.batch = std::min(step, a.batch - m0);
-        b.x = a.x + (size_t)m0 * a.ld_x;
-        b.xs = a.xs + (a.in_feat ? m0 : 0);
-        b.y = static_cast<char*>(a.y) + (size_t)m0 * a.ld_y * type_bytes(y_type);
-        const hipError_t e = with_type(y_type, [&](auto t) { return launch_form<decltype(t)>(b, form, stream); });
-        if (e != hipSuccess) return e;
+        b.out_feat = std::min(n_step, a.out_feat - n0);
+        b.w = a.w + (size_t)n0 * a.ld_w;
+        b.ws = a.in_feat ? a.ws + n0 : a.ws;
+        b.bias = a.bias ? a.bias + n0 : nullptr;
+        const int m_step = (int)std::min<int64_t>(((int64_t)1 << 31) / std::max(b.out_feat, 1024) / 256 * 256, 65535 * 16);
+        for (int m0 = 0; m0 < a.batch; m0 += std::min(m_step, a.batch - m0)) {
+            b.batch = std::min(m_step, a.batch - m0);
+            b.x = a.x + (size_t)m0 * a.ld_x;
+            b.xs = a.in_feat ? a.xs + m0 : a.xs;
+            b.y = static_cast<char*>(a.y) + ((size_t)m0 * a.ld_y + n0) * type_bytes(y_type);
+            const I8Form form = i8_form(b.batch, b.in_feat, b.out_feat);
+            const hipError_t e = with_type(y_type, [&](auto t) { return launch_form<decltype(t)>(b, form, stream); });
+            if (e != hipSuccess) return e;
+        }
     }
     return hipSuccess;
 }

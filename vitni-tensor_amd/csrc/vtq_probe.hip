@@ -10,6 +10,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "vtq_i8_rules.h"
 #include "vtq_rules.h"
 #include "vtq_serve.h"
 
@@ -77,6 +78,12 @@ int vtqp_kquant_form(int type, int batch, int in_feat, int out_feat) {
     if (!vtq::q4k_gemm_faster(batch, in_feat, out_feat)) return 0;
     const int form = vtq::gemm_form(R, out_feat, M, Mt);
     return form == 3 ? 300 + vtq::sk_piece(R, NR * Mt) : form == 2 ? 2 : 1;
+}
+
+// The form that an int8 product takes (I8Form in vtq_i8_rules.h).
+int vtqp_i8_form(int batch, int in_feat, int out_feat) {
+    if (batch <= 0 || in_feat < 0 || out_feat <= 0) return -1;
+    return vtq::i8_form(batch, in_feat, out_feat);
 }
 
 // What the serving operators refuse: the status that a call with these arguments

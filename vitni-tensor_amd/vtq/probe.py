@@ -31,10 +31,20 @@ def lib() -> ctypes.CDLL:
         L.vtqp_check_rope_call.argtypes = [vp, vp, i, vp, sz, sz, vp, sz, sz, vp, sz, sz, sz]
         L.vtqp_check_append.argtypes = [vp, vp, vp, vp, i, sz, vp, sz, sz, vp, sz, sz, sz, vp, sz, sz, vp, sz, sz]
         L.vtqp_check_attention.argtypes = [vp, vp, vp, i, sz, sz, vp, sz, sz, vp, sz, sz, vp, f]
+        L.vtqp_i8_form.argtypes = [i, i, i]
         L.vtqp_slot_of.argtypes = [vp, vp, i, ctypes.c_int64]
         L.vtqp_slot_of.restype = ctypes.c_int64
         _lib = L
     return _lib
+
+
+# forms of the int8 product, in the library's order
+I8_FORMS = ("rows", "slices32", "slices64", "slices128", "tiles128", "pair128", "tiles128x256", "tiles256")
+
+
+def i8_form(batch: int, in_feat: int, out_feat: int) -> str:
+    """The form that vtq_linear_i8_device gives a call."""
+    return I8_FORMS[lib().vtqp_i8_form(batch, in_feat, out_feat)]
 
 
 def refusal(operator: str, *args):
