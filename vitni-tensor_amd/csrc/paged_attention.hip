@@ -72,7 +72,7 @@ struct Tile {
     // in the same bank: K is read 32 rows at one column, V (16 bits) 4 rows x 32
     // bytes, V (f32) two rows x 128 bytes.
     __device__ static int k_chunk(int row, int c) {
-        return kChunks == 8 ? c ^ ((row ^ (row >> 3)) & 7) : c ^ (row & 15);
+        return kChunks == 8 ? c ^ ((row ^ ((row >> 3) & 1)) & 7) : c ^ (row & 15);
     }
     __device__ static int v_chunk(int row, int c) {
         if (sizeof(C) == 4) return c ^ (((row >> 2) & 1) << 3);
@@ -96,14 +96,17 @@ __device__ __forceinline__ void hold_pages(Pages& p, int key) {
     p.held = p.list[min(p.first + lane, last)];
 }
 
-// Loads of a wave: 1 KiB of consecutive keys of K or V to LDS.
+// Loads of a wave, 8 keys of K or V at a time: 8 keys lie in one page, so their address
+// is worked out once, in scalar registers, and the lanes' offsets from it stay the same.
 template <class C, int D>
 struct Loader {
     using T = Tile<C, D>;
-    const char *k, *v;         // of this KV head
+    static constexpr int kLoads8 = 8 / T::kLoadRows;  // loads of 8 keys
+    const char *k, *v;                                 // of this KV head
     int64_t page_bytes;
-    uint32_t slot_bytes;
+    uint32_t slot_bytes, row_bytes;
     int n_pages, page_mask;
+    uint32_t k_off[2][kLoads8], v_off[kLoads8];  // the permutations repeat after 16 (K) and 8 (V) rows
 
     __device__ __forceinline__ void init(const vtq_kv_cache& c, int head) {
         const int64_t at = (int64_t)head * (int64_t)c.head_stride * (int64_t)sizeof(C);
@@ -111,30 +114,57 @@ struct Loader {
         v = static_cast<const char*>(c.v) + at;
         page_bytes = (int64_t)c.page_stride * (int64_t)sizeof(C);
         slot_bytes = (uint32_t)(c.slot_stride * sizeof(C));
+        row_bytes = (uint32_t)c.head_dim * (uint32_t)sizeof(C);
         n_pages = (int)c.n_pages;
         page_mask = c.page_size - 1;
+        const int lane = threadIdx.x & 63, chunk = lane % T::kChunks;
+#pragma unroll
+        for (int i = 0; i < kLoads8; i++) {
+            const int row = i * T::kLoadRows + lane / T::kChunks;
+            // chunks past head_dim read past the end: zeros
+            auto at_chunk = [&](int c) {
+                return (uint32_t)c * 16 < row_bytes ? (uint32_t)row * slot_bytes + (uint32_t)c * 16 : 0x7FFFFFF0u;
+            };
+            k_off[0][i] = at_chunk(T::k_chunk(row, chunk));
+            k_off[1][i] = at_chunk(T::k_chunk(8 + row, chunk));
+            v_off[i] = at_chunk(T::v_chunk(row, chunk));
+        }
     }
-    // byte offset of this lane's 16 bytes in load l of a tile, from the load's first row
-    template <bool V>
-    __device__ __forceinline__ uint32_t offset(int l, int head_dim) const {
-        const int lane = threadIdx.x & 63;
-        const int r = lane / T::kChunks, row = l * T::kLoadRows + r;
-        const int c = V ? T::v_chunk(row, lane % T::kChunks) : T::k_chunk(row, lane % T::kChunks);
-        // chunks past head_dim read past the end: zeros
-        return c * 16 < head_dim * (int)sizeof(C) ? (uint32_t)r * slot_bytes + (uint32_t)c * 16 : 0x7FFFFFF0u;
-    }
-    // Load l of the tile that starts at `key` into lds (the tile's first byte).
-    template <bool V>
-    __device__ __forceinline__ void load(const Pages& p, int key, int l, uint32_t lds, int head_dim) const {
-        const int row = key + l * T::kLoadRows;
-        const int rows = min(T::kLoadRows, p.keys - row);
+    // Where 8 keys from `row` on are, and how many bytes of them exist.
+    struct Run {
+        int64_t at;
+        int bytes;
+    };
+    __device__ __forceinline__ Run run(const Pages& p, int row) const {
         const int page = __builtin_amdgcn_readlane(p.held, ((row >> p.shift) - p.first) & 63);
-        const bool ok = rows > 0 && (uint32_t)page < (uint32_t)n_pages;
-        const int64_t at = ok ? (int64_t)page * page_bytes + (int64_t)(row & page_mask) * slot_bytes : 0;
-        const int bytes = ok ? (rows - 1) * (int)slot_bytes + head_dim * (int)sizeof(C) : 0;
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<char*>((V ? v : k) + at), (short)0, bytes, kWord3);
-        load_to_lds<16>(rs, offset<V>(l, head_dim), lds + (uint32_t)l * 1024u);
+        const int rows = min(8, p.keys - row);
+        Run r;
+        r.at = (int64_t)page * page_bytes + (int64_t)(uint32_t)(row & page_mask) * slot_bytes;
+        r.bytes = (rows - 1) * (int)slot_bytes + (int)row_bytes;
+        r.bytes = rows > 0 ? r.bytes : 0;  // nothing is read at an address of no bytes
+        r.bytes = (uint32_t)page < (uint32_t)n_pages ? r.bytes : 0;
+        return r;
+    }
+    // 8 keys into lds, rows 8 ODD .. of a half tile of 16.
+    template <bool V, int ODD>
+    __device__ __forceinline__ void load8(const Run& r, uint32_t lds) const {
+        const __amdgpu_buffer_rsrc_t rs =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>((V ? v : k) + r.at), (short)0, r.bytes, kWord3);
+#pragma unroll
+        for (int i = 0; i < kLoads8; i++) load_to_lds<16>(rs, V ? v_off[i] : k_off[ODD][i], lds + 1024u * i);
+    }
+    // 16 keys of K or V (or both, v_lds bytes after K), lds at the first one's row
+    __device__ __forceinline__ void load16(const Pages& p, int key, uint32_t lds, bool with_k, bool with_v,
+                                           uint32_t v_lds) const {
+        const Run a = run(p, key), b = run(p, key + 8);
+        if (with_k) {
+            load8<false, 0>(a, lds);
+            load8<false, 1>(b, lds + 8 * T::kRow);
+        }
+        if (with_v) {
+            load8<true, 0>(a, lds + v_lds);
+            load8<true, 1>(b, lds + v_lds + 8 * T::kRow);
+        }
     }
 };
 
@@ -278,17 +308,16 @@ struct Compute {
         return o;
     }
 
-    // Keys key .. key + 31 of the tile at k, v.  limit: keys that this lane's row sees;
-    // low: the least of them over the wave's rows; there: keys that exist (later ones
-    // are zeros in LDS).
-    template <class Between>
-    __device__ static void tile(State<D>& st, const Query& q, const uint8_t* k, const uint8_t* v, int key, int limit,
-                                int low, int there, float c, Between between) {
+    // Keys key .. key + 31 of the tile at k, v.  EDGE: some row may not see all of them.
+    // limit: keys that this lane's row sees; low: the least of them over the wave's rows;
+    // there: keys that exist (later ones are zeros in LDS).
+    template <bool EDGE, class Between>
+    __device__ __forceinline__ static void tile(State<D>& st, const Query& q, const uint8_t* k, const uint8_t* v, int key,
+                                                int limit, int low, int there, float c, Between between) {
         const int h = (threadIdx.x & 63) >> 5;
         v16f s = scores(k, q);
         between();  // K is read; V's loads may still be on their way
-        const bool edge = key + 32 > low;  // uniform: some row does not see all of the tile
-        if (edge) {
+        if constexpr (EDGE) {
 #pragma unroll
             for (int r = 0; r < 16; r++)
                 if (key + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[r] = -INFINITY;
@@ -297,10 +326,12 @@ struct Compute {
 #pragma unroll
         for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
         top = fmaxf(top, swap_halves(top));
-        if (__ballot(top > st.m)) {
-            const float m = fmaxf(st.m, top), base = m == -INFINITY ? 0.0f : m * c;
-            const float shrink = __builtin_amdgcn_exp2f(fmaf(st.m, c, -base));
-            st.m = m;
+        // m follows the maximum only once it is 8 powers of two behind: weights up to 256
+        // cost nothing in a float, and rows rarely rescale
+        const bool moves = (top - st.m) * c > 8.0f;  // each row for itself
+        if (__ballot(moves)) {
+            const float shrink = moves ? __builtin_amdgcn_exp2f(fmaf(st.m, c, -(top * c))) : 1.0f;
+            st.m = moves ? top : st.m;
             st.l *= shrink;
 #pragma unroll
             for (int b = 0; b < D / 32; b++) st.o[b] *= shrink;
@@ -314,14 +345,14 @@ struct Compute {
         }
         st.l += sum;
         const Weights w = weights(s);
-        if (!edge || low >= there) {
+        if (!EDGE || low >= there) {
 #pragma unroll
             for (int b = 0; b < D / 32; b++) st.o[b] = add_values<kAll>(v, w, b, st.o[b]);
             return;
         }
-        // Some row sees less than what is there.  A weight of 0 does not silence a value that is not finite: such values count as
-        // zeros here, and the rows that see one get its infinity (or NaN, the sum of
-        // both) on top.
+        // Some row sees less than what is there.  A weight of 0 does not silence a value
+        // that is not finite: such values count as zeros here, and the rows that see one
+        // get its infinity (or NaN, the sum of both) on top.
         v16f sees;
 #pragma unroll
         for (int r = 0; r < 16; r++) sees[r] = key + 8 * (r / 4) + 4 * h + r % 4 < limit ? 1.0f : 0.0f;
@@ -330,10 +361,11 @@ struct Compute {
         for (int b = 0; b < D / 32; b++) {
             st.o[b] = add_values<kFinite>(v, w, b, st.o[b]);
             const v16f up = add_values<kPlusInfinite>(v, seen, b, v16f{});
+#pragma unroll
+            for (int r = 0; r < 16; r++) st.o[b][r] += up[r] > 0.0f ? INFINITY : 0.0f;
             const v16f down = add_values<kMinusInfinite>(v, seen, b, v16f{});
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                st.o[b][r] += (up[r] > 0.0f ? INFINITY : 0.0f) + (down[r] > 0.0f ? -INFINITY : 0.0f);
+            for (int r = 0; r < 16; r++) st.o[b][r] -= down[r] > 0.0f ? INFINITY : 0.0f;
         }
     }
 };
@@ -440,6 +472,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
         // the last row of the tile sees the most
         const int last_row = min(n_rows, r0 + tile_rows) - 1;
         const int end = prefix ? k1 : min(max(unseen + 1 + last_row / G, 0), k1);
+        const int first_limit = prefix ? k1 : min(max(unseen + 1 + r0 / G, 0), k1);  // the first row's, the least
         const int tiles = end > k0 ? (end - k0 + 31) / 32 : 0;  // of 32 keys
         typename X::Query q;
         X::load_query(q, static_cast<const Q*>(a.q.p) + token * a.q.token_stride + head * a.q.head_stride, valid, hd);
@@ -455,20 +488,16 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
             };
             if (shared) {
                 // stages of W / 2 tiles; wave w loads rows 16w .. 16w + 15 of a stage's
-                constexpr int kStageKeys = 16 * W, kHalf = T::kLoads / 2;
+                constexpr int kStageKeys = 16 * W;
                 constexpr uint32_t kStage = W * T::kBytes;  // K then V
                 const int stages = (end - k0 + kStageKeys - 1) / kStageKeys;
                 auto load_stage = [&](int n) {
-                    const int key = k0 + n * kStageKeys + (wave / 2) * 32, l0 = (wave & 1) * kHalf;
-                    const uint32_t at = lds0 + (n & 1) * kStage + (wave / 2) * T::kBytes;
+                    const int key = k0 + n * kStageKeys + 16 * wave;
                     holds(key);
-#pragma unroll
-                    for (int l = 0; l < kHalf; l++) from.template load<false>(pages, key, l0 + l, at, hd);
-#pragma unroll
-                    for (int l = 0; l < kHalf; l++) from.template load<true>(pages, key, l0 + l, at + kStage / 2, hd);
+                    from.load16(pages, key, lds0 + (n & 1) * kStage + 16 * wave * T::kRow, true, true, kStage / 2);
                 };
                 load_stage(0);
-                for (int n = 0; n < stages; n++) {
+                auto stage = [&](int n, auto edge) {
                     wait_vmcnt<0>();
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
@@ -478,11 +507,17 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
 #pragma unroll 1
                     for (int i = 0; i < W / 2; i++) {
                         const int key = k0 + n * kStageKeys + 32 * i;
-                        if (key < high)
-                            X::tile(st, q, kt + i * T::kBytes, kt + kStage / 2 + i * T::kBytes, key, limit, low,
-                                    pages.keys, j.c, [] {});
+                        if (!decltype(edge)::value || key < high)
+                            X::template tile<decltype(edge)::value>(st, q, kt + i * T::kBytes,
+                                                                    kt + kStage / 2 + i * T::kBytes, key, limit, low,
+                                                                    pages.keys, j.c, [] {});
                     }
-                }
+                };
+                // stages that every row of the workgroup sees whole, then the others
+                const int whole = (first_limit - k0) / kStageKeys;
+                int n = 0;
+                for (; n < min(whole, stages); n++) stage(n, std::false_type{});
+                for (; n < stages; n++) stage(n, std::true_type{});
                 // the next row tile's loads overwrite what other waves may still read
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
@@ -493,24 +528,26 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                 auto load_k = [&](int n) {
                     holds(k0 + 32 * n);
 #pragma unroll
-                    for (int l = 0; l < T::kLoads; l++) from.template load<false>(pages, k0 + 32 * n, l, at, hd);
+                    for (int i = 0; i < 2; i++)
+                        from.load16(pages, k0 + 32 * n + 16 * i, at + 16 * i * T::kRow, true, false, 0);
                 };
                 auto load_v = [&](int n) {
                     holds(k0 + 32 * n);
                     if constexpr (2 * T::kLoads > 63) wait_vmcnt<63 - T::kLoads>();  // the counter's range
 #pragma unroll
-                    for (int l = 0; l < T::kLoads; l++)
-                        from.template load<true>(pages, k0 + 32 * n, l, at + T::kBytes, hd);
+                    for (int i = 0; i < 2; i++)
+                        from.load16(pages, k0 + 32 * n + 16 * i, at + 16 * i * T::kRow, false, true, T::kBytes);
                 };
                 if (wave < tiles) {
                     load_k(wave);
                     load_v(wave);
                 }
-                for (int n = wave; n < tiles; n += W) {
+                auto one = [&](int n, auto edge) {
                     const bool more = n + W < tiles;
                     wait_vmcnt<T::kLoads>();
                     asm volatile("" ::: "memory");
-                    X::tile(st, q, kt, kt + T::kBytes, k0 + 32 * n, limit, low, pages.keys, j.c, [&] {
+                    X::template tile<decltype(edge)::value>(st, q, kt, kt + T::kBytes, k0 + 32 * n, limit, low, pages.keys,
+                                                            j.c, [&] {
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         if (more) {
                             load_k(n + W);
@@ -522,7 +559,11 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                     });
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     if (more) load_v(n + W);
-                }
+                };
+                const int whole = (first_limit - k0) / 32;  // tiles that every row sees whole
+                int n = wave;
+                for (; n < min(whole, tiles); n += W) one(n, std::false_type{});
+                for (; n < tiles; n += W) one(n, std::true_type{});
             }
         }
         st.l += swap_halves(st.l);
