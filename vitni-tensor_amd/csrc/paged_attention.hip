@@ -19,6 +19,7 @@
 // product's operand as they are: the order of keys inside an MFMA is free, so V is
 // read in the order that P has.  V's transpose comes from the LDS transposing read.
 // f32 queries multiply in f32 (32x32x2 MFMAs; 16-bit keys and values widen exactly).
+#include <cstdlib>
 #include <type_traits>
 
 #include "vtq_device.h"
@@ -45,7 +46,7 @@ struct Job {
     int prefix_splits, prefix_chunk;  // key ranges, and keys to one (a multiple of 128)
     int own_rows, own_splits;         // row tiles of a sequence (a workgroup may take several), key ranges
     int shared_prefix, shared_own;    // whether the waves share tiles (else they share rows)
-    int prefix_blocks, own_blocks;
+    int prefix_per_xcd, own_per_xcd;  // workgroups
     float c;          // scale * log2(e)
     float* part_o;    // [splits][tokens * heads][head_dim]
     float2* part_ml;  // [splits][tokens * heads]: maximum (log2) and sum
@@ -145,26 +146,13 @@ struct Loader {
         r.bytes = (uint32_t)page < (uint32_t)n_pages ? r.bytes : 0;
         return r;
     }
-    // 8 keys into lds, rows 8 ODD .. of a half tile of 16.
-    template <bool V, int ODD>
-    __device__ __forceinline__ void load8(const Run& r, uint32_t lds) const {
+    // 8 keys of K or V into lds; odd: the second 8 of 16 rows.
+    template <bool V>
+    __device__ __forceinline__ void load8(const Run& r, bool odd, uint32_t lds) const {
         const __amdgpu_buffer_rsrc_t rs =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>((V ? v : k) + r.at), (short)0, r.bytes, kWord3);
 #pragma unroll
-        for (int i = 0; i < kLoads8; i++) load_to_lds<16>(rs, V ? v_off[i] : k_off[ODD][i], lds + 1024u * i);
-    }
-    // 16 keys of K or V (or both, v_lds bytes after K), lds at the first one's row
-    __device__ __forceinline__ void load16(const Pages& p, int key, uint32_t lds, bool with_k, bool with_v,
-                                           uint32_t v_lds) const {
-        const Run a = run(p, key), b = run(p, key + 8);
-        if (with_k) {
-            load8<false, 0>(a, lds);
-            load8<false, 1>(b, lds + 8 * T::kRow);
-        }
-        if (with_v) {
-            load8<true, 0>(a, lds + v_lds);
-            load8<true, 1>(b, lds + v_lds + 8 * T::kRow);
-        }
+        for (int i = 0; i < kLoads8; i++) load_to_lds<16>(rs, V ? v_off[i] : odd ? k_off[1][i] : k_off[0][i], lds + 1024u * i);
     }
 };
 
@@ -415,19 +403,22 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
     const int hd = a.cache.head_dim, G = j.group, kv_heads = a.cache.kv_heads;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
 
-    // which part of the work: prefix and own workgroups evenly mixed
-    const int64_t blocks = j.prefix_blocks + j.own_blocks, b = blockIdx.x;
-    const int p_before = (int)(b * j.prefix_blocks / blocks), p_after = (int)((b + 1) * j.prefix_blocks / blocks);
-    const bool prefix = p_after > p_before;
-    int unit = prefix ? p_before : (int)b - p_before;
+    // Which part of the work.  Workgroups go to the 8 XCDs in turn: the row tiles of the
+    // same keys follow each other on one XCD, where its L2 has the keys; prefix and own
+    // workgroups are evenly mixed on each.
+    const int xcd = (int)(blockIdx.x & 7);
+    const int64_t s = blockIdx.x >> 3;
+    const bool prefix = s < j.prefix_per_xcd;
+    const int64_t mine = prefix ? s : s - j.prefix_per_xcd;
     const int row_tiles = prefix ? j.prefix_rows : j.own_rows;
     const int splits = prefix ? j.prefix_splits : j.own_splits;
     const bool shared = prefix ? j.shared_prefix : j.shared_own;
-    int row_tile = unit % row_tiles;
-    unit /= row_tiles;
+    const int row_tile = (int)(mine % row_tiles);
+    int unit = (int)(mine / row_tiles) * 8 + xcd;  // KV head, then key range, then sequence
     const int kv_head = unit % kv_heads;
     unit /= kv_heads;
     const int split = unit % splits, seq = unit / splits;
+    if (seq >= (prefix ? 1 : a.batch.batch)) return;
 
     // tokens, keys and the key range
     const int64_t all = min((int64_t)max(uniform(a.batch.q_start[a.batch.batch]), 0), a.tokens);
@@ -482,42 +473,49 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
 #pragma unroll
         for (int i = 0; i < D / 32; i++) st.o[i] = v16f{};
         if (tiles > 0) {
+            const int whole = (first_limit - k0) / 32;  // tiles that every row sees whole
+            pages.keys = end;  // past the last row's sight nothing is read
             hold_pages(pages, k0);
             auto holds = [&](int key) {
                 if (((min(key + 31, pages.keys - 1)) >> pages.shift) - pages.first >= 64) hold_pages(pages, key);
             };
             if (shared) {
-                // stages of W / 2 tiles; wave w loads rows 16w .. 16w + 15 of a stage's
-                constexpr int kStageKeys = 16 * W;
-                constexpr uint32_t kStage = W * T::kBytes;  // K then V
-                const int stages = (end - k0 + kStageKeys - 1) / kStageKeys;
-                auto load_stage = [&](int n) {
-                    const int key = k0 + n * kStageKeys + 16 * wave;
+                // stages of a tile (K, then V); a wave loads 32 / W of the keys
+                constexpr int S = Cfg::kLds / (2 * T::kBytes), kMine = 32 / W, kLoads = 2 * kMine / T::kLoadRows;
+                auto load_stage = [&](int n, int at) {
+                    const int key = k0 + 32 * n + kMine * wave;
                     holds(key);
-                    from.load16(pages, key, lds0 + (n & 1) * kStage + 16 * wave * T::kRow, true, true, kStage / 2);
+#pragma unroll
+                    for (int u = 0; u < kMine / 8; u++) {
+                        const auto run = from.run(pages, key + 8 * u);
+                        const uint32_t to = lds0 + (uint32_t)(at * 2 * T::kBytes + (kMine * wave + 8 * u) * T::kRow);
+                        const bool odd = kMine == 8 ? wave & 1 : u & 1;
+                        from.template load8<false>(run, odd, to);
+                        from.template load8<true>(run, odd, to + T::kBytes);
+                    }
                 };
-                load_stage(0);
+#pragma unroll
+                for (int i = 0; i < S - 1; i++) load_stage(i, i);
+                int at = 0;
+                // Every stage loads the one S - 1 on, past the end too (zeros from nowhere), so
+                // that the count of those in flight stays the same.
                 auto stage = [&](int n, auto edge) {
-                    wait_vmcnt<0>();
+                    wait_vmcnt<(S - 2) * kLoads>();
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
-                    if (n + 1 < stages) load_stage(n + 1);
-                    const uint8_t* kt = lds + (n & 1) * kStage;
-#pragma unroll 1
-                    for (int i = 0; i < W / 2; i++) {
-                        const int key = k0 + n * kStageKeys + 32 * i;
-                        if (!decltype(edge)::value || key < high)
-                            X::template tile<decltype(edge)::value>(st, q, kt + i * T::kBytes,
-                                                                    kt + kStage / 2 + i * T::kBytes, key, limit, low,
-                                                                    pages.keys, j.c, [] {});
-                    }
+                    load_stage(n + S - 1, at == 0 ? S - 1 : at - 1);
+                    const uint8_t* kt = lds + at * 2 * T::kBytes;
+                    const int key = k0 + 32 * n;
+                    if (!decltype(edge)::value || key < high)
+                        X::template tile<decltype(edge)::value>(st, q, kt, kt + T::kBytes, key, limit, low, pages.keys, j.c,
+                                                                [] {});
+                    at = at + 1 == S ? 0 : at + 1;
                 };
-                // stages that every row of the workgroup sees whole, then the others
-                const int whole = (first_limit - k0) / kStageKeys;
                 int n = 0;
-                for (; n < min(whole, stages); n++) stage(n, std::false_type{});
-                for (; n < stages; n++) stage(n, std::true_type{});
+                for (; n < min(whole, tiles); n++) stage(n, std::false_type{});
+                for (; n < tiles; n++) stage(n, std::true_type{});
+                wait_vmcnt<0>();
                 // the next row tile's loads overwrite what other waves may still read
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
@@ -528,15 +526,16 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                 auto load_k = [&](int n) {
                     holds(k0 + 32 * n);
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        from.load16(pages, k0 + 32 * n + 16 * i, at + 16 * i * T::kRow, true, false, 0);
+                    for (int u = 0; u < 4; u++)
+                        from.template load8<false>(from.run(pages, k0 + 32 * n + 8 * u), u & 1, at + 8 * u * T::kRow);
                 };
                 auto load_v = [&](int n) {
                     holds(k0 + 32 * n);
                     if constexpr (2 * T::kLoads > 63) wait_vmcnt<63 - T::kLoads>();  // the counter's range
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        from.load16(pages, k0 + 32 * n + 16 * i, at + 16 * i * T::kRow, false, true, T::kBytes);
+                    for (int u = 0; u < 4; u++)
+                        from.template load8<true>(from.run(pages, k0 + 32 * n + 8 * u), u & 1,
+                                                  at + T::kBytes + 8 * u * T::kRow);
                 };
                 if (wave < tiles) {
                     load_k(wave);
@@ -560,7 +559,6 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     if (more) load_v(n + W);
                 };
-                const int whole = (first_limit - k0) / 32;  // tiles that every row sees whole
                 int n = wave;
                 for (; n < min(whole, tiles); n += W) one(n, std::false_type{});
                 for (; n < tiles; n += W) one(n, std::true_type{});
@@ -625,39 +623,68 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
     }
 }
 
-// Joins the parts of a row: one wave a row, lanes over its elements.
-template <class Q>
+// Joins the parts of a row: one wave a row.  L lanes take the elements, 64 / L groups
+// of them every so many parts; a part without weight (no keys) is not used, its sums
+// may never have been written.
+template <class Q, int L>
 __global__ __launch_bounds__(256) void join_kernel(Job j) {
+    constexpr int N = 64 / L, kAhead = 4;
     const Attention& a = j.a;
     const int lane = threadIdx.x & 63, splits = j.prefix_splits + j.own_splits, hd = a.cache.head_dim;
     const int64_t rows = a.tokens * a.heads, row = (int64_t)blockIdx.x * 4 + wave_id();
     const int64_t token = row / a.heads;
     if (row >= rows || token >= a.batch.q_start[a.batch.batch]) return;
-    float m = -INFINITY;
-    for (int s = lane; s < splits; s += 64) m = fmaxf(m, j.part_ml[s * rows + row].x);
+    // part lane and part 64 + lane
+    float2 ml[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        ml[i] = 64 * i + lane < splits ? j.part_ml[(64 * i + lane) * rows + row] : make_float2(-INFINITY, 0.0f);
+    float m = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 64));
     const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
+    float f[2], l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        f[i] = __builtin_amdgcn_exp2f(ml[i].x - base);
+        l += ml[i].y * f[i];
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x, 64);
+    const int d = 4 * (lane % L), group = lane / L;
+    const bool in = d < hd;
+    const float* from = j.part_o + row * hd + (in ? d : 0);
     float4 o = make_float4(0, 0, 0, 0);
-    const bool in = 4 * lane < hd;
-    for (int s = 0; s < splits; s++) {
-        const float2 ml = j.part_ml[s * rows + row];
-        const float f = __builtin_amdgcn_exp2f(ml.x - base);
-        l = fmaf(ml.y, f, l);
-        if (in && ml.y != 0.0f) {
-            const float4 x = *reinterpret_cast<const float4*>(j.part_o + (s * rows + row) * hd + 4 * lane);
-            o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+    for (int s0 = 0; s0 < splits; s0 += N * kAhead) {
+        float4 x[kAhead];
+        float w[kAhead], has[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const int s = s0 + i * N + group, at = min(s, splits - 1);
+            x[i] = *reinterpret_cast<const float4*>(from + at * rows * hd);
+            w[i] = __shfl(s0 < 64 ? f[0] : f[1], s & 63, 64);
+            has[i] = s < splits ? __shfl(s0 < 64 ? ml[0].y : ml[1].y, s & 63, 64) : 0.0f;
         }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const bool use = has[i] != 0.0f;
+            o.x = use ? fmaf(x[i].x, w[i], o.x) : o.x, o.y = use ? fmaf(x[i].y, w[i], o.y) : o.y;
+            o.z = use ? fmaf(x[i].z, w[i], o.z) : o.z, o.w = use ? fmaf(x[i].w, w[i], o.w) : o.w;
+        }
+    }
+#pragma unroll
+    for (int x = L; x < 64; x *= 2) {
+        o.x += __shfl_xor(o.x, x, 64), o.y += __shfl_xor(o.y, x, 64);
+        o.z += __shfl_xor(o.z, x, 64), o.w += __shfl_xor(o.w, x, 64);
     }
     const bool none = m == -INFINITY && l == 0.0f;
     const float inv = none ? 0.0f : 1.0f / l;
     typedef Q v4q __attribute__((ext_vector_type(4)));
-    if (in) {
+    if (in && group == 0) {
         v4q r;
         r[0] = (Q)(o.x * inv), r[1] = (Q)(o.y * inv), r[2] = (Q)(o.z * inv), r[3] = (Q)(o.w * inv);
-        *reinterpret_cast<v4q*>(static_cast<Q*>(a.y) + token * a.y_token_stride + (row % a.heads) * a.y_head_stride +
-                                4 * lane) = r;
+        *reinterpret_cast<v4q*>(static_cast<Q*>(a.y) + token * a.y_token_stride + (row % a.heads) * a.y_head_stride + d) =
+            r;
     }
     if (a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
@@ -682,20 +709,24 @@ void split_work(Job& j) {
     j.shared_own = own_rows > 32;
     j.prefix_rows = j.prefix_splits = 0;
     j.prefix_chunk = 128;
-    if (a.batch.prefix_len) {
-        j.prefix_rows = (int)up(prefix_rows, j.shared_prefix ? 32 * W : 32);
-        const int64_t units = (int64_t)a.cache.kv_heads * j.prefix_rows;
-        int64_t splits = std::min<int64_t>({up(slots, units), up(a.batch.prefix_len, 256), 64});
-        j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), 128) * 128);
-        j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
-    }
     const int64_t most = (int64_t)a.batch.max_pages << j.page_shift;
     const int64_t len = a.batch.max_len ? std::min<int64_t>(a.batch.max_len, most) : most;
     j.own_rows = (int)up(own_rows, j.shared_own ? 32 * W : 32);
-    const int64_t units = (int64_t)a.cache.kv_heads * j.own_rows * a.batch.batch;
-    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({up(slots, units), up(len, 256), 64}));
-    j.prefix_blocks = a.cache.kv_heads * j.prefix_rows * j.prefix_splits;
-    j.own_blocks = (int)(units * j.own_splits);
+    const int64_t own_units = (int64_t)a.cache.kv_heads * j.own_rows * a.batch.batch;
+    if (a.batch.prefix_len) {
+        j.prefix_rows = (int)up(prefix_rows, j.shared_prefix ? 32 * W : 32);
+        const int64_t units = (int64_t)a.cache.kv_heads * j.prefix_rows;
+        // a workgroup a CU beside the own ones, two where those have little to do
+        static const int e1 = getenv("ATT_P") ? atoi(getenv("ATT_P")) : 0, e2 = getenv("ATT_C") ? atoi(getenv("ATT_C")) : 512;
+        const int64_t own_keys = own_units * len, prefix_keys = units * a.batch.prefix_len;
+        const int64_t want = e1 ? e1 : own_keys * 4 < prefix_keys ? slots : slots / 2;
+        const int64_t splits = std::min<int64_t>({up(want, units), up(a.batch.prefix_len, j.shared_prefix ? e2 : 256), 64});
+        j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), 128) * 128);
+        j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
+    }
+    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({up(slots, own_units), up(len, 256), 64}));
+    j.prefix_per_xcd = (int)up((int64_t)a.cache.kv_heads * j.prefix_splits, 8) * j.prefix_rows;
+    j.own_per_xcd = (int)(up((int64_t)a.cache.kv_heads * j.own_splits * a.batch.batch, 8) * j.own_rows);
 }
 
 }  // namespace
@@ -716,11 +747,11 @@ hipError_t launch_attention_of(const Job& j, hipStream_t stream) {
     using Cfg = Config<Q, C, D>;
     const void* f = reinterpret_cast<const void*>(&attention_kernel<Q, C, D>);
     if (hipError_t e = allow_dynamic_lds(f, Cfg::kLds + 2048)) return e;
-    hipLaunchKernelGGL((attention_kernel<Q, C, D>), dim3((unsigned)(j.prefix_blocks + j.own_blocks)),
+    hipLaunchKernelGGL((attention_kernel<Q, C, D>), dim3(8u * (unsigned)(j.prefix_per_xcd + j.own_per_xcd)),
                        dim3(Cfg::kWaves * 64), Cfg::kLds, stream, j);
     if (hipError_t e = hipGetLastError()) return e;
     if (j.prefix_splits + j.own_splits > 1) {
-        hipLaunchKernelGGL((join_kernel<Q>), dim3((unsigned)((j.a.tokens * j.a.heads + 3) / 4)), dim3(256), 0, stream, j);
+        hipLaunchKernelGGL((join_kernel<Q, D / 4>), dim3((unsigned)((j.a.tokens * j.a.heads + 3) / 4)), dim3(256), 0, stream, j);
         return hipGetLastError();
     }
     return hipSuccess;
