@@ -95,6 +95,9 @@ __device__ __forceinline__ void hold_pages(Pages& p, int key) {
     const int lane = threadIdx.x & 63, last = (p.keys - 1) >> p.shift;
     p.first = key >> p.shift;
     p.held = p.list[min(p.first + lane, last)];
+    // waited for here: left to its use, the wait would stand in every tile, and be one for
+    // all loads to LDS in flight as well
+    asm volatile("" : "+v"(p.held));
 }
 
 // Loads of a wave, 8 keys of K or V at a time: 8 keys lie in one page, so their address
@@ -296,15 +299,47 @@ struct Compute {
         return o;
     }
 
-    // Keys key .. key + 31 of the tile at k, v.  EDGE: some row may not see all of them.
-    // limit: keys that this lane's row sees; low: the least of them over the wave's rows;
-    // there: keys that exist (later ones are zeros in LDS).
-    template <bool EDGE, class Between>
-    __device__ __forceinline__ static void tile(State<D>& st, const Query& q, const uint8_t* k, const uint8_t* v, int key,
-                                                int limit, int low, int there, float c, Between between) {
+    // 16-bit operands of a tile, read ahead of their products
+    struct Keys {
+        v8q v[kWide ? 1 : D / 16];
+    };
+    struct Values {
+        v8q v[kWide ? 1 : D / 32][2];
+    };
+    __device__ static void read_keys(Keys& x, const uint8_t* k) {
+        const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+            x.v[i] = *reinterpret_cast<const v8q*>(k + row * T::kRow + T::k_chunk(row, 2 * i + h) * 16);
+    }
+    __device__ static void read_values(Values& x, const uint8_t* v) {
+#pragma unroll
+        for (int b = 0; b < D / 32; b++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const v4c lo = values4(v, b, 2 * i), hi = values4(v, b, 2 * i + 1);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x.v[b][i][e] = lo[e], x.v[b][i][4 + e] = hi[e];
+            }
+    }
+    __device__ static v16f scores(const Keys& x, const Query& q) {
+        v16f s = {};
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) s = mma(x.v[i], q.v[i], s);
+        return s;
+    }
+    __device__ static void add_values(State<D>& st, const Values& x, const Weights& w) {
+#pragma unroll
+        for (int b = 0; b < D / 32; b++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) st.o[b] = mma(x.v[b][i], w.v[i], st.o[b]);
+    }
+
+    // Scores to weights, with the row's maximum and sum.  EDGE: some row may not see all of
+    // the 32 keys from `key` on; limit: keys that this lane's row sees.
+    template <bool EDGE>
+    __device__ __forceinline__ static Weights softmax(State<D>& st, v16f s, int key, int limit, float c) {
         const int h = (threadIdx.x & 63) >> 5;
-        v16f s = scores(k, q);
-        between();  // K is read; V's loads may still be on their way
         if constexpr (EDGE) {
 #pragma unroll
             for (int r = 0; r < 16; r++)
@@ -332,8 +367,15 @@ struct Compute {
             sum += s[r];
         }
         st.l += sum;
-        const Weights w = weights(s);
-        if (!EDGE || low >= there) {
+        return weights(s);
+    }
+
+    // The values of a tile that some row does not see whole.  low: the keys that the wave's
+    // rows see at least; there: keys that exist (later ones are zeros in LDS).
+    __device__ __forceinline__ static void add_edge(State<D>& st, const Weights& w, const uint8_t* v, int key, int limit,
+                                                    int low, int there) {
+        const int h = (threadIdx.x & 63) >> 5;
+        if (low >= there) {
 #pragma unroll
             for (int b = 0; b < D / 32; b++) st.o[b] = add_values<kAll>(v, w, b, st.o[b]);
             return;
@@ -354,6 +396,21 @@ struct Compute {
             const v16f down = add_values<kMinusInfinite>(v, seen, b, v16f{});
 #pragma unroll
             for (int r = 0; r < 16; r++) st.o[b][r] -= down[r] > 0.0f ? INFINITY : 0.0f;
+        }
+    }
+
+    // A tile from its keys to its values.
+    template <bool EDGE, class Between>
+    __device__ __forceinline__ static void tile(State<D>& st, const Query& q, const uint8_t* k, const uint8_t* v, int key,
+                                                int limit, int low, int there, float c, Between between) {
+        const v16f s = scores(k, q);
+        between();  // K is read; V's loads may still be on their way
+        const Weights w = softmax<EDGE>(st, s, key, limit, c);
+        if constexpr (EDGE) {
+            add_edge(st, w, v, key, limit, low, there);
+        } else {
+#pragma unroll
+            for (int b = 0; b < D / 32; b++) st.o[b] = add_values<kAll>(v, w, b, st.o[b]);
         }
     }
 };
@@ -496,25 +553,51 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                 };
 #pragma unroll
                 for (int i = 0; i < S - 1; i++) load_stage(i, i);
-                int at = 0;
                 // Every stage loads the one S - 1 on, past the end too (zeros from nowhere), so
                 // that the count of those in flight stays the same.
-                auto stage = [&](int n, auto edge) {
-                    wait_vmcnt<(S - 2) * kLoads>();
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                int at = 0, n = 0;
+                auto meet = [&] {
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
                     load_stage(n + S - 1, at == 0 ? S - 1 : at - 1);
+                };
+                if constexpr (!X::kWide) {
+                    if (whole > 0) {
+                        // The next tile's keys are read to registers under this one's softmax,
+                        // its own values under its scores.
+                        typename X::Keys keys;
+                        wait_vmcnt<(S - 2) * kLoads>();
+                        __builtin_amdgcn_s_barrier();
+                        asm volatile("" ::: "memory");
+                        X::read_keys(keys, lds);
+                        for (; n < min(whole, tiles); n++) {
+                            const v16f s = X::scores(keys, q);
+                            typename X::Values values;
+                            X::read_values(values, lds + at * 2 * T::kBytes + T::kBytes);
+                            asm volatile("" ::: "memory");
+                            wait_vmcnt<(S - 3) * kLoads>();
+                            meet();
+                            at = at + 1 == S ? 0 : at + 1;
+                            X::read_keys(keys, lds + at * 2 * T::kBytes);
+                            asm volatile("" ::: "memory");
+                            const auto w = X::template softmax<false>(st, s, k0 + 32 * n, limit, j.c);
+                            X::add_values(st, values, w);
+                        }
+                    }
+                }
+                auto stage = [&](auto edge) {
+                    wait_vmcnt<(S - 2) * kLoads>();
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    meet();
                     const uint8_t* kt = lds + at * 2 * T::kBytes;
-                    const int key = k0 + 32 * n;
-                    if (!decltype(edge)::value || key < high)
-                        X::template tile<decltype(edge)::value>(st, q, kt, kt + T::kBytes, key, limit, low, pages.keys, j.c,
-                                                                [] {});
+                    if (!decltype(edge)::value || k0 + 32 * n < high)
+                        X::template tile<decltype(edge)::value>(st, q, kt, kt + T::kBytes, k0 + 32 * n, limit, low,
+                                                                pages.keys, j.c, [] {});
                     at = at + 1 == S ? 0 : at + 1;
                 };
-                int n = 0;
-                for (; n < min(whole, tiles); n++) stage(n, std::false_type{});
-                for (; n < tiles; n++) stage(n, std::true_type{});
+                if constexpr (X::kWide)
+                    for (; n < min(whole, tiles); n++) stage(std::false_type{});
+                for (; n < tiles; n++) stage(std::true_type{});
                 wait_vmcnt<0>();
                 // the next row tile's loads overwrite what other waves may still read
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
