@@ -121,7 +121,7 @@ BAD_CACHES = [(dict(ggml_type=vtq.Q8_0), NIMP), (dict(page_size=4), SHAPE), (dic
               (dict(head_dim=264), SHAPE), (dict(head_dim=0), SHAPE), (dict(kv_heads=0), SHAPE),
               (dict(n_pages=1 << 31), NIMP), (dict(slot_stride=68), SHAPE), (dict(slot_stride=56), SHAPE),
               (dict(head_stride=56), SHAPE), (dict(head_stride=4), SHAPE), (dict(page_stride=100), SHAPE),
-              (dict(slot_stride=1 << 24), NIMP), (dict(n_pages=2 ** 31 - 1, page_stride=1 << 16), NIMP), (dict(k_ptr=None), ARG), (dict(v_ptr=None), ARG),
+              (dict(slot_stride=1 << 24), NIMP), (dict(page_size=4096, slot_stride=1 << 17), NIMP), (dict(n_pages=2 ** 31 - 1, page_stride=1 << 16), NIMP), (dict(k_ptr=None), ARG), (dict(v_ptr=None), ARG),
               (dict(k_ptr=A + 8), ARG), (dict(v_ptr=A + 2), ARG)]
 BAD_BATCHES = [(dict(batch=-1), ARG), (dict(max_pages=-1), ARG), (dict(prefix_len=-1), ARG), (dict(max_q=-1), ARG),
                (dict(max_len=-1), ARG), (dict(batch=(1 << 20) + 1), NIMP), (dict(max_pages=1 << 28), NIMP),

@@ -60,7 +60,18 @@ struct State {
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ float swap_halves(float x) { return __shfl_xor(x, 32, 64); }
+// x of both half-waves: {lanes 0-31's, lanes 32-63's} in every lane
+__device__ __forceinline__ float2 halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// A lane number that the compiler knows nothing of: what is worked out from it stays
+// behind this point, instead of in registers all through the loops before it.
+__device__ __forceinline__ int late_lane() {
+    int x = threadIdx.x & 63;
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 template <class C, int D>
 struct Tile {
@@ -81,24 +92,15 @@ struct Tile {
     }
 };
 
-// Where keys come from: a page list with its length in keys.  The page numbers of up
-// to 64 pages are held a lane each.
+// Where keys come from: a page list with its length in keys.  The byte offsets of up to
+// 64 pages are held a lane each (-1: outside the cache).
 struct Pages {
     const int32_t* list;
     int keys;     // keys that exist: later ones read as zeros
     int shift;
     int first;    // page that lane 0 holds
-    int held;
+    int low, high;
 };
-
-__device__ __forceinline__ void hold_pages(Pages& p, int key) {
-    const int lane = threadIdx.x & 63, last = (p.keys - 1) >> p.shift;
-    p.first = key >> p.shift;
-    p.held = p.list[min(p.first + lane, last)];
-    // waited for here: left to its use, the wait would stand in every tile, and be one for
-    // all loads to LDS in flight as well
-    asm volatile("" : "+v"(p.held));
-}
 
 // Loads of a wave, 8 keys of K or V at a time: 8 keys lie in one page, so their address
 // is worked out once, in scalar registers, and the lanes' offsets from it stay the same.
@@ -134,19 +136,34 @@ struct Loader {
             v_off[i] = at_chunk(T::v_chunk(row, chunk));
         }
     }
+    // Holds the pages from `key`'s on.
+    __device__ __forceinline__ void hold(Pages& p, int key) const {
+        const int lane = threadIdx.x & 63, last = (p.keys - 1) >> p.shift;
+        p.first = key >> p.shift;
+        const int page = p.list[min(p.first + lane, last)];
+        const int64_t at = (uint32_t)page < (uint32_t)n_pages ? (int64_t)page * page_bytes : -1;
+        p.low = (int)(uint32_t)at;
+        p.high = (int)(at >> 32);
+        // waited for here: left to its use, the wait would stand in every tile, and be one for
+        // all loads to LDS in flight as well
+        asm volatile("" : "+v"(p.low), "+v"(p.high));
+    }
     // Where 8 keys from `row` on are, and how many bytes of them exist.
     struct Run {
         int64_t at;
         int bytes;
     };
     __device__ __forceinline__ Run run(const Pages& p, int row) const {
-        const int page = __builtin_amdgcn_readlane(p.held, ((row >> p.shift) - p.first) & 63);
-        const int rows = min(8, p.keys - row);
+        const int lane = ((row >> p.shift) - p.first) & 63;
+        const uint32_t low = (uint32_t)__builtin_amdgcn_readlane(p.low, lane);
+        const int high = __builtin_amdgcn_readlane(p.high, lane);
         Run r;
-        r.at = (int64_t)page * page_bytes + (int64_t)(uint32_t)(row & page_mask) * slot_bytes;
+        r.at = (int64_t)(((uint64_t)(uint32_t)high << 32) | low) +
+               (int64_t)(uint32_t)((uint32_t)(row & page_mask) * slot_bytes);  // a page's slots span less than 2^31
+        const int rows = min(8, p.keys - row);
         r.bytes = (rows - 1) * (int)slot_bytes + (int)row_bytes;
-        r.bytes = rows > 0 ? r.bytes : 0;  // nothing is read at an address of no bytes
-        r.bytes = (uint32_t)page < (uint32_t)n_pages ? r.bytes : 0;
+        r.bytes = rows > 0 ? r.bytes : 0;
+        r.bytes = high >= 0 ? r.bytes : 0;  // nothing is read at an address of no bytes
         return r;
     }
     // 8 keys of K or V into lds; odd: the second 8 of 16 rows.
@@ -348,7 +365,8 @@ struct Compute {
         float top = s[0];
 #pragma unroll
         for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
-        top = fmaxf(top, swap_halves(top));
+        const float2 both = halves(top);
+        top = fmaxf(both.x, both.y);
         // m follows the maximum only once it is 8 powers of two behind: weights up to 256
         // cost nothing in a float, and rows rarely rescale
         const bool moves = (top - st.m) * c > 8.0f;  // each row for itself
@@ -360,13 +378,13 @@ struct Compute {
             for (int b = 0; b < D / 32; b++) st.o[b] *= shrink;
         }
         const float base = st.m == -INFINITY ? 0.0f : st.m * c;
-        float sum = 0.0f;
+        float sum[4] = {st.l, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -base));
-            sum += s[r];
+            sum[r & 3] += s[r];
         }
-        st.l += sum;
+        st.l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         return weights(s);
     }
 
@@ -532,9 +550,9 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
         if (tiles > 0) {
             const int whole = (first_limit - k0) / 32;  // tiles that every row sees whole
             pages.keys = end;  // past the last row's sight nothing is read
-            hold_pages(pages, k0);
+            from.hold(pages, k0);
             auto holds = [&](int key) {
-                if (((min(key + 31, pages.keys - 1)) >> pages.shift) - pages.first >= 64) hold_pages(pages, key);
+                if (((min(key + 31, pages.keys - 1)) >> pages.shift) - pages.first >= 64) from.hold(pages, key);
             };
             if (shared) {
                 // stages of a tile (K, then V); a wave loads 32 / W of the keys
@@ -647,40 +665,43 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                 for (; n < tiles; n += W) one(n, std::true_type{});
             }
         }
-        st.l += swap_halves(st.l);
+        const float2 sums = halves(st.l);
+        st.l = sums.x + sums.y;
         const float m2 = st.m == -INFINITY ? -INFINITY : st.m * j.c;
         const int out_split = prefix ? split : j.prefix_splits + split;
+        const int late = late_lane(), late_h = late >> 5;
         if (shared) {
-            if (valid) {
+            const int row = r0 + wave * 32 + (late & 31);
+            if (row < n_rows) {
 #pragma unroll
                 for (int db = 0; db < D / 32; db++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int d = 32 * db + 8 * i + 4 * h;
+                        const int d = 32 * db + 8 * i + 4 * late_h;
                         const v16f& o = st.o[db];
                         if (d < hd)
-                            put_row<Q>(j, out_split, token, head, d,
+                            put_row<Q>(j, out_split, t0 + row / G, kv_head * G + row % G, d,
                                        make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]), m2, st.l);
                     }
             }
         } else {
             // merge the waves' parts of the same rows, each in its own part of LDS
             float* mine = reinterpret_cast<float*>(lds + wave * 2 * T::kBytes);
-            const int row = lane & 31;
+            const int row = late & 31;
             asm volatile("" ::: "memory");
 #pragma unroll
             for (int db = 0; db < D / 32; db++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int c = (8 * db + 2 * i + h) ^ (row & 15);
+                    const int c = (8 * db + 2 * i + late_h) ^ (row & 15);
                     const v16f& o = st.o[db];
                     *reinterpret_cast<float4*>(mine + row * D + 4 * c) =
                         make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
-            if (h == 0) wave_ml[wave][row] = make_float2(m2, st.l);
+            if (late_h == 0) wave_ml[wave][row] = make_float2(m2, st.l);
             __syncthreads();
             const int rows = min(32, n_rows - r0);
-            for (int e = threadIdx.x; e < rows * (D / 4); e += W * 64) {
+            for (int e = wave * 64 + late; e < rows * (D / 4); e += W * 64) {
                 const int rr = e / (D / 4), c = e % (D / 4);
                 if (4 * c >= hd) continue;
                 float m = -INFINITY;

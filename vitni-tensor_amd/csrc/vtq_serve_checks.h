@@ -52,6 +52,8 @@ inline Refusal check_cache(const vtq_kv_cache* c) {
     VTQ_REFUSE(c->slot_stride >= (size_t)1 << 24 || c->head_stride >= kMostStride / 65536 ||
                    c->page_stride >= kMostStride / 4,
                VTQ_E_NOT_IMPLEMENTED, "vtq: cache stride too large");
+    VTQ_REFUSE((size_t)c->page_size * c->slot_stride >= (size_t)1 << 29, VTQ_E_NOT_IMPLEMENTED,
+               "vtq: the slots of a page span more than 2^29 elements");
     VTQ_REFUSE(c->n_pages * (c->page_stride / 8) > (size_t)1 << 43, VTQ_E_NOT_IMPLEMENTED, "vtq: cache too large");
     VTQ_REFUSE(c->n_pages && (!c->k || !c->v), VTQ_E_INVALID_ARGUMENT, "vtq: null cache");
     VTQ_REFUSE(!aligned(c->k, 16) || !aligned(c->v, 16), VTQ_E_INVALID_ARGUMENT,
