@@ -68,6 +68,15 @@ def test_prefix_lengths_around_the_tiles(ctx, prefix):
     _case(ctx, [20, 13], [20, 40], prefix, 8, 2, 64, 8, "f16", "f16", seed=prefix)
 
 
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("prefix", [128 * n - 3 for n in (2, 3, 5, 9, 16, 17, 25, 33, 50, 63, 64, 65, 80)])
+def test_every_number_of_parts(ctx, prefix, head_dim):
+    # one row tile of 128 keys a part: the join's groups of lanes see every remainder
+    _case(ctx, [1], [5], prefix, 1, 1, head_dim, 16, "bf16", "bf16", seed=prefix)
+    _case(ctx, [1], [prefix], 0, 1, 1, head_dim, 16, "f32", "f32", seed=prefix)
+    _case(ctx, [1], [prefix], prefix + 1, 1, 1, head_dim, 16, "f16", "f16", seed=prefix)
+
+
 @pytest.mark.parametrize("name,cache", [("bf16", "bf16"), ("f32", "f32"), ("f32", "bf16")])
 def test_slots_before_heads_and_strided_queries(ctx, name, cache):
     p, q, y, lse = _case(ctx, [1, 3], [50, 70], 40, 8, 2, 64, 16, name, cache, order="slots")

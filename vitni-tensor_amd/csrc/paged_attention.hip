@@ -19,7 +19,7 @@
 // product's operand as they are: the order of keys inside an MFMA is free, so V is
 // read in the order that P has.  V's transpose comes from the LDS transposing read.
 // f32 queries multiply in f32 (32x32x2 MFMAs; 16-bit keys and values widen exactly).
-#include <cstdlib>
+#include <algorithm>
 #include <type_traits>
 
 #include "vtq_device.h"
@@ -182,6 +182,7 @@ template <class Q, class C, int D>
 struct Compute {
     using T = Tile<C, D>;
     static constexpr bool kWide = std::is_same_v<Q, float>;  // f32 products
+    static constexpr bool kAhead = !kWide && D <= 128;        // operands read a tile ahead, where registers allow
     static constexpr int kStep = sizeof(C) == 4 ? 8 : 16;     // elements of a head that both half-waves read at once
     typedef Q v8q __attribute__((ext_vector_type(8)));
     typedef C v8c __attribute__((ext_vector_type(8)));
@@ -440,7 +441,8 @@ struct Config {
     static constexpr int kTile = Tile<C, D>::kBytes;         // 32 keys of K or V
     static constexpr int kWaves = kTile > 16384 ? 2 : 4;
     static constexpr int kLds = kWaves * 2 * kTile;           // a tile of K and V a wave, or two stages shared
-    static constexpr int kPerCu = kLds <= 80 * 1024 ? 2 : 1;  // workgroups of a CU
+    // workgroups of a CU: f32 queries of 128 elements and more take the registers of two
+    static constexpr int kPerCu = kLds <= 80 * 1024 && !(std::is_same_v<Q, float> && D > 64) ? 2 : 1;
 };
 
 // Finishes a row: y and lse, or a part.  o0..o3 are elements d..d+3 of the row.
@@ -474,7 +476,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float2 wave_ml[W][32];
     const Attention& a = j.a;
-    const int lane = threadIdx.x & 63, wave = wave_id(), h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = wave_id();
     const int hd = a.cache.head_dim, G = j.group, kv_heads = a.cache.kv_heads;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
 
@@ -579,7 +581,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                     asm volatile("" ::: "memory");
                     load_stage(n + S - 1, at == 0 ? S - 1 : at - 1);
                 };
-                if constexpr (!X::kWide) {
+                if constexpr (X::kAhead) {
                     if (whole > 0) {
                         // The next tile's keys are read to registers under this one's softmax,
                         // its own values under its scores.
@@ -613,7 +615,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                                                                 pages.keys, j.c, [] {});
                     at = at + 1 == S ? 0 : at + 1;
                 };
-                if constexpr (X::kWide)
+                if constexpr (!X::kAhead)
                     for (; n < min(whole, tiles); n++) stage(std::false_type{});
                 for (; n < tiles; n++) stage(std::true_type{});
                 wait_vmcnt<0>();
@@ -767,7 +769,8 @@ __global__ __launch_bounds__(256) void join_kernel(Job j) {
             const int s = s0 + i * N + group, at = min(s, splits - 1);
             x[i] = *reinterpret_cast<const float4*>(from + at * rows * hd);
             w[i] = __shfl(s0 < 64 ? f[0] : f[1], s & 63, 64);
-            has[i] = s < splits ? __shfl(s0 < 64 ? ml[0].y : ml[1].y, s & 63, 64) : 0.0f;
+            const float sum = __shfl(s0 < 64 ? ml[0].y : ml[1].y, s & 63, 64);  // by every lane
+            has[i] = s < splits ? sum : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
@@ -800,7 +803,7 @@ int waves_of(int cache_type, int head_dim) {
     return 32 * d * (int)type_bytes(cache_type) > 16384 ? 2 : 4;
 }
 
-void split_work(Job& j) {
+void split_work(Job& j, int type) {
     const Attention& a = j.a;
     const int W = waves_of(a.cache.type, a.cache.head_dim);
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
@@ -820,28 +823,37 @@ void split_work(Job& j) {
     if (a.batch.prefix_len) {
         j.prefix_rows = (int)up(prefix_rows, j.shared_prefix ? 32 * W : 32);
         const int64_t units = (int64_t)a.cache.kv_heads * j.prefix_rows;
-        // a workgroup a CU beside the own ones, two where those have little to do
-        static const int e1 = getenv("ATT_P") ? atoi(getenv("ATT_P")) : 0, e2 = getenv("ATT_C") ? atoi(getenv("ATT_C")) : 512;
+        // A workgroup a CU beside the own ones, two where those have little to do; keys enough
+        // that the parts' way through memory stays small beside them, but where a tile takes
+        // long (64 sequences, us: 8192 bf16 keys of 128 elements, own 512, least 512 / 768 /
+        // 2048 keys: 46.9 / 44.0 / 60.6; 2048 f32 keys, least 256 / 768: 92 / 122; 4096 keys of
+        // 256 elements, 16 sequences, least 128 / 512: 38.5 / 67).
         const int64_t own_keys = own_units * len, prefix_keys = units * a.batch.prefix_len;
-        const int64_t want = e1 ? e1 : own_keys * 4 < prefix_keys ? slots : slots / 2;
-        const int64_t splits = std::min<int64_t>({up(want, units), up(a.batch.prefix_len, j.shared_prefix ? e2 : 256), 64});
+        const bool alone = own_keys * 4 < prefix_keys;
+        const int64_t least = !j.shared_prefix               ? 128
+                              : type == VTQ_TYPE_F32         ? 256
+                              : a.cache.head_dim > 128       ? 128
+                              : alone                        ? 512
+                                                             : 768;
+        const int64_t splits =
+            std::min<int64_t>({up(alone ? slots : slots / 2, units), up(a.batch.prefix_len, least), 64});
         j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), 128) * 128);
         j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
     }
-    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({up(slots, own_units), up(len, 256), 64}));
+    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({up(slots, own_units), up(len, 128), 64}));
     j.prefix_per_xcd = (int)up((int64_t)a.cache.kv_heads * j.prefix_splits, 8) * j.prefix_rows;
     j.own_per_xcd = (int)(up((int64_t)a.cache.kv_heads * j.own_splits * a.batch.batch, 8) * j.own_rows);
 }
 
 }  // namespace
 
-size_t attention_workspace(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int, int64_t tokens, int heads) {
+size_t attention_workspace(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens, int heads) {
     Job j{};
     j.a.cache = cache;
     j.a.batch = batch;
     j.a.tokens = tokens;
     j.a.heads = heads;
-    split_work(j);
+    split_work(j, type);
     const size_t splits = j.prefix_splits + j.own_splits;
     return splits > 1 ? splits * tokens * heads * (cache.head_dim * sizeof(float) + sizeof(float2)) + 256 : 0;
 }
@@ -864,7 +876,7 @@ hipError_t launch_attention_of(const Job& j, hipStream_t stream) {
 hipError_t launch_attention(const Attention& a, int type, hipStream_t stream) {
     Job j{};
     j.a = a;
-    split_work(j);
+    split_work(j, type);
     j.c = a.scale * kLog2E;
     const size_t rows = (size_t)(j.prefix_splits + j.own_splits) * a.tokens * a.heads;
     j.part_o = static_cast<float*>(a.ws);
