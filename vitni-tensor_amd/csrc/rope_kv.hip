@@ -11,6 +11,7 @@
 // The work is a copy: every element is read and written once.  A workgroup
 // takes some heads of one token and computes that token's cosines and sines
 // once, in LDS.
+#include <algorithm>
 #include <type_traits>
 
 #include "vtq_device.h"
@@ -44,7 +45,7 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t t) {
 }
 
 template <class T, int N>
-struct alignas(sizeof(T) * N) Pack {
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
     T v[N];
 };
 
@@ -177,7 +178,7 @@ hipError_t launch_rope(const RopeJob& j, int type, int cache_type, hipStream_t s
     // N elements to an access: the most that the alignment of every row and the
     // places where the rotation starts and ends allow
     auto fits = [&](int n) {
-        const size_t bytes = es * n;
+        const size_t bytes = std::min<size_t>(es * n, 16);
         if (j.head_dim % n || rot % n || (half && rot / 2 % n)) return false;
         if (j.x_heads && (!rows_aligned(j.x.p, j.x.token_stride, j.x.head_stride, bytes, es) ||
                           !rows_aligned(j.y, j.y_token_stride, j.y_head_stride, bytes, es)))
@@ -185,9 +186,14 @@ hipError_t launch_rope(const RopeJob& j, int type, int cache_type, hipStream_t s
         return !j.kv_heads || (rows_aligned(j.k.p, j.k.token_stride, j.k.head_stride, bytes, es) &&
                                rows_aligned(j.v.p, j.v.token_stride, j.v.head_stride, bytes, es));
     };
-    const int wide = (int)(16 / es), n = fits(wide) ? wide : 1;
+    // (f32 by 8, two 16-byte accesses, or by 4)
+    const int n = fits(8) ? 8 : es == 4 && fits(4) ? 4 : 1;
     const int all = j.x_heads + 2 * j.kv_heads;
-    const int per = all;
+    // a workgroup a token, more where that leaves the chip idle
+    const int64_t units = (int64_t)all * (j.head_dim / n);
+    const int64_t most = (units + kRopeThreads - 1) / kRopeThreads;
+    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>({most, 1024 / j.tokens, (int64_t)all}));
+    const int per = (int)((all + groups - 1) / groups);
     const dim3 grid((unsigned)j.tokens, (unsigned)((all + per - 1) / per));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
@@ -196,9 +202,14 @@ hipError_t launch_rope(const RopeJob& j, int type, int cache_type, hipStream_t s
             if constexpr (!std::is_same_v<T, C> && !std::is_same_v<T, float>) {
                 return hipErrorInvalidValue;
             } else {
-                constexpr int W = 16 / sizeof(T);
-                if (n == W) hipLaunchKernelGGL((rope_kernel<T, C, W>), grid, dim3(kRopeThreads), 0, stream, j, per);
-                else hipLaunchKernelGGL((rope_kernel<T, C, 1>), grid, dim3(kRopeThreads), 0, stream, j, per);
+                if (n == 8) {
+                    hipLaunchKernelGGL((rope_kernel<T, C, 8>), grid, dim3(kRopeThreads), 0, stream, j, per);
+                } else if (n == 4) {
+                    if constexpr (sizeof(T) == 4)
+                        hipLaunchKernelGGL((rope_kernel<T, C, 4>), grid, dim3(kRopeThreads), 0, stream, j, per);
+                } else {
+                    hipLaunchKernelGGL((rope_kernel<T, C, 1>), grid, dim3(kRopeThreads), 0, stream, j, per);
+                }
                 return hipGetLastError();
             }
         });
