@@ -182,7 +182,7 @@ template <class Q, class C, int D>
 struct Compute {
     using T = Tile<C, D>;
     static constexpr bool kWide = std::is_same_v<Q, float>;  // f32 products
-    static constexpr bool kAhead = !kWide && D <= 128;        // operands read a tile ahead, where registers allow
+    static constexpr bool kPairs = !kWide && D <= 128;        // two tiles at a time, where registers allow
     static constexpr int kStep = sizeof(C) == 4 ? 8 : 16;     // elements of a head that both half-waves read at once
     typedef Q v8q __attribute__((ext_vector_type(8)));
     typedef C v8c __attribute__((ext_vector_type(8)));
@@ -340,11 +340,14 @@ struct Compute {
                 for (int e = 0; e < 4; e++) x.v[b][i][e] = lo[e], x.v[b][i][4 + e] = hi[e];
             }
     }
-    __device__ static v16f scores(const Keys& x, const Query& q) {
-        v16f s = {};
+    // two tiles' scores, two chains of products that do not wait for each other
+    __device__ static void scores(v16f (&s)[2], const Keys (&x)[2], const Query& q) {
+        s[0] = s[1] = v16f{};
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) s = mma(x.v[i], q.v[i], s);
-        return s;
+        for (int i = 0; i < D / 16; i++) {
+            s[0] = mma(x[0].v[i], q.v[i], s[0]);
+            s[1] = mma(x[1].v[i], q.v[i], s[1]);
+        }
     }
     __device__ static void add_values(State<D>& st, const Values& x, const Weights& w) {
 #pragma unroll
@@ -353,19 +356,14 @@ struct Compute {
             for (int i = 0; i < 2; i++) st.o[b] = mma(x.v[b][i], w.v[i], st.o[b]);
     }
 
-    // Scores to weights, with the row's maximum and sum.  EDGE: some row may not see all of
-    // the 32 keys from `key` on; limit: keys that this lane's row sees.
-    template <bool EDGE>
-    __device__ __forceinline__ static Weights softmax(State<D>& st, v16f s, int key, int limit, float c) {
-        const int h = (threadIdx.x & 63) >> 5;
-        if constexpr (EDGE) {
+    // Scores of N tiles to weights, with the row's maximum and sum.
+    template <int N>
+    __device__ __forceinline__ static void softmax(State<D>& st, Weights (&w)[N], v16f (&s)[N], float c) {
+        float top = s[0][0];
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (key + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[r] = -INFINITY;
-        }
-        float top = s[0];
+        for (int i = 0; i < N; i++)
 #pragma unroll
-        for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+            for (int r = 0; r < 16; r++) top = fmaxf(top, s[i][r]);
         const float2 both = halves(top);
         top = fmaxf(both.x, both.y);
         // m follows the maximum only once it is 8 powers of two behind: weights up to 256
@@ -381,12 +379,15 @@ struct Compute {
         const float base = st.m == -INFINITY ? 0.0f : st.m * c;
         float sum[4] = {st.l, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -base));
-            sum[r & 3] += s[r];
+        for (int i = 0; i < N; i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], c, -base));
+                sum[r & 3] += s[i][r];
+            }
+            w[i] = weights(s[i]);
         }
         st.l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        return weights(s);
     }
 
     // The values of a tile that some row does not see whole.  low: the keys that the wave's
@@ -418,18 +419,26 @@ struct Compute {
         }
     }
 
-    // A tile from its keys to its values.
+    // A tile from its keys to its values.  EDGE: some row may not see all of the 32 keys from
+    // `key` on; limit: keys that this lane's row sees.
     template <bool EDGE, class Between>
     __device__ __forceinline__ static void tile(State<D>& st, const Query& q, const uint8_t* k, const uint8_t* v, int key,
                                                 int limit, int low, int there, float c, Between between) {
-        const v16f s = scores(k, q);
+        v16f s[1] = {scores(k, q)};
         between();  // K is read; V's loads may still be on their way
-        const Weights w = softmax<EDGE>(st, s, key, limit, c);
         if constexpr (EDGE) {
-            add_edge(st, w, v, key, limit, low, there);
+            const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (key + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[0][r] = -INFINITY;
+        }
+        Weights w[1];
+        softmax<1>(st, w, s, c);
+        if constexpr (EDGE) {
+            add_edge(st, w[0], v, key, limit, low, there);
         } else {
 #pragma unroll
-            for (int b = 0; b < D / 32; b++) st.o[b] = add_values<kAll>(v, w, b, st.o[b]);
+            for (int b = 0; b < D / 32; b++) st.o[b] = add_values<kAll>(v, w[0], b, st.o[b]);
         }
     }
 };
@@ -571,51 +580,57 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                         from.template load8<true>(run, odd, to + T::kBytes);
                     }
                 };
-#pragma unroll
-                for (int i = 0; i < S - 1; i++) load_stage(i, i);
-                // Every stage loads the one S - 1 on, past the end too (zeros from nowhere), so
-                // that the count of those in flight stays the same.
                 int at = 0, n = 0;
+                // all waves have read what the loads after this overwrite
                 auto meet = [&] {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
-                    load_stage(n + S - 1, at == 0 ? S - 1 : at - 1);
                 };
-                if constexpr (X::kAhead) {
-                    if (whole > 0) {
-                        // The next tile's keys are read to registers under this one's softmax,
-                        // its own values under its scores.
-                        typename X::Keys keys;
-                        wait_vmcnt<(S - 2) * kLoads>();
-                        __builtin_amdgcn_s_barrier();
-                        asm volatile("" ::: "memory");
-                        X::read_keys(keys, lds);
-                        for (; n < min(whole, tiles); n++) {
-                            const v16f s = X::scores(keys, q);
-                            typename X::Values values;
-                            X::read_values(values, lds + at * 2 * T::kBytes + T::kBytes);
-                            asm volatile("" ::: "memory");
-                            wait_vmcnt<(S - 3) * kLoads>();
-                            meet();
-                            at = at + 1 == S ? 0 : at + 1;
-                            X::read_keys(keys, lds + at * 2 * T::kBytes);
-                            asm volatile("" ::: "memory");
-                            const auto w = X::template softmax<false>(st, s, k0 + 32 * n, limit, j.c);
-                            X::add_values(st, values, w);
-                        }
+                load_stage(0, 0);
+                if constexpr (X::kPairs) {
+                    // Two tiles a step while the next two load: chains of products side by side,
+                    // one maximum, one meeting of the waves.
+                    static_assert(S == 4, "two stages of two tiles");
+                    load_stage(1, 1);
+                    for (; n + 2 <= min(whole, tiles); n += 2, at ^= 2) {
+                        wait_vmcnt<0>();
+                        meet();
+                        load_stage(n + 2, at ^ 2);
+                        load_stage(n + 3, (at ^ 2) + 1);
+                        const uint8_t* kt = lds + at * 2 * T::kBytes;
+                        typename X::Keys keys[2];
+                        X::read_keys(keys[0], kt);
+                        X::read_keys(keys[1], kt + 2 * T::kBytes);
+                        v16f s[2];
+                        X::scores(s, keys, q);
+                        typename X::Values values;
+                        X::read_values(values, kt + T::kBytes);
+                        typename X::Weights w[2];
+                        X::template softmax<2>(st, w, s, j.c);
+                        X::add_values(st, values, w[0]);
+                        X::read_values(values, kt + 3 * T::kBytes);
+                        X::add_values(st, values, w[1]);
                     }
+                    meet();
+                    load_stage(n + 2, at ^ 2);
+                } else {
+#pragma unroll
+                    for (int i = 1; i < S - 1; i++) load_stage(i, i);
                 }
+                // One tile a step.  Every step loads the stage S - 1 on, past the end too (zeros
+                // from nowhere), so that the count of those in flight stays the same.
                 auto stage = [&](auto edge) {
                     wait_vmcnt<(S - 2) * kLoads>();
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     meet();
+                    load_stage(n + S - 1, at == 0 ? S - 1 : at - 1);
                     const uint8_t* kt = lds + at * 2 * T::kBytes;
                     if (!decltype(edge)::value || k0 + 32 * n < high)
                         X::template tile<decltype(edge)::value>(st, q, kt, kt + T::kBytes, k0 + 32 * n, limit, low,
                                                                 pages.keys, j.c, [] {});
                     at = at + 1 == S ? 0 : at + 1;
                 };
-                if constexpr (!X::kAhead)
+                if constexpr (!X::kPairs)
                     for (; n < min(whole, tiles); n++) stage(std::false_type{});
                 for (; n < tiles; n++) stage(std::true_type{});
                 wait_vmcnt<0>();
