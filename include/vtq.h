@@ -305,7 +305,7 @@ int vtq_kv_append_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_b
  * gives zeros and an lse of -infinity; what stands in slots that a row does not
  * see never reaches it.  Keys in pages outside the cache count as zeros.  type is
  * the queries' and y's: the cache's own, or VTQ_TYPE_F32 with any cache.  lse
- * (f32, tokens x heads, or NULL) is in natural logarithms.  scale is positive.
+ * (f32, tokens x heads, or NULL) is in natural logarithms.  0 < scale <= 1e30.
  * d_ws is at least vtq_attention_workspace bytes, 256-byte aligned, for this call
  * alone until its work is done (calls that may overlap need one each); the size
  * depends on the host's numbers only, not on the lengths in device memory. */

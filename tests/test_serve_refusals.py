@@ -181,7 +181,7 @@ def test_append(change, code):
     ({}, OK), (dict(type=vtq.F32, qt=256), OK), (dict(type=vtq.F16), NIMP), (dict(heads=3), SHAPE), (dict(q=None), ARG),
     (dict(y=None), ARG), (dict(q=A + 8), ARG), (dict(y=A + 2), ARG), (dict(qt=260), ARG), (dict(yh=68), ARG),
     (dict(qh=56), SHAPE), (dict(lse=A), OK), (dict(lse=A + 2), ARG), (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG),
-    (dict(scale=float("nan")), ARG), (dict(scale=float("inf")), ARG), (dict(tokens=0, q=None), OK),
+    (dict(scale=float("nan")), ARG), (dict(scale=float("inf")), ARG), (dict(scale=2e30), ARG), (dict(tokens=0, q=None), OK),
     (dict(heads=0, q=None), OK), (dict(heads=65536), NIMP)])
 def test_attention(change, code):
     rc, text = probe.refusal("attention", *_attention_args(**change))

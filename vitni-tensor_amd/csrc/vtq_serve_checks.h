@@ -243,7 +243,7 @@ inline Refusal check_attention(const vtq_kv_cache* cache, const vtq_kv_batch* ba
     VTQ_REFUSE(tokens > kMostTokens || heads > 65535, VTQ_E_NOT_IMPLEMENTED, "vtq: too many tokens or heads");
     VTQ_REFUSE(heads % cache->kv_heads, VTQ_E_INVALID_SHAPE, "vtq: heads must be a multiple of kv_heads");
     VTQ_REFUSE(!attention_fits(cache, batch, tokens, heads), VTQ_E_NOT_IMPLEMENTED, "vtq: more than 2^25 rows of queries");
-    VTQ_REFUSE(!std::isfinite(scale) || scale <= 0.0f, VTQ_E_INVALID_ARGUMENT, "vtq: scale must be positive");
+    VTQ_REFUSE(!(scale > 0.0f && scale <= 1e30f), VTQ_E_INVALID_ARGUMENT, "vtq: scale must be positive, up to 1e30");
     if (tokens == 0 || heads == 0 || batch->batch == 0) return {};
     const size_t hd = cache->head_dim, es = type_bytes(type);
     if (Refusal r = check_rows(d_q, q_token_stride, q_head_stride, hd, heads, type, tokens)) return r;
