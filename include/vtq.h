@@ -185,7 +185,8 @@ int vtq_linear_device_noalloc(vtq_ctx *ctx, int ggml_type, int regime, const flo
  * and calls on different streams share no memory but the caller's.
  * `type` arguments take VTQ_TYPE_F32, VTQ_TYPE_F16 or VTQ_TYPE_BF16.  Leading
  * dimensions and strides count elements; the last dimension is contiguous.
- * Results do not change from run to run: no sums of a changing order.
+ * Results do not change from run to run: no sums of a changing order.  Outputs
+ * overlap neither each other's rows nor, but where a call says so, inputs.
  * Refusals: VTQ_E_INVALID_ARGUMENT (null or unaligned pointer, value out of its
  * range), VTQ_E_INVALID_SHAPE (sizes or strides that do not fit together) and
  * VTQ_E_NOT_IMPLEMENTED (type combinations and sizes beyond the kernels), with
@@ -193,11 +194,11 @@ int vtq_linear_device_noalloc(vtq_ctx *ctx, int ggml_type, int regime, const flo
 
 /* Rows to 8 bits: scale[m] = max_k |x[m][k]| / 127 (f32, rounded once) and
  * q[m][k] = x[m][k] / scale[m] to the nearest whole number (the exact quotient;
- * ties to even; at most 127 in magnitude), 0 where the scale is 0.  A row that holds an infinity or a NaN
- * gets that as its scale and zeros, so its products are NaN.  x has rows ld_x
- * apart, q rows ld_q bytes apart (a multiple of 16, at least n; q itself 16-byte
- * aligned); the bytes from n to ld_q are set to 0.  n <= 131071.  Weights take
- * the same call, one row per output channel. */
+ * ties to even; at most 127 in magnitude), 0 where the scale is 0.  A row that
+ * holds an infinity or a NaN gets that as its scale and zeros, so its products
+ * are NaN.  x has rows ld_x apart, q rows ld_q bytes apart (a multiple of 16, at
+ * least n; q itself 16-byte aligned); the bytes from n to ld_q are set to 0.
+ * n <= 131071.  Weights take the same call, one row per output channel. */
 int vtq_quantize_i8_device(vtq_ctx *ctx, int x_type, const void *d_x, size_t ld_x, int8_t *d_q, size_t ld_q,
                            float *d_scale, size_t rows, size_t n, void *stream);
 
@@ -223,7 +224,7 @@ int vtq_linear_i8_device(vtq_ctx *ctx, const int8_t *d_xq, size_t ld_x, const fl
  *   YARN    a ramp over the pair index between the pairs that make `high` and `low`
  *           turns (32 and 1 where 0 is given), rounded outwards to whole indices, and
  *           magnitude 0.1 ln(factor) + 1.
- * magnitude, where it is not 0, replaces the rule's own.  A plan is plain memory:
+ * magnitude (at most 1e30), where it is not 0, replaces the rule's own.  A plan is plain memory:
  * it may be copied, and holds f_i as fractions of a turn in 64 bits, so that
  * p * f_i modulo a turn is exact for every 32-bit position. */
 #define VTQ_ROPE_INTERLEAVED 0
@@ -259,7 +260,10 @@ int vtq_rope_device(vtq_ctx *ctx, const vtq_rope *rope, int type, const void *d_
  * at p * page_stride + h * head_stride + s * slot_stride, in k and v alike.
  * page_size is a power of two, 8 to 4096; head_dim a multiple of 8 up to 256; the
  * strides are multiples of 8 with slots and heads apart (at least head_dim), and k
- * and v 16-byte aligned. */
+ * and v 16-byte aligned.  So pages x heads x slots, pages x slots x heads and heads
+ * x pages x slots all fit.  Limits: slot_stride below 2^24 and a page's slots
+ * within 2^29 elements, head_stride and page_stride below 2^38, n_pages up to
+ * INT_MAX, the whole within 2^46 elements. */
 typedef struct {
     int type, page_size, kv_heads, head_dim;
     size_t n_pages;
@@ -306,6 +310,11 @@ int vtq_kv_append_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_b
  * see never reaches it.  Keys in pages outside the cache count as zeros.  type is
  * the queries' and y's: the cache's own, or VTQ_TYPE_F32 with any cache.  lse
  * (f32, tokens x heads, or NULL) is in natural logarithms.  0 < scale <= 1e30.
+ * A row whose every score is -infinity counts as one that sees no key; a score
+ * past the range of f32 gives NaN.  y may be q itself (the same pointer and
+ * strides), and must not overlap it otherwise.  A call takes at most 2^23 tokens,
+ * 2^25 rows (tokens x heads) and 2^22 workgroups (to a sequence, KV head and 32
+ * rows of it).
  * d_ws is at least vtq_attention_workspace bytes, 256-byte aligned, for this call
  * alone until its work is done (calls that may overlap need one each); the size
  * depends on the host's numbers only, not on the lengths in device memory. */

@@ -94,7 +94,8 @@ def rotation_bound(y, size, dtype):
 
 class Paged:
     """A ragged batch over a paged cache whose pages are in no order.  layout "heads": pages x kv_heads x slots x
-    head_dim; "slots": pages x slots x kv_heads x head_dim.  Slots that hold no token are NaN."""
+    head_dim; "slots": pages x slots x kv_heads x head_dim; "major": kv_heads x pages x slots x head_dim.  Slots that
+    hold no token are NaN."""
 
     def __init__(self, q_lens, own_lens, prefix, kv_heads, head_dim, page, cache, seed=0, layout="heads", spare_pages=3,
                  extra_pages=0, device="cuda", fill=True):
@@ -110,12 +111,12 @@ class Paged:
         self.q_start = torch.tensor([0] + list(np.cumsum(q_lens)), dtype=torch.int32)
         self.len = torch.tensor(own_lens, dtype=torch.int32)
         self.tokens = int(self.q_start[-1])
-        shape = (self.n_pages, kv_heads, page, head_dim) if layout == "heads" else (self.n_pages, page, kv_heads, head_dim)
+        shape = {"heads": (self.n_pages, kv_heads, page, head_dim), "slots": (self.n_pages, page, kv_heads, head_dim),
+                 "major": (kv_heads, self.n_pages, page, head_dim)}[layout]
+        self.layout = layout
         self.k = torch.full(shape, float("nan"), dtype=TYPES[cache])
         self.v = torch.full(shape, float("nan"), dtype=TYPES[cache])
-        # views in pages x kv_heads x slots x head_dim
-        self.kh = self.k if layout == "heads" else self.k.transpose(1, 2)
-        self.vh = self.v if layout == "heads" else self.v.transpose(1, 2)
+        self.kh, self.vh = self.view(self.k), self.view(self.v)
         if fill:
             lists = [(self.prefix_pages, prefix)] + [(self.pages[b], n) for b, n in enumerate(own_lens)]
             for pages, n in lists:
@@ -124,18 +125,19 @@ class Paged:
                     for j0 in range(0, n, page):
                         m = min(page, n - j0)
                         view[int(pages[j0 // page]), :, :m] = x[j0:j0 + m].transpose(0, 1)
-        self.layout = layout
         if device == "cuda":
             self.to_device()
+
+    def view(self, x):
+        """A cache tensor as pages x kv_heads x slots x head_dim."""
+        return {"heads": x, "slots": x.transpose(1, 2), "major": x.transpose(0, 1)}[self.layout]
 
     def to_device(self):
         self.dk, self.dv = self.k.cuda(), self.v.cuda()
         self.dlists = [t.cuda() for t in (self.q_start, self.len, self.pages, self.prefix_pages)]
-        es, d = 1, self.head_dim
-        if self.layout == "heads":
-            strides = dict(page_stride=self.kv_heads * self.page * d, head_stride=self.page * d, slot_stride=d)
-        else:
-            strides = dict(page_stride=self.kv_heads * self.page * d, head_stride=d, slot_stride=self.kv_heads * d)
+        d = self.head_dim
+        at = self.view(self.dk).stride()
+        strides = dict(page_stride=at[0], head_stride=at[1], slot_stride=at[2])
         self.cache = vtq.KvCache(TAGS[self.cache_name], self.dk.data_ptr(), self.dv.data_ptr(), self.n_pages, self.page,
                                  self.kv_heads, d, **strides)
         self.desc = self.describe()

@@ -92,6 +92,22 @@ def test_slots_before_heads_and_strided_queries(ctx, name, cache):
     assert torch.equal(y2, y)
 
 
+@pytest.mark.parametrize("name,cache", [("bf16", "bf16"), ("f32", "f16")])
+def test_heads_before_pages(ctx, name, cache):
+    # heads 2^24 elements and more apart
+    _case(ctx, [1, 3], [50, 70], 40, 8, 2, 64, 16, name, cache, order="major", spare_pages=1 << 14)
+
+
+@pytest.mark.parametrize("name,cache", [("bf16", "bf16"), ("f32", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("q_lens,prefix", [([1, 2], 0), ([1, 2], 300), ([40, 70], 0), ([40, 70], 300)])
+def test_in_place(ctx, name, cache, q_lens, prefix):
+    p = Paged(q_lens, [n + 30 for n in q_lens], prefix, 2, 128, 16, cache)
+    q = torch.randn(p.tokens, 8, 128, device="cuda").to(TYPES[name])
+    want, _ = _attend(ctx, p, q, 8, 0.1)
+    y, _ = _attend(ctx, p, q, 8, 0.1, y=q)
+    assert y is q and torch.equal(y, want)
+
+
 def test_rows_behind_the_last_sequence_stay(ctx):
     for prefix, n in ((0, 1), (100, 1), (100, 40), (3000, 1)):
         p = Paged([n, n], [50, 60], prefix, 2, 64, 16, "bf16")

@@ -44,9 +44,7 @@ def _case(ctx, q_lens, own_lens, prefix, heads, kv_heads, head_dim, rot, layout,
         assert (out[p.tokens:] == 7.0).all()
     bound_k = rotation_bound(want_k, size_k, TYPES[cache])
     got_k, got_v = p.dk.cpu(), p.dv.cpu()
-    view_k, view_v = (got_k, got_v) if order == "heads" else (got_k.transpose(1, 2), got_v.transpose(1, 2))
-    old_k, old_v = (before_k, before_v) if order == "heads" else (before_k.transpose(1, 2), before_v.transpose(1, 2))
-    old_k, old_v = old_k.cpu(), old_v.cpu()
+    view_k, view_v, old_k, old_v = (p.view(t) for t in (got_k, got_v, before_k.cpu(), before_v.cpu()))
     for t, (b, place) in enumerate(where):
         if place < 0 or place // page >= p.max_pages or not 0 <= int(p.pages[b, place // page]) < p.n_pages:
             continue
@@ -78,6 +76,7 @@ def test_without_queries_without_rotation_and_slots_before_heads(ctx):
     _case(ctx, [3, 1], [20, 9], 4, 0, 2, 64, 64, HALF, 16, "bf16", "bf16", order="slots")
     _case(ctx, [3, 1], [20, 9], 4, 3, 3, 64, 0, HALF, 16, "f32", "f16", order="slots")
     _case(ctx, [2], [2], 0, 0, 1, 40, 10, INTER, 8, "f32", "f32", order="slots")
+    _case(ctx, [3, 1], [20, 9], 4, 4, 3, 64, 64, HALF, 16, "bf16", "bf16", order="major")
 
 
 def test_rows_behind_the_last_sequence_stay(ctx):

@@ -54,7 +54,8 @@ def test_rope_plans():
             vtq.Rope(**args)
     nan, inf = float("nan"), float("inf")
     for args in (dict(layout=2), dict(scaling=4), dict(scaling=-1), dict(theta=1.0), dict(theta=nan), dict(theta=inf),
-                 dict(magnitude=-1.0), dict(magnitude=nan), dict(scaling=vtq.ROPE_SCALE_LINEAR, factor=0.5),
+                 dict(magnitude=-1.0), dict(magnitude=nan),
+                 dict(magnitude=1e39), dict(scaling=vtq.ROPE_SCALE_LINEAR, factor=0.5),
                  dict(scaling=vtq.ROPE_SCALE_LINEAR, factor=nan),
                  dict(scaling=vtq.ROPE_SCALE_YARN, factor=2.0, original_context=0),
                  dict(scaling=vtq.ROPE_SCALE_BANDS, factor=2.0, original_context=4096, low=4.0, high=4.0),
@@ -121,12 +122,15 @@ BAD_CACHES = [(dict(ggml_type=vtq.Q8_0), NIMP), (dict(page_size=4), SHAPE), (dic
               (dict(head_dim=264), SHAPE), (dict(head_dim=0), SHAPE), (dict(kv_heads=0), SHAPE),
               (dict(n_pages=1 << 31), NIMP), (dict(slot_stride=68), SHAPE), (dict(slot_stride=56), SHAPE),
               (dict(head_stride=56), SHAPE), (dict(head_stride=4), SHAPE), (dict(page_stride=100), SHAPE),
-              (dict(slot_stride=1 << 24), NIMP), (dict(page_size=4096, slot_stride=1 << 17), NIMP), (dict(n_pages=2 ** 31 - 1, page_stride=1 << 16), NIMP), (dict(k_ptr=None), ARG), (dict(v_ptr=None), ARG),
+              (dict(slot_stride=1 << 24), NIMP), (dict(page_size=4096, slot_stride=1 << 17), NIMP),
+              (dict(n_pages=2 ** 31 - 1, page_stride=1 << 16), NIMP), (dict(head_stride=1 << 38, page_stride=1024), NIMP),
+              (dict(k_ptr=None), ARG), (dict(v_ptr=None), ARG),
               (dict(k_ptr=A + 8), ARG), (dict(v_ptr=A + 2), ARG)]
 BAD_BATCHES = [(dict(batch=-1), ARG), (dict(max_pages=-1), ARG), (dict(prefix_len=-1), ARG), (dict(max_q=-1), ARG),
                (dict(max_len=-1), ARG), (dict(batch=(1 << 20) + 1), NIMP), (dict(max_pages=1 << 28), NIMP),
                (dict(prefix_len=1 << 30), NIMP), (dict(q_start_ptr=None), ARG), (dict(len_ptr=None), ARG),
-               (dict(pages_ptr=None), ARG)]
+               (dict(pages_ptr=None), ARG), (dict(q_start_ptr=A + 2), ARG), (dict(len_ptr=A + 1), ARG),
+               (dict(pages_ptr=A + 2), ARG)]
 
 
 def _append_args(cache=None, batch=None, **change):
@@ -182,11 +186,19 @@ def test_append(change, code):
     (dict(y=None), ARG), (dict(q=A + 8), ARG), (dict(y=A + 2), ARG), (dict(qt=260), ARG), (dict(yh=68), ARG),
     (dict(qh=56), SHAPE), (dict(lse=A), OK), (dict(lse=A + 2), ARG), (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG),
     (dict(scale=float("nan")), ARG), (dict(scale=float("inf")), ARG), (dict(scale=2e30), ARG), (dict(tokens=0, q=None), OK),
-    (dict(heads=0, q=None), OK), (dict(heads=65536), NIMP)])
+    (dict(heads=0, q=None), OK), (dict(heads=65536), NIMP), (dict(y=A, yt=512), SHAPE),
+    (dict(y=A + 65536, yt=512), OK)])
 def test_attention(change, code):
     rc, text = probe.refusal("attention", *_attention_args(**change))
     assert rc == code and (text != "") == (code != OK)
-    assert probe.refusal("attention", *_attention_args(batch=_batch(prefix_pages=None)))[0] == ARG
+    for address in (None, A + 2):
+        assert probe.refusal("attention", *_attention_args(batch=_batch(prefix_pages=address)))[0] == ARG
+
+
+def test_heads_before_pages_are_taken():
+    cache = _cache(n_pages=1 << 16, page_stride=16 * 64, head_stride=(1 << 16) * 16 * 64)
+    for operator, args in (("append", _append_args), ("attention", _attention_args)):
+        assert probe.refusal(operator, *args(cache=cache)) == (OK, "")
 
 
 def test_null_contexts_are_refused():

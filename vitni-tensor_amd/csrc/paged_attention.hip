@@ -289,7 +289,7 @@ struct Compute {
         Weights w;
         if constexpr (kWide) {
             w.v[0] = p;
-        } else {  // rounded to the values' type: a relative 2^-9 (bf16) or 2^-12 (f16) of each, the sum stays f32
+        } else {  // rounded to the values' type: off by 2^-8 (bf16) or 2^-11 (f16) of each at most, the sum stays f32
 #pragma unroll
             for (int j = 0; j < 8; j++) w.v[0][j] = (Q)p[j], w.v[1][j] = (Q)p[8 + j];
         }

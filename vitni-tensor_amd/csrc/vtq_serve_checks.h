@@ -49,7 +49,7 @@ inline Refusal check_cache(const vtq_kv_cache* c) {
                "vtq: cache strides must be multiples of 8 elements");
     VTQ_REFUSE(c->slot_stride < (size_t)c->head_dim || (c->kv_heads > 1 && c->head_stride < (size_t)c->head_dim),
                VTQ_E_INVALID_SHAPE, "vtq: cache strides below head_dim");
-    VTQ_REFUSE(c->slot_stride >= (size_t)1 << 24 || c->head_stride >= kMostStride / 65536 ||
+    VTQ_REFUSE(c->slot_stride >= (size_t)1 << 24 || c->head_stride >= kMostStride / 4 ||
                    c->page_stride >= kMostStride / 4,
                VTQ_E_NOT_IMPLEMENTED, "vtq: cache stride too large");
     VTQ_REFUSE((size_t)c->page_size * c->slot_stride >= (size_t)1 << 29, VTQ_E_NOT_IMPLEMENTED,
@@ -70,6 +70,9 @@ inline Refusal check_batch(const vtq_kv_batch* b, const vtq_kv_cache* c, bool re
     VTQ_REFUSE(b->batch && (!b->q_start || !b->len || (b->max_pages && !b->pages)), VTQ_E_INVALID_ARGUMENT,
                "vtq: null list in the batch");
     VTQ_REFUSE(reads_prefix && b->prefix_len && !b->prefix_pages, VTQ_E_INVALID_ARGUMENT, "vtq: null prefix_pages");
+    VTQ_REFUSE(!aligned(b->q_start, 4) || !aligned(b->len, 4) || !aligned(b->pages, 4) ||
+                   (reads_prefix && !aligned(b->prefix_pages, 4)),
+               VTQ_E_INVALID_ARGUMENT, "vtq: list in the batch not aligned to its type");
     return {};
 }
 
@@ -102,8 +105,8 @@ inline Refusal plan_rope(const vtq_rope_params* p, vtq_rope* out) {
     VTQ_REFUSE(p->scaling < VTQ_ROPE_SCALE_NONE || p->scaling > VTQ_ROPE_SCALE_YARN, VTQ_E_INVALID_ARGUMENT,
                "vtq: unknown rope scaling");
     VTQ_REFUSE(!std::isfinite(p->theta) || p->theta <= 1.0, VTQ_E_INVALID_ARGUMENT, "vtq: theta must be above 1");
-    VTQ_REFUSE(!std::isfinite(p->magnitude) || p->magnitude < 0.0, VTQ_E_INVALID_ARGUMENT,
-               "vtq: magnitude must not be negative");
+    VTQ_REFUSE(!(p->magnitude >= 0.0 && p->magnitude <= 1e30), VTQ_E_INVALID_ARGUMENT,
+               "vtq: magnitude must be 0 to 1e30");
     const bool ramp = p->scaling == VTQ_ROPE_SCALE_BANDS || p->scaling == VTQ_ROPE_SCALE_YARN;
     VTQ_REFUSE(p->scaling != VTQ_ROPE_SCALE_NONE && (!std::isfinite(p->factor) || p->factor < 1.0),
                VTQ_E_INVALID_ARGUMENT, "vtq: factor must be at least 1");
@@ -251,6 +254,8 @@ inline Refusal check_attention(const vtq_kv_cache* cache, const vtq_kv_batch* ba
     VTQ_REFUSE(!aligned(d_q, 16) || !aligned(d_y, 16) || q_token_stride * es % 16 || q_head_stride * es % 16 ||
                    y_token_stride * es % 16 || y_head_stride * es % 16,
                VTQ_E_INVALID_ARGUMENT, "vtq: attention rows must start at multiples of 16 bytes");
+    VTQ_REFUSE(d_q == d_y && (q_token_stride != y_token_stride || q_head_stride != y_head_stride),
+               VTQ_E_INVALID_SHAPE, "vtq: attention in place keeps its strides");
     VTQ_REFUSE(d_lse && !aligned(d_lse, 4), VTQ_E_INVALID_ARGUMENT, "vtq: lse not aligned to its type");
     return {};
 }
