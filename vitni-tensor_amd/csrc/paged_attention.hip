@@ -20,6 +20,7 @@
 // read in the order that P has.  V's transpose comes from the LDS transposing read.
 // f32 queries multiply in f32 (32x32x2 MFMAs; 16-bit keys and values widen exactly).
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "vtq_device.h"
@@ -856,6 +857,7 @@ void split_work(Job& j, int type) {
         j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
     }
     j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({up(slots, own_units), up(len, 128), 64}));
+    if (const char* e = getenv("OWNS")) j.own_splits = atoi(e);
     j.prefix_per_xcd = (int)up((int64_t)a.cache.kv_heads * j.prefix_splits, 8) * j.prefix_rows;
     j.own_per_xcd = (int)(up((int64_t)a.cache.kv_heads * j.own_splits * a.batch.batch, 8) * j.own_rows);
 }
