@@ -856,7 +856,12 @@ void split_work(Job& j, int type) {
         j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), 128) * 128);
         j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
     }
-    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({up(slots, own_units), up(len, 128), 64}));
+    // As many parts as run at once beside the prefix: one workgroup more than the chip holds
+    // costs a round (8 KV heads of 128, rounded up / down, us: 48 sequences of 600 keys 28.3 /
+    // 21.6, 24 of 5 x 600 behind 8192 42.9 / 36.7, 8 of 4000 behind 8192 36.1 / 33.9; the worst
+    // of 80 shapes 40 of 600 behind 8192, 32.7 / 34.2).
+    const int64_t beside = slots - (int64_t)a.cache.kv_heads * j.prefix_splits * j.prefix_rows;
+    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({beside / own_units, up(len, 128), 64}));
     if (const char* e = getenv("OWNS")) j.own_splits = atoi(e);
     j.prefix_per_xcd = (int)up((int64_t)a.cache.kv_heads * j.prefix_splits, 8) * j.prefix_rows;
     j.own_per_xcd = (int)(up((int64_t)a.cache.kv_heads * j.own_splits * a.batch.batch, 8) * j.own_rows);
