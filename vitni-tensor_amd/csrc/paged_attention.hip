@@ -20,6 +20,7 @@
 // read in the order that P has.  V's transpose comes from the LDS transposing read.
 // f32 queries multiply in f32 (32x32x2 MFMAs; 16-bit keys and values widen exactly).
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <type_traits>
 
@@ -839,20 +840,29 @@ void split_work(Job& j, int type) {
     if (a.batch.prefix_len) {
         j.prefix_rows = (int)up(prefix_rows, j.shared_prefix ? 32 * W : 32);
         const int64_t units = (int64_t)a.cache.kv_heads * j.prefix_rows;
-        // A workgroup a CU beside the own ones, two where those have little to do; keys enough
-        // that the parts' way through memory stays small beside them, but where a tile takes
-        // long (64 sequences, us: 8192 bf16 keys of 128 elements, own 512, least 512 / 768 /
-        // 2048 keys: 46.9 / 44.0 / 60.6; 2048 f32 keys, least 256 / 768: 92 / 122; 4096 keys of
-        // 256 elements, 16 sequences, least 128 / 512: 38.5 / 67).
+        // A workgroup a CU beside the own ones, two where those have little to do, and keys
+        // enough to each: n keys take n / 32 tiles one after the other, and each part costs
+        // its rows' way through memory and the join, so n = sqrt(32 keys part / tile) (us), at
+        // least 256 where f32 tiles take long.  Where the waves share rows a part is near
+        // free: n lets 192 workgroups have all.  Against 512 keys (768 beside own work, 256 or
+        // 128 of f32 and 256 elements; 128 for shared rows), 8 KV heads of 128, us: 12 x 1003
+        // 22.1 / 16.1, 64 x 8192 29.7 / 28, 2 x 60 tokens x 8192 50 / 42, 1 x 8192 23.7 / 15.9,
+        // f32 43.4 / 28.8; over 654 shapes 3 % less in the mean, the worst 16 x 6 x 8192 of 256
+        // elements (109 for 89: 264 workgroups for 256 CUs).
         const int64_t own_keys = own_units * len, prefix_keys = units * a.batch.prefix_len;
         const bool alone = own_keys * 4 < prefix_keys;
-        const int64_t least = !j.shared_prefix               ? 128
-                              : type == VTQ_TYPE_F32         ? 256
-                              : a.cache.head_dim > 128       ? 128
-                              : alone                        ? 512
-                                                             : 768;
+        int64_t least;
+        if (j.shared_prefix) {
+            const int d = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
+            const double tile = type == VTQ_TYPE_F32 ? 3.6 * d / 128 : d > 128 ? 2.4 : 0.18 + 0.0025 * d;
+            const double part = 0.08 + 2.3e-6 * (double)(a.tokens * a.heads * a.cache.head_dim);
+            least = up((int64_t)std::sqrt(32.0 * a.batch.prefix_len * part / tile), 128) * 128;
+            if (type == VTQ_TYPE_F32) least = std::max<int64_t>(least, 256);
+        } else {
+            least = std::min<int64_t>(512, up(prefix_keys, 192 * 128) * 128);
+        }
         const int64_t splits =
-            std::min<int64_t>({up(alone ? slots : slots / 2, units), up(a.batch.prefix_len, least), 64});
+            std::min<int64_t>({up(alone ? slots : slots / 2, units), up(a.batch.prefix_len, std::max<int64_t>(128, least)), 64});
         j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), 128) * 128);
         j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
     }
