@@ -15,7 +15,7 @@ from test_asm_checks import FLAGS, HIPCC, ROOT, _functions, _scratch_sizes
 CSRC = os.path.join(ROOT, "vitni-tensor_amd", "csrc")
 
 
-@pytest.fixture(scope="module", params=["paged_attention.hip", "i8_linear.hip"])
+@pytest.fixture(scope="module", params=["cache_attention.hip", "i8_linear.hip"])
 def asm(request, tmp_path_factory):
     if not (os.path.exists(HIPCC) or shutil.which("hipcc")):
         pytest.skip("hipcc not available")
@@ -49,7 +49,7 @@ def test_loops_of_the_16_bit_attention_wait_only_for_their_own_loads(asm):
     # with products and loads to LDS) of heads of up to 128 elements none may stand beside
     # the kernel's own, which follow a barrier's place.
     name, functions = asm
-    if name != "paged_attention.hip":
+    if name != "cache_attention.hip":
         pytest.skip("attention only")
     checked = 0
     for kernel, body in functions.items():

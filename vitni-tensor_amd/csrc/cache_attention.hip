@@ -1,4 +1,4 @@
-// paged_attention.hip -- attention of a ragged batch over a prefix that all its
+// cache_attention.hip -- attention of a ragged batch over a prefix that all its
 // sequences share and the pages of their own (gfx950).
 //
 //   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - m),  m = max_j scale q.k_j
@@ -180,7 +180,8 @@ struct Loader {
         const __amdgpu_buffer_rsrc_t rs =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>((V ? v : k) + r.at), (short)0, r.bytes, kWord3);
 #pragma unroll
-        for (int i = 0; i < kLoads8; i++) load_to_lds<16>(rs, V ? v_off[i] : odd ? k_off[1][i] : k_off[0][i], lds + 1024u * i);
+        for (int i = 0; i < kLoads8; i++)
+            load_to_lds<16>(rs, V ? v_off[i] : odd ? k_off[1][i] : k_off[0][i], lds + 1024u * i);
     }
 };
 
@@ -863,13 +864,13 @@ void split_work(Job& j, int type) {
             const int d = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
             const double tile = type == VTQ_TYPE_F32 ? 3.6 * d / 128 : d > 128 ? 2.4 : 0.18 + 0.0025 * d;
             const double part = 0.08 + 2.3e-6 * (double)(a.tokens * a.heads * a.cache.head_dim);
-            least = up((int64_t)std::sqrt(32.0 * a.batch.prefix_len * part / tile), 128) * 128;
+            least = (1 + (int64_t)std::sqrt(32.0 * a.batch.prefix_len * part / tile) / 128) * 128;
             if (type == VTQ_TYPE_F32) least = std::max<int64_t>(least, 256);
         } else {
             least = std::min<int64_t>(512, up(prefix_keys, 192 * 128) * 128);
         }
         const int64_t splits =
-            std::min<int64_t>({up(alone ? slots : slots / 2, units), up(a.batch.prefix_len, std::max<int64_t>(128, least)), 64});
+            std::min<int64_t>({up(alone ? slots : slots / 2, units), up(a.batch.prefix_len, least), 64});
         j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), 128) * 128);
         j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
     }
@@ -906,7 +907,8 @@ hipError_t launch_attention_of(const Job& j, hipStream_t stream) {
                        dim3(Cfg::kWaves * 64), Cfg::kLds, stream, j);
     if (hipError_t e = hipGetLastError()) return e;
     if (j.prefix_splits + j.own_splits > 1) {
-        hipLaunchKernelGGL((join_kernel<Q, D / 4>), dim3((unsigned)((j.a.tokens * j.a.heads + 3) / 4)), dim3(256), 0, stream, j);
+        hipLaunchKernelGGL((join_kernel<Q, D / 4>), dim3((unsigned)((j.a.tokens * j.a.heads + 3) / 4)), dim3(256), 0,
+                           stream, j);
         return hipGetLastError();
     }
     return hipSuccess;
