@@ -755,16 +755,29 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
 
 // Joins the parts of a row: one wave a row.  L lanes take the elements, 64 / L groups
 // of them every so many parts; a part without weight (no keys) is not used, its sums
-// may never have been written.  2048 rows of 128 take 6.0 us, 4096 7.5: two launches'
-// and three loads' latency more than traffic.
+// may never have been written.  2048 rows of 128 take 5.4 us, 4096 6.9: a launch
+// and two loads' latency more than traffic (6.0 and 7.5 where the parts' loads wait for
+// their weights).
 template <class Q, int L>
 __global__ __launch_bounds__(256) void join_kernel(Job j) {
     constexpr int N = 64 / L, kAhead = 4;
     const Attention& a = j.a;
     const int lane = threadIdx.x & 63, splits = j.prefix_splits + j.own_splits, hd = a.cache.head_dim;
     const int64_t rows = a.tokens * a.heads, row = (int64_t)blockIdx.x * 4 + wave_id();
+    if (row >= rows) return;
     const int64_t token = row / a.heads;
-    if (row >= rows || token >= a.batch.q_start[a.batch.batch]) return;
+    const bool live = token < a.batch.q_start[a.batch.batch];
+    // the first parts load while their weights are worked out
+    const int d = 4 * (lane % L), group = lane / L;
+    const bool in = d < hd;
+    const float* from = j.part_o + row * hd + (in ? d : 0);
+    float4 x[kAhead];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+            x[i] = *reinterpret_cast<const float4*>(from + min(s0 + i * N + group, splits - 1) * rows * hd);
+    };
+    load(0);
     // part lane and part 64 + lane
     float2 ml[2];
 #pragma unroll
@@ -782,17 +795,13 @@ __global__ __launch_bounds__(256) void join_kernel(Job j) {
     }
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x, 64);
-    const int d = 4 * (lane % L), group = lane / L;
-    const bool in = d < hd;
-    const float* from = j.part_o + row * hd + (in ? d : 0);
     float4 o = make_float4(0, 0, 0, 0);
     for (int s0 = 0; s0 < splits; s0 += N * kAhead) {
-        float4 x[kAhead];
+        if (s0) load(s0);
         float w[kAhead], has[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            const int s = s0 + i * N + group, at = min(s, splits - 1);
-            x[i] = *reinterpret_cast<const float4*>(from + at * rows * hd);
+            const int s = s0 + i * N + group;
             w[i] = __shfl(s0 < 64 ? f[0] : f[1], s & 63, 64);
             const float sum = __shfl(s0 < 64 ? ml[0].y : ml[1].y, s & 63, 64);  // by every lane
             has[i] = s < splits ? sum : 0.0f;
@@ -812,13 +821,13 @@ __global__ __launch_bounds__(256) void join_kernel(Job j) {
     const bool none = m == -INFINITY && l == 0.0f;
     const float inv = none ? 0.0f : 1.0f / l;
     typedef Q v4q __attribute__((ext_vector_type(4)));
-    if (in && group == 0) {
+    if (live && in && group == 0) {
         v4q r;
         r[0] = (Q)(o.x * inv), r[1] = (Q)(o.y * inv), r[2] = (Q)(o.z * inv), r[3] = (Q)(o.w * inv);
         *reinterpret_cast<v4q*>(static_cast<Q*>(a.y) + token * a.y_token_stride + (row % a.heads) * a.y_head_stride + d) =
             r;
     }
-    if (a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (m + __log2f(l)) * kLn2;
+    if (live && a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 // ------------------------------------------------ how the work is split
