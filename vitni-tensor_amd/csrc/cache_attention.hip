@@ -41,6 +41,7 @@ namespace {
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef uint16_t v8us __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -51,8 +52,9 @@ struct Job {
     int group;        // query heads of a KV head
     int page_shift;
     int prefix_rows;  // row tiles of the prefix
-    int prefix_splits, prefix_chunk;  // key ranges, and keys to one (a multiple of 128)
+    int prefix_splits, prefix_chunk;  // key ranges, and keys to one (a multiple of 32; of 128 where waves share rows)
     int own_rows, own_splits;         // row tiles of a sequence (a workgroup may take several), key ranges
+    int own_grain;                    // which are multiples of this: 32, or 128 where waves share rows
     int shared_prefix, shared_own;    // whether the waves share tiles (else they share rows)
     int prefix_per_xcd, own_per_xcd;  // workgroups
     float c;          // scale * log2(e)
@@ -399,6 +401,30 @@ struct Compute {
         st.l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
 
+    // Whether a tile holds no infinity and no NaN: the largest exponent of all.
+    __device__ __forceinline__ static bool all_finite(const uint8_t* v) {
+        const uint8_t* at = v + 16 * late_lane();
+        if constexpr (sizeof(C) == 4) {
+            uint32_t top = 0;
+#pragma unroll 1  // few registers: all sums are live
+            for (int i = 0; i < T::kBytes / 1024; i++) {
+                const v4u x = *reinterpret_cast<const v4u*>(at + 1024 * i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = max(top, x[e] & 0x7FFFFFFFu);
+            }
+            return __ballot(top >= 0x7F800000u) == 0;
+        } else {
+            v8us top = {};
+#pragma unroll 1  // few registers: all sums are live
+            for (int i = 0; i < T::kBytes / 1024; i++)
+                top = __builtin_elementwise_max(top, *reinterpret_cast<const v8us*>(at + 1024 * i) & (uint16_t)0x7FFF);
+            uint16_t most = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) most = max(most, top[e]);
+            return __ballot(most >= (std::is_same_v<C, __bf16> ? 0x7F80 : 0x7C00)) == 0;
+        }
+    }
+
     // The values of a tile that some row does not see whole.  low: the keys that the wave's
     // rows see at least; there: keys that exist (later ones are zeros in LDS).
     __device__ __forceinline__ static void add_edge(State<D>& st, const Weights& w, const uint8_t* v, int key, int limit,
@@ -409,7 +435,7 @@ struct Compute {
             for (int b = 0; b < D / 32; b++) st.o[b] = add_values<kAll>(v, w, b, st.o[b]);
             return;
         }
-        // Some row sees less than what is there.  A weight of 0 does not silence a value
+        // Some row sees less than what is there, and a weight of 0 does not silence a value
         // that is not finite: such values count as zeros here, and the rows that see one
         // get its infinity (or NaN, the sum of both) on top.
         v16f sees;
@@ -436,6 +462,7 @@ struct Compute {
         v16f s[1] = {scores(k, q)};
         between();  // K is read; V's loads may still be on their way
         if constexpr (EDGE) {
+            if (low < there && all_finite(v)) low = there;
             const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
             for (int r = 0; r < 16; r++)
@@ -533,7 +560,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
         const int len = uniform(min(max(a.batch.len[seq], -(1 << 29)), 1 << 30));
         pages.keys = min(max(len, 0), a.batch.max_pages << j.page_shift);
         unseen = len - (int)(t1 - t0);
-        const int chunk = ((pages.keys + splits - 1) / splits + 127) & ~127;
+        const int chunk = ((pages.keys + splits - 1) / splits + j.own_grain - 1) & -j.own_grain;
         k0 = (int)min((int64_t)split * chunk, (int64_t)pages.keys);
         k1 = min(pages.keys, k0 + chunk);
     }
@@ -854,6 +881,15 @@ void split_work(Job& j, int type) {
     const int64_t len = a.batch.max_len ? std::min<int64_t>(a.batch.max_len, most) : most;
     j.own_rows = (int)up(own_rows, j.shared_own ? 32 * W : 32);
     const int64_t own_units = (int64_t)a.cache.kv_heads * j.own_rows * a.batch.batch;
+    const int d = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
+    const bool slow = type == VTQ_TYPE_F32 || d > 128;  // tiles that take long: parts of less than four
+    const int grain = slow ? 32 : 128;
+    j.own_grain = j.shared_own ? grain : 128;
+    auto least_keys = [&](int64_t keys) {
+        const double tile = type == VTQ_TYPE_F32 ? 3.6 * d / 128 : d > 128 ? 2.4 : 0.18 + 0.0025 * d;
+        const double part = 0.08 + 2.3e-6 * (double)(a.tokens * a.heads * a.cache.head_dim);
+        return (1 + (int64_t)std::sqrt(32.0 * keys * part / tile) / grain) * grain;
+    };
     if (a.batch.prefix_len) {
         j.prefix_rows = (int)up(prefix_rows, j.shared_prefix ? 32 * W : 32);
         const int64_t units = (int64_t)a.cache.kv_heads * j.prefix_rows;
@@ -870,17 +906,16 @@ void split_work(Job& j, int type) {
         const bool alone = own_keys * 4 < prefix_keys;
         int64_t least;
         if (j.shared_prefix) {
-            const int d = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
-            const double tile = type == VTQ_TYPE_F32 ? 3.6 * d / 128 : d > 128 ? 2.4 : 0.18 + 0.0025 * d;
-            const double part = 0.08 + 2.3e-6 * (double)(a.tokens * a.heads * a.cache.head_dim);
-            least = (1 + (int64_t)std::sqrt(32.0 * a.batch.prefix_len * part / tile) / 128) * 128;
-            if (type == VTQ_TYPE_F32) least = std::max<int64_t>(least, 256);
+            least = least_keys(a.batch.prefix_len);
+            if (type == VTQ_TYPE_F32 && units * up(a.batch.prefix_len, least) + own_units > slots / 2)
+                least = std::max<int64_t>(least, 256);
         } else {
             least = std::min<int64_t>(512, up(prefix_keys, 192 * 128) * 128);
         }
         const int64_t splits =
             std::min<int64_t>({up(alone ? slots : slots / 2, units), up(a.batch.prefix_len, least), 64});
-        j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), 128) * 128);
+        const int64_t by = j.shared_prefix ? grain : 128;
+        j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), by) * by);
         j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
     }
     // As many parts as run at once beside the prefix: one workgroup more than the chip holds
@@ -888,7 +923,7 @@ void split_work(Job& j, int type) {
     // 21.6, 24 of 5 x 600 behind 8192 42.9 / 36.7, 8 of 4000 behind 8192 36.1 / 33.9; the worst
     // of 80 shapes 40 of 600 behind 8192, 32.7 / 34.2).
     const int64_t beside = slots - (int64_t)a.cache.kv_heads * j.prefix_splits * j.prefix_rows;
-    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({beside / own_units, up(len, 128), 64}));
+    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({beside / own_units, up(len, j.shared_own && slow ? least_keys(len) : 128), 64}));
     if (const char* e = getenv("OWNS")) j.own_splits = atoi(e);
     j.prefix_per_xcd = (int)up((int64_t)a.cache.kv_heads * j.prefix_splits, 8) * j.prefix_rows;
     j.own_per_xcd = (int)(up((int64_t)a.cache.kv_heads * j.own_splits * a.batch.batch, 8) * j.own_rows);
