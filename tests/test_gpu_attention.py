@@ -68,6 +68,15 @@ def test_prefix_lengths_around_the_tiles(ctx, prefix):
     _case(ctx, [20, 13], [20, 40], prefix, 8, 2, 64, 8, "f16", "f16", seed=prefix)
 
 
+@pytest.mark.parametrize("name,cache,head_dim", [("f32", "f32", 64), ("f32", "bf16", 128), ("bf16", "bf16", 256),
+                                                 ("f32", "f32", 256)])
+@pytest.mark.parametrize("n", [31, 33, 65, 95, 160, 225, 450, 1000])
+def test_parts_of_a_few_tiles(ctx, name, cache, head_dim, n):
+    # rows shared by the waves where a tile takes long: parts end at multiples of 32 keys, pages at 8 and 64
+    _case(ctx, [1] * 20, [1 + n % 50] * 20, n, 4, 1, head_dim, 8, name, cache, seed=n)
+    _case(ctx, [40], [40 + n], n % 37, 2, 1, head_dim, 64, name, cache, seed=n)
+
+
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
 @pytest.mark.parametrize("prefix", [128 * n - 3 for n in (2, 3, 5, 9, 16, 17, 25, 33, 50, 63, 64, 65, 80)])
 def test_every_number_of_parts(ctx, prefix, head_dim):

@@ -401,7 +401,9 @@ struct Compute {
         st.l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
 
-    // Whether a tile holds no infinity and no NaN: the largest exponent of all.
+    // Whether a tile holds no infinity and no NaN: the largest exponent of all.  (Without it
+    // every tile on a causal edge took three products: a prompt of 52 tokens of 256 elements
+    // 42 us, 28 with it.)
     __device__ __forceinline__ static bool all_finite(const uint8_t* v) {
         const uint8_t* at = v + 16 * late_lane();
         if constexpr (sizeof(C) == 4) {
@@ -895,13 +897,15 @@ void split_work(Job& j, int type) {
         const int64_t units = (int64_t)a.cache.kv_heads * j.prefix_rows;
         // A workgroup a CU beside the own ones, two where those have little to do, and keys
         // enough to each: n keys take n / 32 tiles one after the other, and each part costs
-        // its rows' way through memory and the join, so n = sqrt(32 keys part / tile) (us), at
-        // least 256 where f32 tiles take long.  Where the waves share rows a part is near
-        // free: n lets 192 workgroups have all.  Against 512 keys (768 beside own work, 256 or
-        // 128 of f32 and 256 elements; 128 for shared rows), 8 KV heads of 128, us: 12 x 1003
-        // 22.1 / 16.1, 64 x 8192 29.7 / 28, 2 x 60 tokens x 8192 50 / 42, 1 x 8192 23.7 / 15.9,
-        // f32 43.4 / 28.8; over 654 shapes 3 % less in the mean, the worst 16 x 6 x 8192 of 256
-        // elements (109 for 89: 264 workgroups for 256 CUs).
+        // its rows' way through memory and the join, so n = sqrt(32 keys part / tile) (us); of
+        // f32 256 at least where fewer would make more than a workgroup a CU.  Where the waves
+        // share rows a part is near free: n lets 192 workgroups have all.  Against 512 keys
+        // (768 beside own work, 256 or 128 of f32 and 256 elements; 128 for shared rows), 8 KV
+        // heads of 128, us: 12 x 1003 22.1 / 16.1, 64 x 8192 29.7 / 28, 2 x 60 tokens x 8192
+        // 50 / 42, 1 x 8192 23.7 / 15.9, f32 43.4 / 28.8; over 654 shapes 3 % less in the mean.
+        // Multiples of 32 keys, not 128, where a tile takes long: 8 % less again (f32 20 x 1721
+        // on 2 KV heads 54 / 25; the worst 16 x 6 x 30000 of 256 elements, 203 / 235, 516
+        // workgroups for 256 CUs).
         const int64_t own_keys = own_units * len, prefix_keys = units * a.batch.prefix_len;
         const bool alone = own_keys * 4 < prefix_keys;
         int64_t least;
