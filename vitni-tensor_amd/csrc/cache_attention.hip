@@ -27,7 +27,6 @@
 // (the matrix cores are busy 28 % of the time; keys from one hot page are 10 % faster).
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <type_traits>
 
 #include "vtq_device.h"
@@ -928,7 +927,6 @@ void split_work(Job& j, int type) {
     // of 80 shapes 40 of 600 behind 8192, 32.7 / 34.2).
     const int64_t beside = slots - (int64_t)a.cache.kv_heads * j.prefix_splits * j.prefix_rows;
     j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({beside / own_units, up(len, j.shared_own && slow ? least_keys(len) : 128), 64}));
-    if (const char* e = getenv("OWNS")) j.own_splits = atoi(e);
     j.prefix_per_xcd = (int)up((int64_t)a.cache.kv_heads * j.prefix_splits, 8) * j.prefix_rows;
     j.own_per_xcd = (int)(up((int64_t)a.cache.kv_heads * j.own_splits * a.batch.batch, 8) * j.own_rows);
 }
