@@ -25,10 +25,9 @@
 // 3.9 TB/s at once; that prefix alone 97-102 us, 690 TFLOP/s.  Own keys are bound by
 // memory, prefix tiles by one wave's chain of products, exponentials and LDS reads
 // (the matrix cores are busy 28 % of the time; keys from one hot page are 10 % faster).
-#include <algorithm>
-#include <cmath>
 #include <type_traits>
 
+#include "vtq_attention_plan.h"
 #include "vtq_device.h"
 #include "vtq_kernels.h"
 #include "vtq_lds_load.h"
@@ -46,16 +45,8 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kWord3 = 0x00020000;  // raw buffer, stride 0
 
-struct Job {
+struct Job : AttentionPlan {
     Attention a;
-    int group;        // query heads of a KV head
-    int page_shift;
-    int prefix_rows;  // row tiles of the prefix
-    int prefix_splits, prefix_chunk;  // key ranges, and keys to one (a multiple of 32; of 128 where waves share rows)
-    int own_rows, own_splits;         // row tiles of a sequence (a workgroup may take several), key ranges
-    int own_grain;                    // which are multiples of this: 32, or 128 where waves share rows
-    int shared_prefix, shared_own;    // whether the waves share tiles (else they share rows)
-    int prefix_per_xcd, own_per_xcd;  // workgroups
     float c;          // scale * log2(e)
     float* part_o;    // [splits][tokens * heads][head_dim]
     float2* part_ml;  // [splits][tokens * heads]: maximum (log2) and sum
@@ -561,7 +552,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
         const int len = uniform(min(max(a.batch.len[seq], -(1 << 29)), 1 << 30));
         pages.keys = min(max(len, 0), a.batch.max_pages << j.page_shift);
         unseen = len - (int)(t1 - t0);
-        const int chunk = ((pages.keys + splits - 1) / splits + j.own_grain - 1) & -j.own_grain;
+        const int chunk = own_chunk(pages.keys, splits, j.own_grain);
         k0 = (int)min((int64_t)split * chunk, (int64_t)pages.keys);
         k1 = min(pages.keys, k0 + chunk);
     }
@@ -789,6 +780,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
 template <class Q, int L>
 __global__ __launch_bounds__(256) void join_kernel(Job j) {
     constexpr int N = 64 / L, kAhead = 4;
+    static_assert(kMostParts == 2 * 64, "parts lane and 64 + lane");
     const Attention& a = j.a;
     const int lane = threadIdx.x & 63, splits = j.prefix_splits + j.own_splits, hd = a.cache.head_dim;
     const int64_t rows = a.tokens * a.heads, row = (int64_t)blockIdx.x * 4 + wave_id();
@@ -858,89 +850,11 @@ __global__ __launch_bounds__(256) void join_kernel(Job j) {
     if (live && a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
-// ------------------------------------------------ how the work is split
-
-int waves_of(int cache_type, int head_dim) {
-    const int d = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-    return 32 * d * (int)type_bytes(cache_type) > 16384 ? 2 : 4;
-}
-
-void split_work(Job& j, int type) {
-    const Attention& a = j.a;
-    const int W = waves_of(a.cache.type, a.cache.head_dim);
-    auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    const int64_t slots = 512;
-    j.group = a.heads / a.cache.kv_heads;
-    j.page_shift = __builtin_ctz((unsigned)a.cache.page_size);
-    const int64_t prefix_rows = a.tokens * j.group;
-    const int64_t own_rows = std::min<int64_t>(std::max(1, a.batch.max_q), a.tokens) * j.group;
-    j.shared_prefix = prefix_rows > 32;
-    j.shared_own = own_rows > 32;
-    j.prefix_rows = j.prefix_splits = 0;
-    j.prefix_chunk = 128;
-    const int64_t most = (int64_t)a.batch.max_pages << j.page_shift;
-    const int64_t len = a.batch.max_len ? std::min<int64_t>(a.batch.max_len, most) : most;
-    j.own_rows = (int)up(own_rows, j.shared_own ? 32 * W : 32);
-    const int64_t own_units = (int64_t)a.cache.kv_heads * j.own_rows * a.batch.batch;
-    const int d = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
-    const bool slow = type == VTQ_TYPE_F32 || d > 128;  // tiles that take long: parts of less than four
-    const int grain = slow ? 32 : 128;
-    j.own_grain = j.shared_own ? grain : 128;
-    auto least_keys = [&](int64_t keys) {
-        const double tile = type == VTQ_TYPE_F32 ? 3.6 * d / 128 : d > 128 ? 2.4 : 0.18 + 0.0025 * d;
-        const double part = 0.08 + 2.3e-6 * (double)(a.tokens * a.heads * a.cache.head_dim);
-        return (1 + (int64_t)std::sqrt(32.0 * keys * part / tile) / grain) * grain;
-    };
-    if (a.batch.prefix_len) {
-        j.prefix_rows = (int)up(prefix_rows, j.shared_prefix ? 32 * W : 32);
-        const int64_t units = (int64_t)a.cache.kv_heads * j.prefix_rows;
-        // A workgroup a CU beside the own ones, two where those have little to do, and keys
-        // enough to each: n keys take n / 32 tiles one after the other, and each part costs
-        // its rows' way through memory and the join, so n = sqrt(32 keys part / tile) (us); of
-        // f32 256 at least where fewer would make more than a workgroup a CU.  Where the waves
-        // share rows a part is near free: n lets 192 workgroups have all.  Against 512 keys
-        // (768 beside own work, 256 or 128 of f32 and 256 elements; 128 for shared rows), 8 KV
-        // heads of 128, us: 12 x 1003 22.1 / 16.1, 64 x 8192 29.7 / 28, 2 x 60 tokens x 8192
-        // 50 / 42, 1 x 8192 23.7 / 15.9, f32 43.4 / 28.8; over 654 shapes 3 % less in the mean.
-        // Multiples of 32 keys, not 128, where a tile takes long: 8 % less again (f32 20 x 1721
-        // on 2 KV heads 54 / 25; the worst 16 x 6 x 30000 of 256 elements, 203 / 235, 516
-        // workgroups for 256 CUs).
-        const int64_t own_keys = own_units * len, prefix_keys = units * a.batch.prefix_len;
-        const bool alone = own_keys * 4 < prefix_keys;
-        int64_t least;
-        if (j.shared_prefix) {
-            least = least_keys(a.batch.prefix_len);
-            if (type == VTQ_TYPE_F32 && units * up(a.batch.prefix_len, least) + own_units > slots / 2)
-                least = std::max<int64_t>(least, 256);
-        } else {
-            least = std::min<int64_t>(512, up(prefix_keys, 192 * 128) * 128);
-        }
-        const int64_t splits =
-            std::min<int64_t>({up(alone ? slots : slots / 2, units), up(a.batch.prefix_len, least), 64});
-        const int64_t by = j.shared_prefix ? grain : 128;
-        j.prefix_chunk = (int)(up(up(a.batch.prefix_len, splits), by) * by);
-        j.prefix_splits = (int)up(a.batch.prefix_len, j.prefix_chunk);
-    }
-    // As many parts as run at once beside the prefix: one workgroup more than the chip holds
-    // costs a round (8 KV heads of 128, rounded up / down, us: 48 sequences of 600 keys 28.3 /
-    // 21.6, 24 of 5 x 600 behind 8192 42.9 / 36.7, 8 of 4000 behind 8192 36.1 / 33.9; the worst
-    // of 80 shapes 40 of 600 behind 8192, 32.7 / 34.2).
-    const int64_t beside = slots - (int64_t)a.cache.kv_heads * j.prefix_splits * j.prefix_rows;
-    j.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({beside / own_units, up(len, j.shared_own && slow ? least_keys(len) : 128), 64}));
-    j.prefix_per_xcd = (int)up((int64_t)a.cache.kv_heads * j.prefix_splits, 8) * j.prefix_rows;
-    j.own_per_xcd = (int)(up((int64_t)a.cache.kv_heads * j.own_splits * a.batch.batch, 8) * j.own_rows);
-}
-
 }  // namespace
 
 size_t attention_workspace(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens, int heads) {
-    Job j{};
-    j.a.cache = cache;
-    j.a.batch = batch;
-    j.a.tokens = tokens;
-    j.a.heads = heads;
-    split_work(j, type);
-    const size_t splits = j.prefix_splits + j.own_splits;
+    const AttentionPlan plan = plan_attention(cache, batch, type, tokens, heads);
+    const size_t splits = plan.prefix_splits + plan.own_splits;
     return splits > 1 ? splits * tokens * heads * (cache.head_dim * sizeof(float) + sizeof(float2)) + 256 : 0;
 }
 
@@ -962,8 +876,8 @@ hipError_t launch_attention_of(const Job& j, hipStream_t stream) {
 
 hipError_t launch_attention(const Attention& a, int type, hipStream_t stream) {
     Job j{};
+    static_cast<AttentionPlan&>(j) = plan_attention(a.cache, a.batch, type, a.tokens, a.heads);
     j.a = a;
-    split_work(j, type);
     j.c = a.scale * kLog2E;
     const size_t rows = (size_t)(j.prefix_splits + j.own_splits) * a.tokens * a.heads;
     j.part_o = static_cast<float*>(a.ws);

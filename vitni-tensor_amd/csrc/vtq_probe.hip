@@ -10,6 +10,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "vtq_attention_plan.h"
 #include "vtq_i8_rules.h"
 #include "vtq_rules.h"
 #include "vtq_serve.h"
@@ -119,6 +120,22 @@ int vtqp_check_attention(const char** text, const vtq_kv_cache* cache, const vtq
     return told(vtq::check_attention(cache, batch, type, tokens, heads, d_q, q_token_stride, q_head_stride, d_y,
                                      y_token_stride, y_head_stride, d_lse, scale), text);
 }
+
+// How an attention call that is not refused is split: AttentionPlan, 12 numbers in its
+// order (vtq_attention_plan.h), and keys to each own range of a sequence of `keys`.
+int vtqp_attention_plan(const vtq_kv_cache* cache, const vtq_kv_batch* batch, int type, size_t tokens, size_t heads,
+                        int* out) {
+    static_assert(sizeof(vtq::AttentionPlan) == 12 * sizeof(int), "plan");
+    if (vtq::Refusal r = vtq::check_cache(cache)) return r.code;
+    if (vtq::Refusal r = vtq::check_batch(batch, cache, false)) return r.code;
+    if (!vtq::type_bytes(type) || !tokens || tokens > vtq::kMostTokens || !heads || heads > 65535 ||
+        heads % cache->kv_heads || !batch->batch || !vtq::attention_fits(cache, batch, tokens, heads))
+        return VTQ_E_INVALID_ARGUMENT;
+    const vtq::AttentionPlan p = vtq::plan_attention(*cache, *batch, type, (int64_t)tokens, (int)heads);
+    __builtin_memcpy(out, &p, sizeof p);
+    return VTQ_OK;
+}
+int vtqp_own_chunk(int keys, int splits, int grain) { return vtq::own_chunk(keys, splits, grain); }
 
 // Where a place of a sequence begins in the cache (vtq_serve.h).
 int64_t vtqp_slot_of(const vtq_kv_cache* cache, const int32_t* pages, int max_pages, int64_t place) {

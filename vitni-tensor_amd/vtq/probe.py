@@ -32,6 +32,8 @@ def lib() -> ctypes.CDLL:
         L.vtqp_check_append.argtypes = [vp, vp, vp, vp, i, sz, vp, sz, sz, vp, sz, sz, sz, vp, sz, sz, vp, sz, sz]
         L.vtqp_check_attention.argtypes = [vp, vp, vp, i, sz, sz, vp, sz, sz, vp, sz, sz, vp, f]
         L.vtqp_i8_form.argtypes = [i, i, i]
+        L.vtqp_attention_plan.argtypes = [vp, vp, i, sz, sz, ctypes.POINTER(i)]
+        L.vtqp_own_chunk.argtypes = [i, i, i]
         L.vtqp_slot_of.argtypes = [vp, vp, i, ctypes.c_int64]
         L.vtqp_slot_of.restype = ctypes.c_int64
         _lib = L
@@ -53,6 +55,22 @@ def refusal(operator: str, *args):
     text = ctypes.c_char_p()
     rc = getattr(lib(), "vtqp_check_" + operator)(ctypes.byref(text), *args)
     return rc, (text.value or b"").decode()
+
+
+PLAN = ("group", "page_shift", "prefix_rows", "prefix_splits", "prefix_chunk", "own_rows", "own_splits", "own_grain",
+        "shared_prefix", "shared_own", "prefix_per_xcd", "own_per_xcd")
+
+
+def attention_plan(cache, batch, ggml_type, tokens, heads):
+    """How vtq_attention_device splits a call (AttentionPlan of vtq_attention_plan.h); None where it is refused."""
+    out = (ctypes.c_int * len(PLAN))()
+    rc = lib().vtqp_attention_plan(cache.ref, batch.ref, ggml_type, tokens, heads, out)
+    return None if rc else dict(zip(PLAN, out))
+
+
+def own_chunk(keys, splits, grain):
+    """Keys to each range of a sequence's own."""
+    return lib().vtqp_own_chunk(keys, splits, grain)
 
 
 def stream_read(ptr: int, nbytes: int, workgroups: int, sink_ptr: int, stream: int) -> None:
