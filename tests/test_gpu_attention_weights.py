@@ -1,0 +1,83 @@
+"""Attention's softmax weights where rounding shows most: maxima that rise late at large scores, and keys whose
+weights are far below the largest one.  Scores are chosen so that they are exact in f32."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import vtq
+from serving import F32_HALF_STEP, TAGS, TYPES, half_step, smallest, stream, within
+from vtq import probe
+
+pytestmark = pytest.mark.gpu
+U = F32_HALF_STEP
+
+
+def _attend(ctx, name, cache, q, k, v, heads, lens, pages, page, prefix=0, live=None, one_range=False, shared=None):
+    """k, v [n_pages, kv_heads, page, head_dim]; a token each of len(lens) sequences, the first `live` of the call's
+    tokens; the others only choose how the work is split."""
+    kv_heads, d, tokens = k.shape[1], k.shape[3], q.shape[0]
+    live = len(lens) if live is None else live
+    lists = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in
+             (list(range(len(lens) + 1)), lens, pages, [0] * max(1, -(-prefix // page)))]
+    c = vtq.KvCache(TAGS[cache], k.data_ptr(), v.data_ptr(), k.shape[0], page, kv_heads, d)
+    b = vtq.KvBatch(len(lens), lists[0].data_ptr(), lists[1].data_ptr(), lists[2].data_ptr(), len(pages[0]),
+                    max_q=tokens if tokens > len(lens) else 1, prefix_len=prefix,
+                    prefix_pages=lists[3].data_ptr() if prefix else None)
+    plan = probe.attention_plan(c, b, TAGS[name], tokens, heads)
+    if one_range:
+        assert plan["own_splits"] == 1 and plan["prefix_splits"] == 0
+    if shared is not None:
+        assert plan["shared_own"] == shared
+    need = ctx.attention_workspace(c, b, TAGS[name], tokens, heads)
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    y = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    lse = torch.full(q.shape[:2], 7.0, device="cuda")
+    ctx.attention_device(c, b, TAGS[name], tokens, heads, q.data_ptr(), q.stride(0), q.stride(1), y.data_ptr(),
+                         y.stride(0), y.stride(1), 1.0, ws.data_ptr(), need, stream(), lse_ptr=lse.data_ptr())
+    torch.cuda.synchronize()
+    return y[:live].double().cpu(), lse[:live].double().cpu()
+
+
+def _queries(tokens, heads, d, name, *first):
+    q = torch.zeros(tokens, heads, d)
+    for i, x in enumerate(first):
+        q[..., i] = x
+    q = q.to(TYPES[name])
+    assert [float(x) for x in q[0, 0, :len(first)]] == list(first)
+    return q.cuda()
+
+
+@pytest.mark.parametrize("name,cache", [("f32", "f32"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("shared", [True, False])
+def test_a_late_maximum_keeps_the_earlier_weights(ctx, name, cache, d, shared):
+    # 256 keys with a score S of some 2^18, then four that are higher by 6, one in every tile of a wave: weights 1 and
+    # e^6.  S log2(e) in f32 is off by up to 2^-6, which must cancel.
+    c = float(np.float32(1.44269504088896340736))
+    k0 = max(range(200, 257), key=lambda x: abs(1024 * x * c - float(np.float32(1024 * x * c))))
+    lost = abs(1024 * k0 * c - float(np.float32(1024 * k0 * c)))
+    assert lost > 0.01  # of a power of two
+    n, high = 353, torch.tensor([256, 288, 320, 352])
+    kv_heads, batch = (1, 1) if shared else (8, 64)
+    heads = 64 if shared else 8
+    k = torch.zeros(1, kv_heads, 512, d)
+    k[..., 0] = k0
+    k[:, :, high, 1] = 6.0
+    v = torch.ones(1, kv_heads, 512, d)
+    v[:, :, high] = -1.0
+    q = _queries(1024 if shared else batch, heads, d, name, 1024.0, 1.0)
+    y, lse = _attend(ctx, name, cache, q, k.to(TYPES[cache]).cuda(), v.to(TYPES[cache]).cuda(), heads, [n] * batch,
+                     [[0]] * batch, 512, one_range=True, shared=shared)
+    low, top = float(n - 4), 4 * math.exp(6.0)
+    want = torch.full(y.shape, (low - top) / (low + top), dtype=torch.float64)
+    # Differences of 6 times log2(e), which is off by u, and the exponential by 4 u: 6 * 1.45 * 2 u + 4 u; weights are off
+    # by twice that, sums by a u a key; weights and the result round to the type.  (Twice: values of both signs.)
+    rel = 2.1 * (6 * 1.45 * 2 * U + 4 * U) + n * U + (0 if name == "f32" else half_step(q.dtype) * 1.01)
+    bound = rel + half_step(q.dtype) * want.abs() * 1.01 + smallest(q.dtype)
+    # what the lost part of a power of two would do to the 256 keys before the first rise, is more than that
+    assert lost * math.log(2) * 2 * 256 * top / (low + top) ** 2 > 1.2 * float(bound[0, 0, 0])
+    within(y, want, bound, "y")
+    want_l = torch.full(lse.shape, 1024.0 * k0 + math.log(low + top), dtype=torch.float64)
+    within(lse, want_l, 4 * U * want_l + rel, "lse")

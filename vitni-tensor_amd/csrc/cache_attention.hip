@@ -371,7 +371,9 @@ struct Compute {
         // cost nothing in a float, and rows rarely rescale
         const bool moves = (top - st.m) * c > 8.0f;  // each row for itself
         if (__ballot(moves)) {
-            const float shrink = moves ? __builtin_amdgcn_exp2f(fmaf(st.m, c, -(top * c))) : 1.0f;
+            // from one rounded product to the other, as weights are taken: with the old one
+            // unrounded, scores of 2^18 lost 2^-6 of a power of two here
+            const float shrink = moves ? __builtin_amdgcn_exp2f(st.m * c - top * c) : 1.0f;
             st.m = moves ? top : st.m;
             st.l *= shrink;
 #pragma unroll
