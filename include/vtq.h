@@ -310,8 +310,8 @@ int vtq_kv_append_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_b
  * see never reaches it.  Keys in pages outside the cache count as zeros.  type is
  * the queries' and y's: the cache's own, or VTQ_TYPE_F32 with any cache.  lse
  * (f32, tokens x heads, or NULL) is in natural logarithms.  0 < scale <= 1e30.
- * A row whose every score is -infinity counts as one that sees no key; a score
- * past the range of f32 gives NaN.  y may be q itself (the same pointer and
+ * A row whose every score is -infinity counts as one that sees no key; a product
+ * q . k past the range of f32 gives NaN, an lse past it an infinity.  y may be q itself (the same pointer and
  * strides), and must not overlap it otherwise.  A call takes at most 2^23 tokens,
  * 2^25 rows (tokens x heads) and 2^22 workgroups (to a sequence, KV head and 32
  * rows of it).

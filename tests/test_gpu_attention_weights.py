@@ -14,7 +14,8 @@ pytestmark = pytest.mark.gpu
 U = F32_HALF_STEP
 
 
-def _attend(ctx, name, cache, q, k, v, heads, lens, pages, page, prefix=0, live=None, one_range=False, shared=None):
+def _attend(ctx, name, cache, q, k, v, heads, lens, pages, page, prefix=0, live=None, one_range=False, shared=None,
+            scale=1.0):
     """k, v [n_pages, kv_heads, page, head_dim]; a token each of len(lens) sequences, the first `live` of the call's
     tokens; the others only choose how the work is split."""
     kv_heads, d, tokens = k.shape[1], k.shape[3], q.shape[0]
@@ -35,7 +36,7 @@ def _attend(ctx, name, cache, q, k, v, heads, lens, pages, page, prefix=0, live=
     y = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
     lse = torch.full(q.shape[:2], 7.0, device="cuda")
     ctx.attention_device(c, b, TAGS[name], tokens, heads, q.data_ptr(), q.stride(0), q.stride(1), y.data_ptr(),
-                         y.stride(0), y.stride(1), 1.0, ws.data_ptr(), need, stream(), lse_ptr=lse.data_ptr())
+                         y.stride(0), y.stride(1), scale, ws.data_ptr(), need, stream(), lse_ptr=lse.data_ptr())
     torch.cuda.synchronize()
     return y[:live].double().cpu(), lse[:live].double().cpu()
 
@@ -81,3 +82,36 @@ def test_a_late_maximum_keeps_the_earlier_weights(ctx, name, cache, d, shared):
     within(y, want, bound, "y")
     want_l = torch.full(lse.shape, 1024.0 * k0 + math.log(low + top), dtype=torch.float64)
     within(lse, want_l, 4 * U * want_l + rel, "lse")
+
+
+# heads, KV heads, tokens of the call, sequences, own keys, prefix: a wave's own rows and tiles of its own, with and
+# without parts, and the prefix
+SHAPES = [(64, 1, 1024, 1, 500, 0), (64, 1, 1, 1, 500, 0), (8, 8, 64, 64, 500, 0), (4, 1, 1, 1, 500, 0),
+          (4, 2, 20, 20, 32, 500), (2, 1, 1, 1, 32, 500)]
+
+
+@pytest.mark.parametrize("name,cache", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"),
+                                        ("f32", "bf16")])
+@pytest.mark.parametrize("scale", [3.0e7, 1.1e10, 1.3e20, 1.0e30])
+@pytest.mark.parametrize("heads,kv_heads,tokens,batch,n,prefix", SHAPES)
+def test_scores_of_any_size_in_f32(ctx, heads, kv_heads, tokens, batch, n, prefix, scale, name, cache):
+    # products of -7 to 5 times a large scale: the keys of 5 share the weight, the others, 3e7 and more below, have none
+    g = torch.Generator().manual_seed(n + prefix)
+    k = torch.zeros(2, kv_heads, 512, 64)
+    k[..., 0] = torch.randint(-7, 5, (2, kv_heads, 512), generator=g).float()
+    for page, place in ((0, 40), (0, 41), (0, 333), (1, 3), (1, 30), (1, 200), (1, 497)):
+        k[page, :, place, 0] = 5.0
+    v = torch.randn(2, kv_heads, 512, 64, generator=g).to(TYPES[cache])
+    q = _queries(tokens, heads, 64, name, 1.0)
+    y, lse = _attend(ctx, name, cache, q, k.to(TYPES[cache]).cuda(), v.cuda(), heads, [n] * batch, [[1]] * batch, 512,
+                     prefix=prefix, live=min(tokens, batch), scale=scale)
+    ks, vs = (torch.cat([x[0, :, :prefix], x[1, :, :n]], 1).double() for x in (k, v))
+    has = (ks[..., 0] == 5.0).double()[..., None]
+    count = has.sum(1)
+    want = ((has * vs).sum(1) / count).repeat_interleave(heads // kv_heads, 0).expand(y.shape)
+    size = ((has * vs.abs()).sum(1) / count).repeat_interleave(heads // kv_heads, 0).expand(y.shape)
+    # weights of 1, at most 7 of them: sums and the quotient round in f32, then the result to its type
+    within(y, want, 10 * U * size + half_step(q.dtype) * want.abs() * 1.01 + smallest(q.dtype), "y")
+    f32_scale = float(torch.tensor(scale))
+    want_l = (5.0 * f32_scale + count.log()).squeeze(-1).repeat_interleave(heads // kv_heads).expand(lse.shape)
+    within(lse, want_l, 4 * U * want_l, "lse")

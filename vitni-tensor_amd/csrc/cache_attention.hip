@@ -49,7 +49,7 @@ struct Job : AttentionPlan {
     Attention a;
     float c;          // scale * log2(e)
     float* part_o;    // [splits][tokens * heads][head_dim]
-    float2* part_ml;  // [splits][tokens * heads]: maximum (log2) and sum
+    float2* part_ml;  // [splits][tokens * heads]: maximum of q.k and sum
 };
 
 // What a wave has of a 32-row tile.
@@ -371,21 +371,21 @@ struct Compute {
         // cost nothing in a float, and rows rarely rescale
         const bool moves = (top - st.m) * c > 8.0f;  // each row for itself
         if (__ballot(moves)) {
-            // from one rounded product to the other, as weights are taken: with the old one
-            // unrounded, scores of 2^18 lost 2^-6 of a power of two here
-            const float shrink = moves ? __builtin_amdgcn_exp2f(st.m * c - top * c) : 1.0f;
+            const float shrink = moves ? __builtin_amdgcn_exp2f((st.m - top) * c) : 1.0f;
             st.m = moves ? top : st.m;
             st.l *= shrink;
 #pragma unroll
             for (int b = 0; b < D / 32; b++) st.o[b] *= shrink;
         }
-        const float base = st.m == -INFINITY ? 0.0f : st.m * c;
+        // The difference first, then the scale, here and wherever sums meet: the product m c, rounded,
+        // would be off by a power of two and more from scores of 2^24 on, and exp2 leave its range
+        const float base = st.m == -INFINITY ? 0.0f : st.m;
         float sum[4] = {st.l, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < N; i++) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], c, -base));
+                s[i][r] = __builtin_amdgcn_exp2f((s[i][r] - base) * c);
                 sum[r & 3] += s[i][r];
             }
             w[i] = weights(s[i]);
@@ -503,7 +503,7 @@ __device__ __forceinline__ void put_row(const Job& j, int split, int64_t token, 
     v4q r;
     r[0] = (Q)(o.x * inv), r[1] = (Q)(o.y * inv), r[2] = (Q)(o.z * inv), r[3] = (Q)(o.w * inv);
     *reinterpret_cast<v4q*>(y) = r;
-    if (d == 0 && a.lse) a.lse[row] = none ? -INFINITY : (m + __log2f(l)) * kLn2;
+    if (d == 0 && a.lse) a.lse[row] = none ? -INFINITY : fmaf(m, a.scale, __log2f(l) * kLn2);
 }
 
 template <class Q, class C, int D>
@@ -714,7 +714,6 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
         }
         const float2 sums = halves(st.l);
         st.l = sums.x + sums.y;
-        const float m2 = st.m == -INFINITY ? -INFINITY : st.m * j.c;
         const int out_split = prefix ? split : j.prefix_splits + split;
         const int late = late_lane(), late_h = late >> 5;
         if (shared) {
@@ -728,7 +727,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                         const v16f& o = st.o[db];
                         if (d < hd)
                             put_row<Q>(j, out_split, t0 + row / G, kv_head * G + row % G, d,
-                                       make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]), m2, st.l);
+                                       make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]), st.m, st.l);
                     }
             }
         } else {
@@ -745,7 +744,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
                     *reinterpret_cast<float4*>(mine + row * D + 4 * c) =
                         make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
-            if (late_h == 0) wave_ml[wave][row] = make_float2(m2, st.l);
+            if (late_h == 0) wave_ml[wave][row] = make_float2(st.m, st.l);
             __syncthreads();
             const int rows = min(32, n_rows - r0);
             for (int e = wave * 64 + late; e < rows * (D / 4); e += W * 64) {
@@ -760,7 +759,7 @@ __global__ __launch_bounds__((Config<Q, C, D>::kWaves * 64), (Config<Q, C, D>::k
 #pragma unroll
                 for (int w = 0; w < W; w++) {
                     const float2 ml = wave_ml[w][rr];
-                    const float f = __builtin_amdgcn_exp2f(ml.x - base);
+                    const float f = __builtin_amdgcn_exp2f((ml.x - base) * j.c);
                     const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(
                                                                           lds + w * 2 * T::kBytes) +
                                                                       rr * D + 4 * (c ^ (rr & 15)));
@@ -812,7 +811,7 @@ __global__ __launch_bounds__(256) void join_kernel(Job j) {
     float f[2], l = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        f[i] = __builtin_amdgcn_exp2f(ml[i].x - base);
+        f[i] = __builtin_amdgcn_exp2f((ml[i].x - base) * j.c);
         l += ml[i].y * f[i];
     }
 #pragma unroll
@@ -849,7 +848,7 @@ __global__ __launch_bounds__(256) void join_kernel(Job j) {
         *reinterpret_cast<v4q*>(static_cast<Q*>(a.y) + token * a.y_token_stride + (row % a.heads) * a.y_head_stride + d) =
             r;
     }
-    if (live && a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (m + __log2f(l)) * kLn2;
+    if (live && a.lse && lane == 0) a.lse[row] = none ? -INFINITY : fmaf(m, a.scale, __log2f(l) * kLn2);
 }
 
 }  // namespace
