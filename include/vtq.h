@@ -310,11 +310,15 @@ int vtq_kv_append_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_b
  * see never reaches it.  Keys in pages outside the cache count as zeros.  type is
  * the queries' and y's: the cache's own, or VTQ_TYPE_F32 with any cache.  lse
  * (f32, tokens x heads, or NULL) is in natural logarithms.  0 < scale <= 1e30.
+ * Scores, maxima and sums are f32.  Where the queries are 16-bit, each weight is
+ * rounded to their type before it meets its value: off by 2^-8 of itself (BF16), or
+ * by 2^-11 of itself or 2^-32 of the row's largest, whichever is more (F16).  With
+ * F32 queries weights stay f32, over a 16-bit cache too.
  * A row whose every score is -infinity counts as one that sees no key; a product
- * q . k past the range of f32 gives NaN, an lse past it an infinity.  y may be q itself (the same pointer and
- * strides), and must not overlap it otherwise.  A call takes at most 2^23 tokens,
- * 2^25 rows (tokens x heads) and 2^22 workgroups (to a sequence, KV head and 32
- * rows of it).
+ * q . k past the range of f32 gives NaN, an lse past it an infinity.  y may be q
+ * itself (the same pointer and strides), and must not overlap it otherwise.  A call
+ * takes at most 2^23 tokens, 2^25 rows (tokens x heads) and 2^22 workgroups (to a
+ * sequence, KV head and 32 rows of it).
  * d_ws is at least vtq_attention_workspace bytes, 256-byte aligned, for this call
  * alone until its work is done (calls that may overlap need one each); the size
  * depends on the host's numbers only, not on the lengths in device memory. */

@@ -115,3 +115,56 @@ def test_scores_of_any_size_in_f32(ctx, heads, kv_heads, tokens, batch, n, prefi
     f32_scale = float(torch.tensor(scale))
     want_l = (5.0 * f32_scale + count.log()).squeeze(-1).repeat_interleave(heads // kv_heads).expand(lse.shape)
     within(lse, want_l, 4 * U * want_l, "lse")
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("gap", [18.0, 19.5, 21.0])
+@pytest.mark.parametrize("heads,kv_heads,tokens,batch,n,prefix", SHAPES)
+def test_f16_keeps_weights_far_below_the_largest(ctx, heads, kv_heads, tokens, batch, n, prefix, gap, d):
+    # Every tile of 32 keys begins with a key of score 0 and value 0; the others' weights, e^-gap (2^-26 to 2^-30.3),
+    # are all that the result has.
+    g = torch.Generator().manual_seed(int(10 * gap) + d)
+    k = torch.zeros(2, kv_heads, 512, d)
+    k[..., 0] = -gap
+    k[:, :, ::32, 0] = 0.0
+    v = 500.0 + 500.0 * torch.rand(2, kv_heads, 512, d, generator=g)
+    v[:, :, ::32] = 0.0
+    v = v.half()
+    q = _queries(tokens, heads, d, "f16", 1.0)
+    y, lse = _attend(ctx, "f16", "f16", q, k.half().cuda(), v.cuda(), heads, [n] * batch, [[1]] * batch, 512,
+                     prefix=prefix, live=min(tokens, batch))
+    w = math.exp(-gap)
+    vs = torch.cat([v[0, :, :prefix], v[1, :, :n]], 1).double()
+    highs = -(-prefix // 32) + -(-n // 32)
+    total = highs + w * (prefix + n - highs)
+    want = (w * vs.sum(1) / total).repeat_interleave(heads // kv_heads, 0).expand(y.shape)
+    # A weight is rounded to 2^-11 of itself, or to half of 2^-24's step where it is below 2^-14: kept 2^7 times as
+    # large as it counts, that is 2^-32 of the largest.
+    rel = 2.1 * (gap * 1.45 * 2 * U + 4 * U) + (prefix + n) * U + half_step(torch.float16) * 1.01
+    bound = want * (rel + 2.0 ** -32 * 1.01 / w + half_step(torch.float16) * 1.01) + smallest(torch.float16)
+    assert (bound < 0.6 * want).all()
+    within(y, want, bound, "y")
+
+
+def test_f16_keeps_a_million_small_weights(ctx):
+    # one key of score 0 and value 0, and 2^20 - 1 of e^-18, 2^-26, which together are 2^-6 of it
+    n, d, page, heads = 1 << 20, 64, 4096, 64
+    g = torch.Generator().manual_seed(3)
+    k = torch.zeros(2, 1, page, d)
+    k[..., 0] = -18.0
+    k[0, 0, 0, 0] = 0.0
+    v = 1.0 + torch.rand(2, 1, page, d, generator=g)
+    v[0, 0, 0] = 0.0
+    v = v.half()
+    q = _queries(1024, heads, d, "f16", 1.0)
+    y, lse = _attend(ctx, "f16", "f16", q, k.half().cuda(), v.cuda(), heads, [n], [[0] + [1] * (n // page - 1)], page,
+                     one_range=True, shared=True)
+    w = math.exp(-18.0)
+    values = v[0, 0].double().sum(0) + (n // page - 1) * v[1, 0].double().sum(0)
+    want = (w * values / (1 + w * (n - 1))).expand(y.shape)
+    # As above; the products' sum is rounded once for 8 keys at most, the weights' sum at most once a key of a lane
+    # and of the four sums that it has, of which one holds the large weight: n / 8 times in two lanes.
+    rel = (2.1 * (18 * 1.45 * 2 * U + 4 * U) + n / 8 * U + n / 4 * U + half_step(torch.float16) * 2.02
+           + 2.0 ** -32 * 1.01 / w)
+    assert rel < 0.05
+    within(y, want, want * rel + smallest(torch.float16), "y")

@@ -43,6 +43,12 @@ typedef uint16_t v8us __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+// Weights, and what is summed with them, are 2^kUp times as large as they count.  In f16
+// the 2^8 that a weight may be ahead of the maximum times 2^7 stay within 65504, and what
+// is lost below the smallest step is 2^-32 of the largest weight instead of 2^-25 (500 keys
+// of 2^-26 counted for nothing beside one of 1).  bf16 and f32 have exponents enough.
+template <class Q>
+constexpr float kUp = std::is_same_v<Q, _Float16> ? 7.0f : 0.0f;
 constexpr int kWord3 = 0x00020000;  // raw buffer, stride 0
 
 struct Job : AttentionPlan {
@@ -290,7 +296,10 @@ struct Compute {
         Weights w;
         if constexpr (kWide) {
             w.v[0] = p;
-        } else {  // rounded to the values' type: off by 2^-8 (bf16) or 2^-11 (f16) of each at most, the sum stays f32
+        } else {
+            // Rounded to the values' type, so that the second product runs at that type's rate
+            // (f32's is a sixteenth): off by 2^-8 (bf16) or 2^-11 (f16) of each at most, in f16 or
+            // by 2^-32 of the largest.  The sum is of the unrounded ones, in f32.
 #pragma unroll
             for (int j = 0; j < 8; j++) w.v[0][j] = (Q)p[j], w.v[1][j] = (Q)p[8 + j];
         }
@@ -368,7 +377,7 @@ struct Compute {
         const float2 both = halves(top);
         top = fmaxf(both.x, both.y);
         // m follows the maximum only once it is 8 powers of two behind: weights up to 256
-        // cost nothing in a float, and rows rarely rescale
+        // cost nothing, and rows rarely rescale
         const bool moves = (top - st.m) * c > 8.0f;  // each row for itself
         if (__ballot(moves)) {
             const float shrink = moves ? __builtin_amdgcn_exp2f((st.m - top) * c) : 1.0f;
@@ -385,7 +394,7 @@ struct Compute {
         for (int i = 0; i < N; i++) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                s[i][r] = __builtin_amdgcn_exp2f((s[i][r] - base) * c);
+                s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r] - base, c, kUp<Q>));
                 sum[r & 3] += s[i][r];
             }
             w[i] = weights(s[i]);
@@ -503,7 +512,7 @@ __device__ __forceinline__ void put_row(const Job& j, int split, int64_t token, 
     v4q r;
     r[0] = (Q)(o.x * inv), r[1] = (Q)(o.y * inv), r[2] = (Q)(o.z * inv), r[3] = (Q)(o.w * inv);
     *reinterpret_cast<v4q*>(y) = r;
-    if (d == 0 && a.lse) a.lse[row] = none ? -INFINITY : fmaf(m, a.scale, __log2f(l) * kLn2);
+    if (d == 0 && a.lse) a.lse[row] = none ? -INFINITY : fmaf(m, a.scale, (__log2f(l) - kUp<Q>) * kLn2);
 }
 
 template <class Q, class C, int D>
@@ -848,7 +857,7 @@ __global__ __launch_bounds__(256) void join_kernel(Job j) {
         *reinterpret_cast<v4q*>(static_cast<Q*>(a.y) + token * a.y_token_stride + (row % a.heads) * a.y_head_stride + d) =
             r;
     }
-    if (live && a.lse && lane == 0) a.lse[row] = none ? -INFINITY : fmaf(m, a.scale, __log2f(l) * kLn2);
+    if (live && a.lse && lane == 0) a.lse[row] = none ? -INFINITY : fmaf(m, a.scale, (__log2f(l) - kUp<Q>) * kLn2);
 }
 
 }  // namespace
