@@ -225,8 +225,9 @@ int vtq_linear_i8_device(vtq_ctx *ctx, const int8_t *d_xq, size_t ld_x, const fl
  *           turns (32 and 1 where 0 is given), rounded outwards to whole indices, and
  *           magnitude 0.1 ln(factor) + 1.
  * magnitude (at most 1e30), where it is not 0, replaces the rule's own.  A plan is plain memory:
- * it may be copied, and holds f_i as fractions of a turn in 64 bits, so that
- * p * f_i modulo a turn is exact for every 32-bit position. */
+ * it may be copied, and holds f_i as fractions of a turn in 64 bits (off by 4 2^-64
+ * at most where no factor is below 1), so that p * f_i modulo a turn is right to
+ * 2^-31 of a turn for every 32-bit position. */
 #define VTQ_ROPE_INTERLEAVED 0
 #define VTQ_ROPE_HALF 1
 #define VTQ_ROPE_SCALE_NONE 0

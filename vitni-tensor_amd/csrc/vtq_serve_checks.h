@@ -126,23 +126,26 @@ inline Refusal plan_rope(const vtq_rope_params* p, vtq_rope* out) {
         first = std::fmax(std::floor(index_at(high)), 0.0);
         last = std::fmin(std::ceil(index_at(low)), dim - 1.0);
     }
+    // Frequencies in the host's 64-bit mantissas: positions of up to 2^31 multiply what they
+    // are off by, and doubles' 2^-53 would come out as 2^-22 of a radian.
+    const long double full = 6.283185307179586476925286766559005768L;
     for (int i = 0; i < dim / 2; i++) {
-        double f = std::exp(-2.0 * i / dim * std::log(p->theta));
+        long double f = std::exp(-2.0L * i / dim * std::log((long double)p->theta));
         if (p->factors) {
             const double d = p->factors[i];
             VTQ_REFUSE(!std::isfinite(d) || d <= 0.0, VTQ_E_INVALID_ARGUMENT, "vtq: rope factors must be positive");
             f /= d;
         }
-        double keep = 1.0;  // the share of the unscaled frequency
-        if (p->scaling == VTQ_ROPE_SCALE_LINEAR) keep = 0.0;
-        else if (bands) keep = (p->original_context * f / two_pi - low) / (high - low);
-        else if (ramp) keep = 1.0 - (i - first) / std::fmax(last - first, 0.001);
-        keep = std::fmin(1.0, std::fmax(0.0, keep));
-        if (keep < 1.0) f = keep * f + (1.0 - keep) * f / p->factor;
+        long double keep = 1.0L;  // the share of the unscaled frequency
+        if (p->scaling == VTQ_ROPE_SCALE_LINEAR) keep = 0.0L;
+        else if (bands) keep = (p->original_context * f / full - low) / ((long double)high - low);
+        else if (ramp) keep = 1.0L - (i - (long double)first) / std::fmax(last - first, 0.001);
+        keep = std::fmin(1.0L, std::fmax(0.0L, keep));
+        if (keep < 1.0L) f = keep * f + (1.0L - keep) * f / p->factor;
         // f <= 1 radian a position unless a factor below 1 says otherwise; whole turns do not count
-        const double turns = f / two_pi;
-        VTQ_REFUSE(!(turns < 1048576.0), VTQ_E_INVALID_ARGUMENT, "vtq: rope frequency too large");
-        r.turns[i] = (uint64_t)((turns - std::floor(turns)) * 18446744073709551616.0);
+        const long double turns = f / full;
+        VTQ_REFUSE(!(turns < 1048576.0L), VTQ_E_INVALID_ARGUMENT, "vtq: rope frequency too large");
+        r.turns[i] = (uint64_t)((turns - std::floor(turns)) * 18446744073709551616.0L);
     }
     r.magnitude = p->magnitude != 0.0                           ? (float)p->magnitude
                   : p->scaling == VTQ_ROPE_SCALE_YARN ? (float)(0.1 * std::log(p->factor) + 1.0)
