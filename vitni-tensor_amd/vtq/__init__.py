@@ -179,6 +179,17 @@ EXPORTED = (
 )
 
 
+def _fits(lo, hi, **values):
+    """Refuses what a C integer would not hold: ctypes cuts it without a word."""
+    for name, value in values.items():
+        if not lo <= int(value) < hi:
+            raise InvalidArgument(f"vtq: {name} does not fit its C type")
+
+
+def _ints(**values):
+    _fits(-(1 << 31), 1 << 31, **values)
+
+
 class _RopeParams(ctypes.Structure):
     _fields_ = [("layout", ctypes.c_int), ("scaling", ctypes.c_int), ("rot_dim", ctypes.c_int),
                 ("original_context", ctypes.c_int), ("theta", ctypes.c_double), ("factor", ctypes.c_double),
@@ -211,6 +222,7 @@ class Rope:
     def __init__(self, rot_dim, layout=ROPE_HALF, theta=10000.0, scaling=ROPE_SCALE_NONE, factor=1.0,
                  original_context=0, low=0.0, high=0.0, magnitude=0.0, factors=None):
         lib = load_library()
+        _ints(layout=layout, scaling=scaling, rot_dim=rot_dim, original_context=original_context)
         f = None if factors is None else np.ascontiguousarray(factors, dtype=np.float32)
         if f is not None and f.size != int(rot_dim) // 2:
             raise InvalidShape("vtq: one rope factor a pair")
@@ -232,6 +244,8 @@ class KvCache:
         slot = head_dim if slot_stride is None else slot_stride
         head = page_size * slot if head_stride is None else head_stride
         page = kv_heads * head if page_stride is None else page_stride
+        _ints(ggml_type=ggml_type, page_size=page_size, kv_heads=kv_heads, head_dim=head_dim)
+        _fits(0, 1 << 64, n_pages=n_pages, page_stride=page, head_stride=head, slot_stride=slot)
         self.desc = _KvCache(int(ggml_type), page_size, kv_heads, head_dim, n_pages, k_ptr, v_ptr, page, head, slot)
         self.ref = ctypes.byref(self.desc)
 
@@ -241,6 +255,7 @@ class KvBatch:
 
     def __init__(self, batch, q_start_ptr, len_ptr, pages_ptr, max_pages, max_q=1, max_len=0, prefix_len=0,
                  prefix_pages=None):
+        _ints(batch=batch, max_pages=max_pages, max_q=max_q, max_len=max_len, prefix_len=prefix_len)
         self.desc = _KvBatch(batch, max_pages, max_q, max_len, prefix_len, q_start_ptr, len_ptr, pages_ptr,
                              prefix_pages)
         self.ref = ctypes.byref(self.desc)
