@@ -20,11 +20,14 @@
 // read in the order that P has.  V's transpose comes from the LDS transposing read.
 // f32 queries multiply in f32 (32x32x2 MFMAs; 16-bit keys and values widen exactly).
 //
-// bf16, 32 heads on 8 of 128: 64 sequences of up to 512 keys alone 22.7 us, 4.6 TB/s;
-// behind a prefix of 8192 44 us; 128 of up to 1024 behind 32768 137 us, 510 TFLOP/s and
-// 3.9 TB/s at once; that prefix alone 97-102 us, 690 TFLOP/s.  Own keys are bound by
+// bf16, 32 heads on 8 of 128: 64 sequences of up to 512 keys alone 22.8 us, 4.6 TB/s;
+// behind a prefix of 8192 45 us; 128 of up to 1024 behind 32768 138 us, 510 TFLOP/s and
+// 3.9 TB/s at once; that prefix alone 97-103 us, 670-690 TFLOP/s.  Own keys are bound by
 // memory, prefix tiles by one wave's chain of products, exponentials and LDS reads
 // (the matrix cores are busy 28 % of the time; keys from one hot page are 10 % faster).
+// Prompts are far from this: one of 4096 tokens 201 us, 680 TFLOP/s; on 2 KV heads 555,
+// where the row tiles of a KV head stay on one XCD and the others idle.  Heads of 256
+// elements spill in the loops (26 sequences of 7 behind 8099, f16: 120 us, 165 TFLOP/s).
 #include <type_traits>
 
 #include "vtq_attention_plan.h"

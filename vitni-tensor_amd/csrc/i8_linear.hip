@@ -368,7 +368,7 @@ using Tiles256 = Tiles<4, 2, 2, 4, 2, 1>;
 
 // A workgroup owns 32 TM tokens x 32 channels, its 4 waves every fourth 128 bytes of K,
 // each with tiles of its own in LDS, S deep: nothing waits for another wave until the
-// sums are joined.  Bound by the weights: 19 x 11008 -> 4096 12.6 us, 3.6 TB/s.
+// sums are joined.  Bound by the weights: 19 x 11008 -> 4096 12.7 us, 3.6 TB/s.
 template <class O, int TM, int S>
 __global__ __launch_bounds__(256, 1) void i8_slices_kernel(I8Linear a) {
     constexpr int kStage = (TM + 1) * 4096, kLoads = (TM + 1) * 4, BM = 32 * TM;
