@@ -322,7 +322,8 @@ int vtq_kv_append_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_b
  * sequence, KV head and 32 rows of it).
  * d_ws is at least vtq_attention_workspace bytes, 256-byte aligned, for this call
  * alone until its work is done (calls that may overlap need one each); the size
- * depends on the host's numbers only, not on the lengths in device memory. */
+ * depends on the host's numbers only, not on the lengths in device memory.  It is 0
+ * where none is needed, and for numbers that the call refuses. */
 size_t vtq_attention_workspace(const vtq_kv_cache *cache, const vtq_kv_batch *batch, int type, size_t tokens,
                                size_t heads);
 int vtq_attention_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_batch *batch, int type, size_t tokens,

@@ -4,9 +4,10 @@
 // Pair i of a head at position p turns by p * f_i.  f_i is kept as a fraction of
 // a turn in 64 bits, so p * f_i modulo one turn is a 64-bit integer product: it
 // loses nothing, and the fraction's own error (a few 2^-64) is 2^-31 of a turn at
-// position 2^31, where a product in f32 is off by 0.06 rad at position 10^6.  The remainder, within an eighth of a turn of a quarter turn,
-// goes through sine and cosine series in f64 (terms to x^13 and x^14: truncation
-// below 2e-14 and 2e-15 on pi/4), rounded once to f32.
+// position 2^31, where a product in f32 is off by 0.06 rad at position 10^6.  The
+// remainder, within an eighth of a turn of a quarter turn, goes through sine and
+// cosine series in f64 (terms to x^13 and x^14: truncation below 2e-14 and 2e-15 on
+// pi/4), rounded once to f32.
 //
 // The work is a copy: every element is read and written once.  A workgroup
 // takes some heads of one token and computes that token's cosines and sines
