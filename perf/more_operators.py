@@ -221,9 +221,9 @@ def _prepare_batch(case, gen, st):
     else:
         st["q_in"] = _normal(gen, case["dtype"], st["tokens"], case["heads"], d, scale=1.5)
     if own:
+        ctx = _ctx()
         import vtq
 
-        ctx = _ctx()
         st["own_cache"] = vtq.Kv8Cache(st["k_cache"].data_ptr(), st["v_cache"].data_ptr(), st["k_scale"].data_ptr(),
                                        st["v_scale"].data_ptr(), n_pages, page, hkv, d, block=case["block"])
         st["own_batch"] = vtq.KvBatch(case["batch"], st["q_start"].data_ptr(), st["len"].data_ptr(),
@@ -312,9 +312,9 @@ def _prepare_pages(case, gen, st):
     st["copies"] = torch.empty(copies, 3, dtype=torch.int32, device="cuda")
     st["info"] = torch.empty(2, dtype=torch.int32, device="cuda")
     if own:
+        ctx = _ctx()
         import vtq
 
-        ctx = _ctx()
         if case["cache"] == "e4m3":
             st["own_cache"] = vtq.Kv8Cache(st["k_cache"].data_ptr(), st["v_cache"].data_ptr(),
                                            st["k_scale"].data_ptr(), st["v_scale"].data_ptr(), n_pages, page,
