@@ -71,6 +71,7 @@ extern "C" {
 #define VTQ_TYPE_Q4_K 12
 #define VTQ_TYPE_Q6_K 14
 #define VTQ_TYPE_BF16 30 /* activations and caches of the serving operators only */
+#define VTQ_TYPE_E4M3 256 /* 8-bit floats (4 bits exponent, 3 mantissa, no infinities): caches only, no tag of GGUF's */
 
 /* Numerical regime of the Q4_K arm, chosen by a Cargo feature in the
  * reference (src/model/forward_quantized.rs:704-725):
@@ -93,7 +94,8 @@ const char *vtq_last_error(const vtq_ctx *ctx);
  * the ABI of this header and of vtq_runtime.h together; 0.2.0 added the
  * trailing digest_v1 argument of vtqrt_run (a caller built against 0.1.0
  * headers must not load this library); 0.3.0 added vtqrt_set_prompt_mode
- * (no existing signature changed); 0.3.1 added the serving operators. */
+ * (no existing signature changed); 0.3.1 added the serving operators; 0.3.2
+ * those over 8-bit caches, beam selection and the pages' operators. */
 const char *vtq_version(void);
 
 /* ---- host-pointer entry points (synchronous; y is complete on return) ----
@@ -330,6 +332,128 @@ int vtq_attention_device(vtq_ctx *ctx, const vtq_kv_cache *cache, const vtq_kv_b
                          size_t heads, const void *d_q, size_t q_token_stride, size_t q_head_stride, void *d_y,
                          size_t y_token_stride, size_t y_head_stride, float *d_lse, float scale, void *d_ws,
                          size_t ws_bytes, void *stream);
+
+/* A paged KV cache in 8 bits.  cache is as above with type VTQ_TYPE_E4M3, head_dim
+ * and the strides multiples of 16, and page_size at least 16.  An element stands for
+ * its e4m3 value (1 sign, 4 exponent, 3 mantissa bits, bias 7, largest 448, 0x7F and
+ * 0xFF NaN) times its block's scale: `block` tokens (a power of two, 16 to page_size)
+ * of a page and KV head share one, in k and v apart.  A scale is a power of two, held
+ * as a byte b: 2^(b - 127), 10 to 246; other bytes count as the nearest of these.
+ * Block i of page p of head h has its byte at
+ * p * scale_page_stride + h * scale_head_stride + i, in k_scale and v_scale alike. */
+typedef struct {
+    vtq_kv_cache cache;
+    int block, reserved;
+    uint8_t *k_scale, *v_scale;
+    size_t scale_page_stride, scale_head_stride;
+} vtq_kv8_cache;
+
+/* vtq_kv_append_device into an 8-bit cache; type is F32, F16 or BF16.  Of the tokens
+ * that the call writes to a block, e is the least exponent with |x| <= 448 * 2^e for
+ * every finite element x (rotated, in f32), at least -117 and at most 119.  Where the
+ * block holds earlier tokens of the sequence (slots before the call's first), e is at
+ * least their scale's exponent, and if it is above it their elements are divided by the
+ * power of two between (exact, but for those that fall below the smallest normal
+ * value, rounded to the nearest).  The new ones are x / 2^e to the nearest, ties to even (beyond
+ * 448: 448 with the sign); infinities and NaN become NaN.  A token past q_start[batch],
+ * or whose slot does not exist, is not written and has no part in a scale. */
+int vtq_kv8_append_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv_batch *batch, const vtq_rope *rope,
+                          int type, size_t tokens, const void *d_k, size_t k_token_stride, size_t k_head_stride,
+                          const void *d_v, size_t v_token_stride, size_t v_head_stride, size_t heads, const void *d_q,
+                          size_t q_token_stride, size_t q_head_stride, void *d_q_out, size_t q_out_token_stride,
+                          size_t q_out_head_stride, void *stream);
+
+/* vtq_attention_device over an 8-bit cache: its formulas, masks, limits and workspace
+ * rules.  type, the queries' and y's, is F32, F16 or BF16.  Keys and values enter the
+ * products as the numbers they stand for.  BF16 queries multiply as they are, F16
+ * ones as the exact sum of two bf16 parts and F32 ones of three; weights are rounded
+ * to as many: off by 2^-8, 2^-16 and 2^-24 of themselves at most. */
+size_t vtq_kv8_attention_workspace(const vtq_kv8_cache *cache, const vtq_kv_batch *batch, int type, size_t tokens,
+                                   size_t heads);
+int vtq_kv8_attention_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv_batch *batch, int type,
+                             size_t tokens, size_t heads, const void *d_q, size_t q_token_stride, size_t q_head_stride,
+                             void *d_y, size_t y_token_stride, size_t y_head_stride, float *d_lse, float scale,
+                             void *d_ws, size_t ws_bytes, void *stream);
+
+/* ---- choosing tokens and moving a cache's pages ----
+ * Same rules as the operators above.  Which sequence goes on where is decided by
+ * lists in device memory, so that a step with a selection, the tables of the next
+ * batch and the copies that these take may stand in one captured graph. */
+
+/* The best continuations of beams.  groups x beams rows of `vocab` logits (rows ld
+ * apart), each with the sum so far of its beam, score[row] (f32).  A candidate is a
+ * token of a row, worth score + logit - ln sum exp(logits of the row), worked out in
+ * f64.  The n_out greatest of a group come out in falling order, equal ones by falling
+ * logit and then by rising (beam, token): out_score (f32), out_token and out_parent
+ * (the row, counted over all groups), each groups x n_out.  A row whose score or sum
+ * is not finite (a NaN or +infinity among the logits, or -infinity alone) has all its
+ * candidates at -infinity, equal ones.  done (NULL: none) marks rows that ended: such a
+ * row is one candidate, end_token, worth its score alone (its logit counting as 0), and
+ * its logits are not read.  out_done (may be NULL) is 1 where the parent was done or
+ * the token is end_token (where that is negative, which is no token, only for done
+ * parents).  Where a group has fewer candidates than n_out, the rest are -infinity with
+ * token and parent -1 and done 1.  n_out and beams are 1 to 64, vocab 1 to 2^20, groups
+ * x beams at most 2^20.  Where n_out is beams, out_score may be score and out_done done.
+ * d_ws as in attention. */
+size_t vtq_beam_select_workspace(size_t groups, size_t beams, size_t vocab, size_t n_out);
+int vtq_beam_select_device(vtq_ctx *ctx, int type, const void *d_logits, size_t ld, size_t groups, size_t beams,
+                           size_t vocab, const float *d_score, const uint8_t *d_done, int end_token, size_t n_out,
+                           float *d_out_score, int32_t *d_out_token, int32_t *d_out_parent, uint8_t *d_out_done,
+                           void *d_ws, size_t ws_bytes, void *stream);
+
+/* Who holds a cache's pages: refs[page] (int32, n_pages) counts the holders; a page of
+ * count 0 is free.  A sequence holds the pages that its row of a table (max_pages
+ * numbers) names; numbers outside 0 to n_pages - 1 hold nothing.  The pages of a
+ * prefix, or others that a program keeps for itself, have a count that it set.
+ *
+ * The table of the next batch: sequence i goes on where sequence parent[i] of the old
+ * one stands (any number outside 0 to batch - 1: as an empty one) and gets pages for
+ * grow[i] more tokens (NULL, or below 0: for none).  A parent may have several children
+ * (a fork) or none (its pages lose a holder).  Children share the pages that the
+ * parent's len has filled.  What follows these, a part-filled page first, the first of
+ * the children keeps as far as it needs pages and up to the first that others hold too
+ * or that is none.  All other places take free pages, the lowest numbers first, in the
+ * order of sequences and places; pages that the call frees are taken by a later one at
+ * the earliest.  Where such a page takes a part-filled one's place, that is to be
+ * copied: a row (page, new page, slots in use) of copies, in the order of sequences.
+ * new_refs, new_pages (batch_out x max_pages) and new_len are written beside the old
+ * lists, which stay as they are.  copies is batch_out x 3, rows past the count are -1.
+ * info[0] is the count of copies.  info[1] is how many pages are missing, none being
+ * free or max_pages too few: their places are -1, and a part-filled page among them is not
+ * copied.  Where it is not 0 go on with the old lists.  len counts as between 0 and
+ * max_pages * page_size.  Up to 2^16 sequences. */
+size_t vtq_pages_reorder_workspace(size_t n_pages, size_t batch, size_t batch_out);
+int vtq_pages_reorder_device(vtq_ctx *ctx, size_t n_pages, int page_size, size_t max_pages, const int32_t *d_refs,
+                             size_t batch, const int32_t *d_pages, const int32_t *d_len, size_t batch_out,
+                             const int32_t *d_parent, const int32_t *d_grow, int32_t *d_new_refs, int32_t *d_new_pages,
+                             int32_t *d_new_len, int32_t *d_copies, int32_t *d_info, void *d_ws, size_t ws_bytes,
+                             void *stream);
+
+/* The n pages in use (of a count above 0) closed up to the numbers 0 to n - 1: the i-th
+ * of those from n on goes to the i-th that is not in use below n.  copies (n_pages / 2 x
+ * 3) gets a row (page, new page, page_size) of each, rows past the count are -1; info[0]
+ * is the count, info[1] n.  new_refs are the counts at the new numbers, 0 from n on.
+ * new_pages are the n_entries numbers of pages (a table), and new_prefix_pages the
+ * n_prefix of prefix_pages (n_prefix may be 0), as they are now; numbers that are no
+ * page become -1. */
+size_t vtq_pages_compact_workspace(size_t n_pages);
+int vtq_pages_compact_device(vtq_ctx *ctx, size_t n_pages, int page_size, const int32_t *d_refs, size_t n_entries,
+                             const int32_t *d_pages, size_t n_prefix, const int32_t *d_prefix_pages,
+                             int32_t *d_new_refs, int32_t *d_new_pages, int32_t *d_new_prefix_pages, int32_t *d_copies,
+                             int32_t *d_info, void *d_ws, size_t ws_bytes, void *stream);
+
+/* Copies the first slots of pages, keys and values of every head, and for an 8-bit cache
+ * the scales of the blocks that they lie in, on each of `layers` layers: caches of one
+ * layout, layer_stride elements (scales scale_layer_stride bytes) apart; the struct has
+ * the first one's addresses.  count (device memory) is how many rows of copies are
+ * valid, up to max_copies; NULL: all.  Rows whose pages are outside the cache are passed
+ * over; slots count as between 0 and page_size.  A page that is copied to must not occur
+ * again: the lists of the calls above are such. */
+int vtq_pages_copy_device(vtq_ctx *ctx, const vtq_kv_cache *cache, size_t layers, size_t layer_stride,
+                          const int32_t *d_copies, size_t max_copies, const int32_t *d_count, void *stream);
+int vtq_kv8_pages_copy_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, size_t layers, size_t layer_stride,
+                              size_t scale_layer_stride, const int32_t *d_copies, size_t max_copies,
+                              const int32_t *d_count, void *stream);
 
 #ifdef __cplusplus
 }

@@ -15,121 +15,22 @@
 // f32 tokens of 48 heads of 80, appended as f16: 33.6 us, 4.1 TB/s; 8 tokens of
 // 36 heads 2.8 us and 32 appended ones 3.6 us inside a graph, a launch's own
 // time.
-#include <algorithm>
-#include <type_traits>
-
-#include "vtq_device.h"
-#include "vtq_serve.h"
+#include "vtq_rope.h"
 
 namespace vtq {
 namespace {
-
-__device__ __forceinline__ float2 turn_cos_sin(uint64_t t) {
-    const uint64_t quarter = (t + (1ull << 61)) >> 62;  // nearest, 0..3 (4 wraps to 0)
-    const double x = (double)(int64_t)(t - (quarter << 62)) * (6.283185307179586476925286766559 / 18446744073709551616.0);
-    const double z = x * x;
-    double s = 1.0 / 6227020800.0;
-    s = fma(s, z, -1.0 / 39916800.0);
-    s = fma(s, z, 1.0 / 362880.0);
-    s = fma(s, z, -1.0 / 5040.0);
-    s = fma(s, z, 1.0 / 120.0);
-    s = fma(s, z, -1.0 / 6.0);
-    s = fma(s * z, x, x);
-    double c = -1.0 / 87178291200.0;
-    c = fma(c, z, 1.0 / 479001600.0);
-    c = fma(c, z, -1.0 / 3628800.0);
-    c = fma(c, z, 1.0 / 40320.0);
-    c = fma(c, z, -1.0 / 720.0);
-    c = fma(c, z, 1.0 / 24.0);
-    c = fma(c, z, -0.5);
-    c = fma(c, z, 1.0);
-    const float cf = (float)((quarter & 1) ? s : c), sf = (float)((quarter & 1) ? c : s);
-    // quarter 0: (c, s), 1: (-s, c), 2: (-c, -s), 3: (s, -c)
-    return make_float2(quarter == 1 || quarter == 2 ? -cf : cf, quarter >= 2 ? -sf : sf);
-}
-
-template <class T, int N>
-struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
-    T v[N];
-};
-
-template <class T, class O, int N>
-__device__ __forceinline__ void put(O* dst, const float (&f)[N]) {
-    Pack<O, N> o;
-#pragma unroll
-    for (int i = 0; i < N; i++) o.v[i] = (O)f[i];
-    *reinterpret_cast<Pack<O, N>*>(dst) = o;
-}
-
-// One unit of a head: N elements of each half of the pairs (HALF), N elements of
-// whole pairs, or N elements that do not rotate.  cs: cosine and sine a pair.
-template <class T, class O, int N>
-__device__ __forceinline__ void rotate_unit(const T* src, O* dst, const float2* cs, int unit, int rot, bool half) {
-    if (half && rot) {
-        const int per = rot / 2 / N;
-        if (unit < per) {
-            const int i = unit * N;
-            const Pack<T, N> a = *reinterpret_cast<const Pack<T, N>*>(src + i);
-            const Pack<T, N> b = *reinterpret_cast<const Pack<T, N>*>(src + rot / 2 + i);
-            float x[N], y[N];
-#pragma unroll
-            for (int k = 0; k < N; k++) {
-                const float2 w = cs[i + k];
-                x[k] = (float)a.v[k] * w.x - (float)b.v[k] * w.y;
-                y[k] = (float)a.v[k] * w.y + (float)b.v[k] * w.x;
-            }
-            put<T, O, N>(dst + i, x);
-            put<T, O, N>(dst + rot / 2 + i, y);
-            return;
-        }
-        unit += per;  // the units past the rotated ones
-    }
-    if (N == 1 && !half) {  // both elements of a pair, one at a time
-        if (unit < rot / 2) {
-            const float2 w = cs[unit];
-            const float a = (float)src[2 * unit], b = (float)src[2 * unit + 1];
-            dst[2 * unit] = (O)(a * w.x - b * w.y);
-            dst[2 * unit + 1] = (O)(a * w.y + b * w.x);
-            return;
-        }
-        unit += rot / 2;
-    }
-    const int i = unit * N;
-    const Pack<T, N> a = *reinterpret_cast<const Pack<T, N>*>(src + i);
-    float x[N];
-#pragma unroll
-    for (int k = 0; k < N; k++) x[k] = (float)a.v[k];
-    if constexpr (N > 1) {
-        if (!half && i < rot) {
-#pragma unroll
-            for (int k = 0; k < N; k += 2) {
-                const float2 w = cs[(i + k) / 2];
-                const float p = x[k] * w.x - x[k + 1] * w.y, q = x[k] * w.y + x[k + 1] * w.x;
-                x[k] = p, x[k + 1] = q;
-            }
-        }
-    }
-    put<T, O, N>(dst + i, x);
-}
-
-constexpr int kRopeThreads = 256;
 
 // Workgroup (token, group of heads): heads 0..x_heads-1 are x, then the keys, then
 // the values.  N elements to a thread's access; N = 1 takes any alignment.
 template <class T, class C, int N>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeJob j, int heads_per_group) {
     const int64_t t = (int64_t)blockIdx.x;
-    const int lane = threadIdx.x & 63;
     int64_t pos, place = 0;
     int seq = 0;
     if (j.pos) {
         pos = j.pos[t];
     } else {
-        // the sequence whose end is the first one past t; every wave finds it for itself
-        for (int b = 0; b < j.batch.batch; b += 64) {
-            const bool before = b + lane < j.batch.batch && j.batch.q_start[b + lane + 1] <= t;
-            seq += __popcll(__ballot(before));
-        }
+        seq = sequence_of(j.batch, t);
         if (seq >= j.batch.batch) return;
         // the newest token of the sequence is the one before its end
         place = (int64_t)j.batch.len[seq] - (j.batch.q_start[seq + 1] - t);
@@ -148,8 +49,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeJob j, int heads
     const bool half = j.rope.layout == VTQ_ROPE_HALF;
     const int all = j.x_heads + 2 * j.kv_heads;
     const int h0 = (int)blockIdx.y * heads_per_group, h1 = min(all, h0 + heads_per_group);
-    const int rot_units = half || N == 1 ? rot / 2 / N : rot / N;
-    const int units_rot = rot_units + (j.head_dim - rot) / N, units_plain = j.head_dim / N;
+    const int units_rot = rotated_units(j.head_dim, rot, half, N), units_plain = j.head_dim / N;
     const int most = units_plain;
     for (int w = threadIdx.x; w < (h1 - h0) * most; w += kRopeThreads) {
         const int h = h0 + w / most, u = w % most;
@@ -169,29 +69,11 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeJob j, int heads
     }
 }
 
-bool rows_aligned(const void* p, int64_t ts, int64_t hs, size_t bytes, size_t elem) {
-    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ts * elem % bytes == 0 && hs * elem % bytes == 0;
-}
-
 }  // namespace
 
 hipError_t launch_rope(const RopeJob& j, int type, int cache_type, hipStream_t stream) {
     const size_t es = type_bytes(type);
-    const int rot = j.rotate ? j.rope.rot_dim : 0;
-    const bool half = j.rope.layout == VTQ_ROPE_HALF;
-    // N elements to an access: the most that the alignment of every row and the
-    // places where the rotation starts and ends allow
-    auto fits = [&](int n) {
-        const size_t bytes = std::min<size_t>(es * n, 16);
-        if (j.head_dim % n || rot % n || (half && rot / 2 % n)) return false;
-        if (j.x_heads && (!rows_aligned(j.x.p, j.x.token_stride, j.x.head_stride, bytes, es) ||
-                          !rows_aligned(j.y, j.y_token_stride, j.y_head_stride, bytes, es)))
-            return false;
-        return !j.kv_heads || (rows_aligned(j.k.p, j.k.token_stride, j.k.head_stride, bytes, es) &&
-                               rows_aligned(j.v.p, j.v.token_stride, j.v.head_stride, bytes, es));
-    };
-    // (f32 by 8, two 16-byte accesses, or by 4)
-    const int n = fits(8) ? 8 : es == 4 && fits(4) ? 4 : 1;
+    const int n = rope_access(j, es);
     const int all = j.x_heads + 2 * j.kv_heads;
     // a workgroup a token, more where that leaves the chip idle
     const int64_t units = (int64_t)all * (j.head_dim / n);

@@ -37,11 +37,25 @@ inline int attention_waves(int cache_type, int head_dim) {
     return 32 * d * (int)type_bytes(cache_type) > 16384 ? 2 : 4;
 }
 
+// What the split asks of a kernel.
+struct TileCost {
+    int waves;     // of a workgroup
+    bool f32;      // products in f32
+    bool slow;     // tiles that take long: parts of less than four
+    double tile;   // 32 keys against 32 rows, us
+};
+
+inline TileCost attention_cost(int type, int cache_type, int head_dim) {
+    const int d = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    return {attention_waves(cache_type, head_dim), type == VTQ_TYPE_F32, type == VTQ_TYPE_F32 || d > 128,
+            type == VTQ_TYPE_F32 ? 3.6 * d / 128 : d > 128 ? 2.4 : 0.18 + 0.0025 * d};
+}
+
 // The arguments are what the checks let through: tokens, heads and batch above 0.
-inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens,
-                                    int heads) {
+inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batch& batch, const TileCost& cost,
+                                    int64_t tokens, int heads) {
     AttentionPlan p{};
-    const int W = attention_waves(cache.type, cache.head_dim);
+    const int W = cost.waves;
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     const int64_t slots = 512;
     p.group = heads / cache.kv_heads;
@@ -56,14 +70,12 @@ inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batc
     const int64_t len = batch.max_len ? std::min<int64_t>(batch.max_len, most) : most;
     p.own_rows = (int)up(own_rows, p.shared_own ? 32 * W : 32);
     const int64_t own_units = (int64_t)cache.kv_heads * p.own_rows * batch.batch;
-    const int d = cache.head_dim <= 64 ? 64 : cache.head_dim <= 128 ? 128 : 256;
-    const bool slow = type == VTQ_TYPE_F32 || d > 128;  // tiles that take long: parts of less than four
+    const bool slow = cost.slow;
     const int grain = slow ? 32 : 128;
     p.own_grain = p.shared_own ? grain : 128;
     auto least_keys = [&](int64_t keys) {
-        const double tile = type == VTQ_TYPE_F32 ? 3.6 * d / 128 : d > 128 ? 2.4 : 0.18 + 0.0025 * d;
         const double part = 0.08 + 2.3e-6 * (double)(tokens * heads * cache.head_dim);
-        return (1 + (int64_t)std::sqrt(32.0 * keys * part / tile) / grain) * grain;
+        return (1 + (int64_t)std::sqrt(32.0 * keys * part / cost.tile) / grain) * grain;
     };
     if (batch.prefix_len) {
         p.prefix_rows = (int)up(prefix_rows, p.shared_prefix ? 32 * W : 32);
@@ -84,7 +96,7 @@ inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batc
         int64_t least;
         if (p.shared_prefix) {
             least = least_keys(batch.prefix_len);
-            if (type == VTQ_TYPE_F32 && units * up(batch.prefix_len, least) + own_units > slots / 2)
+            if (cost.f32 && units * up(batch.prefix_len, least) + own_units > slots / 2)
                 least = std::max<int64_t>(least, 256);
         } else {
             least = std::min<int64_t>(512, up(prefix_keys, 192 * 128) * 128);
@@ -104,6 +116,22 @@ inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batc
     p.prefix_per_xcd = (int)up((int64_t)cache.kv_heads * p.prefix_splits, 8) * p.prefix_rows;
     p.own_per_xcd = (int)(up((int64_t)cache.kv_heads * p.own_splits * batch.batch, 8) * p.own_rows);
     return p;
+}
+
+inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens,
+                                    int heads) {
+    return plan_attention(cache, batch, attention_cost(type, cache.type, cache.head_dim), tokens, heads);
+}
+
+// Over 8-bit caches: products of one, two or three 16-bit parts.
+inline TileCost kv8_attention_cost(int type, int head_dim) {
+    const int d = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    const int parts = type == VTQ_TYPE_F32 ? 3 : type == VTQ_TYPE_F16 ? 2 : 1;
+    return {4, false, d > 128, (0.18 + 0.0025 * d) * (1 + parts) / 2};
+}
+inline AttentionPlan plan_kv8_attention(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens,
+                                        int heads) {
+    return plan_attention(cache, batch, kv8_attention_cost(type, cache.head_dim), tokens, heads);
 }
 
 }  // namespace vtq

@@ -121,6 +121,53 @@ int vtqp_check_attention(const char** text, const vtq_kv_cache* cache, const vtq
                                      y_token_stride, y_head_stride, d_lse, scale), text);
 }
 
+int vtqp_check_kv8_append(const char** text, const vtq_kv8_cache* cache, const vtq_kv_batch* batch,
+                          const vtq_rope* rope, int type, size_t tokens, const void* d_k, size_t k_token_stride,
+                          size_t k_head_stride, const void* d_v, size_t v_token_stride, size_t v_head_stride,
+                          size_t heads, const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_q_out,
+                          size_t q_out_token_stride, size_t q_out_head_stride) {
+    return told(vtq::check_kv8_append(cache, batch, rope, type, tokens, d_k, k_token_stride, k_head_stride, d_v,
+                                      v_token_stride, v_head_stride, heads, d_q, q_token_stride, q_head_stride, d_q_out,
+                                      q_out_token_stride, q_out_head_stride), text);
+}
+int vtqp_check_kv8_attention(const char** text, const vtq_kv8_cache* cache, const vtq_kv_batch* batch, int type,
+                             size_t tokens, size_t heads, const void* d_q, size_t q_token_stride,
+                             size_t q_head_stride, void* d_y, size_t y_token_stride, size_t y_head_stride,
+                             float* d_lse, float scale) {
+    return told(vtq::check_kv8_attention(cache, batch, type, tokens, heads, d_q, q_token_stride, q_head_stride, d_y,
+                                         y_token_stride, y_head_stride, d_lse, scale), text);
+}
+int vtqp_check_beam_select(const char** text, int type, const void* d_logits, size_t ld, size_t groups, size_t beams,
+                           size_t vocab, const float* d_score, const uint8_t* d_done, int end_token, size_t n_out,
+                           float* d_out_score, int32_t* d_out_token, int32_t* d_out_parent, uint8_t* d_out_done) {
+    return told(vtq::check_beam_select(type, d_logits, ld, groups, beams, vocab, d_score, d_done, end_token, n_out,
+                                       d_out_score, d_out_token, d_out_parent, d_out_done), text);
+}
+int vtqp_check_pages_reorder(const char** text, size_t n_pages, int page_size, size_t max_pages, const int32_t* d_refs,
+                             size_t batch, const int32_t* d_pages, const int32_t* d_len, size_t batch_out,
+                             const int32_t* d_parent, const int32_t* d_grow, int32_t* d_new_refs, int32_t* d_new_pages,
+                             int32_t* d_new_len, int32_t* d_copies, int32_t* d_info) {
+    return told(vtq::check_pages_reorder(n_pages, page_size, max_pages, d_refs, batch, d_pages, d_len, batch_out,
+                                         d_parent, d_grow, d_new_refs, d_new_pages, d_new_len, d_copies, d_info), text);
+}
+int vtqp_check_pages_compact(const char** text, size_t n_pages, int page_size, const int32_t* d_refs, size_t n_entries,
+                             const int32_t* d_pages, size_t n_prefix, const int32_t* d_prefix_pages,
+                             int32_t* d_new_refs, int32_t* d_new_pages, int32_t* d_new_prefix_pages, int32_t* d_copies,
+                             int32_t* d_info) {
+    return told(vtq::check_pages_compact(n_pages, page_size, d_refs, n_entries, d_pages, n_prefix, d_prefix_pages,
+                                         d_new_refs, d_new_pages, d_new_prefix_pages, d_copies, d_info), text);
+}
+int vtqp_check_pages_copy(const char** text, const vtq_kv_cache* cache, size_t layers, size_t layer_stride,
+                          const int32_t* d_copies, size_t max_copies, const int32_t* d_count) {
+    return told(vtq::check_pages_copy(cache, layers, layer_stride, d_copies, max_copies, d_count), text);
+}
+int vtqp_check_kv8_pages_copy(const char** text, const vtq_kv8_cache* cache, size_t layers, size_t layer_stride,
+                              size_t scale_layer_stride, const int32_t* d_copies, size_t max_copies,
+                              const int32_t* d_count) {
+    return told(vtq::check_kv8_pages_copy(cache, layers, layer_stride, scale_layer_stride, d_copies, max_copies,
+                                          d_count), text);
+}
+
 // How an attention call that is not refused is split: AttentionPlan, 12 numbers in its
 // order (vtq_attention_plan.h), and keys to each own range of a sequence of `keys`.
 int vtqp_attention_plan(const vtq_kv_cache* cache, const vtq_kv_batch* batch, int type, size_t tokens, size_t heads,

@@ -79,7 +79,64 @@ struct Attention {
     float scale;
     void* ws;
 };
+// Scales of an 8-bit cache.
+struct Scales {
+    int block;
+    uint8_t *k, *v;
+    int64_t page_stride, head_stride;
+};
+
+// The same append into an 8-bit cache.
+hipError_t launch_kv8_append(const RopeJob& j, const Scales& s, int type, hipStream_t stream);
+
 size_t attention_workspace(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens, int heads);
 hipError_t launch_attention(const Attention& a, int type, hipStream_t stream);
+size_t kv8_attention_workspace(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens, int heads);
+hipError_t launch_kv8_attention(const Attention& a, const Scales& s, int type, hipStream_t stream);
+
+struct BeamSelect {
+    const void* logits;
+    int64_t ld;
+    int groups, beams, vocab, n_out, end_token;
+    const float* score;
+    const uint8_t* done;
+    float* out_score;
+    int32_t *out_token, *out_parent;
+    uint8_t* out_done;
+    void* ws;
+};
+size_t beam_select_workspace(int64_t groups, int64_t beams, int64_t vocab, int64_t n_out);
+hipError_t launch_beam_select(const BeamSelect& a, int type, hipStream_t stream);
+
+struct PagesReorder {
+    int64_t n_pages;
+    int page_size, max_pages, batch, batch_out;
+    const int32_t *refs, *pages, *len, *parent, *grow;
+    int32_t *new_refs, *new_pages, *new_len, *copies, *info;
+    void* ws;
+};
+size_t pages_reorder_workspace(int64_t n_pages, int64_t batch_out);
+hipError_t launch_pages_reorder(const PagesReorder& a, hipStream_t stream);
+
+struct PagesCompact {
+    int64_t n_pages;
+    int page_size;
+    int64_t n_entries, n_prefix;
+    const int32_t *refs, *pages, *prefix_pages;
+    int32_t *new_refs, *new_pages, *new_prefix_pages, *copies, *info;
+    void* ws;
+};
+size_t pages_compact_workspace(int64_t n_pages);
+hipError_t launch_pages_compact(const PagesCompact& a, hipStream_t stream);
+
+struct PagesCopy {
+    vtq_kv_cache cache;
+    Scales scales;  // k null: none
+    int layers;
+    int64_t layer_stride, scale_layer_stride;
+    const int32_t *copies, *count;
+    int64_t max_copies;
+};
+hipError_t launch_pages_copy(const PagesCopy& a, hipStream_t stream);
 
 }  // namespace vtq

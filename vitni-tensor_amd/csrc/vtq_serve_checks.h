@@ -37,8 +37,7 @@ inline Refusal check_rope(const vtq_rope* r) {
     return {};
 }
 
-inline Refusal check_cache(const vtq_kv_cache* c) {
-    VTQ_REFUSE(type_bytes(c->type) == 0, VTQ_E_NOT_IMPLEMENTED, "vtq: cache type not F32 / F16 / BF16");
+inline Refusal check_cache_layout(const vtq_kv_cache* c) {
     VTQ_REFUSE(c->page_size < 8 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)), VTQ_E_INVALID_SHAPE,
                "vtq: page_size must be a power of two, 8 to 4096");
     VTQ_REFUSE(c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8, VTQ_E_INVALID_SHAPE,
@@ -58,6 +57,30 @@ inline Refusal check_cache(const vtq_kv_cache* c) {
     VTQ_REFUSE(c->n_pages && (!c->k || !c->v), VTQ_E_INVALID_ARGUMENT, "vtq: null cache");
     VTQ_REFUSE(!aligned(c->k, 16) || !aligned(c->v, 16), VTQ_E_INVALID_ARGUMENT,
                "vtq: the cache must be 16-byte aligned");
+    return {};
+}
+
+inline Refusal check_cache(const vtq_kv_cache* c) {
+    VTQ_REFUSE(type_bytes(c->type) == 0, VTQ_E_NOT_IMPLEMENTED, "vtq: cache type not F32 / F16 / BF16");
+    return check_cache_layout(c);
+}
+
+inline Refusal check_cache8(const vtq_kv8_cache* c) {
+    VTQ_REFUSE(c->cache.type != VTQ_TYPE_E4M3, VTQ_E_NOT_IMPLEMENTED, "vtq: the type of an 8-bit cache is E4M3");
+    if (Refusal r = check_cache_layout(&c->cache)) return r;
+    const vtq_kv_cache& b = c->cache;
+    VTQ_REFUSE(b.page_size < 16, VTQ_E_INVALID_SHAPE, "vtq: pages of an 8-bit cache hold at least 16 tokens");
+    VTQ_REFUSE(b.head_dim % 16 || b.page_stride % 16 || b.head_stride % 16 || b.slot_stride % 16, VTQ_E_INVALID_SHAPE,
+               "vtq: head_dim and strides of an 8-bit cache must be multiples of 16");
+    VTQ_REFUSE(c->block < 16 || c->block > b.page_size || (c->block & (c->block - 1)), VTQ_E_INVALID_SHAPE,
+               "vtq: tokens to a scale must be a power of two, 16 to page_size");
+    const size_t blocks = (size_t)(b.page_size / c->block);
+    VTQ_REFUSE((b.kv_heads > 1 && c->scale_head_stride < blocks) || (b.n_pages > 1 && c->scale_page_stride < blocks),
+               VTQ_E_INVALID_SHAPE, "vtq: scale strides below the blocks of a page");
+    VTQ_REFUSE(c->scale_page_stride >= kMostStride / 4 || c->scale_head_stride >= kMostStride / 4 ||
+                   b.n_pages * c->scale_page_stride > (size_t)1 << 46,
+               VTQ_E_NOT_IMPLEMENTED, "vtq: scale stride too large");
+    VTQ_REFUSE(b.n_pages && (!c->k_scale || !c->v_scale), VTQ_E_INVALID_ARGUMENT, "vtq: null scales");
     return {};
 }
 
@@ -207,18 +230,15 @@ inline Refusal check_rope_call(const vtq_rope* rope, int type, const void* d_x, 
     return {};
 }
 
-inline Refusal check_append(const vtq_kv_cache* cache, const vtq_kv_batch* batch, const vtq_rope* rope, int type,
+// What an append's arguments have to be with a cache of any type.
+inline Refusal check_append_rows(const vtq_kv_cache* cache, const vtq_kv_batch* batch, const vtq_rope* rope, int type,
                             size_t tokens, const void* d_k, size_t k_token_stride, size_t k_head_stride,
                                     const void* d_v, size_t v_token_stride, size_t v_head_stride, size_t heads,
                                             const void* d_q, size_t q_token_stride, size_t q_head_stride,
                                                     void* d_q_out, size_t q_out_token_stride,
                                                             size_t q_out_head_stride) {
-    VTQ_REFUSE(!cache || !batch, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
-    if (Refusal r = check_cache(cache)) return r;
     if (Refusal r = check_batch(batch, cache, false)) return r;
     VTQ_REFUSE(type_bytes(type) == 0, VTQ_E_NOT_IMPLEMENTED, "vtq: activation type not F32 / F16 / BF16");
-    VTQ_REFUSE(type != VTQ_TYPE_F32 && type != cache->type, VTQ_E_NOT_IMPLEMENTED,
-               "vtq: activations are F32 or of the cache's type");
     VTQ_REFUSE(tokens > kMostTokens || heads > 65535, VTQ_E_NOT_IMPLEMENTED, "vtq: too many tokens or heads");
     if (rope) {
         if (Refusal r = check_rope(rope)) return r;
@@ -238,14 +258,37 @@ inline Refusal check_append(const vtq_kv_cache* cache, const vtq_kv_batch* batch
     return {};
 }
 
-inline Refusal check_attention(const vtq_kv_cache* cache, const vtq_kv_batch* batch, int type, size_t tokens,
-                               size_t heads, const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_y,
-                                       size_t y_token_stride, size_t y_head_stride, float* d_lse, float scale) {
+inline Refusal check_append(const vtq_kv_cache* cache, const vtq_kv_batch* batch, const vtq_rope* rope, int type,
+                            size_t tokens, const void* d_k, size_t k_token_stride, size_t k_head_stride,
+                            const void* d_v, size_t v_token_stride, size_t v_head_stride, size_t heads,
+                            const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_q_out,
+                            size_t q_out_token_stride, size_t q_out_head_stride) {
     VTQ_REFUSE(!cache || !batch, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
     if (Refusal r = check_cache(cache)) return r;
-    if (Refusal r = check_batch(batch, cache, true)) return r;
-    VTQ_REFUSE(type_bytes(type) == 0 || (type != VTQ_TYPE_F32 && type != cache->type), VTQ_E_NOT_IMPLEMENTED,
+    if (Refusal r = check_batch(batch, cache, false)) return r;
+    VTQ_REFUSE(type_bytes(type) != 0 && type != VTQ_TYPE_F32 && type != cache->type, VTQ_E_NOT_IMPLEMENTED,
                "vtq: activations are F32 or of the cache's type");
+    return check_append_rows(cache, batch, rope, type, tokens, d_k, k_token_stride, k_head_stride, d_v, v_token_stride,
+                             v_head_stride, heads, d_q, q_token_stride, q_head_stride, d_q_out, q_out_token_stride,
+                             q_out_head_stride);
+}
+
+inline Refusal check_kv8_append(const vtq_kv8_cache* cache, const vtq_kv_batch* batch, const vtq_rope* rope, int type,
+                                size_t tokens, const void* d_k, size_t k_token_stride, size_t k_head_stride,
+                                const void* d_v, size_t v_token_stride, size_t v_head_stride, size_t heads,
+                                const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_q_out,
+                                size_t q_out_token_stride, size_t q_out_head_stride) {
+    VTQ_REFUSE(!cache || !batch, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    if (Refusal r = check_cache8(cache)) return r;
+    return check_append_rows(&cache->cache, batch, rope, type, tokens, d_k, k_token_stride, k_head_stride, d_v,
+                             v_token_stride, v_head_stride, heads, d_q, q_token_stride, q_head_stride, d_q_out,
+                             q_out_token_stride, q_out_head_stride);
+}
+
+// What attention's arguments have to be with a cache of any type.
+inline Refusal check_attention_rows(const vtq_kv_cache* cache, const vtq_kv_batch* batch, int type, size_t tokens,
+                               size_t heads, const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_y,
+                                       size_t y_token_stride, size_t y_head_stride, float* d_lse, float scale) {
     VTQ_REFUSE(tokens > kMostTokens || heads > 65535, VTQ_E_NOT_IMPLEMENTED, "vtq: too many tokens or heads");
     VTQ_REFUSE(heads % cache->kv_heads, VTQ_E_INVALID_SHAPE, "vtq: heads must be a multiple of kv_heads");
     VTQ_REFUSE(!attention_fits(cache, batch, tokens, heads), VTQ_E_NOT_IMPLEMENTED, "vtq: more than 2^25 rows of queries");
@@ -260,6 +303,141 @@ inline Refusal check_attention(const vtq_kv_cache* cache, const vtq_kv_batch* ba
     VTQ_REFUSE(d_q == d_y && (q_token_stride != y_token_stride || q_head_stride != y_head_stride),
                VTQ_E_INVALID_SHAPE, "vtq: attention in place keeps its strides");
     VTQ_REFUSE(d_lse && !aligned(d_lse, 4), VTQ_E_INVALID_ARGUMENT, "vtq: lse not aligned to its type");
+    return {};
+}
+
+inline Refusal check_attention(const vtq_kv_cache* cache, const vtq_kv_batch* batch, int type, size_t tokens,
+                               size_t heads, const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_y,
+                               size_t y_token_stride, size_t y_head_stride, float* d_lse, float scale) {
+    VTQ_REFUSE(!cache || !batch, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    if (Refusal r = check_cache(cache)) return r;
+    if (Refusal r = check_batch(batch, cache, true)) return r;
+    VTQ_REFUSE(type_bytes(type) == 0 || (type != VTQ_TYPE_F32 && type != cache->type), VTQ_E_NOT_IMPLEMENTED,
+               "vtq: activations are F32 or of the cache's type");
+    return check_attention_rows(cache, batch, type, tokens, heads, d_q, q_token_stride, q_head_stride, d_y,
+                                y_token_stride, y_head_stride, d_lse, scale);
+}
+
+inline Refusal check_kv8_attention(const vtq_kv8_cache* cache, const vtq_kv_batch* batch, int type, size_t tokens,
+                                   size_t heads, const void* d_q, size_t q_token_stride, size_t q_head_stride,
+                                   void* d_y, size_t y_token_stride, size_t y_head_stride, float* d_lse, float scale) {
+    VTQ_REFUSE(!cache || !batch, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    if (Refusal r = check_cache8(cache)) return r;
+    if (Refusal r = check_batch(batch, &cache->cache, true)) return r;
+    VTQ_REFUSE(type_bytes(type) == 0, VTQ_E_NOT_IMPLEMENTED, "vtq: activation type not F32 / F16 / BF16");
+    return check_attention_rows(&cache->cache, batch, type, tokens, heads, d_q, q_token_stride, q_head_stride, d_y,
+                                y_token_stride, y_head_stride, d_lse, scale);
+}
+
+constexpr size_t kMostKept = 64;  // continuations and beams of a group
+
+inline bool beam_select_fits(size_t groups, size_t beams, size_t vocab, size_t n_out) {
+    return beams <= kMostKept && n_out <= kMostKept && vocab <= (size_t)1 << 20 && groups <= (size_t)1 << 20 &&
+           groups * beams <= (size_t)1 << 20;
+}
+
+inline Refusal check_beam_select(int type, const void* d_logits, size_t ld, size_t groups, size_t beams, size_t vocab,
+                                 const float* d_score, const uint8_t* d_done, int end_token, size_t n_out,
+                                 float* d_out_score, int32_t* d_out_token, int32_t* d_out_parent,
+                                 uint8_t* d_out_done) {
+    VTQ_REFUSE(type_bytes(type) == 0, VTQ_E_NOT_IMPLEMENTED, "vtq: logits type not F32 / F16 / BF16");
+    VTQ_REFUSE(!beam_select_fits(groups, beams, vocab, n_out), VTQ_E_NOT_IMPLEMENTED, "vtq: at most 64 beams and continuations, 2^20 tokens and 2^20 rows");
+    VTQ_REFUSE(beams == 0 || vocab == 0 || n_out == 0, VTQ_E_INVALID_SHAPE, "vtq: no beams, tokens or continuations");
+    VTQ_REFUSE(groups * beams > 1 && ld < vocab, VTQ_E_INVALID_SHAPE, "vtq: rows of logits overlap");
+    VTQ_REFUSE(ld >= kMostStride / 4, VTQ_E_NOT_IMPLEMENTED, "vtq: stride too large");
+    VTQ_REFUSE(end_token >= 0 && (size_t)end_token >= vocab, VTQ_E_INVALID_ARGUMENT, "vtq: end_token outside the vocabulary");
+    if (groups == 0) return {};
+    VTQ_REFUSE(!d_logits || !d_score || !d_out_score || !d_out_token || !d_out_parent, VTQ_E_INVALID_ARGUMENT,
+               "vtq: null pointer");
+    VTQ_REFUSE(!aligned(d_logits, type_bytes(type)) || !aligned(d_score, 4) || !aligned(d_out_score, 4) ||
+                   !aligned(d_out_token, 4) || !aligned(d_out_parent, 4),
+               VTQ_E_INVALID_ARGUMENT, "vtq: pointer not aligned to its type");
+    VTQ_REFUSE(n_out != beams && ((d_done && d_done == d_out_done) || d_score == d_out_score), VTQ_E_INVALID_SHAPE,
+               "vtq: scores and ends are replaced in place only where n_out is beams");
+    return {};
+}
+
+inline Refusal check_pages(size_t n_pages, int page_size, const int32_t* d_refs, const int32_t* d_new_refs,
+                           const int32_t* d_copies, const int32_t* d_info) {
+    VTQ_REFUSE(n_pages > (size_t)INT_MAX, VTQ_E_NOT_IMPLEMENTED, "vtq: page count exceeds INT_MAX");
+    VTQ_REFUSE(page_size < 8 || page_size > 4096 || (page_size & (page_size - 1)), VTQ_E_INVALID_SHAPE,
+               "vtq: page_size must be a power of two, 8 to 4096");
+    VTQ_REFUSE((n_pages && (!d_refs || !d_new_refs)) || !d_info, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    VTQ_REFUSE(!aligned(d_refs, 4) || !aligned(d_new_refs, 4) || !aligned(d_copies, 4) || !aligned(d_info, 4),
+               VTQ_E_INVALID_ARGUMENT, "vtq: list not aligned to its type");
+    VTQ_REFUSE(n_pages && d_refs == d_new_refs, VTQ_E_INVALID_ARGUMENT, "vtq: the new lists stand beside the old ones");
+    return {};
+}
+
+// Each sequence looks through the list of parents.
+constexpr size_t kMostReordered = (size_t)1 << 16;
+
+inline Refusal check_pages_reorder(size_t n_pages, int page_size, size_t max_pages, const int32_t* d_refs, size_t batch,
+                                   const int32_t* d_pages, const int32_t* d_len, size_t batch_out,
+                                   const int32_t* d_parent, const int32_t* d_grow, int32_t* d_new_refs,
+                                   int32_t* d_new_pages, int32_t* d_new_len, int32_t* d_copies, int32_t* d_info) {
+    if (Refusal r = check_pages(n_pages, page_size, d_refs, d_new_refs, d_copies, d_info)) return r;
+    VTQ_REFUSE(batch > kMostReordered || batch_out > kMostReordered, VTQ_E_NOT_IMPLEMENTED,
+               "vtq: more than 2^16 sequences");
+    VTQ_REFUSE(max_pages > (size_t)(INT_MAX / 2) / page_size, VTQ_E_NOT_IMPLEMENTED, "vtq: page table too large");
+    VTQ_REFUSE(batch && ((max_pages && !d_pages) || !d_len), VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    VTQ_REFUSE(batch_out && ((max_pages && !d_new_pages) || !d_new_len || !d_parent || !d_copies),
+               VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    VTQ_REFUSE(!aligned(d_pages, 4) || !aligned(d_len, 4) || !aligned(d_parent, 4) || !aligned(d_grow, 4) ||
+                   !aligned(d_new_pages, 4) || !aligned(d_new_len, 4),
+               VTQ_E_INVALID_ARGUMENT, "vtq: list not aligned to its type");
+    VTQ_REFUSE(batch && batch_out && (d_len == d_new_len || (max_pages && d_pages == d_new_pages)),
+               VTQ_E_INVALID_ARGUMENT, "vtq: the new lists stand beside the old ones");
+    return {};
+}
+
+inline Refusal check_pages_compact(size_t n_pages, int page_size, const int32_t* d_refs, size_t n_entries,
+                                   const int32_t* d_pages, size_t n_prefix, const int32_t* d_prefix_pages,
+                                   int32_t* d_new_refs, int32_t* d_new_pages, int32_t* d_new_prefix_pages,
+                                   int32_t* d_copies, int32_t* d_info) {
+    if (Refusal r = check_pages(n_pages, page_size, d_refs, d_new_refs, d_copies, d_info)) return r;
+    VTQ_REFUSE(n_entries > (size_t)INT_MAX || n_prefix > (size_t)INT_MAX, VTQ_E_NOT_IMPLEMENTED,
+               "vtq: page table too large");
+    VTQ_REFUSE((n_pages > 1 && !d_copies) || (n_entries && (!d_pages || !d_new_pages)) ||
+                   (n_prefix && (!d_prefix_pages || !d_new_prefix_pages)),
+               VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    VTQ_REFUSE(!aligned(d_pages, 4) || !aligned(d_prefix_pages, 4) || !aligned(d_new_pages, 4) ||
+                   !aligned(d_new_prefix_pages, 4),
+               VTQ_E_INVALID_ARGUMENT, "vtq: list not aligned to its type");
+    return {};
+}
+
+inline Refusal check_copies(const vtq_kv_cache* c, size_t layers, size_t layer_stride, const int32_t* d_copies,
+                            size_t max_copies, const int32_t* d_count) {
+    VTQ_REFUSE(layers > 65535 || layers * (size_t)c->kv_heads > (size_t)1 << 24 || max_copies > (size_t)INT_MAX,
+               VTQ_E_NOT_IMPLEMENTED, "vtq: too many layers or copies");
+    VTQ_REFUSE(layer_stride >= kMostStride || layers * (layer_stride / 8) > (size_t)1 << 43, VTQ_E_NOT_IMPLEMENTED,
+               "vtq: layer stride too large");
+    VTQ_REFUSE(layers > 1 && layer_stride == 0, VTQ_E_INVALID_SHAPE, "vtq: layers overlap");
+    VTQ_REFUSE(layer_stride % (c->type == VTQ_TYPE_E4M3 ? 16 : 8), VTQ_E_INVALID_SHAPE,
+               "vtq: the layer stride must be a multiple of 8 elements, of 16 in 8 bits");
+    VTQ_REFUSE(layers && max_copies && !d_copies, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    VTQ_REFUSE(!aligned(d_copies, 4) || !aligned(d_count, 4), VTQ_E_INVALID_ARGUMENT,
+               "vtq: list not aligned to its type");
+    return {};
+}
+
+inline Refusal check_pages_copy(const vtq_kv_cache* cache, size_t layers, size_t layer_stride, const int32_t* d_copies,
+                                size_t max_copies, const int32_t* d_count) {
+    VTQ_REFUSE(!cache, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    if (Refusal r = check_cache(cache)) return r;
+    return check_copies(cache, layers, layer_stride, d_copies, max_copies, d_count);
+}
+
+inline Refusal check_kv8_pages_copy(const vtq_kv8_cache* cache, size_t layers, size_t layer_stride,
+                                    size_t scale_layer_stride, const int32_t* d_copies, size_t max_copies,
+                                    const int32_t* d_count) {
+    VTQ_REFUSE(!cache, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
+    if (Refusal r = check_cache8(cache)) return r;
+    if (Refusal r = check_copies(&cache->cache, layers, layer_stride, d_copies, max_copies, d_count)) return r;
+    VTQ_REFUSE(scale_layer_stride >= kMostStride || layers * scale_layer_stride > (size_t)1 << 46, VTQ_E_NOT_IMPLEMENTED,
+               "vtq: layer stride too large");
+    VTQ_REFUSE(layers > 1 && scale_layer_stride == 0, VTQ_E_INVALID_SHAPE, "vtq: layers overlap");
     return {};
 }
 

@@ -25,8 +25,9 @@ LIB_PATH = os.path.join(LIB_DIR, "libvtq.so")
 # GGUF tensor type tags (src/model/gguf.rs:127-139)
 F32, F16, Q4_0, Q5_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 6, 8, 12, 14
 BF16 = 30  # activations and caches of the serving operators only
+E4M3 = 256  # 8-bit caches only
 TYPE_NAMES = {F32: "F32", F16: "F16", Q4_0: "Q4_0", Q5_0: "Q5_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q6_K: "Q6_K",
-              BF16: "BF16"}
+              BF16: "BF16", E4M3: "E4M3"}
 BLOCK = {Q4_0: (32, 18), Q5_0: (32, 22), Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210)}
 
 REGIME_INTEGER = 0       # std-parallel build: integer Q4_K
@@ -166,6 +167,24 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.vtq_attention_workspace.restype = sz
     lib.vtq_attention_device.argtypes = [vp, vp, vp, i, sz, sz, vp, sz, sz, vp, sz, sz, vp, ctypes.c_float, vp, sz, vp]
     lib.vtq_attention_device.restype = i
+    lib.vtq_kv8_append_device.argtypes = lib.vtq_kv_append_device.argtypes
+    lib.vtq_kv8_attention_workspace.argtypes = lib.vtq_attention_workspace.argtypes
+    lib.vtq_kv8_attention_workspace.restype = sz
+    lib.vtq_kv8_attention_device.argtypes = lib.vtq_attention_device.argtypes
+    lib.vtq_beam_select_workspace.argtypes = [sz, sz, sz, sz]
+    lib.vtq_beam_select_workspace.restype = sz
+    lib.vtq_beam_select_device.argtypes = [vp, i, vp, sz, sz, sz, sz, vp, vp, i, sz, vp, vp, vp, vp, vp, sz, vp]
+    lib.vtq_pages_reorder_workspace.argtypes = [sz, sz, sz]
+    lib.vtq_pages_reorder_workspace.restype = sz
+    lib.vtq_pages_reorder_device.argtypes = [vp, sz, i, sz, vp, sz, vp, vp, sz, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.vtq_pages_compact_workspace.argtypes = [sz]
+    lib.vtq_pages_compact_workspace.restype = sz
+    lib.vtq_pages_compact_device.argtypes = [vp, sz, i, vp, sz, vp, sz, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.vtq_pages_copy_device.argtypes = [vp, vp, sz, sz, vp, sz, vp, vp]
+    lib.vtq_kv8_pages_copy_device.argtypes = [vp, vp, sz, sz, sz, vp, sz, vp, vp]
+    for name in ("kv8_append", "kv8_attention", "beam_select", "pages_reorder", "pages_compact", "pages_copy",
+                 "kv8_pages_copy"):
+        getattr(lib, f"vtq_{name}_device").restype = i
     _lib = lib
     return lib
 
@@ -175,7 +194,10 @@ EXPORTED = (
     "vtq_linear_q4_k_integer", "vtq_linear_q6_k_integer", "vtq_linear_q4_k_fused",
     "vtq_linear_q4_0", "vtq_release_weights", "vtq_linear_device", "vtq_linear_device_noalloc",
     "vtq_quantize_i8_device", "vtq_linear_i8_device", "vtq_rope_plan", "vtq_rope_device", "vtq_kv_append_device",
-    "vtq_attention_workspace", "vtq_attention_device",
+    "vtq_attention_workspace", "vtq_attention_device", "vtq_kv8_append_device", "vtq_kv8_attention_workspace",
+    "vtq_kv8_attention_device", "vtq_beam_select_workspace", "vtq_beam_select_device", "vtq_pages_reorder_workspace",
+    "vtq_pages_reorder_device", "vtq_pages_compact_workspace", "vtq_pages_compact_device", "vtq_pages_copy_device",
+    "vtq_kv8_pages_copy_device",
 )
 
 
@@ -207,6 +229,12 @@ class _KvCache(ctypes.Structure):
                 ("head_dim", ctypes.c_int), ("n_pages", ctypes.c_size_t), ("k", ctypes.c_void_p),
                 ("v", ctypes.c_void_p), ("page_stride", ctypes.c_size_t), ("head_stride", ctypes.c_size_t),
                 ("slot_stride", ctypes.c_size_t)]
+
+
+class _Kv8Cache(ctypes.Structure):
+    _fields_ = [("cache", _KvCache), ("block", ctypes.c_int), ("reserved", ctypes.c_int), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("scale_page_stride", ctypes.c_size_t),
+                ("scale_head_stride", ctypes.c_size_t)]
 
 
 class _KvBatch(ctypes.Structure):
@@ -247,6 +275,23 @@ class KvCache:
         _ints(ggml_type=ggml_type, page_size=page_size, kv_heads=kv_heads, head_dim=head_dim)
         _fits(0, 1 << 64, n_pages=n_pages, page_stride=page, head_stride=head, slot_stride=slot)
         self.desc = _KvCache(int(ggml_type), page_size, kv_heads, head_dim, n_pages, k_ptr, v_ptr, page, head, slot)
+        self.ref = ctypes.byref(self.desc)
+
+
+class Kv8Cache:
+    """A paged KV cache of e4m3 numbers with a power of two to each `block` tokens of a page and head
+    (vtq_kv8_cache); the scales are bytes, pages x kv_heads x (page_size / block), or the given strides.  Holds
+    addresses, not the memory."""
+
+    def __init__(self, k_ptr, v_ptr, k_scale_ptr, v_scale_ptr, n_pages, page_size, kv_heads, head_dim, block=16,
+                 page_stride=None, head_stride=None, slot_stride=None, scale_page_stride=None, scale_head_stride=None):
+        cache = KvCache(E4M3, k_ptr, v_ptr, n_pages, page_size, kv_heads, head_dim, page_stride, head_stride,
+                        slot_stride)
+        _ints(block=block)
+        head = page_size // max(1, block) if scale_head_stride is None else scale_head_stride
+        page = kv_heads * head if scale_page_stride is None else scale_page_stride
+        _fits(0, 1 << 64, scale_head_stride=head, scale_page_stride=page)
+        self.desc = _Kv8Cache(cache.desc, block, 0, k_scale_ptr, v_scale_ptr, page, head)
         self.ref = ctypes.byref(self.desc)
 
 
@@ -416,6 +461,89 @@ class Context:
         rc = self.lib.vtq_attention_device(self.handle, cache.ref, batch.ref, ggml_type, tokens, heads, q_ptr,
                                            q_token_stride, q_head_stride, y_ptr, y_token_stride, y_head_stride, lse_ptr,
                                            scale, ws_ptr, ws_bytes, stream)
+        if rc:
+            self._check(rc)
+
+    # -- the same over 8-bit caches; choosing tokens, and a cache's pages (device pointers) --
+
+    def kv8_append_device(self, cache, batch, rope, ggml_type, tokens, k_ptr, k_token_stride, k_head_stride, v_ptr,
+                          v_token_stride, v_head_stride, stream=None, heads=0, q_ptr=None, q_token_stride=0,
+                          q_head_stride=0, q_out_ptr=None, q_out_token_stride=0, q_out_head_stride=0):
+        """vtq_kv8_append_device: rotated keys and plain values to 8 bits and their slots, rotated queries to q_out."""
+        rc = self.lib.vtq_kv8_append_device(self.handle, cache.ref, batch.ref, None if rope is None else rope.ref,
+                                            ggml_type, tokens, k_ptr, k_token_stride, k_head_stride, v_ptr,
+                                            v_token_stride, v_head_stride, heads, q_ptr, q_token_stride, q_head_stride,
+                                            q_out_ptr, q_out_token_stride, q_out_head_stride, stream)
+        if rc:
+            self._check(rc)
+
+    def kv8_attention_workspace(self, cache, batch, ggml_type, tokens, heads):
+        """vtq_kv8_attention_workspace: bytes that kv8_attention_device needs for these numbers."""
+        return self.lib.vtq_kv8_attention_workspace(cache.ref, batch.ref, ggml_type, tokens, heads)
+
+    def kv8_attention_device(self, cache, batch, ggml_type, tokens, heads, q_ptr, q_token_stride, q_head_stride, y_ptr,
+                             y_token_stride, y_head_stride, scale, ws_ptr, ws_bytes, stream=None, lse_ptr=None):
+        """vtq_kv8_attention_device: attention over an 8-bit cache's shared prefix and the sequences' own pages."""
+        rc = self.lib.vtq_kv8_attention_device(self.handle, cache.ref, batch.ref, ggml_type, tokens, heads, q_ptr,
+                                               q_token_stride, q_head_stride, y_ptr, y_token_stride, y_head_stride,
+                                               lse_ptr, scale, ws_ptr, ws_bytes, stream)
+        if rc:
+            self._check(rc)
+
+    def beam_select_workspace(self, groups, beams, vocab, n_out):
+        """vtq_beam_select_workspace: bytes that beam_select_device needs for these numbers."""
+        return self.lib.vtq_beam_select_workspace(groups, beams, vocab, n_out)
+
+    def beam_select_device(self, ggml_type, logits_ptr, ld, groups, beams, vocab, score_ptr, n_out, out_score_ptr,
+                           out_token_ptr, out_parent_ptr, ws_ptr, ws_bytes, stream=None, done_ptr=None, end_token=-1,
+                           out_done_ptr=None):
+        """vtq_beam_select_device: the n_out best continuations of each group of beams."""
+        _ints(end_token=end_token)
+        rc = self.lib.vtq_beam_select_device(self.handle, ggml_type, logits_ptr, ld, groups, beams, vocab, score_ptr,
+                                             done_ptr, end_token, n_out, out_score_ptr, out_token_ptr, out_parent_ptr,
+                                             out_done_ptr, ws_ptr, ws_bytes, stream)
+        if rc:
+            self._check(rc)
+
+    def pages_reorder_workspace(self, n_pages, batch, batch_out):
+        """vtq_pages_reorder_workspace: bytes that pages_reorder_device needs for these numbers."""
+        return self.lib.vtq_pages_reorder_workspace(n_pages, batch, batch_out)
+
+    def pages_reorder_device(self, n_pages, page_size, max_pages, refs_ptr, batch, pages_ptr, len_ptr, batch_out,
+                             parent_ptr, grow_ptr, new_refs_ptr, new_pages_ptr, new_len_ptr, copies_ptr, info_ptr,
+                             ws_ptr, ws_bytes, stream=None):
+        """vtq_pages_reorder_device: the next batch's page tables (forks, ends, growth) and the copies they take."""
+        _ints(page_size=page_size)
+        rc = self.lib.vtq_pages_reorder_device(self.handle, n_pages, page_size, max_pages, refs_ptr, batch, pages_ptr,
+                                               len_ptr, batch_out, parent_ptr, grow_ptr, new_refs_ptr, new_pages_ptr,
+                                               new_len_ptr, copies_ptr, info_ptr, ws_ptr, ws_bytes, stream)
+        if rc:
+            self._check(rc)
+
+    def pages_compact_workspace(self, n_pages):
+        """vtq_pages_compact_workspace: bytes that pages_compact_device needs."""
+        return self.lib.vtq_pages_compact_workspace(n_pages)
+
+    def pages_compact_device(self, n_pages, page_size, refs_ptr, n_entries, pages_ptr, new_refs_ptr, new_pages_ptr,
+                             copies_ptr, info_ptr, ws_ptr, ws_bytes, stream=None, n_prefix=0, prefix_pages_ptr=None,
+                             new_prefix_pages_ptr=None):
+        """vtq_pages_compact_device: the pages in use closed up, in the tables, and the copies that this takes."""
+        _ints(page_size=page_size)
+        rc = self.lib.vtq_pages_compact_device(self.handle, n_pages, page_size, refs_ptr, n_entries, pages_ptr, n_prefix,
+                                               prefix_pages_ptr, new_refs_ptr, new_pages_ptr, new_prefix_pages_ptr,
+                                               copies_ptr, info_ptr, ws_ptr, ws_bytes, stream)
+        if rc:
+            self._check(rc)
+
+    def pages_copy_device(self, cache, layers, layer_stride, copies_ptr, max_copies, count_ptr=None, stream=None,
+                          scale_layer_stride=0):
+        """vtq_pages_copy_device, or vtq_kv8_pages_copy_device for a Kv8Cache: pages of every layer."""
+        if isinstance(cache, Kv8Cache):
+            rc = self.lib.vtq_kv8_pages_copy_device(self.handle, cache.ref, layers, layer_stride, scale_layer_stride,
+                                                    copies_ptr, max_copies, count_ptr, stream)
+        else:
+            rc = self.lib.vtq_pages_copy_device(self.handle, cache.ref, layers, layer_stride, copies_ptr, max_copies,
+                                                count_ptr, stream)
         if rc:
             self._check(rc)
 

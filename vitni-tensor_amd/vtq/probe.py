@@ -31,6 +31,13 @@ def lib() -> ctypes.CDLL:
         L.vtqp_check_rope_call.argtypes = [vp, vp, i, vp, sz, sz, vp, sz, sz, vp, sz, sz, sz]
         L.vtqp_check_append.argtypes = [vp, vp, vp, vp, i, sz, vp, sz, sz, vp, sz, sz, sz, vp, sz, sz, vp, sz, sz]
         L.vtqp_check_attention.argtypes = [vp, vp, vp, i, sz, sz, vp, sz, sz, vp, sz, sz, vp, f]
+        L.vtqp_check_kv8_append.argtypes = L.vtqp_check_append.argtypes
+        L.vtqp_check_kv8_attention.argtypes = L.vtqp_check_attention.argtypes
+        L.vtqp_check_beam_select.argtypes = [vp, i, vp, sz, sz, sz, sz, vp, vp, i, sz, vp, vp, vp, vp]
+        L.vtqp_check_pages_reorder.argtypes = [vp, sz, i, sz, vp, sz, vp, vp, sz, vp, vp, vp, vp, vp, vp, vp]
+        L.vtqp_check_pages_compact.argtypes = [vp, sz, i, vp, sz, vp, sz, vp, vp, vp, vp, vp, vp]
+        L.vtqp_check_pages_copy.argtypes = [vp, vp, sz, sz, vp, sz, vp]
+        L.vtqp_check_kv8_pages_copy.argtypes = [vp, vp, sz, sz, sz, vp, sz, vp]
         L.vtqp_i8_form.argtypes = [i, i, i]
         L.vtqp_attention_plan.argtypes = [vp, vp, i, sz, sz, ctypes.POINTER(i)]
         L.vtqp_own_chunk.argtypes = [i, i, i]
