@@ -356,7 +356,8 @@ typedef struct {
  * power of two between (exact, but for those that fall below the smallest normal
  * value, rounded to the nearest).  The new ones are x / 2^e to the nearest, ties to even (beyond
  * 448: 448 with the sign); infinities and NaN become NaN.  A token past q_start[batch],
- * or whose slot does not exist, is not written and has no part in a scale. */
+ * or whose slot does not exist, is not written and has no part in a scale.  A call takes
+ * at most 2^26 tokens x kv_heads. */
 int vtq_kv8_append_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv_batch *batch, const vtq_rope *rope,
                           int type, size_t tokens, const void *d_k, size_t k_token_stride, size_t k_head_stride,
                           const void *d_v, size_t v_token_stride, size_t v_head_stride, size_t heads, const void *d_q,
@@ -421,7 +422,7 @@ int vtq_beam_select_device(vtq_ctx *ctx, int type, const void *d_logits, size_t 
  * info[0] is the count of copies.  info[1] is how many pages are missing, none being
  * free or max_pages too few: their places are -1, and a part-filled page among them is not
  * copied.  Where it is not 0 go on with the old lists.  len counts as between 0 and
- * max_pages * page_size.  Up to 2^16 sequences. */
+ * max_pages * page_size.  Up to 2^16 sequences and 2^24 pages. */
 size_t vtq_pages_reorder_workspace(size_t n_pages, size_t batch, size_t batch_out);
 int vtq_pages_reorder_device(vtq_ctx *ctx, size_t n_pages, int page_size, size_t max_pages, const int32_t *d_refs,
                              size_t batch, const int32_t *d_pages, const int32_t *d_len, size_t batch_out,
@@ -435,7 +436,7 @@ int vtq_pages_reorder_device(vtq_ctx *ctx, size_t n_pages, int page_size, size_t
  * is the count, info[1] n.  new_refs are the counts at the new numbers, 0 from n on.
  * new_pages are the n_entries numbers of pages (a table), and new_prefix_pages the
  * n_prefix of prefix_pages (n_prefix may be 0), as they are now; numbers that are no
- * page become -1. */
+ * page become -1.  Up to 2^24 pages. */
 size_t vtq_pages_compact_workspace(size_t n_pages);
 int vtq_pages_compact_device(vtq_ctx *ctx, size_t n_pages, int page_size, const int32_t *d_refs, size_t n_entries,
                              const int32_t *d_pages, size_t n_prefix, const int32_t *d_prefix_pages,

@@ -79,6 +79,8 @@ def test_append(change, code):
     rc, text = probe.refusal("kv8_append", *_append_args(**change))
     assert rc == code and (text != "") == (code != OK)
     assert probe.refusal("kv8_append", *_append_args(rope=vtq.Rope(128).ref))[0] == SHAPE  # rot_dim beyond head_dim
+    assert probe.refusal("kv8_append", *_append_args(cache=_cache8(kv_heads=1 << 10), tokens=(1 << 16) + 1, kt=1 << 16,
+                                                     vt=1 << 16))[0] == NIMP  # more than 2^26 keys
     assert probe.refusal("kv8_append", None, *_append_args()[1:])[0] == ARG
     assert probe.refusal("kv8_append", _append_args()[0], None, *_append_args()[2:])[0] == ARG
 
@@ -121,7 +123,7 @@ REORDER = dict(n_pages=10, page=16, max_pages=4, refs=A, batch=3, pages=A, len=A
 
 @pytest.mark.parametrize("change,code", [
     ({}, OK), (dict(grow=A), OK), (dict(grow=A + 1), ARG), (dict(page=12), SHAPE), (dict(page=0), SHAPE),
-    (dict(page=-16), SHAPE), (dict(page=8192), SHAPE), (dict(n_pages=1 << 31), NIMP), (dict(n_pages=0, refs=None, new_refs=None), OK),
+    (dict(page=-16), SHAPE), (dict(page=8192), SHAPE), (dict(n_pages=(1 << 24) + 1), NIMP), (dict(n_pages=0, refs=None, new_refs=None), OK),
     (dict(refs=None), ARG), (dict(new_refs=None), ARG), (dict(new_refs=A), ARG), (dict(refs=A + 2), ARG),
     (dict(batch=(1 << 16) + 1), NIMP), (dict(batch_out=(1 << 16) + 1), NIMP), (dict(max_pages=1 << 27), NIMP),
     (dict(max_pages=1 << 62), NIMP), (dict(pages=None), ARG), (dict(len=None), ARG), (dict(batch=0, pages=None, len=None), OK),
@@ -169,8 +171,8 @@ def test_pages_copy(change, code):
     assert probe.refusal("kv8_pages_copy", eight.ref, 3, 1 << 20, 0, A, 7, None)[0] == SHAPE
     assert probe.refusal("kv8_pages_copy", eight.ref, 3, 1 << 20, 1 << 41, A, 7, None)[0] == NIMP
     assert probe.refusal("kv8_pages_copy", eight.ref, 3, (1 << 20) + 8, 64, A, 7, None)[0] == SHAPE
-    many = vtq.KvCache(vtq.F16, A, A, 10, 16, 65535, 64, head_stride=64)
-    assert probe.refusal("pages_copy", many.ref, 60000, 1 << 20, A, 7, None)[0] == NIMP
+    many = vtq.KvCache(vtq.F16, A, A, 10, 4096, 65535, 64, head_stride=64)
+    assert probe.refusal("pages_copy", many.ref, 3, 1 << 20, A, 7, None)[0] == NIMP
 
 
 def test_workspaces_of_refused_sizes_are_none():
@@ -180,8 +182,8 @@ def test_workspaces_of_refused_sizes_are_none():
                   (1 << 20, 2, 10, 1), (1 << 62, 4, 10, 1)):
         assert lib.vtq_beam_select_workspace(*sizes) == 0
     assert lib.vtq_pages_reorder_workspace(10, 3, 5) > 0 and lib.vtq_pages_compact_workspace(10) > 0
-    assert lib.vtq_pages_reorder_workspace(1 << 31, 3, 5) == lib.vtq_pages_reorder_workspace(10, 3, 1 << 17) == 0
-    assert lib.vtq_pages_compact_workspace(1 << 31) == 0
+    assert lib.vtq_pages_reorder_workspace((1 << 24) + 1, 3, 5) == lib.vtq_pages_reorder_workspace(10, 3, 1 << 17) == 0
+    assert lib.vtq_pages_compact_workspace((1 << 24) + 1) == 0
     assert lib.vtq_kv8_attention_workspace(None, None, vtq.BF16, 3, 4) == 0
 
 

@@ -1,10 +1,10 @@
 // cache_pages.hip -- who holds a cache's pages: the next batch's page tables from the
 // sequences that it goes on with, the pages in use closed up, and copies of pages (gfx950).
 //
-// The lists are small (a table of 256 x 256 pages is 256 KB) and each step needs the
-// one before, so time is launches and latency: a few kernels over all pages at once, with
-// counts of 4096 pages, a scan of the counts by one workgroup, and ranks from both.
-// Free pages are taken lowest first and in the order of sequences, and counts change by
+// The lists are small (a table of 256 x 256 pages is 256 KB) and each step needs the one
+// before, so time is launches and latency: two kernels for a reorder, three to close up,
+// over all pages at once, with counts of 1024 pages that every workgroup adds up for
+// itself.  Free pages are taken lowest first and in the order of sequences, and counts change by
 // atomic additions of whole numbers, whose order changes nothing: the same lists every time.
 #include <algorithm>
 
@@ -14,16 +14,16 @@
 namespace vtq {
 namespace {
 
-constexpr int kSegment = 4096;  // pages to a workgroup
+constexpr int kSegment = 1024;  // pages to a workgroup
 constexpr int kThreads = 256;
+constexpr int kOwnScan = 1024;  // new sequences whose counts every workgroup scans for itself
 
 struct ReorderJob : PagesReorder {
     int segments;
     int32_t *begin, *fresh, *to_copy;     // [batch_out]: first place of free pages, how many, whether a page is copied
-    int64_t* fresh_before;                // [batch_out + 1]
-    int32_t* copies_before;               // [batch_out]
     int32_t* free_in;                     // [segments]
-    int64_t* free_before;                 // [segments + 1]
+    int64_t* fresh_before;                // [batch_out + 1]; these two above kOwnScan sequences
+    int32_t* copies_before;               // [batch_out + 1]
 };
 
 __device__ __forceinline__ int pages_of(int64_t tokens, int page_size) {
@@ -101,14 +101,29 @@ __global__ __launch_bounds__(kThreads) void reorder_share_kernel(ReorderJob j) {
     }
 }
 
-// before[i] = sum of values below i, for i up to n, by one workgroup of 1024.
-template <class T, class S>
-__device__ __forceinline__ S scan(const T* values, int64_t n, S* before, bool total_too) {
-    __shared__ S waves[16];
+// Sum over a workgroup of THREADS.
+template <int THREADS, class S>
+__device__ __forceinline__ S sum_of(S x) {
+    __shared__ S part[THREADS / 64];
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d, 64);
+    __syncthreads();  // the last sum's parts are read
+    if ((threadIdx.x & 63) == 0) part[wave_id()] = x;
+    __syncthreads();
+    S all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) all += part[w];
+    return all;
+}
+
+// before[i] = sum of value(k) for k below i, i up to n, by a workgroup of THREADS; returns the sum.
+template <int THREADS, class S, class Value>
+__device__ __forceinline__ S scan(int64_t n, S* before, Value value) {
+    __shared__ S waves[THREADS / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     S carry = 0;
-    for (int64_t i0 = 0; i0 < n; i0 += 1024) {
-        const S own = i0 + tid < n ? (S)values[i0 + tid] : (S)0;
+    for (int64_t i0 = 0; i0 < n; i0 += THREADS) {
+        const S own = i0 + tid < n ? (S)value(i0 + tid) : (S)0;
         S up_to = own;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -118,7 +133,8 @@ __device__ __forceinline__ S scan(const T* values, int64_t n, S* before, bool to
         if (lane == 63) waves[wave] = up_to;
         __syncthreads();
         S ahead = carry, all = carry;
-        for (int w = 0; w < 16; w++) {
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; w++) {
             if (w < wave) ahead += waves[w];
             all += waves[w];
         }
@@ -126,41 +142,50 @@ __device__ __forceinline__ S scan(const T* values, int64_t n, S* before, bool to
         carry = all;
         __syncthreads();
     }
-    if (total_too && tid == 0) before[n] = carry;
+    if (tid == 0) before[n] = carry;
+    __syncthreads();
     return carry;
 }
 
-__global__ __launch_bounds__(1024) void reorder_scan_kernel(ReorderJob j) {
-    const int64_t free = scan(j.free_in, j.segments, j.free_before, true);
-    const int64_t fresh = scan(j.fresh, j.batch_out, j.fresh_before, true);
-    __syncthreads();
-    // a sequence's copy has a page while pages last, from the first sequence on
-    for (int i = threadIdx.x; i < j.batch_out; i += 1024)
-        if (j.to_copy[i] && j.fresh_before[i] >= free) j.to_copy[i] = 0;
-    __syncthreads();
-    const int copies = scan(j.to_copy, j.batch_out, j.copies_before, false);
-    // places beyond max_pages
-    int64_t beyond = 0;
-    for (int i = threadIdx.x; i < j.batch_out; i += 1024)
-        if (j.grow) beyond += max(pages_of((int64_t)j.new_len[i] + max(j.grow[i], 0), j.page_size) - j.max_pages, 0);
-    __shared__ int64_t part[16];
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) beyond += __shfl_xor(beyond, d, 64);
-    if ((threadIdx.x & 63) == 0) part[wave_id()] = beyond;
-    __syncthreads();
+// Pages that a sequence's growth would take beyond max_pages.
+__device__ __forceinline__ int64_t beyond(const ReorderJob& j, int i) {
+    if (!j.grow) return 0;
+    return max(pages_of((int64_t)j.new_len[i] + max(j.grow[i], 0), j.page_size) - j.max_pages, 0);
+}
+
+// Scans of the new sequences' counts: free pages that go to those before each, and copies.  A
+// sequence's copy has a page while pages last, from the first sequence on.  One workgroup
+// alone tells the counts.
+template <int THREADS>
+__device__ __forceinline__ void scan_sequences(const ReorderJob& j, int64_t free, int64_t* fresh_before,
+                                               int32_t* copies_before, bool tells) {
+    const int64_t fresh = scan<THREADS>(j.batch_out, fresh_before, [&](int64_t i) { return j.fresh[i]; });
+    const int copies = scan<THREADS>(j.batch_out, copies_before, [&](int64_t i) {
+        return j.to_copy[i] && fresh_before[i] < free ? 1 : 0;
+    });
+    if (!tells) return;
+    int64_t over = 0;
+    for (int i = threadIdx.x; i < j.batch_out; i += THREADS) over += beyond(j, i);
+    over = sum_of<THREADS>(over);
     if (threadIdx.x == 0) {
-        int64_t missing = max(fresh - free, (int64_t)0);
-        for (int w = 0; w < 16; w++) missing += part[w];
         j.info[0] = copies;
-        j.info[1] = (int32_t)min(missing, (int64_t)INT32_MAX);
+        j.info[1] = (int32_t)min(max(fresh - free, (int64_t)0) + over, (int64_t)INT32_MAX);
     }
 }
 
-// Workgroups below `segments` hand out their free pages, the others (one to an old sequence)
-// take its pages' holders off and its children on.
+__global__ __launch_bounds__(1024) void reorder_scan_kernel(ReorderJob j) {
+    int64_t free = 0;
+    for (int s = threadIdx.x; s < j.segments; s += 1024) free += j.free_in[s];
+    scan_sequences<1024>(j, sum_of<1024>(free), j.fresh_before, j.copies_before, true);
+}
+
+// Workgroups below `segments` hand out their free pages, the others (one to an old sequence, and
+// the last) take its pages' holders off and its children on.
+template <bool OWN>
 __global__ __launch_bounds__(kThreads) void reorder_apply_kernel(ReorderJob j) {
     const int tid = threadIdx.x, lane = tid & 63;
-    if ((int64_t)blockIdx.x >= j.segments) {
+    const bool tells = (int64_t)blockIdx.x == (int64_t)j.segments + j.batch;
+    if ((int64_t)blockIdx.x >= j.segments && !tells) {
         const int old = (int)(blockIdx.x - j.segments);
         __shared__ int children, eldest;
         if (tid == 0) children = 0, eldest = INT32_MAX;
@@ -180,14 +205,24 @@ __global__ __launch_bounds__(kThreads) void reorder_apply_kernel(ReorderJob j) {
         }
         return;
     }
-    const int64_t total = j.fresh_before[j.batch_out];
-    int64_t rank = j.free_before[blockIdx.x];
-    if (rank >= total) return;
-    __shared__ int waves[kThreads / 64];
-    for (int k0 = 0; k0 < kSegment; k0 += kThreads) {
+    __shared__ int64_t own_fresh[OWN ? kOwnScan + 1 : 1];
+    __shared__ int32_t own_copies[OWN ? kOwnScan + 1 : 1];
+    int64_t before = 0, all = 0;
+    for (int s = tid; s < j.segments; s += kThreads) {
+        const int n = j.free_in[s];
+        all += n;
+        before += s < (int)blockIdx.x ? n : 0;
+    }
+    int64_t rank = sum_of<kThreads>(before);
+    if constexpr (OWN) scan_sequences<kThreads>(j, sum_of<kThreads>(all), own_fresh, own_copies, tells);
+    if (tells) return;
+    auto fresh_before = [&](int i) { return OWN ? own_fresh[i] : j.fresh_before[i]; };
+    const int64_t total = fresh_before(j.batch_out);
+    for (int k0 = 0; k0 < kSegment && rank < total; k0 += kThreads) {
         const int64_t page = (int64_t)blockIdx.x * kSegment + k0 + tid;
         const bool free = page < j.n_pages && j.refs[page] == 0;
         const uint64_t mask = __ballot(free);
+        __shared__ int waves[kThreads / 64];
         if (lane == 0) waves[wave_id()] = __popcll(mask);
         __syncthreads();
         int64_t mine = rank + __popcll(mask & ((1ull << lane) - 1));
@@ -201,21 +236,20 @@ __global__ __launch_bounds__(kThreads) void reorder_apply_kernel(ReorderJob j) {
             int lo = 0, hi = j.batch_out;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (j.fresh_before[mid] <= mine) lo = mid;
+                if (fresh_before(mid) <= mine) lo = mid;
                 else hi = mid;
             }
-            const int at = (int)(mine - j.fresh_before[lo]);
+            const int at = (int)(mine - fresh_before(lo));
             j.new_pages[(int64_t)lo * j.max_pages + j.begin[lo] + at] = (int32_t)page;
             atomicAdd(&j.new_refs[page], 1);
             if (at == 0 && j.to_copy[lo]) {
                 const int parent = j.parent[lo], len = j.new_len[lo];
-                int32_t* c = j.copies + 3 * (int64_t)j.copies_before[lo];
+                int32_t* c = j.copies + 3 * (int64_t)(OWN ? own_copies[lo] : j.copies_before[lo]);
                 c[0] = j.pages[(int64_t)parent * j.max_pages + len / j.page_size];
                 c[1] = (int32_t)page;
                 c[2] = len % j.page_size;
             }
         }
-        if (rank >= total) return;
     }
 }
 
@@ -223,39 +257,36 @@ __global__ __launch_bounds__(kThreads) void reorder_apply_kernel(ReorderJob j) {
 
 struct CompactJob : PagesCompact {
     int segments;
-    int32_t* live_in;      // [segments]
-    int64_t* live_before;  // [segments + 1]
-    int32_t *low, *high;   // [n_pages / 2]: free pages below the count of those in use, and pages in use past it
-    int32_t* rank;         // [n_pages]: of a page among the latter
+    int32_t* live_in;     // [segments]
+    int32_t *low, *high;  // [n_pages / 2]: free pages below the count of those in use, and pages in use past it
+    int32_t* rank;        // [n_pages]: of a page among the latter
 };
 
 __global__ __launch_bounds__(kThreads) void compact_count_kernel(CompactJob j) {
     count_segment(j.refs, nullptr, j.n_pages, (int)blockIdx.x, j.live_in);
 }
 
-__global__ __launch_bounds__(1024) void compact_scan_kernel(CompactJob j) {
-    const int64_t live = scan(j.live_in, j.segments, j.live_before, true);
-    if (threadIdx.x == 0) j.info[0] = 0, j.info[1] = (int32_t)live;
-}
-
 __global__ __launch_bounds__(kThreads) void compact_rank_kernel(CompactJob j) {
     const int tid = threadIdx.x, lane = tid & 63;
-    const int64_t n_live = j.live_before[j.segments];
+    int64_t all = 0, up_to = 0;
+    for (int s = tid; s < j.segments; s += kThreads) {
+        const int n = j.live_in[s];
+        all += n;
+        up_to += s < (int)blockIdx.x ? n : 0;
+    }
+    const int64_t n_live = sum_of<kThreads>(all);
+    int64_t before = sum_of<kThreads>(up_to);
     // pages in use below n_live: those of whole segments, and of the one that it lies in
     const int64_t edge = n_live / kSegment;
-    __shared__ int waves[kThreads / 64];
-    int64_t below = 0;
-    if ((int64_t)blockIdx.x >= edge) {
-        int mine = 0;
-        for (int64_t p = edge * kSegment + tid; p < n_live; p += kThreads) mine += j.refs[p] > 0;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d, 64);
-        if (lane == 0) waves[wave_id()] = mine;
-        __syncthreads();
-        below = j.live_before[edge] + waves[0] + waves[1] + waves[2] + waves[3];
-        __syncthreads();
+    int64_t mine = 0;
+    for (int s = tid; s < edge; s += kThreads) mine += j.live_in[s];
+    for (int64_t p = edge * kSegment + tid; p < n_live; p += kThreads) mine += j.refs[p] > 0;
+    const int64_t below = sum_of<kThreads>(mine);
+    if (blockIdx.x == 0 && tid == 0) {
+        j.info[0] = (int32_t)(n_live - below);
+        j.info[1] = (int32_t)n_live;
     }
-    int64_t before = j.live_before[blockIdx.x];
+    __shared__ int waves[kThreads / 64];
     for (int k0 = 0; k0 < kSegment; k0 += kThreads) {
         const int64_t p = (int64_t)blockIdx.x * kSegment + k0 + tid;
         const bool there = p < j.n_pages;
@@ -280,10 +311,6 @@ __global__ __launch_bounds__(kThreads) void compact_rank_kernel(CompactJob j) {
                 j.rank[p] = (int32_t)(at - below);
             }
         }
-    }
-    if ((int64_t)blockIdx.x == j.segments - 1 && tid == 0) {
-        // the last segment knows how many are past n_live
-        j.info[0] = n_live < j.n_pages ? (int32_t)(j.live_before[j.segments] - below) : 0;
     }
 }
 
@@ -310,50 +337,67 @@ __global__ __launch_bounds__(kThreads) void compact_apply_kernel(CompactJob j) {
 
 struct CopyJob : PagesCopy {
     int elem;
-    int row_chunks;   // 16 bytes of a head's row
-    int64_t units;    // of a copy: layers x heads x 2
+    int row_chunks;  // of 16 bytes, of a head's row
+    int units;       // of a copy: layers x 2
+    int unit_rows;   // units to an XCD
+    int pieces;      // workgroups to a unit
+    int64_t work;
 };
 
-// A wave takes a copy's keys or values of one head and layer at a time.
+// (as the runtime's uint4 the four would be put in LDS, by numbers from the dispatch packet,
+// which is host memory: 13 us)
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+constexpr int kPiece = 4 * kThreads;  // chunks to a workgroup, in flight at once
+
+// A workgroup takes up to 16 KB of a copy's keys or values of a layer.  Pages lie anywhere, and
+// address translation is what a short list of copies waits for: workgroups go to the 8 XCDs
+// in turn, and a layer's keys (or values) stay on one of them.
 __global__ __launch_bounds__(kThreads) void copy_kernel(CopyJob j) {
-    const int lane = threadIdx.x & 63;
+    const int tid = threadIdx.x;
     const int64_t n = j.count ? min(max((int64_t)*j.count, (int64_t)0), j.max_copies) : j.max_copies;
     const vtq_kv_cache& c = j.cache;
-    const int64_t waves = (int64_t)gridDim.x * (kThreads / 64);
-    for (int64_t w = (int64_t)blockIdx.x * (kThreads / 64) + wave_id(); w < n * j.units; w += waves) {
-        const int64_t copy = w / j.units;
-        int unit = (int)(w % j.units);  // below 2^25
+    for (int64_t i = blockIdx.x; i < j.work; i += gridDim.x) {
+        int64_t at = i >> 3;
+        const int unit = (int)(at % j.unit_rows) * 8 + (int)(i & 7);
+        at /= j.unit_rows;
+        const int piece = (int)(at % j.pieces);
+        const int64_t copy = at / j.pieces;
+        if (copy >= n) return;
+        if (unit >= j.units) continue;
         const int32_t from = j.copies[3 * copy], to = j.copies[3 * copy + 1];
         const int slots = min(max(j.copies[3 * copy + 2], 0), c.page_size);
         if (!is_page(from, (int64_t)c.n_pages) || !is_page(to, (int64_t)c.n_pages)) continue;
         const bool is_v = unit & 1;
-        unit /= 2;
-        const int head = unit % c.kv_heads, layer = unit / c.kv_heads;
-        char* base = static_cast<char*>(is_v ? c.v : c.k) +
-                     (layer * j.layer_stride + head * (int64_t)c.head_stride) * j.elem;
+        const int64_t layer = unit / 2;
+        char* base = static_cast<char*>(is_v ? c.v : c.k) + layer * j.layer_stride * j.elem;
         const char* src = base + from * (int64_t)c.page_stride * j.elem;
         char* dst = base + to * (int64_t)c.page_stride * j.elem;
-        const int64_t slot = (int64_t)c.slot_stride * j.elem;
-        const int chunks = slots * j.row_chunks;
-        // four loads in flight
-        for (int i0 = lane; i0 < chunks; i0 += 256) {
-            uint4 x[4];
-            int64_t at[4];
+        const uint32_t of_head = (uint32_t)slots * j.row_chunks, chunks = of_head * c.kv_heads;  // below 2^31
+        const uint32_t first = (uint32_t)piece * kPiece + tid;
+        if (chunks) {
+            // (past the end the last chunk again, which is not stored: every load stands alone)
+            v4u x[4];
+            int64_t where[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const int i = i0 + 64 * k;
-                at[k] = (i / j.row_chunks) * slot + (i % j.row_chunks) * 16;
-                if (i < chunks) x[k] = *reinterpret_cast<const uint4*>(src + at[k]);
+                const uint32_t chunk = min(first + k * kThreads, chunks - 1);
+                const uint32_t head = chunk / of_head, rest = chunk - head * of_head;
+                const uint32_t slot = rest / (uint32_t)j.row_chunks;
+                where[k] = (head * (int64_t)c.head_stride + slot * (int64_t)c.slot_stride) * j.elem +
+                           (rest - slot * j.row_chunks) * 16;
+                x[k] = *reinterpret_cast<const v4u*>(src + where[k]);
             }
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (i0 + 64 * k < chunks) *reinterpret_cast<uint4*>(dst + at[k]) = x[k];
+                if (first + k * kThreads < chunks) *reinterpret_cast<v4u*>(dst + where[k]) = x[k];
         }
-        if (j.scales.k) {
-            uint8_t* scale = (is_v ? j.scales.v : j.scales.k) + layer * j.scale_layer_stride + head * j.scales.head_stride;
+        if (piece == 0 && j.scales.k) {
+            uint8_t* scale = (is_v ? j.scales.v : j.scales.k) + layer * j.scale_layer_stride;
             const int blocks = (slots + j.scales.block - 1) / j.scales.block;
-            for (int i = lane; i < blocks; i += 64)
-                scale[to * j.scales.page_stride + i] = scale[from * j.scales.page_stride + i];
+            for (int k = tid; k < blocks * c.kv_heads; k += kThreads) {
+                uint8_t* s = scale + (k / blocks) * j.scales.head_stride + k % blocks;
+                s[to * j.scales.page_stride] = s[from * j.scales.page_stride];
+            }
         }
     }
 }
@@ -377,10 +421,9 @@ size_t reorder_parts(ReorderJob& j, int64_t n_pages, int64_t batch_out, void* ws
     p.take(j.begin, batch_out);
     p.take(j.fresh, batch_out);
     p.take(j.to_copy, batch_out);
-    p.take(j.fresh_before, batch_out + 1);
-    p.take(j.copies_before, batch_out);
     p.take(j.free_in, j.segments);
-    p.take(j.free_before, j.segments + 1);
+    p.take(j.fresh_before, batch_out > kOwnScan ? batch_out + 1 : 0);
+    p.take(j.copies_before, batch_out > kOwnScan ? batch_out + 1 : 0);
     return p.used;
 }
 
@@ -388,7 +431,6 @@ size_t compact_parts(CompactJob& j, int64_t n_pages, void* ws) {
     Parts p{static_cast<char*>(ws)};
     j.segments = (int)((n_pages + kSegment - 1) / kSegment);
     p.take(j.live_in, j.segments);
-    p.take(j.live_before, j.segments + 1);
     p.take(j.low, n_pages / 2);
     p.take(j.high, n_pages / 2);
     p.take(j.rank, n_pages);
@@ -415,9 +457,13 @@ hipError_t launch_pages_reorder(const PagesReorder& a, hipStream_t stream) {
     reorder_parts(j, a.n_pages, a.batch_out, a.ws);
     if (j.segments + a.batch_out)
         hipLaunchKernelGGL(reorder_share_kernel, dim3((unsigned)(j.segments + a.batch_out)), dim3(kThreads), 0, stream, j);
-    hipLaunchKernelGGL(reorder_scan_kernel, dim3(1), dim3(1024), 0, stream, j);
-    if (j.segments + a.batch)
-        hipLaunchKernelGGL(reorder_apply_kernel, dim3((unsigned)(j.segments + a.batch)), dim3(kThreads), 0, stream, j);
+    const dim3 grid((unsigned)(j.segments + a.batch + 1));
+    if (a.batch_out > kOwnScan) {
+        hipLaunchKernelGGL(reorder_scan_kernel, dim3(1), dim3(1024), 0, stream, j);
+        hipLaunchKernelGGL((reorder_apply_kernel<false>), grid, dim3(kThreads), 0, stream, j);
+    } else {
+        hipLaunchKernelGGL((reorder_apply_kernel<true>), grid, dim3(kThreads), 0, stream, j);
+    }
     return hipGetLastError();
 }
 
@@ -427,8 +473,8 @@ hipError_t launch_pages_compact(const PagesCompact& a, hipStream_t stream) {
     compact_parts(j, a.n_pages, a.ws);
     if (j.segments)
         hipLaunchKernelGGL(compact_count_kernel, dim3((unsigned)j.segments), dim3(kThreads), 0, stream, j);
-    hipLaunchKernelGGL(compact_scan_kernel, dim3(1), dim3(1024), 0, stream, j);
-    if (j.segments) hipLaunchKernelGGL(compact_rank_kernel, dim3((unsigned)j.segments), dim3(kThreads), 0, stream, j);
+    // (a workgroup at least: it tells the counts)
+    hipLaunchKernelGGL(compact_rank_kernel, dim3((unsigned)std::max(j.segments, 1)), dim3(kThreads), 0, stream, j);
     const int64_t most = std::max({a.n_pages / 2, a.n_entries, a.n_prefix});
     if (most) hipLaunchKernelGGL(compact_apply_kernel, dim3(groups_of(most)), dim3(kThreads), 0, stream, j);
     return hipGetLastError();
@@ -439,9 +485,11 @@ hipError_t launch_pages_copy(const PagesCopy& a, hipStream_t stream) {
     static_cast<PagesCopy&>(j) = a;
     j.elem = a.cache.type == VTQ_TYPE_E4M3 ? 1 : (int)type_bytes(a.cache.type);
     j.row_chunks = a.cache.head_dim * j.elem / 16;
-    j.units = (int64_t)a.layers * a.cache.kv_heads * 2;
-    const int64_t waves = a.max_copies * j.units;
-    const int64_t groups = std::min<int64_t>((waves + 3) / 4, 256 * 16);
+    j.units = a.layers * 2;
+    j.unit_rows = (j.units + 7) / 8;
+    j.pieces = (int)(((int64_t)a.cache.kv_heads * a.cache.page_size * j.row_chunks + kPiece - 1) / kPiece);
+    j.work = 8 * a.max_copies * j.pieces * j.unit_rows;
+    const int64_t groups = std::min<int64_t>(j.work, 1 << 16);
     hipLaunchKernelGGL(copy_kernel, dim3((unsigned)groups), dim3(kThreads), 0, stream, j);
     return hipGetLastError();
 }

@@ -9,9 +9,10 @@
 // requantized: only what drops below e4m3's smallest normal value rounds again (a full
 // scale would gain half a bit at most: e4m3 is a float, and 448 / 2^e lies within two).
 //
-// A workgroup takes a block of a sequence (the one that holds the call's first token in
-// it) and some of its heads; a wave a head's keys or values: the maximum first, then the
-// elements again, from the caches near by.  Queries are rotated by workgroups of their own in the same launch.
+// A workgroup takes a block of a sequence and some of its heads, a wave a head's keys or
+// values.  What the wave's lanes hold at once, 16 tokens of up to 128 elements, stays in
+// registers between the maximum and the stores; longer blocks are read again, from the
+// caches near by.  Queries are rotated by workgroups of their own in the same launch.
 #include "vtq_rope.h"
 
 namespace vtq {
@@ -19,11 +20,14 @@ namespace {
 
 constexpr int kCosTokens = 16;  // tokens whose cosines are held at a time
 constexpr int kMostRows = 32;   // heads' keys and values to a workgroup
+constexpr int kHeld = 4;        // units of a row that a lane has at a time
 constexpr int kLeast = -117, kMost = 119;  // exponents of scales: what they scale stays a normal bf16
 
 struct Kv8Job : RopeJob {
     Scales s;
-    int q_groups, q_per, rows_per;  // workgroups of queries and their heads; heads' keys and values to one
+    int64_t q_work;            // workgroups that rotate queries: tokens x q_groups
+    int q_groups, q_per;       // to a token, and their heads
+    int kv_groups, rows_per;   // to a block, and their heads' keys and values
 };
 
 // Least e with top <= 448 * 2^e, 448 being 1.75 * 2^8.
@@ -65,21 +69,135 @@ __device__ __forceinline__ uint32_t shifted4(uint32_t w, int shift) {
     return (uint32_t)v;
 }
 
+// A token's sequence, and its place among the sequence's own tokens.
+struct Spot {
+    int seq;
+    int64_t place;
+};
+
+// The first token, of those that the call adds to it, of the index-th block that the batch's
+// tokens lie in, and how many they are (0: there is no such block).  Every wave finds it for
+// itself; tokens before place 0 have none.
+__device__ __forceinline__ int block_tokens(const vtq_kv_batch& b, int64_t tokens, int block_shift, int64_t index,
+                                            int64_t& token, Spot& spot) {
+    const int lane = threadIdx.x & 63;
+    for (int i0 = 0; i0 < b.batch; i0 += 64) {
+        const int i = min(i0 + lane, b.batch - 1);
+        const int64_t q0 = b.q_start[i], q1 = b.q_start[i + 1], len = b.len[i];
+        const int64_t end = min(q1, tokens);  // of the tokens; the newest of all is the one before q1
+        const int64_t from = max(len - (q1 - q0), (int64_t)0), to = len - (q1 - end);
+        const bool some = i0 + lane < b.batch && q0 >= 0 && to > from && end > q0;
+        const int64_t blocks = some ? ((to - 1) >> block_shift) - (from >> block_shift) + 1 : 0;
+        int64_t up_to = blocks;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int64_t o = __shfl_up(up_to, d, 64);
+            if (lane >= d) up_to += o;
+        }
+        const uint64_t past = __ballot(up_to > index);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            const int64_t mine = index - (__shfl(up_to, at, 64) - __shfl(blocks, at, 64));
+            const int64_t f = __shfl(from, at, 64), t = __shfl(to, at, 64), q = __shfl(q0, at, 64);
+            const int64_t behind = __shfl(len - (q1 - q0), at, 64);  // place of the first token, maybe below 0
+            const int64_t block0 = (f >> block_shift) + mine;
+            spot.seq = i0 + at;
+            spot.place = max(f, block0 << block_shift);
+            token = q + (spot.place - behind);
+            return (int)(min(t, (block0 + 1) << block_shift) - spot.place);
+        }
+        index -= __shfl(up_to, 63, 64);
+    }
+    return 0;
+}
+
+// Units of a row of some tokens, kHeld to a lane: their elements, rotated.
+template <class T, int N>
+struct Held {
+    float x[kHeld][2][N];
+    int at[kHeld][2];   // first element of each part; -1: there is none
+    int token[kHeld];
+
+    // Units w0 + 64 k + lane of n tokens' `units` each.
+    __device__ __forceinline__ void load(const T* src, int64_t token_stride, int w0, int n, int units, const float2 (*cs)[128],
+                                         int rot, bool half) {
+        const int lane = threadIdx.x & 63, per = half || N == 1 ? rot / 2 / N : rot / N, step = half ? rot / 2 : 1;
+        Pack<T, N> a[kHeld], b[kHeld];
+        bool turns[kHeld];
+        int pair[kHeld];
+        // all loads first
+#pragma unroll
+        for (int k = 0; k < kHeld; k++) {
+            const int w = w0 + 64 * k + lane, last = min(w, n * units - 1), unit = last % units;
+            token[k] = last / units;
+            turns[k] = unit < per;
+            const bool two = turns[k] && (half || N == 1);
+            // where the unit begins; a pair's elements stand side by side, or half the rotated part apart
+            int first;
+            if (turns[k]) first = half ? unit * N : N == 1 ? 2 * unit : unit * N;
+            else first = (half || N == 1 ? rot : per * N) + (unit - per) * N;
+            pair[k] = half || N == 1 ? unit * N : unit * N / 2;
+            at[k][0] = w < n * units ? first : -1;
+            at[k][1] = w < n * units && two ? first + step : -1;
+            const T* from = src + token[k] * token_stride + first;
+            a[k] = *reinterpret_cast<const Pack<T, N>*>(from);
+            b[k] = *reinterpret_cast<const Pack<T, N>*>(two ? from + step : from);
+        }
+#pragma unroll
+        for (int k = 0; k < kHeld; k++) {
+            const float2* c = cs[token[k]] + (turns[k] ? pair[k] : 0);
+            if (half || N == 1) {
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const float2 w = c[e];
+                    const float p = (float)a[k].v[e], q = (float)b[k].v[e];
+                    x[k][0][e] = turns[k] ? p * w.x - q * w.y : p;
+                    x[k][1][e] = turns[k] ? p * w.y + q * w.x : p;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    const float2 w = c[e / 2];
+                    const float p = (float)a[k].v[e], q = (float)a[k].v[e + 1 < N ? e + 1 : e];
+                    x[k][0][e] = turns[k] ? p * w.x - q * w.y : p;
+                    if (e + 1 < N) x[k][0][e + 1] = turns[k] ? p * w.y + q * w.x : q;
+                }
+#pragma unroll
+                for (int e = 0; e < N; e++) x[k][1][e] = x[k][0][e];
+            }
+        }
+    }
+    __device__ __forceinline__ float top() const {
+        float most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kHeld; k++)
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const float v = fabsf(x[k][p][e]);
+                    most = fmaxf(most, v < INFINITY ? v : 0.0f);
+                }
+        return most;
+    }
+    __device__ __forceinline__ void put(uint8_t* dst, int64_t slot, int e) const {
+#pragma unroll
+        for (int k = 0; k < kHeld; k++)
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+                if (at[k][p] >= 0) put8<N>(dst + token[k] * slot + at[k][p], x[k][p], e);
+    }
+};
+
 template <class T, int N>
 __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
-    const int64_t t = (int64_t)blockIdx.x;
     const int lane = threadIdx.x & 63, wave = wave_id();
-    const int seq = sequence_of(j.batch, t);
-    if (seq >= j.batch.batch) return;
-    const int64_t end = min((int64_t)j.batch.q_start[seq + 1], j.tokens);
-    // the newest token of the sequence is the one before its end
-    const int64_t place = (int64_t)j.batch.len[seq] - (j.batch.q_start[seq + 1] - t);
     const int rot = j.rotate ? j.rope.rot_dim : 0;
     const bool half = j.rope.layout == VTQ_ROPE_HALF;
     const int units_rot = rotated_units(j.head_dim, rot, half, N), units_plain = j.head_dim / N;
     __shared__ float2 cs[kCosTokens][128];
-    __shared__ float top[kMostRows];
-    // cosines and sines of `n` tokens from the one at `from` on
+    __shared__ float tops[kMostRows];
+    // cosines and sines of n tokens from the place `from` on
     auto turn = [&](int64_t from, int n) {
         for (int i = threadIdx.x; i < n * (rot / 2); i += kRopeThreads) {
             const int token = i / (rot / 2), pair = i % (rot / 2);
@@ -88,10 +206,14 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
             cs[token][pair] = make_float2(w.x * j.rope.magnitude, w.y * j.rope.magnitude);
         }
     };
-    if ((int)blockIdx.y < j.q_groups) {
-        turn(place, 1);
+    if ((int64_t)blockIdx.x < j.q_work) {
+        const int64_t t = blockIdx.x / j.q_groups;
+        const int group = blockIdx.x % j.q_groups;
+        const int seq = sequence_of(j.batch, t);
+        if (seq >= j.batch.batch) return;
+        turn((int64_t)j.batch.len[seq] - (j.batch.q_start[seq + 1] - t), 1);
         __syncthreads();
-        const int h0 = (int)blockIdx.y * j.q_per, h1 = min(j.x_heads, h0 + j.q_per);
+        const int h0 = group * j.q_per, h1 = min(j.x_heads, h0 + j.q_per);
         for (int w = threadIdx.x; w < (h1 - h0) * units_plain; w += kRopeThreads) {
             const int h = h0 + w / units_plain, u = w % units_plain;
             if (u >= units_rot) continue;
@@ -100,76 +222,79 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
         }
         return;
     }
-    // the call's first token in the block has the block
-    const int block = j.s.block, before = (int)(place & (block - 1));
-    if (place < 0 || (before != 0 && t != j.batch.q_start[seq])) return;
-    const int64_t at = slot_of(j.cache, j.batch.pages + (int64_t)seq * j.batch.max_pages, j.batch.max_pages, place);
+    const int64_t work = blockIdx.x - j.q_work;
+    int64_t t;
+    Spot spot;
+    const int block = j.s.block;
+    const int count = block_tokens(j.batch, j.tokens, __builtin_ctz(block), work / j.kv_groups, t, spot);
+    if (!count) return;
+    const int32_t* list = j.batch.pages + (int64_t)spot.seq * j.batch.max_pages;
+    const int64_t at = slot_of(j.cache, list, j.batch.max_pages, spot.place);
     if (at < 0) return;
-    const int64_t page = j.batch.pages[(int64_t)seq * j.batch.max_pages + place / j.cache.page_size];
-    const int count = (int)min(end - t, (int64_t)(block - before));
-    const int64_t scale_at = page * j.s.page_stride + (place & (j.cache.page_size - 1)) / block;
-    const int r0 = ((int)blockIdx.y - j.q_groups) * j.rows_per, r1 = min(2 * j.kv_heads, r0 + j.rows_per);
+    const int before = (int)(spot.place & (block - 1));
+    const int64_t scale_at = list[spot.place / j.cache.page_size] * j.s.page_stride +
+                             (spot.place & (j.cache.page_size - 1)) / block;
+    const int group = (int)(work % j.kv_groups);
+    const int r0 = group * j.rows_per, r1 = min(2 * j.kv_heads, r0 + j.rows_per);
     const bool keys = r0 < j.kv_heads && rot;
-    // f(i, x, token) with the elements of a row (keys of a head, then values of a head) of n tokens
-    auto each = [&](int r, int c0, int n, auto f) {
-        const bool is_v = r >= j.kv_heads;
-        const int h = is_v ? r - j.kv_heads : r, units = is_v ? units_plain : units_rot;
-        const HeadRows& in = is_v ? j.v : j.k;
-        const T* src = static_cast<const T*>(in.p) + (t + c0) * in.token_stride + h * in.head_stride;
-        for (int w = lane; w < n * units; w += 64) {
-            const int token = w / units, u = w % units;
-            rotated_unit<T, N>(src + token * in.token_stride, cs[token], u, is_v ? 0 : rot, half,
-                               [&](int i, const float (&x)[N]) { f(i, x, c0 + token); });
-        }
-    };
-    for (int c0 = 0; c0 < count; c0 += kCosTokens) {
-        const int n = min(kCosTokens, count - c0);
-        if (keys) {
-            if (c0) __syncthreads();
-            turn(place + c0, n);
-            __syncthreads();
-        }
-        for (int r = r0 + wave; r < r1; r += 4) {
-            float most = 0.0f;
-            each(r, c0, n, [&](int, const float (&x)[N], int) {
-#pragma unroll
-                for (int k = 0; k < N; k++) most = fmaxf(most, fabsf(x[k]) < INFINITY ? fabsf(x[k]) : 0.0f);
-            });
-#pragma unroll
-            for (int x = 1; x < 64; x *= 2) most = fmaxf(most, __shfl_xor(most, x, 64));
-            if (lane == 0) top[r - r0] = c0 ? fmaxf(top[r - r0], most) : most;  // the same wave throughout
-        }
-    }
-    __builtin_amdgcn_wave_barrier();
-    for (int c0 = 0; c0 < count; c0 += kCosTokens) {
-        const int n = min(kCosTokens, count - c0);
-        if (keys && count > kCosTokens) {
-            __syncthreads();
-            turn(place + c0, n);
-            __syncthreads();
-        }
-        for (int r = r0 + wave; r < r1; r += 4) {
-            const bool is_v = r >= j.kv_heads;
-            const int h = is_v ? r - j.kv_heads : r;
-            uint8_t* dst = static_cast<uint8_t*>(is_v ? j.cache.v : j.cache.k) + at + h * (int64_t)j.cache.head_stride;
-            uint8_t* scale = (is_v ? j.s.v : j.s.k) + scale_at + h * j.s.head_stride;
-            const int slot = (int)j.cache.slot_stride;
-            int e = exponent_for(top[r - r0]);
-            if (before) {
-                // (a second pass finds the scale that the first wrote, which is e already)
-                const int old = min(max((int)*scale - 127, kLeast), kMost);
-                if (e > old && c0 == 0)
-                    for (int w = lane; w < before * (j.head_dim / 4); w += 64) {
-                        uint32_t* x = reinterpret_cast<uint32_t*>(dst - (int64_t)(before - w / (j.head_dim / 4)) * slot) +
-                                      w % (j.head_dim / 4);
-                        *x = shifted4(*x, old - e);
-                    }
-                e = max(e, old);
+    // One pass where a row of all tokens is held at once, else one for the maxima and one for the stores.
+    const int most_units = max(units_rot, units_plain);
+    const bool once = count <= kCosTokens && count * most_units <= 64 * kHeld;
+    for (int pass = once ? 1 : 0; pass < 2; pass++)
+        for (int c0 = 0; c0 < count; c0 += kCosTokens) {
+            const int n = min(kCosTokens, count - c0);
+            if (keys && (pass == 0 || once || count > kCosTokens)) {
+                if (pass || c0) __syncthreads();
+                turn(spot.place + c0, n);
+                __syncthreads();
             }
-            if (lane == 0 && c0 == 0) *scale = (uint8_t)(e + 127);
-            each(r, c0, n, [&](int i, const float (&x)[N], int token) { put8<N>(dst + (int64_t)token * slot + i, x, e); });
+            for (int r = r0 + wave; r < r1; r += 4) {
+                const bool is_v = r >= j.kv_heads;
+                const int h = is_v ? r - j.kv_heads : r, units = is_v ? units_plain : units_rot;
+                const HeadRows& in = is_v ? j.v : j.k;
+                const T* src = static_cast<const T*>(in.p) + (t + c0) * in.token_stride + h * in.head_stride;
+                uint8_t* scale = (is_v ? j.s.v : j.s.k) + scale_at + h * j.s.head_stride;
+                const int old = before ? min(max((int)*scale - 127, kLeast), kMost) : kLeast;
+                Held<T, N> held;
+                float top = 0.0f;
+                if (pass == 0 || once) {
+                    for (int w0 = 0; w0 < n * units; w0 += 64 * kHeld) {
+                        held.load(src, in.token_stride, w0, n, units, cs, is_v ? 0 : rot, half);
+                        top = fmaxf(top, held.top());
+                    }
+#pragma unroll
+                    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
+                    if (!once) {
+                        // the same wave has the row in both passes
+                        if (lane == 0) tops[r - r0] = c0 ? fmaxf(tops[r - r0], top) : top;
+                        continue;
+                    }
+                } else {
+                    top = tops[r - r0];
+                }
+                const int e = max(exponent_for(top), old);
+                const int slot = (int)j.cache.slot_stride;
+                uint8_t* dst = static_cast<uint8_t*>(is_v ? j.cache.v : j.cache.k) + at + h * (int64_t)j.cache.head_stride;
+                if (c0 == 0) {  // (later, `old` is what is stored here, which is e)
+                    const int words = j.head_dim / 4;
+                    if (before && e > old)
+                        for (int w = lane; w < before * words; w += 64) {
+                            uint32_t* x = reinterpret_cast<uint32_t*>(dst - (int64_t)(before - w / words) * slot) + w % words;
+                            *x = shifted4(*x, old - e);
+                        }
+                    if (lane == 0) *scale = (uint8_t)(e + 127);
+                }
+                dst += (int64_t)c0 * slot;
+                if (once) {
+                    held.put(dst, slot, e);
+                } else {
+                    for (int w0 = 0; w0 < n * units; w0 += 64 * kHeld) {
+                        held.load(src, in.token_stride, w0, n, units, cs, is_v ? 0 : rot, half);
+                        held.put(dst, slot, e);
+                    }
+                }
+            }
         }
-    }
 }
 
 }  // namespace
@@ -179,22 +304,21 @@ hipError_t launch_kv8_append(const RopeJob& job, const Scales& s, int type, hipS
     static_cast<RopeJob&>(j) = job;
     j.s = s;
     const int n = rope_access(j, type_bytes(type));
-    // workgroups to a token: the queries' heads and the rows of keys and values over as many
-    // as keep the chip busy
-    auto groups = [&](int rows, int64_t units, int least) {
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>({units, 1024 / j.tokens, (int64_t)rows}));
-        return (int)std::max<int64_t>(most, least);
-    };
-    j.q_groups = j.x_heads ? groups(j.x_heads, ((int64_t)j.x_heads * (j.head_dim / n) + kRopeThreads - 1) / kRopeThreads, 1) : 0;
-    if (j.q_groups) {
-        j.q_per = (j.x_heads + j.q_groups - 1) / j.q_groups;
-        j.q_groups = (j.x_heads + j.q_per - 1) / j.q_per;
-    }
+    // Queries: workgroups to a token as many as keep the chip busy.
+    const int64_t units = (int64_t)j.x_heads * (j.head_dim / n);
+    j.q_groups = (int)std::max<int64_t>(1, std::min<int64_t>({(units + kRopeThreads - 1) / kRopeThreads, 1024 / j.tokens,
+                                                              (int64_t)j.x_heads}));
+    j.q_per = (j.x_heads + j.q_groups - 1) / j.q_groups;
+    j.q_groups = j.q_per ? (j.x_heads + j.q_per - 1) / j.q_per : 1;
+    j.q_work = j.x_heads ? j.tokens * j.q_groups : 0;
+    // Keys and values: a row a wave where blocks are few, up to 8 where cosines of a block's
+    // tokens would be worked out by many workgroups.
+    const int64_t blocks = std::min<int64_t>(j.tokens, j.tokens / s.block + 2 * (int64_t)j.batch.batch);
     const int rows = 2 * j.kv_heads;
-    int kv_groups = groups(rows, (rows + 3) / 4, (rows + kMostRows - 1) / kMostRows);
-    j.rows_per = (rows + kv_groups - 1) / kv_groups;
-    kv_groups = (rows + j.rows_per - 1) / j.rows_per;
-    const dim3 grid((unsigned)j.tokens, (unsigned)(j.q_groups + kv_groups));
+    const int64_t wanted = std::max<int64_t>((rows + kMostRows - 1) / kMostRows, std::min<int64_t>((rows + 3) / 4, 2048 / blocks));
+    j.rows_per = (int)((rows + wanted - 1) / wanted);
+    j.kv_groups = (rows + j.rows_per - 1) / j.rows_per;
+    const dim3 grid((unsigned)(j.q_work + blocks * j.kv_groups));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         if (n == 8) {

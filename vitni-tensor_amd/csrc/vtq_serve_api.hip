@@ -1,8 +1,6 @@
 // vtq_serve_api.hip -- C entry points of the serving operators (the last part of
 // include/vtq.h): the checks of vtq_serve_checks.h, then the launchers of
 // vtq_serve.h.
-#include <climits>
-
 #include "vtq_serve.h"
 
 namespace {
@@ -265,7 +263,7 @@ int vtq_beam_select_device(vtq_ctx* ctx, int type, const void* d_logits, size_t 
 }
 
 size_t vtq_pages_reorder_workspace(size_t n_pages, size_t batch, size_t batch_out) {
-    if (n_pages > (size_t)INT_MAX || batch > kMostReordered || batch_out > kMostReordered) return 0;
+    if (n_pages > kMostPages || batch > kMostReordered || batch_out > kMostReordered) return 0;
     return pages_reorder_workspace((int64_t)n_pages, (int64_t)batch_out);
 }
 
@@ -289,7 +287,7 @@ int vtq_pages_reorder_device(vtq_ctx* ctx, size_t n_pages, int page_size, size_t
 }
 
 size_t vtq_pages_compact_workspace(size_t n_pages) {
-    return n_pages > (size_t)INT_MAX ? 0 : pages_compact_workspace((int64_t)n_pages);
+    return n_pages > kMostPages ? 0 : pages_compact_workspace((int64_t)n_pages);
 }
 
 int vtq_pages_compact_device(vtq_ctx* ctx, size_t n_pages, int page_size, const int32_t* d_refs, size_t n_entries,

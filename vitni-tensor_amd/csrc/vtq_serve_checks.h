@@ -280,6 +280,9 @@ inline Refusal check_kv8_append(const vtq_kv8_cache* cache, const vtq_kv_batch* 
                                 size_t q_out_token_stride, size_t q_out_head_stride) {
     VTQ_REFUSE(!cache || !batch, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
     if (Refusal r = check_cache8(cache)) return r;
+    // workgroups, one to 16 heads of a token at least, stay below 2^24 of 256 threads
+    VTQ_REFUSE(tokens > kMostTokens || tokens * (size_t)cache->cache.kv_heads > (size_t)1 << 26, VTQ_E_NOT_IMPLEMENTED,
+               "vtq: too many tokens or heads");
     return check_append_rows(&cache->cache, batch, rope, type, tokens, d_k, k_token_stride, k_head_stride, d_v,
                              v_token_stride, v_head_stride, heads, d_q, q_token_stride, q_head_stride, d_q_out,
                              q_out_token_stride, q_out_head_stride);
@@ -357,9 +360,12 @@ inline Refusal check_beam_select(int type, const void* d_logits, size_t ld, size
     return {};
 }
 
+// Each workgroup adds up the counts of 1024 pages.
+constexpr size_t kMostPages = (size_t)1 << 24;
+
 inline Refusal check_pages(size_t n_pages, int page_size, const int32_t* d_refs, const int32_t* d_new_refs,
                            const int32_t* d_copies, const int32_t* d_info) {
-    VTQ_REFUSE(n_pages > (size_t)INT_MAX, VTQ_E_NOT_IMPLEMENTED, "vtq: page count exceeds INT_MAX");
+    VTQ_REFUSE(n_pages > kMostPages, VTQ_E_NOT_IMPLEMENTED, "vtq: more than 2^24 pages");
     VTQ_REFUSE(page_size < 8 || page_size > 4096 || (page_size & (page_size - 1)), VTQ_E_INVALID_SHAPE,
                "vtq: page_size must be a power of two, 8 to 4096");
     VTQ_REFUSE((n_pages && (!d_refs || !d_new_refs)) || !d_info, VTQ_E_INVALID_ARGUMENT, "vtq: null pointer");
@@ -409,8 +415,9 @@ inline Refusal check_pages_compact(size_t n_pages, int page_size, const int32_t*
 
 inline Refusal check_copies(const vtq_kv_cache* c, size_t layers, size_t layer_stride, const int32_t* d_copies,
                             size_t max_copies, const int32_t* d_count) {
-    VTQ_REFUSE(layers > 65535 || layers * (size_t)c->kv_heads > (size_t)1 << 24 || max_copies > (size_t)INT_MAX,
-               VTQ_E_NOT_IMPLEMENTED, "vtq: too many layers or copies");
+    VTQ_REFUSE(layers > 65535 || max_copies > (size_t)INT_MAX, VTQ_E_NOT_IMPLEMENTED, "vtq: too many layers or copies");
+    VTQ_REFUSE((size_t)c->kv_heads * c->page_size * c->head_dim > (size_t)1 << 31, VTQ_E_NOT_IMPLEMENTED,
+               "vtq: pages of more than 2^31 elements");
     VTQ_REFUSE(layer_stride >= kMostStride || layers * (layer_stride / 8) > (size_t)1 << 43, VTQ_E_NOT_IMPLEMENTED,
                "vtq: layer stride too large");
     VTQ_REFUSE(layers > 1 && layer_stride == 0, VTQ_E_INVALID_SHAPE, "vtq: layers overlap");
