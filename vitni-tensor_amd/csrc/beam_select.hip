@@ -6,11 +6,9 @@
 // up to 8192 of a row in its registers, sums their exponentials below their maximum, and
 // leaves its n greatest.  A second launch, a workgroup a group, joins sums and lists.
 //
-// Which of two sums is greater decides about tokens, so s is f64, and a row's sum of
-// exponentials right to some 2^-30 (f32 would leave s wrong by 2^-20 of itself and more,
-// and equal where it is not).  The few logits near the maximum go through a polynomial in
-// f64, gathered so that all lanes have some; the many below, which count for little, through
-// f32.  Where many are near, all go through f64.
+// Which of two sums is greater decides about tokens, so s and a row's sum of exponentials
+// are f64 (f32 would leave s wrong by 2^-20 of itself and more, and equal where it is
+// not); f64 additions and products run at the f32 rate here.
 //
 // The n greatest of a workgroup: with T the n-th greatest of the 64 lanes' maxima of a
 // wave, n elements at least reach T, so only those that do are looked at (a few times
@@ -25,8 +23,7 @@ namespace vtq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kNear = 1024;      // logits near the maximum that are gathered
-constexpr int kGather = 512;     // candidates that a workgroup ranks by counting
+constexpr int kGather = 192;     // candidates that a wave gathers to be ranked by counting
 constexpr int kJoinGather = 1024;
 
 struct Part {
@@ -36,7 +33,7 @@ struct Part {
 
 struct BeamJob : BeamSelect {
     int splits;      // workgroups of a row
-    uint2* lists;    // [rows][splits][n_out], falling: logit (f32 bits) and token; token -1: no more
+    uint2* lists;    // [rows][n_out][splits], falling: logit (f32 bits) and token; token -1: no more
     Part* parts;     // [rows][splits]
 };
 
@@ -49,26 +46,27 @@ __device__ __forceinline__ float from_ordered(uint32_t u) {
     return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
 
-// exp(y), y <= 0, to 2^-40 of itself; 0 below -80.
+// exp(y), y <= 0, to 2^-34 of itself; below -700, exp(-700).  Two to the nearest whole number of
+// y log2 e, times the polynomial through e^z at the 8 Chebyshev points of |z| <= ln 2 / 2.
 __device__ __forceinline__ double exp_of(double y) {
-    const double t = y * 1.4426950408889634074;
     const double round = 6755399441055744.0;  // 1.5 * 2^52: the sum's last bits are the nearest whole number
-    const double shifted = t + round;
-    const double z = (t - (shifted - round)) * 0.69314718055994530942;
-    double p = 1.0 / 3628800.0;
-    p = fma(p, z, 1.0 / 362880.0);
-    p = fma(p, z, 1.0 / 40320.0);
-    p = fma(p, z, 1.0 / 5040.0);
-    p = fma(p, z, 1.0 / 720.0);
-    p = fma(p, z, 1.0 / 120.0);
-    p = fma(p, z, 1.0 / 24.0);
-    p = fma(p, z, 1.0 / 6.0);
-    p = fma(p, z, 0.5);
-    p = fma(p, z, 1.0);
-    p = fma(p, z, 1.0);
-    const uint64_t bits = (uint64_t)__double_as_longlong(p) + ((uint64_t)(uint32_t)__double_as_longlong(shifted) << 52);
-    return y < -80.0 ? 0.0 : __longlong_as_double((long long)bits);
+    y = fmax(y, -700.0);
+    const double shifted = fma(y, 1.4426950408889634074, round);
+    const double z = fma(shifted - round, -0.69314718055994530942, y);
+    double p = 0.00019907569324043077;
+    p = fma(p, z, 0.0013948578338415058);
+    p = fma(p, z, 0.008333283538688762);
+    p = fma(p, z, 0.041666218319112464);
+    p = fma(p, z, 0.16666666786308657);
+    p = fma(p, z, 0.500000010772923);
+    p = fma(p, z, 0.999999999995509);
+    p = fma(p, z, 0.9999999999595617);
+    // times two to that number
+    return __hiloint2double(__double2hiint(p) + (__double2loint(shifted) << 20), __double2loint(p));
 }
+
+// The greater number; NaN if one is none.
+__device__ __forceinline__ float greater(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
@@ -77,7 +75,7 @@ __device__ __forceinline__ double wave_sum(double x) {
 }
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) x = fmaxf(x, __shfl_xor(x, d, 64));
+    for (int d = 1; d < 64; d *= 2) x = greater(x, __shfl_xor(x, d, 64));
     return x;
 }
 
@@ -96,25 +94,6 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&key)[K], int n) 
     return t;
 }
 
-// Calls put(place, key) for each of the n greatest of c different numbers in LDS.
-template <class Put>
-__device__ __forceinline__ void rank_keys(const uint64_t* keys, int c, int n, Put put) {
-    for (int i = threadIdx.x; i < c; i += kThreads) {
-        const uint64_t mine = keys[i];
-        int above = 0, k = 0;
-        // LDS's latency is what this costs: 8 numbers at a time
-        for (; k + 8 <= c; k += 8) {
-            uint64_t other[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) other[e] = keys[k + e];
-#pragma unroll
-            for (int e = 0; e < 8; e++) above += other[e] > mine;
-        }
-        for (; k < c; k++) above += keys[k] > mine;
-        if (above < n) put(above, mine);
-    }
-}
-
 // ------------------------------------------------ lists of a row's parts
 
 template <class T, int E>
@@ -126,24 +105,23 @@ __global__ __launch_bounds__(kThreads) void list_kernel(BeamJob j) {
     const T* x0 = static_cast<const T*>(j.logits) + row * j.ld;
     const int first = split * kThreads * E;
     // element l V + e of this thread is token first + (l 256 + tid) V + e
-    float x[E];
+    // Rows start at any element.  (Loads from the next multiple of 16 bytes on would give a
+    // row's sum another order for each start, and rows of the same logits another sum.)
+    typedef T vec __attribute__((ext_vector_type(V)));
+    typedef T vec_anywhere __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    vec raw[L];
 #pragma unroll
     for (int l = 0; l < L; l++) {
         const int at = first + (l * kThreads + tid) * V;
-        // Rows start at any element.  (Loads from the next multiple of 16 bytes on would give a
-        // row's sum another order for each start, and rows of the same logits another sum.)
-        typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
         if (at + V <= j.vocab) {
-            const vec v = *reinterpret_cast<const vec*>(x0 + at);
-#pragma unroll
-            for (int e = 0; e < V; e++) x[l * V + e] = (float)v[e];
+            raw[l] = *reinterpret_cast<const vec_anywhere*>(x0 + at);
         } else {
             // past the row: below every number, so that only a comparison by token tells it from -infinity
 #pragma unroll
-            for (int e = 0; e < V; e++)
-                x[l * V + e] = at + e < j.vocab ? (float)x0[at + e] : -INFINITY;
+            for (int e = 0; e < V; e++) raw[l][e] = at + e < j.vocab ? x0[at + e] : (T)-INFINITY;
         }
     }
+    auto x = [&](int i) { return (float)raw[i / V][i % V]; };
     auto token_of = [&](int i) { return first + (i / V * kThreads + tid) * V + i % V; };
     auto in_row = [&](int token) { return token < j.vocab; };
 
@@ -151,11 +129,11 @@ __global__ __launch_bounds__(kThreads) void list_kernel(BeamJob j) {
     float part[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        part[k] = x[k];
+        part[k] = x(k);
 #pragma unroll
-        for (int i = k + 4; i < E; i += 4) part[k] = fmaxf(part[k], x[i]);
+        for (int i = k + 4; i < E; i += 4) part[k] = greater(part[k], x(i));
     }
-    float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    float top = greater(greater(part[0], part[1]), greater(part[2], part[3]));  // NaN if a logit is
     uint32_t reach;
     if (n <= 16) {
         const uint32_t key[1] = {ordered(top)};
@@ -167,96 +145,94 @@ __global__ __launch_bounds__(kThreads) void list_kernel(BeamJob j) {
     top = wave_max(top);
     __shared__ float tops[4];
     __shared__ uint32_t reaches[4];
-    __shared__ int nears[4], reachings[4], more;
+    __shared__ int counts[4];  // candidates that a wave gathered; more than kGather: too many
     __shared__ double sums[4];
-    __shared__ float near[kNear];
-    __shared__ __attribute__((aligned(16))) uint64_t keys[kGather];
+    __shared__ __attribute__((aligned(16))) uint64_t keys[4][kGather];
     if (lane == 0) tops[wave] = top, reaches[wave] = reach;
-    if (tid == 0) more = 0;
     __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    top = greater(greater(tops[0], tops[1]), greater(tops[2], tops[3]));
     reach = max(max(reaches[0], reaches[1]), max(reaches[2], reaches[3]));
     const int64_t list = (int64_t)row * j.splits + split;
-    const float base = top == -INFINITY ? 0.0f : top;
+    if (!(top < INFINITY)) {
+        // the row's candidates are all alike: its lists are not read
+        if (tid == 0) j.parts[list] = Part{__longlong_as_double(0x7FF8000000000000ll), 0.0f};
+        return;
+    }
+    const double base = top == -INFINITY ? 0.0 : (double)top;
     // T; no number, or -infinity, where fewer than n lanes hold any: then all that is finite
     const float limit = from_ordered(reach);
     const bool masks = !(limit > -INFINITY);
     const float least = masks ? -3.402823466e38f : limit;
-    // Near the top: within 5, where the exponential's own error of 2^-24 is what an element's
-    // below is off by; of f32 logits, whose differences round, within 8.
-    const float close = base - (sizeof(T) == 4 ? 8.0f : 5.0f);
-    uint64_t is_near[E], reaches_t[E];
-    int n_near = 0, n_reach = 0;
-    float small = 0.0f;  // sum of the others; no number if a logit is none
-#pragma unroll
-    for (int i = 0; i < E; i++) {
-        const bool in = x[i] >= close;
-        is_near[i] = __ballot(in);
-        reaches_t[i] = __ballot(x[i] >= least);
-        n_near += __popcll(is_near[i]);
-        n_reach += __popcll(reaches_t[i]);
-        const float y = in ? -INFINITY : x[i] - base;
-        // 2^(y log2 e), the product's rounding and the constant's put back
-        const float t = y * 1.44269504088896340736f;
-        const float rest = fmaf(y, 1.44269504088896340736f, -t) + y * 1.92596299112661746e-8f;
-        const float p = __builtin_amdgcn_exp2f(t);
-        small += y > -200.0f ? fmaf(p, rest * 0.69314718055994530942f, p) : y == y ? 0.0f : y;
-    }
-    // places in the order of waves, so that sums have one order
-    if (lane == 0) nears[wave] = n_near, reachings[wave] = n_reach;
-    __syncthreads();
-    int near_at = 0, reach_at = 0;
-    n_near = n_reach = 0;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        near_at += w < wave ? nears[w] : 0, reach_at += w < wave ? reachings[w] : 0;
-        n_near += nears[w], n_reach += reachings[w];
-    }
-    const bool few_near = n_near <= kNear, few = n_reach <= kGather;
     auto below = [&](uint64_t mask) {
         return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
     };
     // a candidate as a number: greater logits, then lower tokens are greater
     auto key_of = [&](float v, int token) { return (uint64_t)ordered(v) << 32 | (uint32_t)~token; };
+    int n_reach = 0;
+    double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; i++) {
-        if (few_near && is_near[i]) {
-            if (is_near[i] >> lane & 1) near[near_at + below(is_near[i])] = x[i];
-            near_at += __popcll(is_near[i]);
+        const float v = x(i);
+        const bool reaches_t = v >= least;
+        sum += exp_of((double)v - base);
+        const uint64_t reaching = __ballot(reaches_t);
+        if (reaching) {
+            const int to = n_reach + below(reaching);
+            if (reaches_t && to < kGather) keys[wave][to] = key_of(v, token_of(i));
+            n_reach += __popcll(reaching);
         }
-        if (few && reaches_t[i]) {
-            if (reaches_t[i] >> lane & 1) keys[reach_at + below(reaches_t[i])] = key_of(x[i], token_of(i));
-            reach_at += __popcll(reaches_t[i]);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // more at once would not fit the registers
+    }
+    // What is rare reads the logits again, where they are near by, and keeps no registers.
+    auto again = [&](int token) { return token < j.vocab ? (float)x0[token] : -INFINITY; };
+    // Of masked tokens, of which there may be many, n will do that come first: n of the wave's
+    // first n + n_reach tokens are masked.
+    const int window = n + n_reach;
+    if (masks && n_reach + window <= kGather) {
+        for (int i0 = 0; i0 < window; i0 += 64) {
+            const int i = i0 + lane, token = first + (i / (64 * V) * kThreads + wave * 64) * V + i % (64 * V);
+            const bool takes = i < window && i < 64 * E && token < j.vocab && again(token) == -INFINITY;
+            const uint64_t taking = __ballot(takes);
+            if (takes) keys[wave][n_reach + below(taking)] = key_of(-INFINITY, token);
+            n_reach += __popcll(taking);
         }
-    }
-    // Of masked tokens, of which there may be many, n will do that come first: n of the first
-    // n + n_reach tokens are masked.
-    const int window = masks ? min(n + n_reach, min(kThreads * E, j.vocab - first)) : 0;
-    const bool fits = few && n_reach + window <= kGather;
-    if (fits && window) {
-#pragma unroll
-        for (int i = 0; i < E; i++)
-            if (x[i] == -INFINITY && token_of(i) < first + window) keys[n_reach + atomicAdd(&more, 1)] = key_of(x[i], token_of(i));
-    }
-    __syncthreads();
-    double sum = (double)(few_near ? small : small * 0.0f);
-    if (few_near) {
-        for (int i = tid; i < n_near; i += kThreads) sum += exp_of((double)near[i] - (double)base);
-    } else {
-#pragma unroll
-        for (int i = 0; i < E; i++) sum += exp_of((double)x[i] - (double)base);
+    } else if (masks) {
+        n_reach = kGather + 1;
     }
     sum = wave_sum(sum);
-    if (lane == 0) sums[wave] = sum;
-    uint2* out = j.lists + list * n;
-    auto put = [&](int at, float v, int token) { out[at] = make_uint2(__float_as_uint(v), (uint32_t)token); };
-    const int c = n_reach + more;
-    if (fits) rank_keys(keys, c, n, [&](int at, uint64_t key) { put(at, from_ordered((uint32_t)(key >> 32)), ~(int)(uint32_t)key); });
+    if (lane == 0) {
+        counts[wave] = min(n_reach, kGather + 1);
+        sums[wave] = sum;
+    }
     __syncthreads();
-    if (tid == 0)
-        j.parts[list] = Part{top < INFINITY ? (sums[0] + sums[1]) + (sums[2] + sums[3])
-                                            : __longlong_as_double(0x7FF8000000000000ll), top};
+    const int at1 = counts[0], at2 = at1 + counts[1], at3 = at2 + counts[2], c = at3 + counts[3];
+    const bool fits = max(max(counts[0], counts[1]), max(counts[2], counts[3])) <= kGather;
+    // (-infinities alone add up to nothing)
+    if (tid == 0) j.parts[list] = Part{top > -INFINITY ? (sums[0] + sums[1]) + (sums[2] + sums[3]) : 0.0, top};
+    uint2* out = j.lists + (int64_t)row * n * j.splits + split;
+    auto put = [&](int at, float v, int token) {
+        out[at * j.splits] = make_uint2(__float_as_uint(v), (uint32_t)token);
+    };
     if (fits) {
+        for (int i = tid; i < c; i += kThreads) {
+            const int w0 = (i >= at1) + (i >= at2) + (i >= at3);
+            const uint64_t mine = keys[w0][i - (w0 > 2 ? at3 : w0 > 1 ? at2 : w0 > 0 ? at1 : 0)];
+            int above = 0;
+            for (int w = 0; w < 4; w++) {
+                const int m = counts[w];
+                int k = 0;
+                // LDS's latency is what this costs: 8 numbers at a time
+                for (; k + 8 <= m; k += 8) {
+                    uint64_t other[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) other[e] = keys[w][k + e];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) above += other[e] > mine;
+                }
+                for (; k < m; k++) above += keys[w][k] > mine;
+            }
+            if (above < n) put(above, from_ordered((uint32_t)(mine >> 32)), ~(int)(uint32_t)mine);
+        }
         for (int i = c + tid; i < n; i += kThreads) put(i, -INFINITY, -1);
         return;
     }
@@ -268,11 +244,12 @@ __global__ __launch_bounds__(kThreads) void list_kernel(BeamJob j) {
     for (int k = 0; k < n; k++) {
         float best = -INFINITY;
         int best_at = INT32_MAX;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < E; i++) {
             const int token = token_of(i);
-            const bool after = x[i] < last_x || (x[i] == last_x && token > last_at);
-            if (in_row(token) && after && (x[i] > best || (x[i] == best && token < best_at))) best = x[i], best_at = token;
+            const float v = again(token);
+            const bool after = v < last_x || (v == last_x && token > last_at);
+            if (in_row(token) && after && (v > best || (v == best && token < best_at))) best = v, best_at = token;
         }
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -308,77 +285,86 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
     return a.row != b.row ? a.row < b.row : a.token < b.token;
 }
 
-// HELD entries of the lists to a thread, in registers, all at once; 0: any number of lists,
-// read as far as they matter.
-template <int HELD>
-__global__ __launch_bounds__(kThreads) void join_kernel(BeamJob j) {
+// The number that e^y is, to 2^-33 of it: one step of Newton's from f32's.
+__device__ __forceinline__ double log_of(double x) {
+    const double y = (double)(__builtin_amdgcn_logf((float)x) * 0.69314718055994530942f);
+    return y + (x * exp_of(-y) - 1.0);
+}
+
+// HELD entries of a list to a thread, in registers: a power of two of threads, 2^list_bits,
+// have the lists side by side, and the next as many their next places.  HELD 0: any number of
+// lists, read as far as they matter.  (A group is one workgroup, which goes through its code
+// once: what it waits for is memory, and the code is part of that.)
+template <int HELD, int THREADS>
+__global__ __launch_bounds__(THREADS) void join_kernel(BeamJob j, int list_bits) {
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int n = j.n_out, beams = j.beams, splits = j.splits, lists = beams * splits;
     const int64_t row0 = (int64_t)blockIdx.x * beams;
     const uint2* entries = j.lists + row0 * splits * n;
+    constexpr int W = THREADS / 64;
     __shared__ double norm[64];  // ln of a row's sum
     __shared__ float score[64];
     __shared__ int kind[64];     // 0 lists, 1 one candidate, 2 all alike
-    __shared__ uint32_t reaches[4];
+    __shared__ uint32_t reaches[W];
     __shared__ int count;
     __shared__ __attribute__((aligned(16))) double got_s[kJoinGather];
     __shared__ float got_x[kJoinGather];
     __shared__ int got_at[kJoinGather], got_row[kJoinGather];
+    // heads first: many lanes have a great one, and few entries reach what n lanes do
+    const int own_list = tid & ((1 << list_bits) - 1), own_row = min(own_list, lists - 1) / splits;
+    const int own_split = min(own_list, lists - 1) - own_row * splits;
     uint2 held[HELD ? HELD : 1];
+    auto place_of = [&](int i) { return (tid >> list_bits) + i * (THREADS >> list_bits); };
 #pragma unroll
-    for (int i = 0; i < HELD; i++) held[i] = entries[min(i * kThreads + tid, lists * n - 1)];
+    for (int i = 0; i < HELD; i++) held[i] = entries[(own_row * n + min(place_of(i), n - 1)) * splits + own_split];
     if (tid == 0) count = 0;
     // `width` lanes to a row
-    int width = 1;
-    while (width < 64 && width < splits) width *= 2;
-    for (int r0 = 0; r0 < beams; r0 += kThreads / width) {
-        const int r = r0 + tid / width;
-        const bool there = r < beams, ended = there && j.done && j.done[row0 + r];
-        const Part* parts = j.parts + (row0 + (there ? r : 0)) * splits;
-        float top = -INFINITY;
-        if (there && !ended)
-            for (int s = tid % width; s < splits; s += width) top = fmaxf(top, parts[s].top);
-        for (int d = 1; d < width; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    int width_bits = 0;
+    while (width_bits < 6 && 1 << width_bits < splits) width_bits++;
+    const int width = 1 << width_bits;
+    for (int r0 = 0; r0 < beams; r0 += THREADS >> width_bits) {
+        const int r = r0 + (tid >> width_bits), s0 = tid & (width - 1);
+        const bool there = r < beams;
+        // all loads at once (of an ended row's parts too, which nobody wrote)
+        const int64_t row = row0 + (there ? r : 0);
+        const Part* parts = j.parts + row * splits;
+        const Part own = parts[min(s0, splits - 1)];
+        const bool ended = j.done && j.done[row];
+        const float cum = j.score[row];
+        float top = s0 < splits ? own.top : -INFINITY;
+        for (int s = s0 + width; s < splits; s += width) top = greater(top, parts[s].top);
+        for (int d = 1; d < width; d *= 2) top = greater(top, __shfl_xor(top, d, 64));
         double sum = 0.0;
-        if (there && !ended)
-            for (int s = tid % width; s < splits; s += width) {
-                // (a part of -infinities alone: its sum is 0)
-                const Part p = parts[s];
-                sum += p.sum == p.sum ? p.sum * exp_of((double)p.top - (double)top) : p.sum;
-            }
+        for (int s = s0; s < splits; s += width) {
+            const Part p = s == s0 ? own : parts[s];
+            sum += p.sum == p.sum ? p.sum * exp_of((double)p.top - (double)top) : p.sum;
+        }
         for (int d = 1; d < width; d *= 2) sum += __shfl_xor(sum, d, 64);
-        if (there && tid % width == 0) {
-            const double ln = (double)top + log(sum);
-            const float cum = j.score[row0 + r];
+        if (there && s0 == 0) {
+            // a row of -infinities alone, or of no numbers, has no logarithm
+            const double ln = sum > 0.0 ? (double)top + log_of(sum) : __longlong_as_double(0x7FF8000000000000ll);
             norm[r] = ln;
             score[r] = cum;
-            kind[r] = ended ? 1 : isfinite(ln) && isfinite(cum) ? 0 : 2;
+            kind[r] = ended ? 1 : ln == ln && fabsf(cum) < INFINITY ? 0 : 2;
         }
     }
     __syncthreads();
-    // entry `pos` of list l of the group; false: there is none
-    auto candidate = [&](int l, int pos, uint2 entry, Candidate& c) {
-        c.row = l / splits;
-        const int split = l - c.row * splits, what = kind[c.row];
-        if (what == 0) {
-            c.token = (int)entry.y;
-            c.x = __uint_as_float(entry.x);
-            c.s = (double)score[c.row] + ((double)c.x - norm[c.row]);
-            return c.token >= 0;
-        }
-        c.x = -INFINITY;
-        if (what == 1) {
-            c.token = j.end_token;
-            c.s = (double)score[c.row];
-            if (!isfinite(c.s)) c.s = -INFINITY;
-            else c.x = 0.0f;
-            return split == 0 && pos == 0;
-        }
-        c.token = pos;
-        c.s = -INFINITY;
-        return split == 0 && pos < j.vocab;
+    // entry `pos` of a row's list of `split`; false: there is none
+    auto candidate = [&](int row, int split, int pos, uint2 entry, Candidate& c) {
+        const int what = kind[row];
+        const float cum = score[row];
+        c.row = row;
+        c.token = what == 0 ? (int)entry.y : what == 1 ? j.end_token : pos;
+        const bool is = what == 0 ? c.token >= 0 : split == 0 && (what == 1 ? pos == 0 : pos < j.vocab);
+        const bool counts = what == 0 || (what == 1 && fabsf(cum) < INFINITY);
+        c.x = what == 0 ? __uint_as_float(entry.x) : counts ? 0.0f : -INFINITY;
+        c.s = counts ? (double)cum + (what == 0 ? (double)c.x - norm[row] : 0.0) : -INFINITY;
+        return is;
     };
-    auto load = [&](int l, int pos, Candidate& c) { return candidate(l, pos, entries[(int64_t)l * n + pos], c); };
+    auto load = [&](int l, int pos, Candidate& c) {
+        const int r = l / splits, split = l - r * splits;
+        return candidate(r, split, pos, entries[(r * n + pos) * splits + split], c);
+    };
     auto gather = [&](const Candidate& c) {
         const int at = atomicAdd(&count, 1);
         if (at < kJoinGather) got_s[at] = c.s, got_x[at] = c.x, got_row[at] = c.row, got_at[at] = c.token;
@@ -386,30 +372,32 @@ __global__ __launch_bounds__(kThreads) void join_kernel(BeamJob j) {
     // a thread's greatest, and what n threads of a wave reach
     uint32_t key[1] = {0};
     Candidate mine[HELD ? HELD : 1];
-    bool is[HELD ? HELD : 1];
+    uint32_t keys[HELD ? HELD : 1];
     if constexpr (HELD > 0) {
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
-            const int e = i * kThreads + tid, l = e / n;
-            is[i] = e < lists * n && candidate(l, e - l * n, held[i], mine[i]);
-            if (is[i]) key[0] = max(key[0], ordered((float)mine[i].s));
+            const bool is = own_list < lists && place_of(i) < n && candidate(own_row, own_split, place_of(i), held[i], mine[i]);
+            keys[i] = is ? ordered((float)mine[i].s) : 0;
+            key[0] = max(key[0], keys[i]);
         }
     } else {
-        for (int l = tid; l < max(lists, kThreads); l += kThreads) {
+        for (int l = tid; l < max(lists, THREADS); l += THREADS) {
             Candidate c;
             if (l / lists < n && load(l % lists, l / lists, c)) key[0] = max(key[0], ordered((float)c.s));
         }
     }
-    const uint32_t reached = reached_by<1, 32>(key, n);
+    const uint32_t reached = reached_by<1, 24>(key, n);
     if (lane == 0) reaches[wave] = reached;
     __syncthreads();
-    const uint32_t reach = max(max(reaches[0], reaches[1]), max(reaches[2], reaches[3]));
+    uint32_t reach = 1;
+#pragma unroll
+    for (int w = 0; w < W; w++) reach = max(reach, reaches[w]);
     if constexpr (HELD > 0) {
 #pragma unroll
         for (int i = 0; i < HELD; i++)
-            if (is[i] && ordered((float)mine[i].s) >= reach) gather(mine[i]);
+            if (keys[i] >= reach) gather(mine[i]);
     } else {
-        for (int l = tid; l < lists; l += kThreads) {
+        for (int l = tid; l < lists; l += THREADS) {
             Candidate c;
             for (int pos = 0; pos < n && load(l, pos, c) && ordered((float)c.s) >= reach; pos++) gather(c);
         }
@@ -430,16 +418,16 @@ __global__ __launch_bounds__(kThreads) void join_kernel(BeamJob j) {
     };
     if (count <= kJoinGather) {
         const int c = count;
-        for (int i = tid; i < c; i += kThreads) {
+        for (int i = tid; i < c; i += THREADS) {
             const Candidate a{got_s[i], got_x[i], got_row[i], got_at[i]};
-            // by the sums, 8 at a time; where some are equal, by the rest too
+            // by the sums, 4 at a time; where some are equal, by the rest too
             int above = 0, equal = 0, k = 0;
-            for (; k + 8 <= c; k += 8) {
-                double other[8];
+            for (; k + 4 <= c; k += 4) {
+                double other[4];
 #pragma unroll
-                for (int e = 0; e < 8; e++) other[e] = got_s[k + e];
+                for (int e = 0; e < 4; e++) other[e] = got_s[k + e];
 #pragma unroll
-                for (int e = 0; e < 8; e++) above += other[e] > a.s, equal += other[e] == a.s;
+                for (int e = 0; e < 4; e++) above += other[e] > a.s, equal += other[e] == a.s;
             }
             for (; k < c; k++) above += got_s[k] > a.s, equal += got_s[k] == a.s;
             if (equal > 1 && above < n)
@@ -447,14 +435,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(BeamJob j) {
                     above += got_s[k] == a.s && before(Candidate{a.s, got_x[k], got_row[k], got_at[k]}, a);
             if (above < n) put(above, a);
         }
-        for (int i = c + tid; i < n; i += kThreads) put_none(i);
+        for (int i = c + tid; i < n; i += THREADS) put_none(i);
         return;
     }
     // Many alike: the first of all, n times.
     Candidate last{INFINITY, INFINITY, -1, -1};
     for (int k = 0; k < n; k++) {
         Candidate best{-INFINITY, -INFINITY, INT32_MAX, INT32_MAX};
-        for (int l = tid; l < lists; l += kThreads) {
+        for (int l = tid; l < lists; l += THREADS) {
             // the first of the list after the last one taken: a list falls
             Candidate c;
             int lo = 0, hi = n;
@@ -471,11 +459,11 @@ __global__ __launch_bounds__(kThreads) void join_kernel(BeamJob j) {
                               __shfl_xor(best.token, d, 64)};
             if (before(o, best)) best = o;
         }
-        const int slot = (k & 1) * 4;
+        const int slot = (k & 1) * W;
         if (lane == 0) got_s[slot + wave] = best.s, got_x[slot + wave] = best.x, got_row[slot + wave] = best.row,
                        got_at[slot + wave] = best.token;
         __syncthreads();
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < W; w++) {
             const Candidate o{got_s[slot + w], got_x[slot + w], got_row[slot + w], got_at[slot + w]};
             if (before(o, best)) best = o;
         }
@@ -529,11 +517,15 @@ hipError_t launch_beam_select(const BeamSelect& a, int type, hipStream_t stream)
         return hipSuccess;
     });
     if (e != hipSuccess) return e;
-    const int64_t entries = (int64_t)a.beams * j.splits * a.n_out;
-    const dim3 grid((unsigned)a.groups), block(kThreads);
-    if (entries <= 2 * kThreads) hipLaunchKernelGGL((join_kernel<2>), grid, block, 0, stream, j);
-    else if (entries <= 8 * kThreads) hipLaunchKernelGGL((join_kernel<8>), grid, block, 0, stream, j);
-    else hipLaunchKernelGGL((join_kernel<0>), grid, block, 0, stream, j);
+    const int lists_of = a.beams * j.splits;
+    int bits = 0;
+    while (1 << bits < lists_of) bits++;
+    const dim3 grid((unsigned)a.groups);
+    // places of a list that THREADS have at once, `held` to each
+    auto holds = [&](int threads, int held) { return 1 << bits <= threads && a.n_out <= held * (threads >> bits); };
+    if (holds(256, 2)) hipLaunchKernelGGL((join_kernel<2, 256>), grid, dim3(256), 0, stream, j, bits);
+    else if (holds(1024, 4)) hipLaunchKernelGGL((join_kernel<4, 1024>), grid, dim3(1024), 0, stream, j, bits);
+    else hipLaunchKernelGGL((join_kernel<0, 256>), grid, dim3(256), 0, stream, j, 0);
     return hipGetLastError();
 }
 
