@@ -8,14 +8,19 @@
 // and O^T += V^T P^T on 32x32 MFMAs, one pass with a running maximum and sum.  Tiles stay
 // 8 bits wide from memory to the registers, half the bytes of a 16-bit cache; the conversion to
 // bf16, two elements an instruction, multiplies by the block's power of two at no cost
-// and loses nothing (4 significant bits of 8).  Queries of 16 and 32 bits become sums of
-// one (bf16), two (f16) or three (f32) bf16 parts, exactly, and weights as many, so that every type
-// runs at the 16-bit products' rate.
+// and loses nothing (4 significant bits of 8).  bf16 queries meet bf16 keys; f16 ones meet
+// keys as f16, whose scores are scaled after; f32 ones are split into three bf16 parts,
+// exactly.  Weights are rounded to one (bf16), two (f16) or three (f32) bf16 parts, so
+// that every type runs at the 16-bit products' rate.
 //
 // K: a lane reads 16 elements of its key at once, for two products; the order of a head's
 // elements inside them is free as long as the query has the same.  V's transpose is the
 // 8-bit transposing read: 16 lanes give 8 keys x 16 elements and get an element of all 8
 // each, which are the keys that this half-wave's weights are of.
+//
+// Heads of more than 128 elements: a workgroup has half of the values' elements, and works
+// out all scores for them.  (The sums of all in one wave, 128 registers beside the query's 64,
+// spilled in every loop: 26 sequences of 7 behind 8099 keys, f16, 565 us.)
 #include <type_traits>
 
 #include "vtq_attention_rows.h"
@@ -68,41 +73,47 @@ struct Runs {
     int scale_k, scale_v;  // f32 bits
 };
 
-template <int D>
+template <int DK, int DV>
 struct Loader8 {
-    using T = Tile8<D>;
-    const char *k, *v;  // of this KV head
+    using TK = Tile8<DK>;
+    using TV = Tile8<DV>;
+    const char *k, *v;  // of this KV head; v: of this part of its elements
     const uint8_t *k_scale, *v_scale;
     int64_t page_bytes, scale_page;
     uint32_t slot_bytes;
-    int row_bytes, n_pages, page_shift, page_mask, block_shift;
-    uint32_t k_off[T::kLoads], v_off[T::kLoads];
+    int k_bytes, v_bytes, n_pages, page_shift, page_mask, block_shift;  // of a key's, of a value's row
+    uint32_t k_off[TK::kLoads], v_off[TV::kLoads];
 
-    __device__ __forceinline__ void init(const Job8& j, int head) {
+    __device__ __forceinline__ void init(const Job8& j, int head, int part) {
         const vtq_kv_cache& c = j.a.cache;
         const int64_t at = (int64_t)head * (int64_t)c.head_stride;
         k = static_cast<const char*>(c.k) + at;
-        v = static_cast<const char*>(c.v) + at;
+        v = static_cast<const char*>(c.v) + at + part * DV;
         k_scale = j.s.k + head * j.s.head_stride;
         v_scale = j.s.v + head * j.s.head_stride;
         page_bytes = (int64_t)c.page_stride;
         scale_page = j.s.page_stride;
         slot_bytes = (uint32_t)c.slot_stride;
-        row_bytes = c.head_dim;
+        k_bytes = c.head_dim;
+        v_bytes = min(c.head_dim - part * DV, DV);
         n_pages = (int)c.n_pages;
         page_shift = j.page_shift;
         page_mask = c.page_size - 1;
         block_shift = j.block_shift;
-        const int lane = threadIdx.x & 63, chunk = lane % T::kChunks;
+        const int lane = threadIdx.x & 63;
+        // chunks past head_dim read past the end: zeros
+        auto at_chunk = [&](int row, int c, int bytes) {
+            return c * 16 < bytes ? (uint32_t)row * slot_bytes + (uint32_t)c * 16 : 0x7FFFFFF0u;
+        };
 #pragma unroll
-        for (int i = 0; i < T::kLoads; i++) {
-            const int row = i * T::kLoadRows + lane / T::kChunks;
-            // chunks past head_dim read past the end: zeros
-            auto at_chunk = [&](int c) {
-                return c * 16 < row_bytes ? (uint32_t)row * slot_bytes + (uint32_t)c * 16 : 0x7FFFFFF0u;
-            };
-            k_off[i] = at_chunk(T::k_chunk(row, chunk));
-            v_off[i] = at_chunk(T::v_chunk(row, chunk));
+        for (int i = 0; i < TK::kLoads; i++) {
+            const int row = i * TK::kLoadRows + lane / TK::kChunks;
+            k_off[i] = at_chunk(row, TK::k_chunk(row, lane % TK::kChunks), k_bytes);
+        }
+#pragma unroll
+        for (int i = 0; i < TV::kLoads; i++) {
+            const int row = i * TV::kLoadRows + lane / TV::kChunks;
+            v_off[i] = at_chunk(row, TV::v_chunk(row, lane % TV::kChunks), v_bytes);
         }
     }
     // Holds the runs from `key`'s on.
@@ -133,56 +144,51 @@ struct Loader8 {
         s.v1 = __int_as_float(__builtin_amdgcn_readlane(p.scale_v, b));
         return s;
     }
-    // 16 keys from `key` on: K to lds, V to lds + v_at.
-    __device__ __forceinline__ void load16(const Runs& p, int key, uint32_t lds, uint32_t v_at) const {
+    // 16 keys from `key` on: K to k_lds, V to v_lds.
+    static constexpr int kLoads = TK::kLoads + TV::kLoads;
+    __device__ __forceinline__ void load16(const Runs& p, int key, uint32_t k_lds, uint32_t v_lds) const {
         const int lane = lane_of(p, key);
         const uint32_t low = (uint32_t)__builtin_amdgcn_readlane(p.low, lane);
         const int high = __builtin_amdgcn_readlane(p.high, lane);
         const int64_t at = (int64_t)(((uint64_t)(uint32_t)high << 32) | low);
         const int rows = min(16, p.keys - key);
-        int bytes = (rows - 1) * (int)slot_bytes + row_bytes;
-        bytes = rows > 0 ? bytes : 0;
-        bytes = high >= 0 ? bytes : 0;  // nothing is read at an address of no bytes
-        const __amdgpu_buffer_rsrc_t rk =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(k + at), (short)0, bytes, kWord3);
-        const __amdgpu_buffer_rsrc_t rv =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(v + at), (short)0, bytes, kWord3);
+        const int before = (rows - 1) * (int)slot_bytes;
+        const bool there = rows > 0 && high >= 0;  // nothing is read at an address of no bytes
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(k + at), (short)0,
+                                                                            there ? before + k_bytes : 0, kWord3);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(v + at), (short)0,
+                                                                            there ? before + v_bytes : 0, kWord3);
 #pragma unroll
-        for (int i = 0; i < T::kLoads; i++) load_to_lds<16>(rk, k_off[i], lds + 1024u * i);
+        for (int i = 0; i < TK::kLoads; i++) load_to_lds<16>(rk, k_off[i], k_lds + 1024u * i);
 #pragma unroll
-        for (int i = 0; i < T::kLoads; i++) load_to_lds<16>(rv, v_off[i], lds + v_at + 1024u * i);
+        for (int i = 0; i < TV::kLoads; i++) load_to_lds<16>(rv, v_off[i], v_lds + 1024u * i);
     }
 };
 
 // ------------------------------------------------ one tile of 32 keys
 
-template <class Q, int D>
+template <class Q, int DK, int DV>
 struct Compute8 {
-    using T = Tile8<D>;
-    static constexpr int P = std::is_same_v<Q, float> ? 3 : std::is_same_v<Q, _Float16> ? 2 : 1;  // parts
-    static constexpr bool kPairs = D <= 128;  // two tiles at a time, where registers allow
+    using TK = Tile8<DK>;
+    using TV = Tile8<DV>;
+    static constexpr bool kHalf = std::is_same_v<Q, _Float16>;
+    static constexpr int P = std::is_same_v<Q, float> ? 3 : kHalf ? 2 : 1;  // parts of a weight
+    static constexpr int PQ = kHalf ? 1 : P;                                 // parts of a query
+    static constexpr bool kPairs = DK <= 128 && P < 3;  // two tiles at a time, where registers allow
+    using K = std::conditional_t<kHalf, _Float16, __bf16>;
+    typedef K v8k __attribute__((ext_vector_type(8)));
     // q of row lane & 31: element d of 32 c + 16 h + 8 s + 0..7 is v[part][2 c + s]
     struct Query {
-        v8bf v[P][D / 16];
+        v8k v[PQ][DK / 16];
     };
     struct Weights {
         v8bf v[P][2];
     };
 
-    // x as a sum of P bf16 numbers (exact for a query's type)
-    __device__ __forceinline__ static void split(float x, __bf16 (&out)[P]) {
-#pragma unroll
-        for (int i = 0; i < P; i++) {
-            out[i] = (__bf16)x;
-            // an infinity's remainder would be no number: the first part has it all
-            if (i + 1 < P) x = fabsf(x) < INFINITY ? x - (float)out[i] : 0.0f;
-        }
-    }
-
     __device__ static void load_query(Query& q, const Q* p, bool valid, int head_dim) {
         const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
-        for (int s = 0; s < D / 16; s++) {
+        for (int s = 0; s < DK / 16; s++) {
             const int d = 32 * (s / 2) + 16 * h + 8 * (s & 1);
             const bool in = valid && d < head_dim;
             typedef Q v8q __attribute__((ext_vector_type(8)));
@@ -190,13 +196,16 @@ struct Compute8 {
             if (in) x = *reinterpret_cast<const v8q*>(p + d);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                if constexpr (P == 1) {
+                if constexpr (PQ == 1) {
                     q.v[0][s][e] = x[e];
                 } else {
-                    __bf16 part[P];
-                    split((float)x[e], part);
+                    float rest = x[e];
 #pragma unroll
-                    for (int i = 0; i < P; i++) q.v[i][s][e] = part[i];
+                    for (int i = 0; i < PQ; i++) {
+                        q.v[i][s][e] = (__bf16)rest;
+                        // an infinity's remainder would be no number: the first part has it all
+                        rest = fabsf(rest) < INFINITY ? rest - (float)q.v[i][s][e] : 0.0f;
+                    }
                 }
             }
         }
@@ -211,35 +220,110 @@ struct Compute8 {
         r[0] = x[0], r[1] = x[1], r[2] = y[0], r[3] = y[1], r[4] = z[0], r[5] = z[1], r[6] = w[0], r[7] = w[1];
         return r;
     }
+    // 8 elements of a key, scaled, or (f16 has not the exponents) as they are
+    __device__ __forceinline__ static v8k widen_key(uint32_t a, uint32_t b, float scale) {
+        if constexpr (kHalf) {
+            v8k r;
+            const auto x = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
+            const auto y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
+            const auto z = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false);
+            const auto w = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+            r[0] = x[0], r[1] = x[1], r[2] = y[0], r[3] = y[1], r[4] = z[0], r[5] = z[1], r[6] = w[0], r[7] = w[1];
+            return r;
+        } else {
+            return widen(a, b, scale);
+        }
+    }
     __device__ __forceinline__ static v16f mma(v8bf a, v8bf b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
-
-    // scores of 32 keys: register 4i + e is key 8i + 4h + e, row lane & 31
-    __device__ static v16f scores(const uint8_t* k, const Query& q, TileScales sc) {
-        const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
-        const float scale = row & 16 ? sc.k1 : sc.k0;
-        v16f s = {};
+    __device__ __forceinline__ static v16f mma_key(v8k a, v8k b, v16f c) {
+        if constexpr (kHalf) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+        else return mma(a, b, c);
+    }
+    // f16: scores of keys in the two blocks of 16 (registers 0 to 7, 8 to 15)
+    __device__ __forceinline__ static void scale_scores(v16f& s, TileScales sc) {
+        if constexpr (kHalf) {
 #pragma unroll
-        for (int c = 0; c < D / 32; c++) {
-            const v4u x = *reinterpret_cast<const v4u*>(k + row * T::kRow + T::k_chunk(row, 2 * c + h) * 16);
-            const v8bf a = widen(x[0], x[1], scale), b = widen(x[2], x[3], scale);
-#pragma unroll
-            for (int i = P - 1; i >= 0; i--) {  // small parts first
-                s = mma(a, q.v[i][2 * c], s);
-                s = mma(b, q.v[i][2 * c + 1], s);
-            }
+            for (int r = 0; r < 16; r++) s[r] *= r < 8 ? sc.k0 : sc.k1;
         }
-        return s;
     }
 
-    // elements 32 db + (lane & 31) of keys 16 i + 4 h + {0..3, 8..11}
-    __device__ __forceinline__ static v8bf values(const uint8_t* v, int db, int i, TileScales sc) {
+    // A tile's operands as they are in LDS, read ahead of their products.
+    struct Keys {
+        v4u x[DK / 32];
+    };
+    struct Values {
+        v2i x[DV / 32][2];
+    };
+    __device__ __forceinline__ static v4u key_at(const uint8_t* k, int c) {
+        const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+        return *reinterpret_cast<const v4u*>(k + row * TK::kRow + TK::k_chunk(row, 2 * c + h) * 16);
+    }
+    // elements 32 b + (lane & 31) of keys 16 i + 4 h + {0..3, 8..11}
+    __device__ __forceinline__ static v2i values_at(const uint8_t* v, int b, int i) {
         const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 15, r = n >> 1;
-        const int row = 16 * i + 4 * h + (r & 3) + 8 * (r >> 2), c = 2 * db + ((lane >> 4) & 1);
-        const uint8_t* at = v + row * T::kRow + T::v_chunk(row, c) * 16 + (n & 1) * 8;
-        const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(at));
-        return widen((uint32_t)x[0], (uint32_t)x[1], i ? sc.v1 : sc.v0);
+        const int row = 16 * i + 4 * h + (r & 3) + 8 * (r >> 2), c = 2 * b + ((lane >> 4) & 1);
+        const uint8_t* at = v + row * TV::kRow + TV::v_chunk(row, c) * 16 + (n & 1) * 8;
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(at));
+    }
+    __device__ __forceinline__ static void read_keys(Keys& r, const uint8_t* k) {
+#pragma unroll
+        for (int c = 0; c < DK / 32; c++) r.x[c] = key_at(k, c);
+    }
+    __device__ __forceinline__ static void read_values(Values& r, const uint8_t* v) {
+#pragma unroll
+        for (int b = 0; b < DV / 32; b++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) r.x[b][i] = values_at(v, b, i);
+    }
+    __device__ __forceinline__ static float key_scale(TileScales sc) { return threadIdx.x & 16 ? sc.k1 : sc.k0; }
+    // scores of 32 keys: register 4i + e is key 8i + 4h + e, row lane & 31
+    __device__ __forceinline__ static v16f scores(const uint8_t* k, const Query& q, TileScales sc) {
+        const float scale = key_scale(sc);
+        v16f s = {};
+#pragma unroll
+        for (int c = 0; c < DK / 32; c++) {
+            const v4u x = key_at(k, c);
+            const v8k a = widen_key(x[0], x[1], scale), b = widen_key(x[2], x[3], scale);
+#pragma unroll
+            for (int i = PQ - 1; i >= 0; i--) {  // small parts first
+                s = mma_key(a, q.v[i][2 * c], s);
+                s = mma_key(b, q.v[i][2 * c + 1], s);
+            }
+        }
+        scale_scores(s, sc);
+        return s;
+    }
+    // two tiles' scores, two chains of products that do not wait for each other
+    __device__ __forceinline__ static void scores(v16f (&s)[2], const Keys& k0, const Keys& k1, const Query& q, TileScales sc0,
+                                                  TileScales sc1) {
+        const float scale0 = key_scale(sc0), scale1 = key_scale(sc1);
+        s[0] = s[1] = v16f{};
+#pragma unroll
+        for (int c = 0; c < DK / 32; c++) {
+            const v8k a0 = widen_key(k0.x[c][0], k0.x[c][1], scale0), a1 = widen_key(k1.x[c][0], k1.x[c][1], scale1);
+            const v8k b0 = widen_key(k0.x[c][2], k0.x[c][3], scale0), b1 = widen_key(k1.x[c][2], k1.x[c][3], scale1);
+#pragma unroll
+            for (int i = PQ - 1; i >= 0; i--) {
+                s[0] = mma_key(a0, q.v[i][2 * c], s[0]);
+                s[1] = mma_key(a1, q.v[i][2 * c], s[1]);
+                s[0] = mma_key(b0, q.v[i][2 * c + 1], s[0]);
+                s[1] = mma_key(b1, q.v[i][2 * c + 1], s[1]);
+            }
+        }
+        scale_scores(s[0], sc0);
+        scale_scores(s[1], sc1);
+    }
+    __device__ __forceinline__ static void add_values(State<DV>& st, const Values& v, const Weights& w, TileScales sc) {
+#pragma unroll
+        for (int b = 0; b < DV / 32; b++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const v8bf x = widen((uint32_t)v.x[b][i][0], (uint32_t)v.x[b][i][1], i ? sc.v1 : sc.v0);
+#pragma unroll
+                for (int p = P - 1; p >= 0; p--) st.o[b] = mma(x, w.v[p][i], st.o[b]);
+            }
     }
 
     __device__ __forceinline__ static Weights weights(const v16f& p) {
@@ -248,29 +332,20 @@ struct Compute8 {
         for (int r = 0; r < 16; r++) {
             // As many parts as the query has: off by 2^-8 (bf16), 2^-16 (f16) or 2^-24 (f32) of each
             // at most.  The sum is of the unrounded ones, in f32.
-            __bf16 part[P];
-            split(p[r], part);
+            float rest = p[r];
 #pragma unroll
-            for (int i = 0; i < P; i++) w.v[i][r / 8][r & 7] = part[i];
+            for (int i = 0; i < P; i++) {
+                const __bf16 part = (__bf16)rest;
+                w.v[i][r / 8][r & 7] = part;
+                rest -= (float)part;
+            }
         }
         return w;
     }
 
-    __device__ __forceinline__ static void add_values(State<D>& st, const uint8_t* v, const Weights& w,
-                                                      TileScales sc) {
-#pragma unroll
-        for (int b = 0; b < D / 32; b++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const v8bf x = values(v, b, i, sc);
-#pragma unroll
-                for (int p = P - 1; p >= 0; p--) st.o[b] = mma(x, w.v[p][i], st.o[b]);
-            }
-    }
-
     // Scores of N tiles to weights, with the row's maximum and sum.
     template <int N>
-    __device__ __forceinline__ static void softmax(State<D>& st, Weights (&w)[N], v16f (&s)[N], float c) {
+    __device__ __forceinline__ static void softmax(State<DV>& st, Weights (&w)[N], v16f (&s)[N], float c) {
         float top = s[0][0];
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -286,7 +361,7 @@ struct Compute8 {
             st.m = moves ? top : st.m;
             st.l *= shrink;
 #pragma unroll
-            for (int b = 0; b < D / 32; b++) st.o[b] *= shrink;
+            for (int b = 0; b < DV / 32; b++) st.o[b] *= shrink;
         }
         // the difference first, then the scale: see cache_attention.hip
         const float base = st.m == -INFINITY ? 0.0f : st.m;
@@ -308,7 +383,7 @@ struct Compute8 {
         const uint8_t* at = v + 16 * late_lane();
         uint32_t any = 0;
 #pragma unroll 1
-        for (int i = 0; i < T::kBytes / 1024; i++) {
+        for (int i = 0; i < TV::kBytes / 1024; i++) {
             const v4u x = *reinterpret_cast<const v4u*>(at + 1024 * i);
 #pragma unroll
             for (int e = 0; e < 4; e++) any |= (x[e] & 0x7F7F7F7Fu) + 0x01010101u;
@@ -316,60 +391,63 @@ struct Compute8 {
         return __ballot((any & 0x80808080u) != 0) == 0;
     }
 
-    // The values of a tile that some row does not see whole.  low: the keys that the wave's
-    // rows see at least; there: keys that exist (later ones are zeros in LDS).
-    __device__ __forceinline__ static void add_edge(State<D>& st, const Weights& w, const uint8_t* v, int key, int limit,
-                                                    int low, int there, TileScales sc) {
-        if (low >= there) {
-            add_values(st, v, w, sc);
-            return;
-        }
-        // Some row sees less than what is there, and a weight of 0 does not silence a NaN: NaNs
-        // count as zeros here, and the rows that see one get it on top.
+    // The values of a tile that holds NaNs and that some row does not see whole: a weight of 0
+    // does not silence a NaN.  They count as zeros here, and the rows that see one get it on top.
+    __device__ __forceinline__ static void add_some(State<DV>& st, const Weights& w, const uint8_t* v, int key, int limit,
+                                                    TileScales sc) {
         const int h = (threadIdx.x & 63) >> 5;
         v8bf seen[2];
 #pragma unroll
         for (int r = 0; r < 16; r++)
             seen[r / 8][r & 7] = (__bf16)(key + 8 * (r / 4) + 4 * h + r % 4 < limit ? 1.0f : 0.0f);
 #pragma unroll
-        for (int b = 0; b < D / 32; b++) {
+        for (int b = 0; b < DV / 32; b++) {
             v16f bad = {};
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                v8bf x = values(v, b, i, sc), none;
+                const v2i x = values_at(v, b, i);
+                uint32_t number[2], none[2];  // codes: the numbers, and 1 (0x38) where there is none
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const bool number = (float)x[e] == (float)x[e];
-                    none[e] = number ? (__bf16)0.0f : (__bf16)1.0f;
-                    x[e] = number ? x[e] : (__bf16)0.0f;
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t is = ((((uint32_t)x[e] & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u;
+                    number[e] = (uint32_t)x[e] & ~(is * 255u);
+                    none[e] = is * 0x38u;
                 }
+                const v8bf y = widen(number[0], number[1], i ? sc.v1 : sc.v0);
 #pragma unroll
-                for (int p = P - 1; p >= 0; p--) st.o[b] = mma(x, w.v[p][i], st.o[b]);
-                bad = mma(none, seen[i], bad);
+                for (int p = P - 1; p >= 0; p--) st.o[b] = mma(y, w.v[p][i], st.o[b]);
+                bad = mma(widen(none[0], none[1], 1.0f), seen[i], bad);
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) st.o[b][r] += bad[r] > 0.0f ? __uint_as_float(0x7FC00000u) : 0.0f;
+            __builtin_amdgcn_sched_barrier(0);  // rare: few registers
         }
     }
 
     // Two tiles that every row sees whole: chains of products side by side, one maximum.
-    __device__ __forceinline__ static void pair(State<D>& st, const Query& q, const uint8_t* k, const uint8_t* v,
+    __device__ __forceinline__ static void pair(State<DV>& st, const Query& q, const uint8_t* k, const uint8_t* v,
                                                 TileScales s0, TileScales s1, float c) {
-        v16f s[2] = {scores(k, q, s0), scores(k + T::kBytes, q, s1)};
+        Keys k0, k1;
+        read_keys(k0, k);
+        read_keys(k1, k + TK::kBytes);
+        Values v0, v1;
+        read_values(v0, v);
+        v16f s[2];
+        scores(s, k0, k1, q, s0, s1);
+        read_values(v1, v + TV::kBytes);
         Weights w[2];
         softmax<2>(st, w, s, c);
-        add_values(st, v, w[0], s0);
-        add_values(st, v + T::kBytes, w[1], s1);
+        add_values(st, v0, w[0], s0);
+        add_values(st, v1, w[1], s1);
     }
 
-    // A tile from its keys to its values.  EDGE: some row may not see all of the 32 keys from
-    // `key` on; limit: keys that this lane's row sees.
-    template <bool EDGE>
-    __device__ __forceinline__ static void tile(State<D>& st, const Query& q, const uint8_t* k, const uint8_t* v,
-                                                TileScales sc, int key, int limit, int low, int there, float c) {
+    // A tile from its keys to its values.  edge: some row may not see all of the 32 keys from
+    // `key` on; limit: keys that this lane's row sees; low: that the wave's rows see at least;
+    // there: keys that exist (later ones are zeros in LDS).
+    __device__ __forceinline__ static void tile(State<DV>& st, const Query& q, const uint8_t* k, const uint8_t* v,
+                                                TileScales sc, bool edge, int key, int limit, int low, int there, float c) {
         v16f s[1] = {scores(k, q, sc)};
-        if constexpr (EDGE) {
-            if (low < there && all_numbers(v)) low = there;
+        if (edge) {
             const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
             for (int r = 0; r < 16; r++)
@@ -377,8 +455,13 @@ struct Compute8 {
         }
         Weights w[1];
         softmax<1>(st, w, s, c);
-        if constexpr (EDGE) add_edge(st, w[0], v, key, limit, low, there, sc);
-        else add_values(st, v, w[0], sc);
+        if (edge && low < there && !all_numbers(v)) {
+            add_some(st, w[0], v, key, limit, sc);
+        } else {
+            Values x;
+            read_values(x, v);
+            add_values(st, x, w[0], sc);
+        }
     }
 };
 
@@ -386,20 +469,23 @@ struct Compute8 {
 
 constexpr int kWaves8 = 4;
 
-template <class Q, int D>
+template <class Q, int DK, int DV>
 struct Config8 {
-    static constexpr int kTile = Tile8<D>::kBytes;
-    // two stages: of a tile of K and V a wave, or of two tiles shared.  The merge of the waves' rows
-    // takes 32 x D x 4 bytes of each.
-    static constexpr int kLds = kWaves8 * 4 * kTile;
-    static constexpr int kPerCu = kLds <= 80 * 1024 && !(std::is_same_v<Q, float> && D > 64) ? 2 : 1;
+    static constexpr int kTile = Tile8<DK>::kBytes + Tile8<DV>::kBytes;  // 32 keys of K and V
+    // two stages of a tile a wave, or four of two tiles shared; the merge of the waves' rows takes
+    // 32 x DV x 4 bytes of each
+    static constexpr int kLds = kWaves8 * 2 * kTile;
+    static_assert(2 * kTile >= 128 * DV, "the merge");
+    static constexpr int kPerCu = kLds <= 80 * 1024 && !(std::is_same_v<Q, float> && DK > 64) ? 2 : 1;
 };
 
-template <class Q, int D>
-__global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_attention_kernel(Job8 j) {
-    using T = Tile8<D>;
-    using X = Compute8<Q, D>;
-    constexpr int W = kWaves8;
+template <class Q, int DK, int DV>
+__global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void kv8_attention_kernel(Job8 j) {
+    using Cfg = Config8<Q, DK, DV>;
+    using TK = Tile8<DK>;
+    using TV = Tile8<DV>;
+    using X = Compute8<Q, DK, DV>;
+    constexpr int W = kWaves8, kParts = DK / DV;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float2 wave_ml[W][32];
     const Attention& a = j.a;
@@ -416,8 +502,8 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
     const int row_tiles = prefix ? j.prefix_rows : j.own_rows;
     const int splits = prefix ? j.prefix_splits : j.own_splits;
     const bool shared = prefix ? j.shared_prefix : j.shared_own;
-    const int row_tile = (int)(mine % row_tiles);
-    int unit = (int)(mine / row_tiles) * 8 + xcd;  // KV head, then key range, then sequence
+    const int row_tile = (int)(mine % row_tiles), part = (int)(mine / row_tiles % kParts);
+    int unit = (int)(mine / row_tiles / kParts) * 8 + xcd;  // KV head, then key range, then sequence
     const int kv_head = unit % kv_heads;
     unit /= kv_heads;
     const int split = unit % splits, seq = unit / splits;
@@ -446,8 +532,8 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
     }
     const int n_rows = (int)min((t1 - t0) * G, (int64_t)INT32_MAX);
     const int tile_rows = shared ? W * 32 : 32;
-    Loader8<D> from;
-    from.init(j, kv_head);
+    Loader8<DK, DV> from;
+    from.init(j, kv_head, part);
 
     // own workgroups take every row_tiles-th tile of a sequence's rows
     for (int r0 = row_tile * tile_rows; r0 < n_rows; r0 += row_tiles * tile_rows) {
@@ -469,11 +555,11 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
         const int tiles = end > k0 ? (end - k0 + 31) / 32 : 0;  // of 32 keys
         typename X::Query q;
         X::load_query(q, static_cast<const Q*>(a.q.p) + token * a.q.token_stride + head * a.q.head_stride, valid, hd);
-        State<D> st;
+        State<DV> st;
         st.m = -INFINITY;
         st.l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) st.o[i] = v16f{};
+        for (int i = 0; i < DV / 32; i++) st.o[i] = v16f{};
         if (tiles > 0) {
             const int whole = (first_limit - k0) / 32;  // tiles that every row sees whole
             runs.keys = end;  // past the last row's sight nothing is read
@@ -482,47 +568,51 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
                 if ((min(key + keys, runs.keys) - 1) / 16 - runs.first >= 64) from.hold(runs, key);
             };
             if (shared) {
-                // stages of two tiles (K, then V); a wave loads 16 of the 64 keys
-                constexpr int kStage = 4 * T::kBytes;
-                TileScales ahead0, ahead1;
-                auto load_stage = [&](int n, int at) {
-                    const int key = k0 + 64 * n;
-                    holds(key, 64);
-                    from.load16(runs, key + 16 * wave, lds0 + (uint32_t)(at * kStage + 16 * wave * T::kRow), 2 * T::kBytes);
-                    ahead0 = from.scales(runs, key);
-                    ahead1 = from.scales(runs, key + 32);
-                };
-                load_stage(0, 0);
+                // stages of two tiles (K, then V), S - 1 of them ahead; a wave loads 16 of the 64 keys
+                constexpr int kStage = 2 * Cfg::kTile, S = Cfg::kLds / kStage;
                 const int stages = (tiles + 1) / 2;
-                int n = 0;
+                int n = 0, at = 0;
+                // Every step loads a stage, past the end too (zeros from nowhere), so that the count of
+                // those in flight stays the same.
+                auto load_stage = [&](int m, int to) {
+                    const int key = k0 + 64 * m;
+                    // (what is held begins at the tiles at hand, whose scales are read from it too)
+                    if ((min(key + 64, runs.keys) - 1) / 16 - runs.first >= 64) from.hold(runs, k0 + 64 * n);
+                    const uint32_t stage = lds0 + (uint32_t)(to * kStage);
+                    from.load16(runs, key + 16 * wave, stage + 16 * wave * TK::kRow,
+                                stage + 2 * TK::kBytes + 16 * wave * TV::kRow);
+                };
+#pragma unroll
+                for (int i = 0; i < S - 1; i++) load_stage(i, i);
                 TileScales here0, here1;
-                // the stage that n is, and the next one's loads
+                // the stage that n is, and a later one's loads
                 auto next_stage = [&] {
-                    wait_vmcnt<0>();
+                    wait_vmcnt<(S - 2) * from.kLoads>();
                     // all waves have read what the loads after this overwrite
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
-                    here0 = ahead0, here1 = ahead1;
-                    load_stage(n + 1, (n & 1) ^ 1);  // past the end: zeros from nowhere
-                    return lds + (n & 1) * kStage;
+                    load_stage(n + S - 1, at == 0 ? S - 1 : at - 1);
+                    here0 = from.scales(runs, k0 + 64 * n), here1 = from.scales(runs, k0 + 64 * n + 32);
+                    const uint8_t* k = lds + at * kStage;
+                    at = at + 1 == S ? 0 : at + 1;
+                    return k;
                 };
                 if constexpr (X::kPairs) {
                     for (; 2 * n + 2 <= min(whole, tiles); n++) {
                         const uint8_t* k = next_stage();
-                        X::pair(st, q, k, k + 2 * T::kBytes, here0, here1, j.c);
+                        X::pair(st, q, k, k + 2 * TK::kBytes, here0, here1, j.c);
                     }
                 }
                 for (; n < stages; n++) {
                     const uint8_t* k = next_stage();
 #pragma unroll 1
-                    for (int i = 0; i < 2; i++, k += T::kBytes) {
+                    for (int i = 0; i < 2; i++) {
                         const int key = k0 + 64 * n + 32 * i;
                         const TileScales sc = i ? here1 : here0;
-                        if (!X::kPairs && 2 * n + i < whole)
-                            X::template tile<false>(st, q, k, k + 2 * T::kBytes, sc, key, limit, low, runs.keys, j.c);
-                        else if (2 * n + i < tiles && key < high)
-                            X::template tile<true>(st, q, k, k + 2 * T::kBytes, sc, key, limit, low, runs.keys, j.c);
+                        if (2 * n + i < tiles && key < high)
+                            X::tile(st, q, k + i * TK::kBytes, k + 2 * TK::kBytes + i * TV::kBytes, sc, 2 * n + i >= whole, key,
+                                    limit, low, runs.keys, j.c);
                     }
                 }
                 wait_vmcnt<0>();
@@ -532,13 +622,14 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
                 asm volatile("" ::: "memory");
             } else {
                 // a wave's two stages of a tile
-                uint8_t* mine8 = lds + wave * 4 * T::kBytes;
-                const uint32_t to = lds0 + (uint32_t)wave * 4 * T::kBytes;
+                uint8_t* mine8 = lds + wave * 2 * Cfg::kTile;
+                const uint32_t to = lds0 + (uint32_t)wave * 2 * Cfg::kTile;
                 auto load = [&](int n, int at) {
                     const int key = k0 + 32 * n;
                     holds(key, 32);
-                    from.load16(runs, key, to + at * 2 * T::kBytes, T::kBytes);
-                    from.load16(runs, key + 16, to + at * 2 * T::kBytes + 16 * T::kRow, T::kBytes);
+                    const uint32_t stage = to + (uint32_t)(at * Cfg::kTile);
+                    from.load16(runs, key, stage, stage + TK::kBytes);
+                    from.load16(runs, key + 16, stage + 16 * TK::kRow, stage + TK::kBytes + 16 * TV::kRow);
                     return from.scales(runs, key);
                 };
                 if (wave < tiles) {
@@ -546,19 +637,15 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
                     int n = wave, at = 0;
                     // Every step loads the tile two steps on, past the end too (zeros from nowhere), so
                     // that the count of those in flight stays the same.
-                    auto one = [&](auto edge) {
-                        const uint8_t* k = mine8 + at * 2 * T::kBytes;
-                        wait_vmcnt<4 * T::kLoads>();
+                    for (; n < tiles; n += W, at ^= 1) {
+                        const uint8_t* k = mine8 + at * Cfg::kTile;
+                        wait_vmcnt<2 * from.kLoads>();
                         asm volatile("" ::: "memory");
-                        X::template tile<decltype(edge)::value>(st, q, k, k + T::kBytes, here, k0 + 32 * n, limit, low,
-                                                                runs.keys, j.c);
+                        X::tile(st, q, k, k + TK::kBytes, here, n >= whole, k0 + 32 * n, limit, low, runs.keys, j.c);
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         here = next;
                         next = load(n + 2 * W, at);
-                        n += W, at ^= 1;
-                    };
-                    while (n < min(whole, tiles)) one(std::false_type{});
-                    while (n < tiles) one(std::true_type{});
+                    }
                     wait_vmcnt<0>();
                     asm volatile("" ::: "memory");
                 }
@@ -572,10 +659,10 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
             const int row = r0 + wave * 32 + (late & 31);
             if (row < n_rows) {
 #pragma unroll
-                for (int db = 0; db < D / 32; db++)
+                for (int db = 0; db < DV / 32; db++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int d = 32 * db + 8 * i + 4 * late_h;
+                        const int d = DV * part + 32 * db + 8 * i + 4 * late_h;
                         const v16f& o = st.o[db];
                         if (d < hd)
                             put_row<Q, 0>(j, out_split, t0 + row / G, kv_head * G + row % G, d,
@@ -584,24 +671,24 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
             }
         } else {
             // merge the waves' parts of the same rows, each in its own part of LDS
-            float* mine = reinterpret_cast<float*>(lds + wave * 4 * T::kBytes);
+            float* mine = reinterpret_cast<float*>(lds + wave * 2 * Cfg::kTile);
             const int row = late & 31;
             asm volatile("" ::: "memory");
 #pragma unroll
-            for (int db = 0; db < D / 32; db++)
+            for (int db = 0; db < DV / 32; db++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int c = (8 * db + 2 * i + late_h) ^ (row & 15);
                     const v16f& o = st.o[db];
-                    *reinterpret_cast<float4*>(mine + row * D + 4 * c) =
+                    *reinterpret_cast<float4*>(mine + row * DV + 4 * c) =
                         make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
             if (late_h == 0) wave_ml[wave][row] = make_float2(st.m, st.l);
             __syncthreads();
             const int rows = min(32, n_rows - r0);
-            for (int e = wave * 64 + late; e < rows * (D / 4); e += W * 64) {
-                const int rr = e / (D / 4), c = e % (D / 4);
-                if (4 * c >= hd) continue;
+            for (int e = wave * 64 + late; e < rows * (DV / 4); e += W * 64) {
+                const int rr = e / (DV / 4), c = e % (DV / 4), d = DV * part + 4 * c;
+                if (d >= hd) continue;
                 float m = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < W; w++) m = fmaxf(m, wave_ml[w][rr].x);
@@ -613,26 +700,26 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, D>::kPerCu)) void kv8_a
                     const float2 ml = wave_ml[w][rr];
                     const float f = __builtin_amdgcn_exp2f((ml.x - base) * j.c);
                     const float4 x = *reinterpret_cast<const float4*>(
-                        reinterpret_cast<const float*>(lds + w * 4 * T::kBytes) + rr * D + 4 * (c ^ (rr & 15)));
+                        reinterpret_cast<const float*>(lds + w * 2 * Cfg::kTile) + rr * DV + 4 * (c ^ (rr & 15)));
                     l = fmaf(ml.y, f, l);
                     o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
                 }
-                put_row<Q, 0>(j, out_split, t0 + (r0 + rr) / G, kv_head * G + (r0 + rr) % G, 4 * c, o, m, l);
+                put_row<Q, 0>(j, out_split, t0 + (r0 + rr) / G, kv_head * G + (r0 + rr) % G, d, o, m, l);
             }
             __syncthreads();
         }
     }
 }
 
-template <class Q, int D>
+template <class Q, int DK, int DV>
 hipError_t launch_of(const Job8& j, hipStream_t stream) {
-    constexpr int kLds = Config8<Q, D>::kLds;
-    const void* f = reinterpret_cast<const void*>(&kv8_attention_kernel<Q, D>);
+    constexpr int kLds = Config8<Q, DK, DV>::kLds;
+    const void* f = reinterpret_cast<const void*>(&kv8_attention_kernel<Q, DK, DV>);
     if (hipError_t e = allow_dynamic_lds(f, kLds + 2048)) return e;
-    hipLaunchKernelGGL((kv8_attention_kernel<Q, D>), dim3(8u * (unsigned)(j.prefix_per_xcd + j.own_per_xcd)),
+    hipLaunchKernelGGL((kv8_attention_kernel<Q, DK, DV>), dim3(8u * (unsigned)(j.prefix_per_xcd + j.own_per_xcd)),
                        dim3(kWaves8 * 64), kLds, stream, j);
     if (hipError_t e = hipGetLastError()) return e;
-    return launch_join<Q, D, 0>(j, stream);
+    return launch_join<Q, DK, 0>(j, stream);
 }
 
 }  // namespace
@@ -652,9 +739,9 @@ hipError_t launch_kv8_attention(const Attention& a, const Scales& s, int type, h
     place_parts(j);
     return with_type(type, [&](auto q) {
         using Q = decltype(q);
-        if (a.cache.head_dim <= 64) return launch_of<Q, 64>(j, stream);
-        if (a.cache.head_dim <= 128) return launch_of<Q, 128>(j, stream);
-        return launch_of<Q, 256>(j, stream);
+        if (a.cache.head_dim <= 64) return launch_of<Q, 64, 64>(j, stream);
+        if (a.cache.head_dim <= 128) return launch_of<Q, 128, 128>(j, stream);
+        return launch_of<Q, 256, 128>(j, stream);
     });
 }
 

@@ -123,15 +123,25 @@ inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batc
     return plan_attention(cache, batch, attention_cost(type, cache.type, cache.head_dim), tokens, heads);
 }
 
-// Over 8-bit caches: products of one, two or three 16-bit parts.
+// Over 8-bit caches: products of one, two or three 16-bit parts; heads of more than 128
+// elements in two parts, each a workgroup's, so twice as many of both.
 inline TileCost kv8_attention_cost(int type, int head_dim) {
-    const int d = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    const int d = head_dim <= 64 ? 64 : 128;
     const int parts = type == VTQ_TYPE_F32 ? 3 : type == VTQ_TYPE_F16 ? 2 : 1;
-    return {4, false, d > 128, (0.18 + 0.0025 * d) * (1 + parts) / 2};
+    return {4, false, head_dim > 128, (0.18 + 0.0025 * d) * (1 + parts) / 2};
 }
 inline AttentionPlan plan_kv8_attention(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens,
                                         int heads) {
-    return plan_attention(cache, batch, kv8_attention_cost(type, cache.head_dim), tokens, heads);
+    const int parts = cache.head_dim > 128 ? 2 : 1;
+    vtq_kv_cache part = cache;
+    part.kv_heads *= parts;
+    part.head_dim = cache.head_dim / parts;
+    AttentionPlan p = plan_attention(part, batch, kv8_attention_cost(type, cache.head_dim), tokens, heads * parts);
+    // a part's workgroups follow the other's on its XCD, where its L2 has the keys
+    auto up8 = [](int64_t x) { return (x + 7) / 8; };
+    p.prefix_per_xcd = (int)(up8((int64_t)cache.kv_heads * p.prefix_splits) * p.prefix_rows * parts);
+    p.own_per_xcd = (int)(up8((int64_t)cache.kv_heads * p.own_splits * batch.batch) * p.own_rows * parts);
+    return p;
 }
 
 }  // namespace vtq
