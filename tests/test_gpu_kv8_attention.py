@@ -117,6 +117,17 @@ def test_in_place(ctx, name, q_lens, prefix):
     assert y is q and torch.equal(y, want)
 
 
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("q_lens,own", [([1] * 64, 20), ([200, 70], 300), ([3] * 300, 40)])
+def test_in_place_of_long_heads(ctx, name, q_lens, own):
+    # two workgroups read a row of more than 128 elements, and each writes half of it
+    p = Paged8(q_lens, [max(own, n) for n in q_lens], 0, 2, 256, 16)
+    q = torch.randn(p.tokens, 8, 256, device="cuda").to(TYPES[name])
+    want, _ = _attend(ctx, p, q, 8, 0.1)
+    y, _ = _attend(ctx, p, q, 8, 0.1, y=q)
+    assert y is q and torch.equal(y, want)
+
+
 def test_rows_behind_the_last_sequence_stay(ctx):
     for prefix, n in ((0, 1), (100, 1), (100, 40), (3000, 1)):
         p = Paged8([n, n], [50, 60], prefix, 2, 64, 16)
@@ -190,6 +201,21 @@ def test_bytes_of_scales_outside_their_range(ctx):
     want, _, by, _ = attention8_exact(p, q, 1, 0.25)
     within(y2, want, by, "y of the largest scale")
     assert y2.isfinite().all()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_sums_of_the_largest_values(ctx, name):
+    # every value 448 x 2^119: their weighted mean is one too, their sum is none in f32
+    for q_lens, own, prefix in (([1, 1], [20, 300], 0), ([1, 3], [700, 40], 900), ([40], [70], 40), ([1], [33], 2000)):
+        for head_dim in (64, 128, 192):
+            p = Paged8(q_lens, own, prefix, 1, head_dim, 16)
+            p.vc.fill_(0x7E)
+            p.vs.fill_(246)
+            p.to_device()
+            q = torch.randn(p.tokens, 4, head_dim, generator=torch.Generator().manual_seed(3)).to(TYPES[name])
+            y, _ = _attend(ctx, p, q.cuda(), 4, head_dim**-0.5)
+            # sums of weights in f32, their rounded parts, the quotient and y: 2^-7 of bf16, 2^-13 of f32 at most
+            assert (y.double() / (448 * 2.0**119) - 1).abs().max() <= (2**-7 if name == "bf16" else 2**-13)
 
 
 def test_large_scores_and_one_dominant_key(ctx):

@@ -277,6 +277,9 @@ struct Compute8 {
 #pragma unroll
             for (int i = 0; i < 2; i++) r.x[b][i] = values_at(v, b, i);
     }
+    __device__ __forceinline__ static bool near_end(TileScales sc) {  // scales above 2^95; scalar as integers
+        return max(__float_as_int(sc.v0), __float_as_int(sc.v1)) > (222 << 23);
+    }
     __device__ __forceinline__ static float key_scale(TileScales sc) { return threadIdx.x & 16 ? sc.k1 : sc.k0; }
     // scores of 32 keys: register 4i + e is key 8i + 4h + e, row lane & 31
     __device__ __forceinline__ static v16f scores(const uint8_t* k, const Query& q, TileScales sc) {
@@ -345,7 +348,7 @@ struct Compute8 {
 
     // Scores of N tiles to weights, with the row's maximum and sum.
     template <int N>
-    __device__ __forceinline__ static void softmax(State<DV>& st, Weights (&w)[N], v16f (&s)[N], float c) {
+    __device__ __forceinline__ static void softmax(State<DV>& st, Weights (&w)[N], v16f (&s)[N], bool raise, float c) {
         float top = s[0][0];
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -354,11 +357,15 @@ struct Compute8 {
         const float2 both = halves(top);
         top = fmaxf(both.x, both.y);
         // m follows the maximum only once it is 8 powers of two behind: weights up to 256
-        // cost nothing, and rows rarely rescale
-        const bool moves = (top - st.m) * c > 8.0f;  // each row for itself
+        // cost nothing, and rows rarely rescale.  Beside values near f32's end m is 24 powers above
+        // the maximum, so that sums of them do not pass it
+        const float before = st.m;
+        float most = 8.0f;
+        if (raise) top += 24.0f / c, most = 0.0f;
+        const bool moves = (top - before) * c > most;  // each row for itself
         if (__ballot(moves)) {
-            const float shrink = moves ? __builtin_amdgcn_exp2f((st.m - top) * c) : 1.0f;
-            st.m = moves ? top : st.m;
+            const float shrink = moves ? __builtin_amdgcn_exp2f((before - top) * c) : 1.0f;
+            st.m = moves ? top : before;
             st.l *= shrink;
 #pragma unroll
             for (int b = 0; b < DV / 32; b++) st.o[b] *= shrink;
@@ -430,13 +437,14 @@ struct Compute8 {
         Keys k0, k1;
         read_keys(k0, k);
         read_keys(k1, k + TK::kBytes);
+        __builtin_amdgcn_sched_barrier(0);  // all on their way before the first is waited for
         Values v0, v1;
         read_values(v0, v);
         v16f s[2];
         scores(s, k0, k1, q, s0, s1);
         read_values(v1, v + TV::kBytes);
         Weights w[2];
-        softmax<2>(st, w, s, c);
+        softmax<2>(st, w, s, near_end(s0) || near_end(s1), c);
         add_values(st, v0, w[0], s0);
         add_values(st, v1, w[1], s1);
     }
@@ -454,7 +462,7 @@ struct Compute8 {
                 if (key + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[0][r] = -INFINITY;
         }
         Weights w[1];
-        softmax<1>(st, w, s, c);
+        softmax<1>(st, w, s, near_end(sc), c);
         if (edge && low < there && !all_numbers(v)) {
             add_some(st, w[0], v, key, limit, sc);
         } else {

@@ -137,6 +137,8 @@ inline AttentionPlan plan_kv8_attention(const vtq_kv_cache& cache, const vtq_kv_
     part.kv_heads *= parts;
     part.head_dim = cache.head_dim / parts;
     AttentionPlan p = plan_attention(part, batch, kv8_attention_cost(type, cache.head_dim), tokens, heads * parts);
+    // y may be q: no part writes rows that the other still reads, so they are joined even if alone
+    if (parts > 1 && p.prefix_splits + p.own_splits == 1) p.own_splits = 2;
     // a part's workgroups follow the other's on its XCD, where its L2 has the keys
     auto up8 = [](int64_t x) { return (x + 7) / 8; };
     p.prefix_per_xcd = (int)(up8((int64_t)cache.kv_heads * p.prefix_splits) * p.prefix_rows * parts);
