@@ -366,9 +366,11 @@ int vtq_kv8_append_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv
 
 /* vtq_attention_device over an 8-bit cache: its formulas, masks, limits and workspace
  * rules.  type, the queries' and y's, is F32, F16 or BF16.  Keys and values enter the
- * products as the numbers they stand for.  BF16 queries multiply as they are, F16
- * ones as the exact sum of two bf16 parts and F32 ones of three; weights are rounded
- * to as many: off by 2^-8, 2^-16 and 2^-24 of themselves at most. */
+ * products as the numbers they stand for.  BF16 and F16 queries multiply as they
+ * are, F32 ones as the exact sum of three bf16 parts; weights are rounded to one
+ * (BF16), two (F16) and three (F32) bf16 parts: off by 2^-8, 2^-16 and 2^-24 of
+ * themselves at most.  Heads of more than 128 elements count four times in the
+ * limit of workgroups. */
 size_t vtq_kv8_attention_workspace(const vtq_kv8_cache *cache, const vtq_kv_batch *batch, int type, size_t tokens,
                                    size_t heads);
 int vtq_kv8_attention_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv_batch *batch, int type,

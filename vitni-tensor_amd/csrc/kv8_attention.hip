@@ -361,7 +361,7 @@ struct Compute8 {
         // the maximum, so that sums of them do not pass it
         const float before = st.m;
         float most = 8.0f;
-        if (raise) top += 24.0f / c, most = 0.0f;
+        if (raise) top += fminf(24.0f / c, 1e38f), most = 0.0f;
         const bool moves = (top - before) * c > most;  // each row for itself
         if (__ballot(moves)) {
             const float shrink = moves ? __builtin_amdgcn_exp2f((before - top) * c) : 1.0f;

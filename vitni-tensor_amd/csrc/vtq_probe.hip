@@ -182,6 +182,19 @@ int vtqp_attention_plan(const vtq_kv_cache* cache, const vtq_kv_batch* batch, in
     __builtin_memcpy(out, &p, sizeof p);
     return VTQ_OK;
 }
+int vtqp_kv8_attention_plan(const vtq_kv8_cache* cache, const vtq_kv_batch* batch, int type, size_t tokens,
+                            size_t heads, int* out) {
+    if (vtq::Refusal r = vtq::check_cache8(cache)) return r.code;
+    const vtq_kv_cache* c = &cache->cache;
+    if (vtq::Refusal r = vtq::check_batch(batch, c, false)) return r.code;
+    if (!vtq::type_bytes(type) || !tokens || tokens > vtq::kMostTokens || !heads || heads > 65535 ||
+        heads % c->kv_heads || !batch->batch ||
+        !vtq::attention_fits(c, batch, tokens, heads, vtq::most_kv8_workgroups(c)))
+        return VTQ_E_INVALID_ARGUMENT;
+    const vtq::AttentionPlan p = vtq::plan_kv8_attention(*c, *batch, type, (int64_t)tokens, (int)heads);
+    __builtin_memcpy(out, &p, sizeof p);
+    return VTQ_OK;
+}
 int vtqp_own_chunk(int keys, int splits, int grain) { return vtq::own_chunk(keys, splits, grain); }
 
 // Where a place of a sequence begins in the cache (vtq_serve.h).

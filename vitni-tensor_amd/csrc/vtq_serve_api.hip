@@ -204,7 +204,7 @@ size_t vtq_kv8_attention_workspace(const vtq_kv8_cache* cache, const vtq_kv_batc
                                    size_t heads) {
     if (!cache || !batch || check_cache8(cache) || check_batch(batch, &cache->cache, false)) return 0;
     if (type_bytes(type) == 0 || tokens > kMostTokens || heads > 65535 || heads % cache->cache.kv_heads) return 0;
-    if (!attention_fits(&cache->cache, batch, tokens, heads)) return 0;
+    if (!attention_fits(&cache->cache, batch, tokens, heads, most_kv8_workgroups(&cache->cache))) return 0;
     if (tokens == 0 || heads == 0 || batch->batch == 0) return 0;
     return kv8_attention_workspace(cache->cache, *batch, type, (int64_t)tokens, (int)heads);
 }

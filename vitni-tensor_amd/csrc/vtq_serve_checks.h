@@ -112,11 +112,14 @@ inline Refusal check_rows(const void* p, size_t token_stride, size_t head_stride
 
 // Whether the launches stay below 2^32 threads: 256 of them to 4 rows of queries, and
 // to a sequence, KV head and 32 rows.
-inline bool attention_fits(const vtq_kv_cache* c, const vtq_kv_batch* b, size_t tokens, size_t heads) {
+inline bool attention_fits(const vtq_kv_cache* c, const vtq_kv_batch* b, size_t tokens, size_t heads,
+                           size_t most = (size_t)1 << 22) {
     const size_t max_q = (size_t)b->max_q < tokens ? (size_t)b->max_q : tokens;
     return tokens * heads <= (size_t)1 << 25 &&
-           (size_t)b->batch * (size_t)c->kv_heads * (max_q * (heads / (size_t)c->kv_heads) / 32 + 1) <= (size_t)1 << 22;
+           (size_t)b->batch * (size_t)c->kv_heads * (max_q * (heads / (size_t)c->kv_heads) / 32 + 1) <= most;
 }
+// Over an 8-bit cache two workgroups take a head of more than 128 elements, in two ranges at least.
+inline size_t most_kv8_workgroups(const vtq_kv_cache* c) { return (size_t)1 << (c->head_dim > 128 ? 20 : 22); }
 
 // A plan from its parameters.
 inline Refusal plan_rope(const vtq_rope_params* p, vtq_rope* out) {
@@ -290,11 +293,12 @@ inline Refusal check_kv8_append(const vtq_kv8_cache* cache, const vtq_kv_batch* 
 
 // What attention's arguments have to be with a cache of any type.
 inline Refusal check_attention_rows(const vtq_kv_cache* cache, const vtq_kv_batch* batch, int type, size_t tokens,
-                               size_t heads, const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_y,
-                                       size_t y_token_stride, size_t y_head_stride, float* d_lse, float scale) {
+                                    size_t heads, const void* d_q, size_t q_token_stride, size_t q_head_stride, void* d_y,
+                                    size_t y_token_stride, size_t y_head_stride, float* d_lse, float scale,
+                                    size_t most = (size_t)1 << 22) {
     VTQ_REFUSE(tokens > kMostTokens || heads > 65535, VTQ_E_NOT_IMPLEMENTED, "vtq: too many tokens or heads");
     VTQ_REFUSE(heads % cache->kv_heads, VTQ_E_INVALID_SHAPE, "vtq: heads must be a multiple of kv_heads");
-    VTQ_REFUSE(!attention_fits(cache, batch, tokens, heads), VTQ_E_NOT_IMPLEMENTED, "vtq: more than 2^25 rows of queries");
+    VTQ_REFUSE(!attention_fits(cache, batch, tokens, heads, most), VTQ_E_NOT_IMPLEMENTED, "vtq: more than 2^25 rows of queries");
     VTQ_REFUSE(!(scale > 0.0f && scale <= 1e30f), VTQ_E_INVALID_ARGUMENT, "vtq: scale must be positive, up to 1e30");
     if (tokens == 0 || heads == 0 || batch->batch == 0) return {};
     const size_t hd = cache->head_dim, es = type_bytes(type);
@@ -329,7 +333,7 @@ inline Refusal check_kv8_attention(const vtq_kv8_cache* cache, const vtq_kv_batc
     if (Refusal r = check_batch(batch, &cache->cache, true)) return r;
     VTQ_REFUSE(type_bytes(type) == 0, VTQ_E_NOT_IMPLEMENTED, "vtq: activation type not F32 / F16 / BF16");
     return check_attention_rows(&cache->cache, batch, type, tokens, heads, d_q, q_token_stride, q_head_stride, d_y,
-                                y_token_stride, y_head_stride, d_lse, scale);
+                                y_token_stride, y_head_stride, d_lse, scale, most_kv8_workgroups(&cache->cache));
 }
 
 constexpr size_t kMostKept = 64;  // continuations and beams of a group

@@ -6,7 +6,7 @@ from __future__ import annotations
 import ctypes
 import os
 
-from . import F32, LIB_DIR, Q4_0, Q4_K, Q5_0, Q6_K, Q8_0, REGIME_INTEGER, load_library
+from . import F32, Kv8Cache, LIB_DIR, Q4_0, Q4_K, Q5_0, Q6_K, Q8_0, REGIME_INTEGER, load_library
 
 _lib = None
 
@@ -40,6 +40,7 @@ def lib() -> ctypes.CDLL:
         L.vtqp_check_kv8_pages_copy.argtypes = [vp, vp, sz, sz, sz, vp, sz, vp]
         L.vtqp_i8_form.argtypes = [i, i, i]
         L.vtqp_attention_plan.argtypes = [vp, vp, i, sz, sz, ctypes.POINTER(i)]
+        L.vtqp_kv8_attention_plan.argtypes = [vp, vp, i, sz, sz, ctypes.POINTER(i)]
         L.vtqp_own_chunk.argtypes = [i, i, i]
         L.vtqp_slot_of.argtypes = [vp, vp, i, ctypes.c_int64]
         L.vtqp_slot_of.restype = ctypes.c_int64
@@ -69,9 +70,11 @@ PLAN = ("group", "page_shift", "prefix_rows", "prefix_splits", "prefix_chunk", "
 
 
 def attention_plan(cache, batch, ggml_type, tokens, heads):
-    """How vtq_attention_device splits a call (AttentionPlan of vtq_attention_plan.h); None where it is refused."""
+    """How vtq_attention_device, or for a Kv8Cache vtq_kv8_attention_device, splits a call (AttentionPlan of
+    vtq_attention_plan.h); None where it is refused."""
     out = (ctypes.c_int * len(PLAN))()
-    rc = lib().vtqp_attention_plan(cache.ref, batch.ref, ggml_type, tokens, heads, out)
+    ask = lib().vtqp_kv8_attention_plan if isinstance(cache, Kv8Cache) else lib().vtqp_attention_plan
+    rc = ask(cache.ref, batch.ref, ggml_type, tokens, heads, out)
     return None if rc else dict(zip(PLAN, out))
 
 
