@@ -204,18 +204,28 @@ def compact(refs, entries, prefix, page):
 @pytest.mark.parametrize("n_pages", [0, 1, 2, 3, 64, 255, 1000, 4095, 4096, 4097, 8192, 20011])
 @pytest.mark.parametrize("share", [0.0, 0.02, 0.5, 0.97, 1.0])
 def test_compact(ctx, n_pages, share):
+    _compact(ctx, n_pages, share, 700)
+
+
+@pytest.mark.parametrize("n_pages,places", [(0, 5), (3, 0), (100, 1 << 16), (4096, 1 << 16), (4096, (1 << 16) + 1),
+                                            (37, 100000), (0, 100000)])
+def test_compact_of_many_places(ctx, n_pages, places):
+    _compact(ctx, n_pages, 0.6, places)
+
+
+def _compact(ctx, n_pages, share, places):
     rng = random.Random(n_pages)
     refs = [rng.randint(1, 5) if rng.random() < share else 0 for _ in range(n_pages)]
-    entries = [rng.randint(-2, n_pages + 1) for _ in range(700)]
+    entries = [rng.randint(-2, n_pages + 1) for _ in range(places)]
     prefix = [rng.randint(-2, n_pages + 1) for _ in range(9)]
     want = compact(refs, entries, prefix, 32)
     r, e, x = _ints(refs, -1), _ints(entries, -1), _ints(prefix, -1)
-    new_r, new_e, new_x = (torch.full((n,), 77, dtype=torch.int32, device="cuda") for n in (n_pages, 700, 9))
+    new_r, new_e, new_x = (torch.full((n,), 77, dtype=torch.int32, device="cuda") for n in (n_pages, places, 9))
     copies = torch.full((n_pages // 2 + 1, 3), 77, dtype=torch.int32, device="cuda")  # one row to spare
     info = torch.full((2,), 77, dtype=torch.int32, device="cuda")
     need = ctx.pages_compact_workspace(n_pages)
     ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
-    ctx.pages_compact_device(n_pages, 32, r.data_ptr(), 700, e.data_ptr(), new_r.data_ptr(), new_e.data_ptr(),
+    ctx.pages_compact_device(n_pages, 32, r.data_ptr(), places, e.data_ptr(), new_r.data_ptr(), new_e.data_ptr(),
                              copies.data_ptr(), info.data_ptr(), ws.data_ptr(), need, stream(), n_prefix=9,
                              prefix_pages_ptr=x.data_ptr(), new_prefix_pages_ptr=new_x.data_ptr())
     torch.cuda.synchronize()
