@@ -84,6 +84,23 @@ def test_without_queries_without_rotation_and_other_orders(ctx):
     _case(ctx, [3, 1], [20, 9], 4, 4, 3, 64, 64, HALF, 32, 16, "bf16", order="major")
 
 
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("head_dim,rot,layout,page", [(128, 128, HALF, 64), (64, 32, INTER, 16), (48, 10, HALF, 32)])
+def test_the_longest_sequence_is_only_a_hint(ctx, name, head_dim, rot, layout, page):
+    # by tokens of a sequence a wave holds one unit of a row at a time or four; every hint gives the same cache
+    seen = []
+    for max_q in (0, 1, 3, 100, 100000):
+        p = Paged8([1, 70, 5, 33], [30, 90, 5, 40], 7, 3, head_dim, page, page, seed=4)
+        g = torch.Generator(device="cuda").manual_seed(5)
+        x = torch.randn(p.tokens, 2 * 3 + 5, head_dim, generator=g, device="cuda").to(TYPES[name])
+        q, k, v = x.split([5, 3, 3], 1)
+        out = torch.full((p.tokens, 5, head_dim), 7.0, dtype=x.dtype, device="cuda")
+        _append(ctx, p, vtq.Rope(rot, layout), name, k, v, q, out, desc=p.describe(max_q=max_q))
+        seen.append([t.clone() for t in (p.dk, p.dv, p.dks, p.dvs, out.view(torch.uint8))])
+    for other in seen[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(seen[0], other))
+
+
 @pytest.mark.parametrize("seed", range(4))
 def test_scales_grow_and_stay(ctx, seed):
     # tokens louder and quieter than those before them in the block, by up to some powers of two

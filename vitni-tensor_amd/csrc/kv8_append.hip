@@ -14,9 +14,10 @@
 // registers between the maximum and the stores; longer blocks are read again, from the
 // caches near by.  Queries are rotated by workgroups of their own in the same launch.
 //
-// A step of 32 sequences, 8 KV heads of 128 and 32 query heads in bf16, takes 8.3 us: the
-// launch and four reads that wait for each other (lengths, angles, page, scale).  Prompts of
-// 4,500 tokens in f32 (124 MB to read and write, 24 us at a large copy's rate) take 35.6.
+// A step of 32 sequences, 8 KV heads of 128 and 32 query heads in bf16, takes 6.4 us in a graph:
+// the launch and three reads that wait for each other (lengths, page, scale; 8.3 where the row
+// and the angles wait for the page too).  Prompts of 4,500 tokens in f32 (124 MB to read and
+// write, 24 us at a large copy's rate) take 35.6.
 #include "vtq_rope.h"
 
 namespace vtq {
@@ -25,7 +26,6 @@ namespace {
 constexpr int kCosTokens = 16;  // tokens whose cosines are held at a time
 constexpr int kMostRows = 32;   // heads' keys and values to a workgroup
 constexpr int kQueryTokens = 4;  // tokens at most whose queries a workgroup rotates: one a wave
-constexpr int kHeld = 4;        // units of a row that a lane has at a time
 constexpr int kLeast = -117, kMost = 119;  // exponents of scales: what they scale stays a normal bf16
 
 struct Kv8Job : RopeJob {
@@ -116,23 +116,21 @@ __device__ __forceinline__ int block_tokens(const vtq_kv_batch& b, int64_t token
     return 0;
 }
 
-// Units of a row of some tokens, kHeld to a lane: their elements, rotated.
-template <class T, int N>
+// Units of a row of some tokens, H to a lane: their elements, rotated.
+template <class T, int N, int H>
 struct Held {
-    float x[kHeld][2][N];
-    int at[kHeld][2];   // first element of each part; -1: there is none
-    int token[kHeld];
+    float x[H][2][N];
+    int at[H][2];   // first element of each part; -1: there is none
+    int token[H];
+    Pack<T, N> a[H], b[H];
+    bool turns[H];
+    int pair[H];
 
-    // Units w0 + 64 k + lane of n tokens' `units` each.
-    __device__ __forceinline__ void load(const T* src, int64_t token_stride, int w0, int n, int units, const float2 (*cs)[128],
-                                         int rot, bool half) {
+    // Units w0 + 64 k + lane of n tokens' `units` each: their loads, all at once
+    __device__ __forceinline__ void fetch(const T* src, int64_t token_stride, int w0, int n, int units, int rot, bool half) {
         const int lane = threadIdx.x & 63, per = half || N == 1 ? rot / 2 / N : rot / N, step = half ? rot / 2 : 1;
-        Pack<T, N> a[kHeld], b[kHeld];
-        bool turns[kHeld];
-        int pair[kHeld];
-        // all loads first
 #pragma unroll
-        for (int k = 0; k < kHeld; k++) {
+        for (int k = 0; k < H; k++) {
             const int w = w0 + 64 * k + lane, last = min(w, n * units - 1), unit = last % units;
             token[k] = last / units;
             turns[k] = unit < per;
@@ -148,8 +146,10 @@ struct Held {
             a[k] = *reinterpret_cast<const Pack<T, N>*>(from);
             b[k] = *reinterpret_cast<const Pack<T, N>*>(two ? from + step : from);
         }
+    }
+    __device__ __forceinline__ void rotate(const float2 (*cs)[128], bool half) {
 #pragma unroll
-        for (int k = 0; k < kHeld; k++) {
+        for (int k = 0; k < H; k++) {
             const float2* c = cs[token[k]] + (turns[k] ? pair[k] : 0);
             if (half || N == 1) {
 #pragma unroll
@@ -175,7 +175,7 @@ struct Held {
     __device__ __forceinline__ float top() const {
         float most = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kHeld; k++)
+        for (int k = 0; k < H; k++)
 #pragma unroll
             for (int p = 0; p < 2; p++)
 #pragma unroll
@@ -187,14 +187,16 @@ struct Held {
     }
     __device__ __forceinline__ void put(uint8_t* dst, int64_t slot, int e) const {
 #pragma unroll
-        for (int k = 0; k < kHeld; k++)
+        for (int k = 0; k < H; k++)
 #pragma unroll
             for (int p = 0; p < 2; p++)
                 if (at[k][p] >= 0) put8<N>(dst + token[k] * slot + at[k][p], x[k][p], e);
     }
 };
 
-template <class T, int N>
+// H: 1 where a sequence's tokens fit a wave by the hint, and a row is on its way while the angles
+// are worked out (with four units to a lane that takes 235 registers); else 4.
+template <class T, int N, int H>
 __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int rot = j.rotate ? j.rope.rot_dim : 0;
@@ -246,38 +248,49 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int block = j.s.block;
     const int count = block_tokens(j.batch, j.tokens, __builtin_ctz(block), work / j.kv_groups, t, spot);
     if (!count) return;
-    const int32_t* list = j.batch.pages + (int64_t)spot.seq * j.batch.max_pages;
-    const int64_t at = slot_of(j.cache, list, j.batch.max_pages, spot.place);
-    if (at < 0) return;
-    const int before = (int)(spot.place & (block - 1));
-    const int64_t scale_at = list[spot.place / j.cache.page_size] * j.s.page_stride +
-                             (spot.place & (j.cache.page_size - 1)) / block;
     const int group = (int)(work % j.kv_groups);
     const int r0 = group * j.rows_per, r1 = min(2 * j.kv_heads, r0 + j.rows_per);
     const bool keys = r0 < j.kv_heads && rot;
+    if (spot.place / j.cache.page_size >= j.batch.max_pages) return;
+    const int page = j.batch.pages[(int64_t)spot.seq * j.batch.max_pages + spot.place / j.cache.page_size];
     // One pass where a row of all tokens is held at once, else one for the maxima and one for the stores.
     const int most_units = max(units_rot, units_plain);
-    const bool once = count <= kCosTokens && count * most_units <= 64 * kHeld;
+    const bool once = count <= kCosTokens && count * most_units <= 64 * H;
+    Held<T, N, H> held;
+    auto row_of = [&](int r, int c0) {  // from token c0 of the block on
+        const HeadRows& in = r >= j.kv_heads ? j.v : j.k;
+        return static_cast<const T*>(in.p) + (t + c0) * in.token_stride + (r % j.kv_heads) * in.head_stride;
+    };
+    auto fetch = [&](int r, int c0, int w0, int n) {
+        const bool is_v = r >= j.kv_heads;
+        held.fetch(row_of(r, c0), (is_v ? j.v : j.k).token_stride, w0, n, is_v ? units_plain : units_rot, is_v ? 0 : rot, half);
+    };
+    const bool early = H == 1 && once;  // the page, the first row and the angles together
+    if (early && r0 + wave < r1) fetch(r0 + wave, 0, 0, count);
+    if (keys && once) turn(spot.place, count);
+    if (page < 0 || page >= (int64_t)j.cache.n_pages) return;
+    const int64_t at = page * (int64_t)j.cache.page_stride +
+                       (spot.place & (j.cache.page_size - 1)) * (int64_t)j.cache.slot_stride;
+    const int before = (int)(spot.place & (block - 1));
+    const int64_t scale_at = page * j.s.page_stride + (spot.place & (j.cache.page_size - 1)) / block;
     for (int pass = once ? 1 : 0; pass < 2; pass++)
         for (int c0 = 0; c0 < count; c0 += kCosTokens) {
             const int n = min(kCosTokens, count - c0);
-            if (keys && (pass == 0 || once || count > kCosTokens)) {
+            if (keys && !once && (pass == 0 || count > kCosTokens)) {
                 if (pass || c0) __syncthreads();
                 turn(spot.place + c0, n);
-                __syncthreads();
             }
+            if (keys) __syncthreads();
             for (int r = r0 + wave; r < r1; r += 4) {
                 const bool is_v = r >= j.kv_heads;
                 const int h = is_v ? r - j.kv_heads : r, units = is_v ? units_plain : units_rot;
-                const HeadRows& in = is_v ? j.v : j.k;
-                const T* src = static_cast<const T*>(in.p) + (t + c0) * in.token_stride + h * in.head_stride;
                 uint8_t* scale = (is_v ? j.s.v : j.s.k) + scale_at + h * j.s.head_stride;
                 const int old = before ? min(max((int)*scale - 127, kLeast), kMost) : kLeast;
-                Held<T, N> held;
                 float top = 0.0f;
                 if (pass == 0 || once) {
-                    for (int w0 = 0; w0 < n * units; w0 += 64 * kHeld) {
-                        held.load(src, in.token_stride, w0, n, units, cs, is_v ? 0 : rot, half);
+                    for (int w0 = 0; w0 < n * units; w0 += 64 * H) {
+                        if (!early || r != r0 + wave) fetch(r, c0, w0, n);
+                        held.rotate(cs, half);
                         top = fmaxf(top, held.top());
                     }
 #pragma unroll
@@ -306,8 +319,9 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
                 if (once) {
                     held.put(dst, slot, e);
                 } else {
-                    for (int w0 = 0; w0 < n * units; w0 += 64 * kHeld) {
-                        held.load(src, in.token_stride, w0, n, units, cs, is_v ? 0 : rot, half);
+                    for (int w0 = 0; w0 < n * units; w0 += 64 * H) {
+                        fetch(r, c0, w0, n);
+                        held.rotate(cs, half);
                         held.put(dst, slot, e);
                     }
                 }
@@ -342,16 +356,20 @@ hipError_t launch_kv8_append(const RopeJob& job, const Scales& s, int type, hipS
     j.kv_groups = (rows + j.rows_per - 1) / j.rows_per;
     j.kv_work = blocks * j.kv_groups;
     const dim3 grid((unsigned)(j.kv_work + q_work));
+    const int most_units = std::max(rotated_units(j.head_dim, j.rotate ? j.rope.rot_dim : 0,
+                                                  j.rope.layout == VTQ_ROPE_HALF, n), j.head_dim / n);
+    const bool few = j.batch.max_q > 0 && std::min<int64_t>(j.batch.max_q, j.tokens) * most_units <= 64;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (n == 8) {
-            hipLaunchKernelGGL((kv8_append_kernel<T, 8>), grid, dim3(kRopeThreads), 0, stream, j);
-        } else if (n == 4) {
-            if constexpr (sizeof(T) == 4)
-                hipLaunchKernelGGL((kv8_append_kernel<T, 4>), grid, dim3(kRopeThreads), 0, stream, j);
-        } else {
-            hipLaunchKernelGGL((kv8_append_kernel<T, 1>), grid, dim3(kRopeThreads), 0, stream, j);
-        }
+        auto launch = [&](auto n_of) {
+            constexpr int N = decltype(n_of)::value;
+            if (few) hipLaunchKernelGGL((kv8_append_kernel<T, N, 1>), grid, dim3(kRopeThreads), 0, stream, j);
+            else hipLaunchKernelGGL((kv8_append_kernel<T, N, 4>), grid, dim3(kRopeThreads), 0, stream, j);
+        };
+        if (n == 8) launch(std::integral_constant<int, 8>{});
+        else if constexpr (sizeof(T) == 4)
+            if (n == 4) launch(std::integral_constant<int, 4>{});
+        if (n == 1) launch(std::integral_constant<int, 1>{});
         return hipGetLastError();
     });
 }
