@@ -15,8 +15,6 @@ from vtq import probe
 A = 1 << 20  # an aligned address; nothing is read
 CSRC = os.path.join(ROOT, "vitni-tensor_amd", "csrc")
 SOURCES = ("kv8_append.hip", "kv8_attention.hip", "beam_select.hip", "cache_pages.hip")
-# bytes a lane at most, of heads of up to 128 elements: registers of what follows the loops
-SCRATCH = {("DF16_", 128): 48, ("DF16b", 128): 16}
 
 
 def _check(ggml_type, kv_heads, group, head_dim, page, batch, max_q, max_len, max_pages, prefix, tokens):
@@ -133,7 +131,4 @@ def test_scratch_memory_and_the_dispatch_packet(asm):
     kernels = [k for k in sizes if "kernel" in k]
     assert len(kernels) >= 3 and len(packet) >= 3
     assert not any(packet.values()), packet
-    for kernel in kernels:
-        m = re.search(r"kv8_attention_kernelI(f|DF16_|DF16b)Li(\d+)", kernel)
-        allowed = SCRATCH.get((m.group(1), int(m.group(2))), 0) if m else 0
-        assert sizes[kernel] <= allowed, (kernel, sizes[kernel])
+    assert not {k: sizes[k] for k in kernels if sizes[k]}

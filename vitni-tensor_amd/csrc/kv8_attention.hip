@@ -37,6 +37,7 @@ namespace {
 
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) v2i lds_v2i;
+typedef __attribute__((address_space(3))) const v4u lds_v4u;
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
@@ -60,8 +61,7 @@ struct Tile8 {
         return kChunks == 8 ? c ^ ((row ^ ((row >> 3) & 1)) & 7) : c ^ (row & 15);
     }
     __device__ static int v_chunk(int row, int c) {
-        if (kChunks == 4) return c ^ ((row >> 2) & 2);
-        return kChunks == 8 ? c ^ ((row & 2) | ((row >> 1) & 4)) : c ^ (((row & 3) | ((row >> 1) & 4)) << 1);
+        return kChunks == 4 ? c ^ ((row >> 2) & 2) : c ^ ((row & 2) | ((row >> 1) & 4));
     }
 };
 
@@ -77,7 +77,7 @@ struct Runs {
     int keys;   // keys that exist: later ones read as zeros
     int first;  // in 16 keys
     int low, high;      // bytes from the head's start, -1: outside the cache
-    int scale_k, scale_v;  // f32 bits
+    int scales;         // bytes: the keys' scale, the values' 16 bits above
 };
 
 template <int DK, int DV>
@@ -134,21 +134,21 @@ struct Loader8 {
         p.low = (int)(uint32_t)byte;
         p.high = (int)(byte >> 32);
         const int64_t scale = there ? (int64_t)page * scale_page + (slot >> block_shift) : 0;
-        p.scale_k = there ? min(max((int)k_scale[scale], 10), 246) << 23 : 0x3F800000;
-        p.scale_v = there ? min(max((int)v_scale[scale], 10), 246) << 23 : 0x3F800000;
+        p.scales = there ? min(max((int)k_scale[scale], 10), 246) | min(max((int)v_scale[scale], 10), 246) << 16 : 127 * 0x10001;
         // waited for here: left to its use, the wait would stand in every tile, and be one for
         // all loads to LDS in flight as well
-        asm volatile("" : "+v"(p.low), "+v"(p.high), "+v"(p.scale_k), "+v"(p.scale_v));
+        asm volatile("" : "+v"(p.low), "+v"(p.high), "+v"(p.scales));
     }
     // the lane of `key`'s 16 keys (those past the end have any)
     __device__ __forceinline__ int lane_of(const Runs& p, int key) const { return ((key >> 4) - p.first) & 63; }
     __device__ __forceinline__ TileScales scales(const Runs& p, int key) const {
-        const int a = lane_of(p, key), b = lane_of(p, key + 16);
+        const int a = __builtin_amdgcn_readlane(p.scales, lane_of(p, key));
+        const int b = __builtin_amdgcn_readlane(p.scales, lane_of(p, key + 16));
         TileScales s;
-        s.k0 = __int_as_float(__builtin_amdgcn_readlane(p.scale_k, a));
-        s.k1 = __int_as_float(__builtin_amdgcn_readlane(p.scale_k, b));
-        s.v0 = __int_as_float(__builtin_amdgcn_readlane(p.scale_v, a));
-        s.v1 = __int_as_float(__builtin_amdgcn_readlane(p.scale_v, b));
+        s.k0 = __int_as_float((a & 0xFF) << 23);
+        s.k1 = __int_as_float((b & 0xFF) << 23);
+        s.v0 = __int_as_float(a >> 16 << 23);
+        s.v1 = __int_as_float(b >> 16 << 23);
         return s;
     }
     // 16 keys from `key` on: K to k_lds, V to v_lds.
@@ -263,26 +263,35 @@ struct Compute8 {
     struct Values {
         v2i x[DV / 32][2];
     };
-    __device__ __forceinline__ static v4u key_at(const uint8_t* k, int c) {
+    // A row's chunks differ in bits that the permutation only flips, so one address makes them all
+    // (tiles begin at multiples of a row): kept ones for each spilled.
+    __device__ __forceinline__ static uint32_t keys_from(const uint8_t* k) {
         const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
-        return *reinterpret_cast<const v4u*>(k + row * TK::kRow + TK::k_chunk(row, 2 * c + h) * 16);
+        return (uint32_t)(uintptr_t)(lds_u8*)k + (uint32_t)(row * TK::kRow + TK::k_chunk(row, h) * 16);
+    }
+    __device__ __forceinline__ static v4u key_at(uint32_t from, int c) {
+        return *(lds_v4u*)(uintptr_t)(from ^ (uint32_t)(32 * c));
     }
     // elements 32 b + (lane & 31) of keys 16 i + 4 h + {0..3, 8..11}
-    __device__ __forceinline__ static v2i values_at(const uint8_t* v, int b, int i) {
+    __device__ __forceinline__ static uint32_t values_from(const uint8_t* v) {
         const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 15, r = n >> 1;
-        const int row = 16 * i + 4 * h + (r & 3) + 8 * (r >> 2), c = 2 * b + ((lane >> 4) & 1);
-        const uint8_t* at = v + row * TV::kRow + TV::v_chunk(row, c) * 16 + (n & 1) * 8;
-        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(at));
+        const int row = 4 * h + (r & 3) + 8 * (r >> 2), c = (lane >> 4) & 1;
+        return (uint32_t)(uintptr_t)(lds_u8*)v + (uint32_t)(row * TV::kRow + TV::v_chunk(row, c) * 16 + (n & 1) * 8);
+    }
+    __device__ __forceinline__ static v2i values_at(uint32_t from, int b, int i) {
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(uintptr_t)((from ^ (uint32_t)(32 * b)) + 16 * TV::kRow * i));
     }
     __device__ __forceinline__ static void read_keys(Keys& r, const uint8_t* k) {
+        const uint32_t from = keys_from(k);
 #pragma unroll
-        for (int c = 0; c < DK / 32; c++) r.x[c] = key_at(k, c);
+        for (int c = 0; c < DK / 32; c++) r.x[c] = key_at(from, c);
     }
     __device__ __forceinline__ static void read_values(Values& r, const uint8_t* v) {
+        const uint32_t from = values_from(v);
 #pragma unroll
         for (int b = 0; b < DV / 32; b++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) r.x[b][i] = values_at(v, b, i);
+            for (int i = 0; i < 2; i++) r.x[b][i] = values_at(from, b, i);
     }
     __device__ __forceinline__ static bool near_end(TileScales sc) {  // scales above 2^95; scalar as integers
         return max(__float_as_int(sc.v0), __float_as_int(sc.v1)) > (222 << 23);
@@ -291,10 +300,11 @@ struct Compute8 {
     // scores of 32 keys: register 4i + e is key 8i + 4h + e, row lane & 31
     __device__ __forceinline__ static v16f scores(const uint8_t* k, const Query& q, TileScales sc) {
         const float scale = key_scale(sc);
+        const uint32_t from = keys_from(k);
         v16f s = {};
 #pragma unroll
         for (int c = 0; c < DK / 32; c++) {
-            const v4u x = key_at(k, c);
+            const v4u x = key_at(from, c);
             const v8k a = widen_key(x[0], x[1], scale), b = widen_key(x[2], x[3], scale);
 #pragma unroll
             for (int i = PQ - 1; i >= 0; i--) {  // small parts first
@@ -419,7 +429,7 @@ struct Compute8 {
             v16f bad = {};
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const v2i x = values_at(v, b, i);
+                const v2i x = values_at(values_from(v), b, i);
                 uint32_t number[2], none[2];  // codes: the numbers, and 1 (0x38) where there is none
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -444,7 +454,6 @@ struct Compute8 {
         Keys k0, k1;
         read_keys(k0, k);
         read_keys(k1, k + TK::kBytes);
-        __builtin_amdgcn_sched_barrier(0);  // all on their way before the first is waited for
         Values v0, v1;
         read_values(v0, v);
         v16f s[2];
