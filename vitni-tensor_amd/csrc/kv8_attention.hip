@@ -40,6 +40,7 @@ typedef __attribute__((address_space(3))) v2i lds_v2i;
 typedef __attribute__((address_space(3))) const v4u lds_v4u;
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 
 struct Job8 : Job {
     Scales s;
@@ -191,30 +192,36 @@ struct Compute8 {
     struct Weights {
         v8bf v[P][2];
     };
+    using Rows = State<DV>;
 
+    // 8 elements in parts: give(part, element, it)
+    template <class Give>
+    __device__ __forceinline__ static void split(const Q* p, bool in, Give give) {
+        typedef Q v8q __attribute__((ext_vector_type(8)));
+        v8q x = {};
+        if (in) x = *reinterpret_cast<const v8q*>(p);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if constexpr (PQ == 1) {
+                give(0, e, x[e]);
+            } else {
+                float rest = x[e];
+#pragma unroll
+                for (int i = 0; i < PQ; i++) {
+                    const __bf16 part = (__bf16)rest;
+                    give(i, e, part);
+                    // an infinity's remainder would be no number: the first part has it all
+                    rest = fabsf(rest) < INFINITY ? rest - (float)part : 0.0f;
+                }
+            }
+        }
+    }
     __device__ static void load_query(Query& q, const Q* p, bool valid, int head_dim) {
         const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
         for (int s = 0; s < DK / 16; s++) {
             const int d = 32 * (s / 2) + 16 * h + 8 * (s & 1);
-            const bool in = valid && d < head_dim;
-            typedef Q v8q __attribute__((ext_vector_type(8)));
-            v8q x = {};
-            if (in) x = *reinterpret_cast<const v8q*>(p + d);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if constexpr (PQ == 1) {
-                    q.v[0][s][e] = x[e];
-                } else {
-                    float rest = x[e];
-#pragma unroll
-                    for (int i = 0; i < PQ; i++) {
-                        q.v[i][s][e] = (__bf16)rest;
-                        // an infinity's remainder would be no number: the first part has it all
-                        rest = fabsf(rest) < INFINITY ? rest - (float)q.v[i][s][e] : 0.0f;
-                    }
-                }
-            }
+            split(p + d, valid && d < head_dim, [&](int part, int e, auto x) { q.v[part][s][e] = x; });
         }
     }
 
@@ -363,6 +370,17 @@ struct Compute8 {
         return w;
     }
 
+    // m follows the maximum only once it is 8 powers of two behind: weights up to 256
+    // cost nothing, and rows rarely rescale.  Beside values near f32's end (raise) m is 24 powers
+    // above the maximum, so that sums of them do not pass it.
+    __device__ __forceinline__ static bool moved(float top, float m, bool raise, float c) {
+        return (top - m) * c > (raise ? 0.0f : 8.0f);
+    }
+    // Whether some row's does; top as it is to be.
+    __device__ __forceinline__ static bool moves(float& top, float m, bool raise, float c) {
+        if (raise) top += fminf(24.0f / c, 1e38f);
+        return __ballot(moved(top, m, raise, c)) != 0;
+    }
     // Scores of N tiles to weights, with the row's maximum and sum.
     template <int N>
     __device__ __forceinline__ static void softmax(State<DV>& st, Weights (&w)[N], v16f (&s)[N], bool raise, float c) {
@@ -373,16 +391,11 @@ struct Compute8 {
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[i][r]);
         const float2 both = halves(top);
         top = fmaxf(both.x, both.y);
-        // m follows the maximum only once it is 8 powers of two behind: weights up to 256
-        // cost nothing, and rows rarely rescale.  Beside values near f32's end m is 24 powers above
-        // the maximum, so that sums of them do not pass it
         const float before = st.m;
-        float most = 8.0f;
-        if (raise) top += fminf(24.0f / c, 1e38f), most = 0.0f;
-        const bool moves = (top - before) * c > most;  // each row for itself
-        if (__ballot(moves)) {
-            const float shrink = moves ? __builtin_amdgcn_exp2f((before - top) * c) : 1.0f;
-            st.m = moves ? top : before;
+        if (moves(top, before, raise, c)) {
+            const bool mine = moved(top, before, raise, c);  // each row for itself
+            const float shrink = mine ? __builtin_amdgcn_exp2f((before - top) * c) : 1.0f;
+            st.m = mine ? top : before;
             st.l *= shrink;
 #pragma unroll
             for (int b = 0; b < DV / 32; b++) st.o[b] *= shrink;
@@ -415,6 +428,15 @@ struct Compute8 {
         return __ballot((any & 0x80808080u) != 0) == 0;
     }
 
+    // Codes: the numbers, and 1 (0x38) where there is none.
+    __device__ __forceinline__ static void part_numbers(v2i x, uint32_t (&number)[2], uint32_t (&none)[2]) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t is = ((((uint32_t)x[e] & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u;
+            number[e] = (uint32_t)x[e] & ~(is * 255u);
+            none[e] = is * 0x38u;
+        }
+    }
     // The values of a tile that holds NaNs and that some row does not see whole: a weight of 0
     // does not silence a NaN.  They count as zeros here, and the rows that see one get it on top.
     __device__ __forceinline__ static void add_some(State<DV>& st, const Weights& w, const uint8_t* v, int key, int limit,
@@ -429,14 +451,8 @@ struct Compute8 {
             v16f bad = {};
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const v2i x = values_at(values_from(v), b, i);
-                uint32_t number[2], none[2];  // codes: the numbers, and 1 (0x38) where there is none
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint32_t is = ((((uint32_t)x[e] & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u;
-                    number[e] = (uint32_t)x[e] & ~(is * 255u);
-                    none[e] = is * 0x38u;
-                }
+                uint32_t number[2], none[2];
+                part_numbers(values_at(values_from(v), b, i), number, none);
                 const v8bf y = widen(number[0], number[1], i ? sc.v1 : sc.v0);
 #pragma unroll
                 for (int p = P - 1; p >= 0; p--) st.o[b] = mma(y, w.v[p][i], st.o[b]);
@@ -487,6 +503,197 @@ struct Compute8 {
             add_values(st, x, w[0], sc);
         }
     }
+    __device__ __forceinline__ static float sum(float l) {
+        const float2 both = halves(l);
+        return both.x + both.y;
+    }
+    // Four elements at a time: give(row, element / 4, them)
+    template <class Give>
+    __device__ __forceinline__ static void each(const State<DV>& st, Give give) {
+        const int lane = late_lane();
+#pragma unroll
+        for (int b = 0; b < DV / 32; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const v16f& o = st.o[b];
+                give(lane & 31, 8 * b + 2 * i + (lane >> 5), make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+            }
+    }
+};
+
+// The same for 16 rows or fewer, a step's tokens of a group, by 16x16 products: half the products
+// and half the weights.  A score of register r of tile t (of 16 keys) is key 8 t + 4 (g / 2) +
+// 16 (g % 2) + r, g = lane / 16, so that a lane's keys lie in one block and its values in 8 rows.
+template <class Q, int DK, int DV>
+struct Few8 {
+    using X = Compute8<Q, DK, DV>;
+    using TK = Tile8<DK>;
+    using TV = Tile8<DV>;
+    using v8k = typename X::v8k;
+    static constexpr int P = X::P, PQ = X::PQ;
+    // q of row lane & 15: element d of 64 c + 16 g + 8 s + 0..7 is v[part][2 c + s]
+    struct Query {
+        v8k v[PQ][DK / 32];
+    };
+    struct Rows {
+        v4f o[DV / 16];  // register r of o[b]: element 16 b + 4 g + r
+        float m, l;
+    };
+    struct Weights {
+        v8bf v[P];
+    };
+
+    __device__ __forceinline__ static int group() { return (threadIdx.x & 63) >> 4; }
+    __device__ static void load_query(Query& q, const Q* p, bool valid, int head_dim) {
+#pragma unroll
+        for (int s = 0; s < DK / 32; s++) {
+            const int d = 64 * (s / 2) + 16 * group() + 8 * (s & 1);
+            X::split(p + d, valid && d < head_dim, [&](int part, int e, auto x) { q.v[part][s][e] = x; });
+        }
+    }
+    __device__ __forceinline__ static int key_of(int t, int g, int r) { return 8 * t + 4 * (g >> 1) + 16 * (g & 1) + r; }
+    __device__ __forceinline__ static v4f mma(v8bf a, v8bf b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    __device__ __forceinline__ static v4f mma_key(v8k a, v8k b, v4f c) {
+        if constexpr (X::kHalf) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+        else return mma(a, b, c);
+    }
+    // where this lane reads values: rows of its keys
+    __device__ __forceinline__ static uint32_t values_from(const uint8_t* v) {
+        const int n = threadIdx.x & 15, row = key_of(n >> 3, group(), (n >> 1) & 3);
+        return (uint32_t)(uintptr_t)(lds_u8*)v + (uint32_t)(row * TV::kRow + TV::v_chunk(row, 0) * 16 + (n & 1) * 8);
+    }
+    __device__ __forceinline__ static v2i values_at(uint32_t from, int b) {
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(uintptr_t)(from ^ (uint32_t)(16 * b)));
+    }
+    __device__ __forceinline__ static void scores(v4f (&s)[2], const uint8_t* k, const Query& q, TileScales sc) {
+        const int m = threadIdx.x & 15;
+        const float scale = m & 4 ? sc.k1 : sc.k0;
+        v4u x[2][DK / 64];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int row = key_of(t, m >> 2, m & 3);
+            const uint32_t from = (uint32_t)(uintptr_t)(lds_u8*)k + (uint32_t)(row * TK::kRow + TK::k_chunk(row, group()) * 16);
+#pragma unroll
+            for (int c = 0; c < DK / 64; c++) x[t][c] = *(lds_v4u*)(uintptr_t)(from ^ (uint32_t)(64 * c));
+        }
+        s[0] = s[1] = v4f{};
+#pragma unroll
+        for (int c = 0; c < DK / 64; c++)
+#pragma unroll
+            for (int half = 0; half < 2; half++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const v8k a = X::widen_key(x[t][c][2 * half], x[t][c][2 * half + 1], scale);
+#pragma unroll
+                    for (int i = PQ - 1; i >= 0; i--) s[t] = mma_key(a, q.v[i][2 * c + half], s[t]);
+                }
+        if constexpr (X::kHalf) {
+            const float mine = group() & 1 ? sc.k1 : sc.k0;
+#pragma unroll
+            for (int t = 0; t < 2; t++) s[t] *= mine;
+        }
+    }
+    // x of the lane's row in the four groups
+    template <class F>
+    __device__ __forceinline__ static float of_groups(float x, F join) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        const float2 y = halves(join(__uint_as_float(r[0]), __uint_as_float(r[1])));
+        return join(y.x, y.y);
+    }
+    __device__ __forceinline__ static float sum(float l) {
+        return of_groups(l, [](float a, float b) { return a + b; });
+    }
+    __device__ __forceinline__ static void softmax(Rows& st, Weights& w, v4f (&s)[2], bool raise, float c) {
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int r = 1; r < 4; r++) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
+        top = of_groups(top, [](float a, float b) { return fmaxf(a, b); });
+        const float before = st.m;
+        if (X::moves(top, before, raise, c)) {
+            const bool mine = X::moved(top, before, raise, c);
+            const float shrink = mine ? __builtin_amdgcn_exp2f((before - top) * c) : 1.0f;
+            st.m = mine ? top : before;
+            st.l *= shrink;
+#pragma unroll
+            for (int b = 0; b < DV / 16; b++) st.o[b] *= shrink;
+        }
+        const float base = st.m == -INFINITY ? 0.0f : st.m;
+        float sum[2] = {st.l, 0.0f};
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float rest = __builtin_amdgcn_exp2f((s[t][r] - base) * c);
+                sum[t] += rest;
+#pragma unroll
+                for (int i = 0; i < P; i++) {
+                    const __bf16 part = (__bf16)rest;
+                    w.v[i][4 * t + r] = part;
+                    rest -= (float)part;
+                }
+            }
+        st.l = sum[0] + sum[1];
+    }
+    __device__ __forceinline__ static float value_scale(TileScales sc) { return group() & 1 ? sc.v1 : sc.v0; }
+    __device__ __forceinline__ static void add_some(Rows& st, const Weights& w, const uint8_t* v, int key, int limit,
+                                                    TileScales sc) {
+        const uint32_t from = values_from(v);
+        const float scale = value_scale(sc);
+        v8bf seen;
+#pragma unroll
+        for (int e = 0; e < 8; e++) seen[e] = (__bf16)(key + key_of(e / 4, group(), e % 4) < limit ? 1.0f : 0.0f);
+#pragma unroll
+        for (int b = 0; b < DV / 16; b++) {
+            uint32_t number[2], none[2];
+            X::part_numbers(values_at(from, b), number, none);
+            const v8bf y = X::widen(number[0], number[1], scale);
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--) st.o[b] = mma(y, w.v[p], st.o[b]);
+            const v4f bad = mma(X::widen(none[0], none[1], 1.0f), seen, v4f{});
+#pragma unroll
+            for (int r = 0; r < 4; r++) st.o[b][r] += bad[r] > 0.0f ? __uint_as_float(0x7FC00000u) : 0.0f;
+            __builtin_amdgcn_sched_barrier(0);  // rare: few registers
+        }
+    }
+    __device__ __forceinline__ static void tile(Rows& st, const Query& q, const uint8_t* k, const uint8_t* v, TileScales sc,
+                                                bool edge, int key, int limit, int low, int there, float c) {
+        v4f s[2];
+        scores(s, k, q, sc);
+        if (edge) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (key + key_of(t, group(), r) >= limit) s[t][r] = -INFINITY;
+        }
+        Weights w;
+        softmax(st, w, s, X::near_end(sc), c);
+        if (edge && low < there && !X::all_numbers(v)) {
+            add_some(st, w, v, key, limit, sc);
+            return;
+        }
+        const uint32_t from = values_from(v);
+        const float scale = value_scale(sc);
+        v2i x[DV / 16];
+#pragma unroll
+        for (int b = 0; b < DV / 16; b++) x[b] = values_at(from, b);
+#pragma unroll
+        for (int b = 0; b < DV / 16; b++) {
+            const v8bf a = X::widen((uint32_t)x[b][0], (uint32_t)x[b][1], scale);
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--) st.o[b] = mma(a, w.v[p], st.o[b]);
+        }
+    }
+    // Four elements at a time: give(row, element / 4, them)
+    template <class Give>
+    __device__ __forceinline__ static void each(const Rows& st, Give give) {
+        const int lane = late_lane();
+#pragma unroll
+        for (int b = 0; b < DV / 16; b++)
+            give(lane & 15, 4 * b + (lane >> 4), make_float4(st.o[b][0], st.o[b][1], st.o[b][2], st.o[b][3]));
+    }
 };
 
 // ------------------------------------------------ workgroups
@@ -503,12 +710,14 @@ struct Config8 {
     static constexpr int kPerCu = kLds <= 80 * 1024 && !(std::is_same_v<Q, float> && DK > 64) ? 2 : 1;
 };
 
-template <class Q, int DK, int DV>
+// R: rows of a tile that the waves share, 16 or 32.
+template <class Q, int DK, int DV, int R>
 __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void kv8_attention_kernel(Job8 j) {
     using Cfg = Config8<Q, DK, DV>;
     using TK = Tile8<DK>;
     using TV = Tile8<DV>;
     using X = Compute8<Q, DK, DV>;
+    using Y = std::conditional_t<R == 16, Few8<Q, DK, DV>, X>;  // of rows that the waves share
     constexpr int W = kWaves8, kParts = DK / DV;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float2 wave_ml[W][32];
@@ -555,13 +764,14 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
         k1 = min(runs.keys, k0 + chunk);
     }
     const int n_rows = (int)min((t1 - t0) * G, (int64_t)INT32_MAX);
-    const int tile_rows = shared ? W * 32 : 32;
+    const int tile_rows = shared ? W * 32 : R;
     Loader8<DK, DV> from;
     from.init(j, kv_head, part);
 
     // own workgroups take every row_tiles-th tile of a sequence's rows
     for (int r0 = row_tile * tile_rows; r0 < n_rows; r0 += row_tiles * tile_rows) {
-        const int r = r0 + (shared ? wave * 32 : 0) + (lane & 31);
+        const int rows = min(tile_rows, n_rows - r0);
+        const int r = r0 + (shared ? wave * 32 + (lane & 31) : lane & (R - 1));
         const bool valid = r < n_rows;
         const int64_t token = t0 + r / G;
         const int head = kv_head * G + r % G;
@@ -573,25 +783,29 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
         low = uniform(low);
         high = uniform(high);
         // the last row of the tile sees the most
-        const int last_row = min(n_rows, r0 + tile_rows) - 1;
+        const int last_row = r0 + rows - 1;
         const int end = prefix ? k1 : min(max(unseen + 1 + last_row / G, 0), k1);
         const int first_limit = prefix ? k1 : min(max(unseen + 1 + r0 / G, 0), k1);  // the first row's, the least
         const int tiles = end > k0 ? (end - k0 + 31) / 32 : 0;  // of 32 keys
-        typename X::Query q;
-        X::load_query(q, static_cast<const Q*>(a.q.p) + token * a.q.token_stride + head * a.q.head_stride, valid, hd);
-        State<DV> st;
-        st.m = -INFINITY;
-        st.l = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DV / 32; i++) st.o[i] = v16f{};
-        if (tiles > 0) {
-            const int whole = (first_limit - k0) / 32;  // tiles that every row sees whole
+        const int whole = (first_limit - k0) / 32;              // tiles that every row sees whole
+        const Q* q_row = static_cast<const Q*>(a.q.p) + token * a.q.token_stride + head * a.q.head_stride;
+        const int out_split = prefix ? split : j.prefix_splits + split;
+        auto begin = [&](auto& q, auto& st, auto of) {
+            decltype(of)::load_query(q, q_row, valid, hd);
             runs.keys = end;  // past the last row's sight nothing is read
-            from.hold(runs, k0);
-            auto holds = [&](int key, int keys) {
-                if ((min(key + keys, runs.keys) - 1) / 16 - runs.first >= 64) from.hold(runs, key);
-            };
-            if (shared) {
+            if (tiles > 0) from.hold(runs, k0);
+            // waited for here, as in hold()
+            for (auto& part : q.v)
+                for (auto& x : part) asm volatile("" : "+v"(x));
+            st.m = -INFINITY;
+            st.l = 0.0f;
+            for (auto& o : st.o) o = std::remove_reference_t<decltype(o)>{};
+        };
+        if (shared) {
+            typename X::Query q;
+            State<DV> st;
+            begin(q, st, X{});
+            if (tiles > 0) {
                 // stages of two tiles (K, then V), S - 1 of them ahead; a wave loads 16 of the 64 keys
                 constexpr int kStage = 2 * Cfg::kTile, S = Cfg::kLds / kStage;
                 const int stages = (tiles + 1) / 2;
@@ -644,105 +858,99 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-            } else {
+            }
+            st.l = X::sum(st.l);
+            const int first_row = r0 + wave * 32;
+            X::each(st, [&](int late_row, int chunk, float4 o) {
+                const int row = first_row + late_row, d = DV * part + 4 * chunk;
+                if (row < n_rows && d < hd)
+                    put_row<Q, 0>(j, out_split, t0 + row / G, kv_head * G + row % G, d, o, st.m, st.l);
+            });
+            continue;
+        }
+        // The waves share the rows: each takes every fourth tile.
+        {
+            typename Y::Query q;
+            typename Y::Rows st;
+            begin(q, st, Y{});
+            if (wave < tiles) {
                 // a wave's two stages of a tile
-                uint8_t* mine8 = lds + wave * 2 * Cfg::kTile;
+                const uint8_t* mine8 = lds + wave * 2 * Cfg::kTile;
                 const uint32_t to = lds0 + (uint32_t)wave * 2 * Cfg::kTile;
                 auto load = [&](int n, int at) {
                     const int key = k0 + 32 * n;
-                    holds(key, 32);
+                    if ((min(key + 32, runs.keys) - 1) / 16 - runs.first >= 64) from.hold(runs, key);
                     const uint32_t stage = to + (uint32_t)(at * Cfg::kTile);
                     from.load16(runs, key, stage, stage + TK::kBytes);
                     from.load16(runs, key + 16, stage + 16 * TK::kRow, stage + TK::kBytes + 16 * TV::kRow);
                     return from.scales(runs, key);
                 };
-                if (wave < tiles) {
-                    TileScales here = load(wave, 0), next = load(wave + W, 1);
-                    int n = wave, at = 0;
-                    // Every step loads the tile two steps on, past the end too (zeros from nowhere), so
-                    // that the count of those in flight stays the same.
-                    for (; n < tiles; n += W, at ^= 1) {
-                        const uint8_t* k = mine8 + at * Cfg::kTile;
-                        wait_vmcnt<2 * from.kLoads>();
-                        asm volatile("" ::: "memory");
-                        X::tile(st, q, k, k + TK::kBytes, here, n >= whole, k0 + 32 * n, limit, low, runs.keys, j.c);
-                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                        here = next;
-                        next = load(n + 2 * W, at);
-                    }
-                    wait_vmcnt<0>();
+                TileScales here = load(wave, 0), next = load(wave + W, 1);
+                int n = wave, at = 0;
+                // Every step loads the tile two steps on, past the end too (zeros from nowhere), so
+                // that the count of those in flight stays the same.
+                for (; n < tiles; n += W, at ^= 1) {
+                    const uint8_t* k = mine8 + at * Cfg::kTile;
+                    wait_vmcnt<2 * from.kLoads>();
                     asm volatile("" ::: "memory");
+                    Y::tile(st, q, k, k + TK::kBytes, here, n >= whole, k0 + 32 * n, limit, low, runs.keys, j.c);
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    here = next;
+                    next = load(n + 2 * W, at);
                 }
+                wait_vmcnt<0>();
+                asm volatile("" ::: "memory");
             }
-        }
-        const float2 sums = halves(st.l);
-        st.l = sums.x + sums.y;
-        const int out_split = prefix ? split : j.prefix_splits + split;
-        const int late = late_lane(), late_h = late >> 5;
-        if (shared) {
-            const int row = r0 + wave * 32 + (late & 31);
-            if (row < n_rows) {
-#pragma unroll
-                for (int db = 0; db < DV / 32; db++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int d = DV * part + 32 * db + 8 * i + 4 * late_h;
-                        const v16f& o = st.o[db];
-                        if (d < hd)
-                            put_row<Q, 0>(j, out_split, t0 + row / G, kv_head * G + row % G, d,
-                                          make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]), st.m, st.l);
-                    }
-            }
-        } else {
-            // merge the waves' parts of the same rows, each in its own part of LDS
+            st.l = Y::sum(st.l);
+            // each wave's part of the rows in its own part of LDS
             float* mine = reinterpret_cast<float*>(lds + wave * 2 * Cfg::kTile);
-            const int row = late & 31;
             asm volatile("" ::: "memory");
-#pragma unroll
-            for (int db = 0; db < DV / 32; db++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int c = (8 * db + 2 * i + late_h) ^ (row & 15);
-                    const v16f& o = st.o[db];
-                    *reinterpret_cast<float4*>(mine + row * DV + 4 * c) =
-                        make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                }
-            if (late_h == 0) wave_ml[wave][row] = make_float2(st.m, st.l);
-            __syncthreads();
-            const int rows = min(32, n_rows - r0);
-            for (int e = wave * 64 + late; e < rows * (DV / 4); e += W * 64) {
-                const int rr = e / (DV / 4), c = e % (DV / 4), d = DV * part + 4 * c;
-                if (d >= hd) continue;
-                float m = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < W; w++) m = fmaxf(m, wave_ml[w][rr].x);
-                const float base = m == -INFINITY ? 0.0f : m;
-                float l = 0.0f;
-                float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    const float2 ml = wave_ml[w][rr];
-                    const float f = __builtin_amdgcn_exp2f((ml.x - base) * j.c);
-                    const float4 x = *reinterpret_cast<const float4*>(
-                        reinterpret_cast<const float*>(lds + w * 2 * Cfg::kTile) + rr * DV + 4 * (c ^ (rr & 15)));
-                    l = fmaf(ml.y, f, l);
-                    o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
-                }
-                put_row<Q, 0>(j, out_split, t0 + (r0 + rr) / G, kv_head * G + (r0 + rr) % G, d, o, m, l);
-            }
-            __syncthreads();
+            Y::each(st, [&](int row, int chunk, float4 o) {
+                *reinterpret_cast<float4*>(mine + row * DV + 4 * (chunk ^ (row & 15))) = o;
+            });
+            const int late = late_lane();
+            if (late < R) wave_ml[wave][late] = make_float2(st.m, st.l);
         }
+        __syncthreads();
+        const int late = late_lane();
+        for (int e = wave * 64 + late; e < rows * (DV / 4); e += W * 64) {
+            const int rr = e / (DV / 4), c = e % (DV / 4), d = DV * part + 4 * c;
+            if (d >= hd) continue;
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < W; w++) m = fmaxf(m, wave_ml[w][rr].x);
+            const float base = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f;
+            float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const float2 ml = wave_ml[w][rr];
+                const float f = __builtin_amdgcn_exp2f((ml.x - base) * j.c);
+                const float4 x = *reinterpret_cast<const float4*>(
+                    reinterpret_cast<const float*>(lds + w * 2 * Cfg::kTile) + rr * DV + 4 * (c ^ (rr & 15)));
+                l = fmaf(ml.y, f, l);
+                o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+            }
+            put_row<Q, 0>(j, out_split, t0 + (r0 + rr) / G, kv_head * G + (r0 + rr) % G, d, o, m, l);
+        }
+        __syncthreads();
     }
 }
 
 template <class Q, int DK, int DV>
 hipError_t launch_of(const Job8& j, hipStream_t stream) {
     constexpr int kLds = Config8<Q, DK, DV>::kLds;
-    const void* f = reinterpret_cast<const void*>(&kv8_attention_kernel<Q, DK, DV>);
-    if (hipError_t e = allow_dynamic_lds(f, kLds + 2048)) return e;
-    hipLaunchKernelGGL((kv8_attention_kernel<Q, DK, DV>), dim3(8u * (unsigned)(j.prefix_per_xcd + j.own_per_xcd)),
-                       dim3(kWaves8 * 64), kLds, stream, j);
-    if (hipError_t e = hipGetLastError()) return e;
+    const int64_t prefix_rows = j.prefix_splits ? j.a.tokens * j.group : 0;
+    const int64_t own_rows = std::min<int64_t>(std::max(1, j.a.batch.max_q), j.a.tokens) * j.group;
+    // 16 rows by the hint are two tiles, or more, where it is wrong
+    const bool few = !j.shared_own && own_rows <= 16 && (j.shared_prefix || prefix_rows <= 16);
+    auto launch = [&](void (*kernel)(Job8)) {
+        if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds + 2048)) return e;
+        hipLaunchKernelGGL(kernel, dim3(8u * (unsigned)(j.prefix_per_xcd + j.own_per_xcd)), dim3(kWaves8 * 64), kLds,
+                           stream, j);
+        return hipGetLastError();
+    };
+    if (hipError_t e = few ? launch(kv8_attention_kernel<Q, DK, DV, 16>) : launch(kv8_attention_kernel<Q, DK, DV, 32>)) return e;
     return launch_join<Q, DK, 0>(j, stream);
 }
 
