@@ -428,19 +428,24 @@ struct Compute8 {
         return __ballot((any & 0x80808080u) != 0) == 0;
     }
 
-    // Codes: the numbers, and 1 (0x38) where there is none.
-    __device__ __forceinline__ static void part_numbers(v2i x, uint32_t (&number)[2], uint32_t (&none)[2]) {
+    // The numbers among codes, zeros for the others; 1 (0x38) for each of these, else 0.
+    __device__ __forceinline__ static v8bf without_nans(v2i& x) {
+        uint32_t none[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const uint32_t is = ((((uint32_t)x[e] & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u;
-            number[e] = (uint32_t)x[e] & ~(is * 255u);
+            x[e] = (int)((uint32_t)x[e] & ~(is * 255u));
             none[e] = is * 0x38u;
         }
+        return widen(none[0], none[1], 1.0f);
     }
-    // The values of a tile that holds NaNs and that some row does not see whole: a weight of 0
-    // does not silence a NaN.  They count as zeros here, and the rows that see one get it on top.
-    __device__ __forceinline__ static void add_some(State<DV>& st, const Weights& w, const uint8_t* v, int key, int limit,
-                                                    TileScales sc) {
+    // x, or NaN where the bit is set (bits all the way: a mask of lanes for each would fill the scalars)
+    __device__ __forceinline__ static float nan_where(float x, uint32_t bits, int bit) {
+        return __uint_as_float(__float_as_uint(x) | ((uint32_t)((int)(bits << (31 - bit)) >> 31) & 0x7FC00000u));
+    }
+    // A tile that holds NaNs and that some row does not see whole: a weight of 0 does not silence a
+    // NaN.  They become zeros here, and the elements of rows that see one are told: bit 16 (b % 2) + r of bits[b / 2].
+    __device__ __forceinline__ static void take_nans(uint32_t (&bits)[DV / 64], Values& v, int key, int limit) {
         const int h = (threadIdx.x & 63) >> 5;
         v8bf seen[2];
 #pragma unroll
@@ -450,16 +455,10 @@ struct Compute8 {
         for (int b = 0; b < DV / 32; b++) {
             v16f bad = {};
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                uint32_t number[2], none[2];
-                part_numbers(values_at(values_from(v), b, i), number, none);
-                const v8bf y = widen(number[0], number[1], i ? sc.v1 : sc.v0);
+            for (int i = 0; i < 2; i++) bad = mma(without_nans(v.x[b][i]), seen[i], bad);
 #pragma unroll
-                for (int p = P - 1; p >= 0; p--) st.o[b] = mma(y, w.v[p][i], st.o[b]);
-                bad = mma(widen(none[0], none[1], 1.0f), seen[i], bad);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; r++) st.o[b][r] += bad[r] > 0.0f ? __uint_as_float(0x7FC00000u) : 0.0f;
+            for (int r = 0; r < 16; r++) bits[b / 2] |= bad[r] > 0.0f ? 1u << (16 * (b & 1) + r) : 0u;
+            asm volatile("" : "+v"(bits[b / 2]));       // bits, not 64 masks of lanes
             __builtin_amdgcn_sched_barrier(0);  // rare: few registers
         }
     }
@@ -495,12 +494,18 @@ struct Compute8 {
         }
         Weights w[1];
         softmax<1>(st, w, s, near_end(sc), c);
-        if (edge && low < there && !all_numbers(v)) {
-            add_some(st, w[0], v, key, limit, sc);
-        } else {
-            Values x;
-            read_values(x, v);
-            add_values(st, x, w[0], sc);
+        Values x;
+        read_values(x, v);
+        const bool nans = edge && low < there && !all_numbers(v);
+        uint32_t bad[DV / 64] = {};
+        if (nans) take_nans(bad, x, key, limit);
+        add_values(st, x, w[0], sc);
+        if (nans) {
+#pragma unroll
+            for (int b = 0; b < DV / 32; b++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    st.o[b][r] = nan_where(st.o[b][r], bad[b / 2], 16 * (b & 1) + r);
         }
     }
     __device__ __forceinline__ static float sum(float l) {
@@ -637,25 +642,21 @@ struct Few8 {
         st.l = sum[0] + sum[1];
     }
     __device__ __forceinline__ static float value_scale(TileScales sc) { return group() & 1 ? sc.v1 : sc.v0; }
-    __device__ __forceinline__ static void add_some(Rows& st, const Weights& w, const uint8_t* v, int key, int limit,
-                                                    TileScales sc) {
-        const uint32_t from = values_from(v);
-        const float scale = value_scale(sc);
+    // bit 4 b + r, as above
+    __device__ __forceinline__ static uint32_t take_nans(v2i (&x)[DV / 16], int key, int limit) {
         v8bf seen;
 #pragma unroll
         for (int e = 0; e < 8; e++) seen[e] = (__bf16)(key + key_of(e / 4, group(), e % 4) < limit ? 1.0f : 0.0f);
+        uint32_t bits = 0;
 #pragma unroll
         for (int b = 0; b < DV / 16; b++) {
-            uint32_t number[2], none[2];
-            X::part_numbers(values_at(from, b), number, none);
-            const v8bf y = X::widen(number[0], number[1], scale);
+            const v4f bad = mma(X::without_nans(x[b]), seen, v4f{});
 #pragma unroll
-            for (int p = P - 1; p >= 0; p--) st.o[b] = mma(y, w.v[p], st.o[b]);
-            const v4f bad = mma(X::widen(none[0], none[1], 1.0f), seen, v4f{});
-#pragma unroll
-            for (int r = 0; r < 4; r++) st.o[b][r] += bad[r] > 0.0f ? __uint_as_float(0x7FC00000u) : 0.0f;
+            for (int r = 0; r < 4; r++) bits |= bad[r] > 0.0f ? 1u << (4 * b + r) : 0u;
+            asm volatile("" : "+v"(bits));
             __builtin_amdgcn_sched_barrier(0);  // rare: few registers
         }
+        return bits;
     }
     __device__ __forceinline__ static void tile(Rows& st, const Query& q, const uint8_t* k, const uint8_t* v, TileScales sc,
                                                 bool edge, int key, int limit, int low, int there, float c) {
@@ -670,20 +671,26 @@ struct Few8 {
         }
         Weights w;
         softmax(st, w, s, X::near_end(sc), c);
-        if (edge && low < there && !X::all_numbers(v)) {
-            add_some(st, w, v, key, limit, sc);
-            return;
-        }
         const uint32_t from = values_from(v);
         const float scale = value_scale(sc);
         v2i x[DV / 16];
 #pragma unroll
         for (int b = 0; b < DV / 16; b++) x[b] = values_at(from, b);
+        const bool nans = edge && low < there && !X::all_numbers(v);
+        uint32_t bad = 0;
+        if (nans) bad = take_nans(x, key, limit);
 #pragma unroll
         for (int b = 0; b < DV / 16; b++) {
             const v8bf a = X::widen((uint32_t)x[b][0], (uint32_t)x[b][1], scale);
 #pragma unroll
             for (int p = P - 1; p >= 0; p--) st.o[b] = mma(a, w.v[p], st.o[b]);
+        }
+        if (nans) {
+#pragma unroll
+            for (int b = 0; b < DV / 16; b++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    st.o[b][r] = X::nan_where(st.o[b][r], bad, 4 * b + r);
         }
     }
     // Four elements at a time: give(row, element / 4, them)
