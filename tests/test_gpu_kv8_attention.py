@@ -139,6 +139,38 @@ def test_rows_behind_the_last_sequence_stay(ctx):
 
 
 @pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("head_dim", [64, 128, 144])
+@pytest.mark.parametrize("prefix", [0, 70])
+def test_the_longest_sequence_is_only_a_hint(ctx, name, head_dim, prefix):
+    # which rows are multiplied 16, 32 or 128 at a time is chosen by it
+    p = Paged8([1, 70, 5, 33], [30, 90, 5, 400], prefix, 2, head_dim, 16, seed=4)
+    q = torch.randn(p.tokens, 8, head_dim, generator=torch.Generator().manual_seed(6)).to(TYPES[name])
+    want, want_l, by, bl = attention8_exact(p, q, 8, 0.125)
+    for max_q, max_len in ((0, 0), (1, 0), (4, 1), (5, 400), (70, 100000), (100000, 17)):
+        y, lse = _attend(ctx, p, q.cuda(), 8, 0.125, desc=p.describe(max_q=max_q, max_len=max_len))
+        within(y, want, by, f"y by {max_q}, {max_len}")
+        within(lse, want_l, bl, "lse")
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (5, 1), (16, 1), (17, 1), (14, 2)])
+def test_rows_of_a_group_around_16(ctx, name, heads, kv_heads):
+    for head_dim in (64, 128, 256):
+        _case(ctx, [1, 1, 1], [1, 333, 2000], 45, heads, kv_heads, head_dim, 16, name, seed=heads)
+        _case(ctx, [3, 2], [40, 2], 0, heads, kv_heads, head_dim, 32, name, block=32, seed=heads)
+        # the last key of each row no number, which the row before does not see
+        p, q, y, lse = _case(ctx, [3], [50], 0, heads, kv_heads, head_dim, 16, name, seed=heads + 1)
+        p.view(p.vc)[int(p.pages[0, 49 // 16]), :, 49 % 16, ::7] = 0x7F
+        p.refresh()
+        p.to_device()
+        y2, _ = _attend(ctx, p, q.cuda(), heads, 1.0 / math.sqrt(head_dim))
+        assert torch.equal(y2[:2], y[:2])
+        assert y2[2, :, ::7].isnan().all()
+        rest = torch.arange(head_dim) % 7 != 0
+        assert torch.equal(y2[2][:, rest], y[2][:, rest])
+
+
+@pytest.mark.parametrize("name", NAMES)
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
 def test_what_a_row_does_not_see_never_reaches_it(ctx, name, head_dim):
     # tokens from 2 on of one sequence hold NaN in elements 3 and 4: tokens 0 and 1 do not see them
