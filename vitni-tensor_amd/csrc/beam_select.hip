@@ -15,8 +15,10 @@
 // n): gathered in LDS and ranked by counting.  T's first 16 bits do.
 //
 // 512 rows of 128000 bf16 logits (116 MB, 22 us at a large copy's rate), 16 of each group of 8:
-// 60 us, where each element is 16 f64 operations of 4.3 cycles a wave, and 13 to join.  Four
-// rows of 32000 in f32: 5.6 and 4.9, two launches.
+// 58 us, of which 24 are memory's, 27 exponentials' (10 f64 operations and an LDS read each) and
+// 9 the lists'; 13 to join.  Twice the elements to a workgroup take 56 and 17; a workgroup that
+// goes through parts with the next one's loads ahead, 100 (its registers).  Four rows of 32000 in
+// f32: 5.6 and 4.9, two launches.
 #include <algorithm>
 #include <type_traits>
 
@@ -67,6 +69,42 @@ __device__ __forceinline__ double exp_of(double y) {
     p = fma(p, z, 0.9999999999595617);
     // times two to that number
     return __hiloint2double(__double2hiint(p) + (__double2loint(shifted) << 20), __double2loint(p));
+}
+
+// 2^(i / 64)
+__device__ const double kPowers[64] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
+};
+// sum + exp(y), y <= 0, exp to 2^-37 of itself; below -700, exp(-700).  Two to the nearest 64th of
+// y log2 e, a whole number's from its bits and the rest's from the powers in LDS, times
+// 1 + z + z^2 / 2 + z^3 / 6 for what is left, |z| <= h = ln 2 / 128, where z^4 / 24 has become its
+// nearest parabola, h^2 z^2 / 24 - h^4 / 192.  10 f64 operations; 14 with a polynomial alone.
+__device__ __forceinline__ double add_exp(double sum, double y, const double* powers) {
+    const double round = 6755399441055744.0;
+    y = fmax(y, -700.0);
+    const double shifted = fma(y, 92.33248261689366, round);
+    const double z = fma(shifted - round, -0.010830424696249145, y);
+    const int n = __double2loint(shifted);
+    const double power = powers[n & 63];
+    double p = fma(1.0 / 6, z, 0.500001221855199);
+    p = fma(p, z, 1.0);
+    p = fma(p, z, 0.9999999999955212);
+    return fma(__hiloint2double(__double2hiint(power) + ((n & ~63) << 14), __double2loint(power)), p, sum);
 }
 
 // The greater number; NaN if one is none.
@@ -152,7 +190,9 @@ __global__ __launch_bounds__(kThreads) void list_kernel(BeamJob j) {
     __shared__ int counts[4];  // candidates that a wave gathered; more than kGather: too many
     __shared__ double sums[4];
     __shared__ __attribute__((aligned(16))) uint64_t keys[4][kGather];
+    __shared__ double powers[64];
     if (lane == 0) tops[wave] = top, reaches[wave] = reach;
+    if (tid < 64) powers[tid] = kPowers[tid];
     __syncthreads();
     top = greater(greater(tops[0], tops[1]), greater(tops[2], tops[3]));
     reach = max(max(reaches[0], reaches[1]), max(reaches[2], reaches[3]));
@@ -172,23 +212,26 @@ __global__ __launch_bounds__(kThreads) void list_kernel(BeamJob j) {
     };
     // a candidate as a number: greater logits, then lower tokens are greater
     auto key_of = [&](float v, int token) { return (uint64_t)ordered(v) << 32 | (uint32_t)~token; };
-    int n_reach = 0;
     double sum = 0.0;
+    uint32_t reaching = 0;  // of this thread's elements, the first in bit E - 1
 #pragma unroll
     for (int i = 0; i < E; i++) {
         const float v = x(i);
-        const bool reaches_t = v >= least;
-        sum += exp_of((double)v - base);
-        const uint64_t reaching = __ballot(reaches_t);
-        if (reaching) {
-            const int to = n_reach + below(reaching);
-            if (reaches_t && to < kGather) keys[wave][to] = key_of(v, token_of(i));
-            n_reach += __popcll(reaching);
-        }
-        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // more at once would not fit the registers
+        sum = add_exp(sum, (double)v - base, powers);
+        reaching = 2 * reaching + (v >= least ? 1 : 0);
+        if (i % 4 == 3) asm volatile("" : "+v"(sum));  // more at once would not fit the registers
     }
-    // What is rare reads the logits again, where they are near by, and keeps no registers.
+    // What is rare reads the logits again, where they are near by, and keeps no registers: a lane has
+    // one or two that reach T.
     auto again = [&](int token) { return token < j.vocab ? (float)x0[token] : -INFINITY; };
+    int n_reach = 0;
+    for (uint64_t turn = __ballot(reaching != 0); turn && n_reach <= kGather; turn = __ballot(reaching != 0)) {
+        const int i = E - 32 + __builtin_clz(reaching | 1), token = token_of(i);
+        const int to = n_reach + below(turn);
+        if (reaching && to < kGather) keys[wave][to] = key_of(again(token), token);
+        reaching &= ~(1u << (E - 1 - i));
+        n_reach += __popcll(turn);
+    }
     // Of masked tokens, of which there may be many, n will do that come first: n of the wave's
     // first n + n_reach tokens are masked.
     const int window = n + n_reach;
