@@ -20,14 +20,14 @@
 //
 // Heads of more than 128 elements: a workgroup has half of the values' elements, and works
 // out all scores for them.  (The sums of all in one wave, 128 registers beside the query's 64,
-// spilled in every loop: 26 sequences of 7 behind 8099 keys, f16, 565 us against 107.)
+// spilled in every loop: 26 sequences of 7 behind 8099 keys, f16, 565 us against 100.)
 //
 // Measured (8 KV heads of 128, groups of 4, bf16; 16-bit keys in brackets): 128 sequences behind
-// 32768 keys with up to 1024 of their own 120 to 130 us (148); the prefix alone 101 (97), 700
+// 32768 keys with up to 1024 of their own 111 and 6 to join (148); the prefix alone 101 (97), 700
 // TFLOP/s at 2.05 GHz, the same with one workgroup a CU and with two: vector instructions, of
 // which a SIMD starts one every 4.3 cycles, 180 to a tile beside its 16 products (without the
-// softmax 15 us less, without the conversions 7).  The own keys alone 44 (88), 4.6 TB/s; 8
-// sequences of 32000 90 (160).
+// softmax 15 us less, without the conversions 7).  The own keys alone 41 (88), 4.9 TB/s; 8
+// sequences of 32000 87 (160).
 #include <type_traits>
 
 #include "vtq_attention_rows.h"
@@ -527,8 +527,9 @@ struct Compute8 {
 };
 
 // The same for 16 rows or fewer, a step's tokens of a group, by 16x16 products: half the products
-// and half the weights.  A score of register r of tile t (of 16 keys) is key 8 t + 4 (g / 2) +
-// 16 (g % 2) + r, g = lane / 16, so that a lane's keys lie in one block and its values in 8 rows.
+// and half the weights (128 sequences behind 32768 keys 133 -> 127 us, 64 behind 8192 37 -> 34).
+// A score of register r of tile t (of 16 keys) is key 8 t + 4 (g / 2) + 16 (g % 2) + r, g = lane / 16,
+// so that a lane's keys lie in one block and its values in 8 rows.
 template <class Q, int DK, int DV>
 struct Few8 {
     using X = Compute8<Q, DK, DV>;
