@@ -132,3 +132,23 @@ def test_scratch_memory_and_the_dispatch_packet(asm):
     assert len(kernels) >= 3 and len(packet) >= 3
     assert not any(packet.values()), packet
     assert not {k: sizes[k] for k in kernels if sizes[k]}
+
+
+def test_no_wait_for_all_loads_stands_beside_products(asm):
+    # the tiles ahead load to LDS, which the compiler does not count: a wait of its own for an ordinary load inside a
+    # loop would be one for all of them
+    name, text = asm
+    if name != "kv8_attention.hip":
+        pytest.skip("attention only")
+    blocks = 0
+    for kernel, body in _functions(text).items():
+        block = []
+        for line in body + [".LBB"]:
+            if not line.startswith(".LBB"):
+                block.append(line)
+                continue
+            if sum(l.startswith("v_mfma") for l in block) >= 4:
+                blocks += 1
+                assert not [l for l in block if re.match(r"s_waitcnt.*vmcnt\(0\)", l)], kernel
+            block = []
+    assert blocks >= 18 * 3

@@ -743,7 +743,9 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
     const int row_tiles = prefix ? j.prefix_rows : j.own_rows;
     const int splits = prefix ? j.prefix_splits : j.own_splits;
     const bool shared = prefix ? j.shared_prefix : j.shared_own;
-    const int row_tile = (int)(mine % row_tiles), part = (int)(mine / row_tiles % kParts);
+    const int part = (int)(mine / row_tiles % kParts);
+    // a prompt's last rows, which see the most keys, first
+    const int row_tile = prefix ? (int)(mine % row_tiles) : row_tiles - 1 - (int)(mine % row_tiles);
     int unit = (int)(mine / row_tiles / kParts) * 8 + xcd;  // KV head, then key range, then sequence
     const int kv_head = unit % kv_heads;
     unit /= kv_heads;
