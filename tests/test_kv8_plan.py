@@ -43,6 +43,21 @@ def _check(ggml_type, kv_heads, group, head_dim, page, batch, max_q, max_len, ma
     assert p["own_rows"] >= 1 and p["shared_prefix"] == (tokens * group > 32)
     assert 8 * p["prefix_per_xcd"] >= halves * kv_heads * p["prefix_splits"] * p["prefix_rows"]
     assert 8 * p["own_per_xcd"] >= halves * kv_heads * p["own_splits"] * batch * p["own_rows"]
+    # as the kernel takes them: every row tile of every range of keys once
+    for units, rows, per in ((kv_heads * p["prefix_splits"], halves * p["prefix_rows"], p["prefix_per_xcd"]),
+                             (kv_heads * p["own_splits"] * batch, halves * p["own_rows"], p["own_per_xcd"])):
+        if units * rows > 2000 or not units:
+            continue
+        turns, last = units // 8, units % 8
+        share = 8 // last if last else 1
+        seen = []
+        for xcd in range(8):
+            for mine in range(per):
+                if mine < turns * rows:
+                    seen.append((mine // rows * 8 + xcd, mine % rows))
+                elif xcd < last * share and (mine - turns * rows) * share + xcd // last < rows:
+                    seen.append((turns * 8 + xcd % last, (mine - turns * rows) * share + xcd // last))
+        assert sorted(seen) == [(u, t) for u in range(units) for t in range(rows)]
     assert p["prefix_per_xcd"] >= 0 and 8 * (p["prefix_per_xcd"] + p["own_per_xcd"]) * 256 < 1 << 32
     return p
 
@@ -71,7 +86,8 @@ def test_plans_cover_the_work(ggml_type, kv_heads):
 @pytest.mark.parametrize("ggml_type", [vtq.F32, vtq.F16, vtq.BF16])
 def test_plans_of_the_largest_calls(ggml_type):
     for head_dim, most in ((128, 22), (256, 20)):
-        for args in ((1, 8, head_dim, 16, 1, 8192, 0, 512, 0, 8192),
+        for args in ((1, 8, head_dim, 16, 1, 8192, 0, 512, 0, 8192), (3, 8, head_dim, 16, 1, 500, 0, 32, 0, 500),
+                     (4, 8, head_dim, 16, 1, 1000, 0, 64, 0, 1000), (2, 16, head_dim, 16, 1, 333, 0, 64, 70, 333),
                      (1, 8, head_dim, 16, 1, 1 << (most - 3), 0, (1 << 30) // 16 - 1, (1 << 30) - 1, 1 << (most - 3)),
                      (8, 1, head_dim, 16, 1 << (most - 3), 1, 0, 4, 7, 1 << (most - 3)),
                      (8, 1, head_dim, 16, 1 << (most - 3), 1, 0, 4, 0, 1 << (most - 3)),

@@ -734,8 +734,8 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
     const int hd = a.cache.head_dim, G = j.group, kv_heads = a.cache.kv_heads;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
 
-    // Which part of the work: as in cache_attention.hip.  Workgroups go to the 8 XCDs in
-    // turn; the row tiles of the same keys follow each other on one.
+    // Which part of the work.  Workgroups go to the 8 XCDs in turn; the row tiles of the same keys
+    // follow each other on one, or on as many as share them.
     const int xcd = (int)(blockIdx.x & 7);
     const int64_t s = blockIdx.x >> 3;
     const bool prefix = s < j.prefix_per_xcd;
@@ -743,14 +743,25 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
     const int row_tiles = prefix ? j.prefix_rows : j.own_rows;
     const int splits = prefix ? j.prefix_splits : j.own_splits;
     const bool shared = prefix ? j.shared_prefix : j.shared_own;
-    const int part = (int)(mine / row_tiles % kParts);
+    const int all_tiles = row_tiles * kParts;
+    const int64_t units = (int64_t)kv_heads * splits * (prefix ? 1 : a.batch.batch), turns = units / 8;
+    int unit, tile;  // KV head, then key range, then sequence; row tiles of the parts
+    if (mine < turns * all_tiles) {
+        unit = (int)(mine / all_tiles) * 8 + xcd;
+        tile = (int)(mine % all_tiles);
+    } else {
+        const int last = (int)(units % 8), share = xcds_of(last);
+        if (xcd >= last * share) return;
+        unit = (int)turns * 8 + xcd % last;
+        tile = (int)(mine - turns * all_tiles) * share + xcd / last;
+        if (tile >= all_tiles) return;
+    }
+    const int part = tile / row_tiles;
     // a prompt's last rows, which see the most keys, first
-    const int row_tile = prefix ? (int)(mine % row_tiles) : row_tiles - 1 - (int)(mine % row_tiles);
-    int unit = (int)(mine / row_tiles / kParts) * 8 + xcd;  // KV head, then key range, then sequence
+    const int row_tile = prefix ? tile % row_tiles : row_tiles - 1 - tile % row_tiles;
     const int kv_head = unit % kv_heads;
     unit /= kv_heads;
     const int split = unit % splits, seq = unit / splits;
-    if (seq >= (prefix ? 1 : a.batch.batch)) return;
 
     // tokens, keys and the key range
     const int64_t all = min((int64_t)max(uniform(a.batch.q_start[a.batch.batch]), 0), a.tokens);
