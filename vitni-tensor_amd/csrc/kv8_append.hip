@@ -10,14 +10,14 @@
 // of more bits would gain little: e4m3 is a float, its rounding relative to the element.
 //
 // A workgroup takes a block of a sequence and some of its heads, a wave a head's keys or
-// values.  What the wave's lanes hold at once, 16 tokens of up to 128 elements, stays in
+// values.  What the wave's lanes hold at once, four tokens of 128 elements, stays in
 // registers between the maximum and the stores; longer blocks are read again, from the
 // caches near by.  Queries are rotated by workgroups of their own in the same launch.
 //
-// A step of 32 sequences, 8 KV heads of 128 and 32 query heads in bf16, takes 6.4 us in a graph:
+// A step of 32 sequences, 8 KV heads of 128 and 32 query heads in bf16, takes 6.5 us in a graph:
 // the launch and three reads that wait for each other (lengths, page, scale; 8.3 where the row
-// and the angles wait for the page too).  Prompts of 4,500 tokens in f32 (124 MB to read and
-// write, 24 us at a large copy's rate) take 35.6.
+// and the angles wait for the page too).  Prompts of 4,500 tokens in f32 (121 MB to read and
+// write, 23.4 us at a large copy's rate) take 26.5; of 4000 in bf16 by blocks of 64 38 (17).
 #include "vtq_rope.h"
 
 namespace vtq {
@@ -116,87 +116,77 @@ __device__ __forceinline__ int block_tokens(const vtq_kv_batch& b, int64_t token
     return 0;
 }
 
-// Units of a row of some tokens, H to a lane: their elements, rotated.
-template <class T, int N, int H>
+// A unit of a row of some tokens to each lane: its elements, rotated.  (Four units to a lane hold
+// 16 tokens of 128 elements at once, and 173 registers: prompts of 4,500 tokens in f32 take 35 us
+// against 26, which read longer blocks again.  Two take 31.)
+template <class T, int N>
 struct Held {
-    float x[H][2][N];
-    int at[H][2];   // first element of each part; -1: there is none
-    int token[H];
-    Pack<T, N> a[H], b[H];
-    bool turns[H];
-    int pair[H];
+    float x[2][N];
+    int at[2];  // first element of each part; -1: there is none
+    int token;
+    Pack<T, N> a, b;
+    bool turns;
+    int pair;
 
-    // Units w0 + 64 k + lane of n tokens' `units` each: their loads, all at once
+    // Unit w0 + lane of n tokens' `units` each: its loads
     __device__ __forceinline__ void fetch(const T* src, int64_t token_stride, int w0, int n, int units, int rot, bool half) {
         const int lane = threadIdx.x & 63, per = half || N == 1 ? rot / 2 / N : rot / N, step = half ? rot / 2 : 1;
-#pragma unroll
-        for (int k = 0; k < H; k++) {
-            const int w = w0 + 64 * k + lane, last = min(w, n * units - 1), unit = last % units;
-            token[k] = last / units;
-            turns[k] = unit < per;
-            const bool two = turns[k] && (half || N == 1);
-            // where the unit begins; a pair's elements stand side by side, or half the rotated part apart
-            int first;
-            if (turns[k]) first = half ? unit * N : N == 1 ? 2 * unit : unit * N;
-            else first = (half || N == 1 ? rot : per * N) + (unit - per) * N;
-            pair[k] = half || N == 1 ? unit * N : unit * N / 2;
-            at[k][0] = w < n * units ? first : -1;
-            at[k][1] = w < n * units && two ? first + step : -1;
-            const T* from = src + token[k] * token_stride + first;
-            a[k] = *reinterpret_cast<const Pack<T, N>*>(from);
-            b[k] = *reinterpret_cast<const Pack<T, N>*>(two ? from + step : from);
-        }
+        const int w = w0 + lane, last = min(w, n * units - 1), unit = last % units;
+        token = last / units;
+        turns = unit < per;
+        const bool two = turns && (half || N == 1);
+        // where the unit begins; a pair's elements stand side by side, or half the rotated part apart
+        int first;
+        if (turns) first = half ? unit * N : N == 1 ? 2 * unit : unit * N;
+        else first = (half || N == 1 ? rot : per * N) + (unit - per) * N;
+        pair = half || N == 1 ? unit * N : unit * N / 2;
+        at[0] = w < n * units ? first : -1;
+        at[1] = w < n * units && two ? first + step : -1;
+        const T* from = src + token * token_stride + first;
+        a = *reinterpret_cast<const Pack<T, N>*>(from);
+        b = *reinterpret_cast<const Pack<T, N>*>(two ? from + step : from);
     }
     __device__ __forceinline__ void rotate(const float2 (*cs)[128], bool half) {
+        const float2* c = cs[token] + (turns ? pair : 0);
+        if (half || N == 1) {
 #pragma unroll
-        for (int k = 0; k < H; k++) {
-            const float2* c = cs[token[k]] + (turns[k] ? pair[k] : 0);
-            if (half || N == 1) {
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const float2 w = c[e];
-                    const float p = (float)a[k].v[e], q = (float)b[k].v[e];
-                    x[k][0][e] = turns[k] ? p * w.x - q * w.y : p;
-                    x[k][1][e] = turns[k] ? p * w.y + q * w.x : p;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    const float2 w = c[e / 2];
-                    const float p = (float)a[k].v[e], q = (float)a[k].v[e + 1 < N ? e + 1 : e];
-                    x[k][0][e] = turns[k] ? p * w.x - q * w.y : p;
-                    if (e + 1 < N) x[k][0][e + 1] = turns[k] ? p * w.y + q * w.x : q;
-                }
-#pragma unroll
-                for (int e = 0; e < N; e++) x[k][1][e] = x[k][0][e];
+            for (int e = 0; e < N; e++) {
+                const float2 w = c[e];
+                const float p = (float)a.v[e], q = (float)b.v[e];
+                x[0][e] = turns ? p * w.x - q * w.y : p;
+                x[1][e] = turns ? p * w.y + q * w.x : p;
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                const float2 w = c[e / 2];
+                const float p = (float)a.v[e], q = (float)a.v[e + 1 < N ? e + 1 : e];
+                x[0][e] = turns ? p * w.x - q * w.y : p;
+                if (e + 1 < N) x[0][e + 1] = turns ? p * w.y + q * w.x : q;
+            }
+#pragma unroll
+            for (int e = 0; e < N; e++) x[1][e] = x[0][e];
         }
     }
     __device__ __forceinline__ float top() const {
         float most = 0.0f;
 #pragma unroll
-        for (int k = 0; k < H; k++)
+        for (int p = 0; p < 2; p++)
 #pragma unroll
-            for (int p = 0; p < 2; p++)
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const float v = fabsf(x[k][p][e]);
-                    most = fmaxf(most, v < INFINITY ? v : 0.0f);
-                }
+            for (int e = 0; e < N; e++) {
+                const float v = fabsf(x[p][e]);
+                most = fmaxf(most, v < INFINITY ? v : 0.0f);
+            }
         return most;
     }
     __device__ __forceinline__ void put(uint8_t* dst, int64_t slot, int e) const {
 #pragma unroll
-        for (int k = 0; k < H; k++)
-#pragma unroll
-            for (int p = 0; p < 2; p++)
-                if (at[k][p] >= 0) put8<N>(dst + token[k] * slot + at[k][p], x[k][p], e);
+        for (int p = 0; p < 2; p++)
+            if (at[p] >= 0) put8<N>(dst + token * slot + at[p], x[p], e);
     }
 };
 
-// H: 1 where a sequence's tokens fit a wave by the hint, and a row is on its way while the angles
-// are worked out (with four units to a lane that takes 235 registers); else 4.
-template <class T, int N, int H>
+template <class T, int N>
 __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int rot = j.rotate ? j.rope.rot_dim : 0;
@@ -255,8 +245,8 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int page = j.batch.pages[(int64_t)spot.seq * j.batch.max_pages + spot.place / j.cache.page_size];
     // One pass where a row of all tokens is held at once, else one for the maxima and one for the stores.
     const int most_units = max(units_rot, units_plain);
-    const bool once = count <= kCosTokens && count * most_units <= 64 * H;
-    Held<T, N, H> held;
+    const bool once = count <= kCosTokens && count * most_units <= 64;
+    Held<T, N> held;
     auto row_of = [&](int r, int c0) {  // from token c0 of the block on
         const HeadRows& in = r >= j.kv_heads ? j.v : j.k;
         return static_cast<const T*>(in.p) + (t + c0) * in.token_stride + (r % j.kv_heads) * in.head_stride;
@@ -265,8 +255,8 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
         const bool is_v = r >= j.kv_heads;
         held.fetch(row_of(r, c0), (is_v ? j.v : j.k).token_stride, w0, n, is_v ? units_plain : units_rot, is_v ? 0 : rot, half);
     };
-    const bool early = H == 1 && once;  // the page, the first row and the angles together
-    if (early && r0 + wave < r1) fetch(r0 + wave, 0, 0, count);
+    // the page, the first row and the angles on their way together
+    if (once && r0 + wave < r1) fetch(r0 + wave, 0, 0, count);
     if (keys && once) turn(spot.place, count);
     if (page < 0 || page >= (int64_t)j.cache.n_pages) return;
     const int64_t at = page * (int64_t)j.cache.page_stride +
@@ -288,8 +278,8 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
                 const int old = before ? min(max((int)*scale - 127, kLeast), kMost) : kLeast;
                 float top = 0.0f;
                 if (pass == 0 || once) {
-                    for (int w0 = 0; w0 < n * units; w0 += 64 * H) {
-                        if (!early || r != r0 + wave) fetch(r, c0, w0, n);
+                    for (int w0 = 0; w0 < n * units; w0 += 64) {
+                        if (!once || r != r0 + wave) fetch(r, c0, w0, n);
                         held.rotate(cs, half);
                         top = fmaxf(top, held.top());
                     }
@@ -319,7 +309,7 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
                 if (once) {
                     held.put(dst, slot, e);
                 } else {
-                    for (int w0 = 0; w0 < n * units; w0 += 64 * H) {
+                    for (int w0 = 0; w0 < n * units; w0 += 64) {
                         fetch(r, c0, w0, n);
                         held.rotate(cs, half);
                         held.put(dst, slot, e);
@@ -337,9 +327,9 @@ hipError_t launch_kv8_append(const RopeJob& job, const Scales& s, int type, hipS
     j.s = s;
     const int n = rope_access(j, type_bytes(type));
     // Queries: a workgroup takes up to four tokens of a long call, a token a wave to find and four
-    // tokens' angles at once, and some heads of a short one, so that they keep the chip busy
-    // (prompts of 4,500 tokens, 32 heads of 80 in f32, with the keys and values: 42.5 us against
-    // 49 with a token each; 35.6 with the keys and values, which take longer, first).
+    // tokens' angles at once, and some heads of a short one, so that they keep the chip busy.  The
+    // keys and values, which take longer, go first.  (Prompts of 4,500 tokens in f32, with four units
+    // to a lane: a token each 49 us, four 42.5, the keys and values first 35.6.)
     const int64_t units = (int64_t)j.x_heads * (j.head_dim / n);
     j.q_tokens = (int)std::max<int64_t>(1, std::min<int64_t>(kQueryTokens, j.tokens / 1024));
     j.q_groups = (int)std::max<int64_t>(1, std::min<int64_t>({(units + kRopeThreads - 1) / kRopeThreads, 1024 / j.tokens,
@@ -356,20 +346,12 @@ hipError_t launch_kv8_append(const RopeJob& job, const Scales& s, int type, hipS
     j.kv_groups = (rows + j.rows_per - 1) / j.rows_per;
     j.kv_work = blocks * j.kv_groups;
     const dim3 grid((unsigned)(j.kv_work + q_work));
-    const int most_units = std::max(rotated_units(j.head_dim, j.rotate ? j.rope.rot_dim : 0,
-                                                  j.rope.layout == VTQ_ROPE_HALF, n), j.head_dim / n);
-    const bool few = j.batch.max_q > 0 && std::min<int64_t>(j.batch.max_q, j.tokens) * most_units <= 64;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        auto launch = [&](auto n_of) {
-            constexpr int N = decltype(n_of)::value;
-            if (few) hipLaunchKernelGGL((kv8_append_kernel<T, N, 1>), grid, dim3(kRopeThreads), 0, stream, j);
-            else hipLaunchKernelGGL((kv8_append_kernel<T, N, 4>), grid, dim3(kRopeThreads), 0, stream, j);
-        };
-        if (n == 8) launch(std::integral_constant<int, 8>{});
-        else if constexpr (sizeof(T) == 4)
-            if (n == 4) launch(std::integral_constant<int, 4>{});
-        if (n == 1) launch(std::integral_constant<int, 1>{});
+        if (n == 8) hipLaunchKernelGGL((kv8_append_kernel<T, 8>), grid, dim3(kRopeThreads), 0, stream, j);
+        if constexpr (sizeof(T) == 4)
+            if (n == 4) hipLaunchKernelGGL((kv8_append_kernel<T, 4>), grid, dim3(kRopeThreads), 0, stream, j);
+        if (n == 1) hipLaunchKernelGGL((kv8_append_kernel<T, 1>), grid, dim3(kRopeThreads), 0, stream, j);
         return hipGetLastError();
     });
 }
