@@ -17,13 +17,14 @@
 // A step of 32 sequences, 8 KV heads of 128 and 32 query heads in bf16, takes 6.5 us in a graph:
 // the launch and three reads that wait for each other (lengths, page, scale; 8.3 where the row
 // and the angles wait for the page too).  Prompts of 4,500 tokens in f32 (121 MB to read and
-// write, 23.4 us at a large copy's rate) take 26.5; of 4000 in bf16 by blocks of 64 38 (17).
+// write, 23.4 us at a large copy's rate) take 26.5; of 4000 in bf16 by blocks of 64 35 (17; 38 with angles of 16 tokens
+// at a time, worked out twice).
 #include "vtq_rope.h"
 
 namespace vtq {
 namespace {
 
-constexpr int kCosTokens = 16;  // tokens whose cosines are held at a time
+constexpr int kAngles = 4096;   // cosines and sines that are held at a time: 64 tokens of 128 rotated elements
 constexpr int kMostRows = 32;   // heads' keys and values to a workgroup
 constexpr int kQueryTokens = 4;  // tokens at most whose queries a workgroup rotates: one a wave
 constexpr int kLeast = -117, kMost = 119;  // exponents of scales: what they scale stays a normal bf16
@@ -146,8 +147,8 @@ struct Held {
         a = *reinterpret_cast<const Pack<T, N>*>(from);
         b = *reinterpret_cast<const Pack<T, N>*>(two ? from + step : from);
     }
-    __device__ __forceinline__ void rotate(const float2 (*cs)[128], bool half) {
-        const float2* c = cs[token] + (turns ? pair : 0);
+    __device__ __forceinline__ void rotate(const float2* cs, int rot, bool half) {
+        const float2* c = cs + token * (rot / 2) + (turns ? pair : 0);
         if (half || N == 1) {
 #pragma unroll
             for (int e = 0; e < N; e++) {
@@ -192,7 +193,8 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int rot = j.rotate ? j.rope.rot_dim : 0;
     const bool half = j.rope.layout == VTQ_ROPE_HALF;
     const int units_rot = rotated_units(j.head_dim, rot, half, N), units_plain = j.head_dim / N;
-    __shared__ float2 cs[kCosTokens][128];
+    __shared__ float2 cs[kAngles];
+    const int at_once = rot ? min(kAngles / (rot / 2), 64) : 64;  // tokens
     __shared__ float tops[kMostRows];
     // cosine and sine of a pair of the token at `place` (behind the prefix)
     auto turn_pair = [&](int64_t place, int pair) {
@@ -202,7 +204,7 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     auto turn = [&](int64_t from, int n) {  // of n tokens from the place `from` on
         for (int i = threadIdx.x; i < n * (rot / 2); i += kRopeThreads) {
             const int token = i / (rot / 2), pair = i % (rot / 2);
-            cs[token][pair] = turn_pair(from + token, pair);
+            cs[i] = turn_pair(from + token, pair);
         }
     };
     if ((int64_t)blockIdx.x >= j.kv_work) {
@@ -221,14 +223,14 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
         __syncthreads();
         if (rot)
             for (int i = threadIdx.x; i < n * (rot / 2); i += kRopeThreads)
-                cs[i / (rot / 2)][i % (rot / 2)] = turn_pair(places[i / (rot / 2)], i % (rot / 2));
+                cs[i] = turn_pair(places[i / (rot / 2)], i % (rot / 2));
         __syncthreads();
         const int h0 = group * j.q_per, heads = min(j.x_heads, h0 + j.q_per) - h0;
         for (int w = threadIdx.x; w < n * heads * units_rot; w += kRopeThreads) {
             const int u = w % units_rot, h = h0 + w / units_rot % heads, i = w / units_rot / heads;
             if (!there[i]) continue;
             rotate_unit<T, T, N>(static_cast<const T*>(j.x.p) + (t0 + i) * j.x.token_stride + h * j.x.head_stride,
-                                 static_cast<T*>(j.y) + (t0 + i) * j.y_token_stride + h * j.y_head_stride, cs[i], u, rot, half);
+                                 static_cast<T*>(j.y) + (t0 + i) * j.y_token_stride + h * j.y_head_stride, cs + i * (rot / 2), u, rot, half);
         }
         return;
     }
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int page = j.batch.pages[(int64_t)spot.seq * j.batch.max_pages + spot.place / j.cache.page_size];
     // One pass where a row of all tokens is held at once, else one for the maxima and one for the stores.
     const int most_units = max(units_rot, units_plain);
-    const bool once = count <= kCosTokens && count * most_units <= 64;
+    const bool once = count <= at_once && count * most_units <= 64;
     Held<T, N> held;
     auto row_of = [&](int r, int c0) {  // from token c0 of the block on
         const HeadRows& in = r >= j.kv_heads ? j.v : j.k;
@@ -264,9 +266,9 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int before = (int)(spot.place & (block - 1));
     const int64_t scale_at = page * j.s.page_stride + (spot.place & (j.cache.page_size - 1)) / block;
     for (int pass = once ? 1 : 0; pass < 2; pass++)
-        for (int c0 = 0; c0 < count; c0 += kCosTokens) {
-            const int n = min(kCosTokens, count - c0);
-            if (keys && !once && (pass == 0 || count > kCosTokens)) {
+        for (int c0 = 0; c0 < count; c0 += at_once) {
+            const int n = min(at_once, count - c0);
+            if (keys && !once && (pass == 0 || count > at_once)) {
                 if (pass || c0) __syncthreads();
                 turn(spot.place + c0, n);
             }
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
                 if (pass == 0 || once) {
                     for (int w0 = 0; w0 < n * units; w0 += 64) {
                         if (!once || r != r0 + wave) fetch(r, c0, w0, n);
-                        held.rotate(cs, half);
+                        held.rotate(cs, rot, half);
                         top = fmaxf(top, held.top());
                     }
 #pragma unroll
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
                 } else {
                     for (int w0 = 0; w0 < n * units; w0 += 64) {
                         fetch(r, c0, w0, n);
-                        held.rotate(cs, half);
+                        held.rotate(cs, rot, half);
                         held.put(dst, slot, e);
                     }
                 }
