@@ -17,8 +17,8 @@
 // A step of 32 sequences, 8 KV heads of 128 and 32 query heads in bf16, takes 6.5 us in a graph:
 // the launch and three reads that wait for each other (lengths, page, scale; 8.3 where the row
 // and the angles wait for the page too).  Prompts of 4,500 tokens in f32 (121 MB to read and
-// write, 23.4 us at a large copy's rate) take 26.5; of 4000 in bf16 by blocks of 64 35 (17; 38 with angles of 16 tokens
-// at a time, worked out twice).
+// write, 23.4 us at a large copy's rate) take 26.5; of 4000 in bf16 by blocks of 64 35 (17; 38
+// with angles of 16 tokens at a time, worked out twice).
 #include "vtq_rope.h"
 
 namespace vtq {
