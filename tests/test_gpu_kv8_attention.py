@@ -7,6 +7,7 @@ import torch
 import vtq
 from kv8 import Paged8, attention8_exact
 from serving import TAGS, TYPES, stream, within
+from vtq import probe
 
 pytestmark = pytest.mark.gpu
 
@@ -150,6 +151,25 @@ def test_the_longest_sequence_is_only_a_hint(ctx, name, head_dim, prefix):
         y, lse = _attend(ctx, p, q.cuda(), 8, 0.125, desc=p.describe(max_q=max_q, max_len=max_len))
         within(y, want, by, f"y by {max_q}, {max_len}")
         within(lse, want_l, bl, "lse")
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("head_dim,prefix", [(64, 1), (64, 70), (128, 33), (128, 200), (256, 64)])
+def test_prompts_behind_a_short_prefix(ctx, name, head_dim, prefix):
+    # prompts that fill the chip take the prefix's keys in their own workgroups; among them tokens without a slot, which
+    # see the prefix alone, and a sequence without tokens
+    q_lens = [33] * 30 + [1, 0, 70, 40, 5] + [20] * 31
+    own = [40] * 30 + [1, 7, 90, 30, 0] + [25] * 31
+    p = Paged8(q_lens, own, prefix, 4, head_dim, 16, seed=prefix)
+    assert probe.attention_plan(p.cache, p.desc, TAGS[name], p.tokens, 8)["prefix_splits"] == 0
+    q = torch.randn(p.tokens, 8, head_dim, generator=torch.Generator().manual_seed(8)).to(TYPES[name])
+    y, lse = _attend(ctx, p, q.cuda(), 8, 0.2)
+    want, want_l, by, bl = attention8_exact(p, q, 8, 0.2)
+    within(y, want, by, "y")
+    within(lse, want_l, bl, "lse")
+    z = q.cuda()
+    _attend(ctx, p, z, 8, 0.2, y=z)
+    assert torch.equal(z, y)
 
 
 @pytest.mark.parametrize("name", NAMES)

@@ -45,6 +45,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 struct Job8 : Job {
     Scales s;
     int block_shift;
+    int prefix_inside;  // own workgroups take the prefix's keys first
 };
 
 template <int D>
@@ -767,6 +768,7 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
     const int64_t all = min((int64_t)max(uniform(a.batch.q_start[a.batch.batch]), 0), a.tokens);
     int64_t t0 = 0, t1 = all;
     Runs runs;
+    const int32_t* own_list = nullptr;
     int k0, k1, unseen = 0;  // row of token t sees keys below  t - t0 + 1 + unseen  (own keys)
     if (prefix) {
         runs.list = a.batch.prefix_pages;
@@ -776,7 +778,7 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
     } else {
         t0 = min(max((int64_t)uniform(a.batch.q_start[seq]), (int64_t)0), all);
         t1 = min(max((int64_t)uniform(a.batch.q_start[seq + 1]), t0), all);
-        runs.list = a.batch.pages + (int64_t)seq * a.batch.max_pages;
+        runs.list = own_list = a.batch.pages + (int64_t)seq * a.batch.max_pages;
         const int len = uniform(min(max(a.batch.len[seq], -(1 << 29)), 1 << 30));
         runs.keys = min(max(len, 0), a.batch.max_pages << j.page_shift);
         unseen = len - (int)(t1 - t0);
@@ -811,22 +813,34 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
         const int whole = (first_limit - k0) / 32;              // tiles that every row sees whole
         const Q* q_row = static_cast<const Q*>(a.q.p) + token * a.q.token_stride + head * a.q.head_stride;
         const int out_split = prefix ? split : j.prefix_splits + split;
-        auto begin = [&](auto& q, auto& st, auto of) {
-            decltype(of)::load_query(q, q_row, valid, hd);
-            runs.keys = end;  // past the last row's sight nothing is read
-            if (tiles > 0) from.hold(runs, k0);
-            // waited for here, as in hold()
-            for (auto& part : q.v)
-                for (auto& x : part) asm volatile("" : "+v"(x));
+        auto clear = [&](auto& st) {
             st.m = -INFINITY;
             st.l = 0.0f;
             for (auto& o : st.o) o = std::remove_reference_t<decltype(o)>{};
         };
+        // the query's loads are waited for before the loops, as those of hold()
+        auto wait_for = [&](auto& q) {
+            for (auto& part : q.v)
+                for (auto& x : part) asm volatile("" : "+v"(x));
+        };
         if (shared) {
             typename X::Query q;
             State<DV> st;
-            begin(q, st, X{});
-            if (tiles > 0) {
+            X::load_query(q, q_row, valid, hd);
+            clear(st);
+            // the prefix's keys, where they are this workgroup's too (never beside 16 rows), then its own
+            const bool inside = R == 32 && j.prefix_inside;
+            for (int of_prefix = inside && !prefix && split == 0; of_prefix >= 0; of_prefix--) {
+                const int begin = of_prefix ? 0 : k0, stop = of_prefix ? a.batch.prefix_len : end;
+                const int tiles = stop > begin ? (stop - begin + 31) / 32 : 0;  // of 32 keys
+                if (tiles == 0) continue;
+                // tiles that every row sees whole; keys that this row, and the wave's rows at least and at most, see
+                const int whole = ((of_prefix ? stop : first_limit) - begin) / 32, sees = of_prefix ? stop : limit;
+                const int least = of_prefix ? stop : low, most = !of_prefix ? high : __ballot(valid) ? stop : 0;
+                if (inside) runs.list = of_prefix ? a.batch.prefix_pages : own_list;
+                runs.keys = stop;  // past the last row's sight nothing is read
+                from.hold(runs, begin);
+                wait_for(q);
                 // stages of two tiles (K, then V), S - 1 of them ahead; a wave loads 16 of the 64 keys
                 constexpr int kStage = 2 * Cfg::kTile, S = Cfg::kLds / kStage;
                 const int stages = (tiles + 1) / 2;
@@ -834,9 +848,9 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                 // Every step loads a stage, past the end too (zeros from nowhere), so that the count of
                 // those in flight stays the same.
                 auto load_stage = [&](int m, int to) {
-                    const int key = k0 + 64 * m;
+                    const int key = begin + 64 * m;
                     // (what is held begins at the tiles at hand, whose scales are read from it too)
-                    if ((min(key + 64, runs.keys) - 1) / 16 - runs.first >= 64) from.hold(runs, k0 + 64 * n);
+                    if ((min(key + 64, runs.keys) - 1) / 16 - runs.first >= 64) from.hold(runs, begin + 64 * n);
                     const uint32_t stage = lds0 + (uint32_t)(to * kStage);
                     from.load16(runs, key + 16 * wave, stage + 16 * wave * TK::kRow,
                                 stage + 2 * TK::kBytes + 16 * wave * TV::kRow);
@@ -852,7 +866,7 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
                     load_stage(n + S - 1, at == 0 ? S - 1 : at - 1);
-                    here0 = from.scales(runs, k0 + 64 * n), here1 = from.scales(runs, k0 + 64 * n + 32);
+                    here0 = from.scales(runs, begin + 64 * n), here1 = from.scales(runs, begin + 64 * n + 32);
                     const uint8_t* k = lds + at * kStage;
                     at = at + 1 == S ? 0 : at + 1;
                     return k;
@@ -867,15 +881,15 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                     const uint8_t* k = next_stage();
 #pragma unroll 1
                     for (int i = 0; i < 2; i++) {
-                        const int key = k0 + 64 * n + 32 * i;
+                        const int key = begin + 64 * n + 32 * i;
                         const TileScales sc = i ? here1 : here0;
-                        if (2 * n + i < tiles && key < high)
+                        if (2 * n + i < tiles && key < most)
                             X::tile(st, q, k + i * TK::kBytes, k + 2 * TK::kBytes + i * TV::kBytes, sc, 2 * n + i >= whole, key,
-                                    limit, low, runs.keys, j.c);
+                                    sees, least, runs.keys, j.c);
                     }
                 }
                 wait_vmcnt<0>();
-                // the next row tile's loads overwrite what other waves may still read
+                // the next keys' or row tile's loads overwrite what other waves may still read
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
@@ -893,7 +907,11 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
         {
             typename Y::Query q;
             typename Y::Rows st;
-            begin(q, st, Y{});
+            Y::load_query(q, q_row, valid, hd);
+            clear(st);
+            runs.keys = end;  // past the last row's sight nothing is read
+            if (tiles > 0) from.hold(runs, k0);
+            wait_for(q);
             if (wave < tiles) {
                 // a wave's two stages of a tile
                 const uint8_t* mine8 = lds + wave * 2 * Cfg::kTile;
@@ -984,7 +1002,9 @@ size_t kv8_attention_workspace(const vtq_kv_cache& cache, const vtq_kv_batch& ba
 
 hipError_t launch_kv8_attention(const Attention& a, const Scales& s, int type, hipStream_t stream) {
     Job8 j{};
-    static_cast<AttentionPlan&>(j) = plan_kv8_attention(a.cache, a.batch, type, a.tokens, a.heads);
+    bool inside;
+    static_cast<AttentionPlan&>(j) = plan_kv8_attention(a.cache, a.batch, type, a.tokens, a.heads, &inside);
+    j.prefix_inside = inside;
     j.a = a;
     j.c = a.scale * kLog2E;
     j.s = s;
