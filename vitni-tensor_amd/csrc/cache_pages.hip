@@ -435,7 +435,9 @@ struct CopyJob : PagesCopy {
     int row_chunks;  // of 16 bytes, of a head's row
     int units;       // of a copy: layers x 2
     int unit_rows;   // units to an XCD
+    int share;       // XCDs to a unit, where units are few
     int pieces;      // workgroups to a unit
+    int turns;       // of an XCD, for its share of them
     int64_t work;
 };
 
@@ -446,19 +448,21 @@ constexpr int kPiece = 4 * kThreads;  // chunks to a workgroup, in flight at onc
 
 // A workgroup takes up to 16 KB of a copy's keys or values of a layer.  Pages lie anywhere, and
 // address translation is what a short list of copies waits for: workgroups go to the 8 XCDs
-// in turn, and a layer's keys (or values) stay on one of them.
+// in turn, and a layer's keys (or values) stay on one of them, or on some where layers are few
+// (240 pages of 256 KB on one layer, with the lists: 56 us against 137).
 __global__ __launch_bounds__(kThreads) void copy_kernel(CopyJob j) {
     const int tid = threadIdx.x;
     const int64_t n = j.count ? min(max((int64_t)*j.count, (int64_t)0), j.max_copies) : j.max_copies;
     const vtq_kv_cache& c = j.cache;
     for (int64_t i = blockIdx.x; i < j.work; i += gridDim.x) {
         int64_t at = i >> 3;
-        const int unit = (int)(at % j.unit_rows) * 8 + (int)(i & 7);
+        const int xcd = (int)(i & 7), of = j.share > 1 ? xcd / j.units : 0;
+        const int unit = j.share > 1 ? xcd % j.units : (int)(at % j.unit_rows) * 8 + xcd;
         at /= j.unit_rows;
-        const int piece = (int)(at % j.pieces);
-        const int64_t copy = at / j.pieces;
+        const int piece = (int)(at % j.turns) * j.share + of;
+        const int64_t copy = at / j.turns;
         if (copy >= n) return;
-        if (unit >= j.units) continue;
+        if (unit >= j.units || of >= j.share || piece >= j.pieces) continue;
         const int32_t from = j.copies[3 * copy], to = j.copies[3 * copy + 1];
         const int slots = min(max(j.copies[3 * copy + 2], 0), c.page_size);
         if (!is_page(from, (int64_t)c.n_pages) || !is_page(to, (int64_t)c.n_pages)) continue;
@@ -589,7 +593,9 @@ hipError_t launch_pages_copy(const PagesCopy& a, hipStream_t stream) {
     j.units = a.layers * 2;
     j.unit_rows = (j.units + 7) / 8;
     j.pieces = (int)(((int64_t)a.cache.kv_heads * a.cache.page_size * j.row_chunks + kPiece - 1) / kPiece);
-    j.work = 8 * a.max_copies * j.pieces * j.unit_rows;
+    j.share = j.units <= 4 ? 8 / j.units : 1;
+    j.turns = (j.pieces + j.share - 1) / j.share;
+    j.work = 8 * a.max_copies * j.turns * j.unit_rows;
     const int64_t groups = std::min<int64_t>(j.work, 1 << 16);
     hipLaunchKernelGGL(copy_kernel, dim3((unsigned)groups), dim3(kThreads), 0, stream, j);
     return hipGetLastError();
