@@ -102,6 +102,15 @@ def test_the_longest_sequence_is_only_a_hint(ctx, name, head_dim, rot, layout, p
 
 
 @pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("name,head_dim,rot,layout,block", [("f32", 128, 0, HALF, 64), ("bf16", 256, 256, HALF, 32),
+                                                            ("f16", 64, 32, INTER, 128), ("f32", 48, 10, HALF, 64)])
+def test_long_blocks_grow(ctx, seed, name, head_dim, rot, layout, block):
+    # rows of a block that all waves of a workgroup share, behind tokens that are quieter or louder
+    _case(ctx, [30, 50, 1, 7], [40, 61, 9, 130], 3, 4, 2, head_dim, rot, layout, 128, name=name, block=block, seed=seed,
+          loud=4.0)
+
+
+@pytest.mark.parametrize("seed", range(4))
 def test_scales_grow_and_stay(ctx, seed):
     # tokens louder and quieter than those before them in the block, by up to some powers of two
     _case(ctx, [1] * 12, [2 + i for i in range(12)], 0, 0, 2, 64, 0, HALF, 32, 32, "f32", seed=seed, loud=4.0)

@@ -187,7 +187,8 @@ struct Held {
     }
 };
 
-template <class T, int N>
+// SHARE: a row that a wave does not hold is all waves', not one's.
+template <class T, int N, bool SHARE>
 __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int rot = j.rotate ? j.rope.rot_dim : 0;
@@ -195,7 +196,9 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
     const int units_rot = rotated_units(j.head_dim, rot, half, N), units_plain = j.head_dim / N;
     __shared__ float2 cs[kAngles];
     const int at_once = rot ? min(kAngles / (rot / 2), 64) : 64;  // tokens
-    __shared__ float tops[kMostRows];
+    constexpr int kTops = SHARE ? kRopeThreads / 64 : 1;
+    __shared__ float tops[kMostRows][kTops];
+    __shared__ int olds[kMostRows];
     // cosine and sine of a pair of the token at `place` (behind the prefix)
     auto turn_pair = [&](int64_t place, int pair) {
         const float2 w = turn_cos_sin((uint64_t)(j.batch.prefix_len + place) * j.rope.turns[pair]);
@@ -265,6 +268,8 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
                        (spot.place & (j.cache.page_size - 1)) * (int64_t)j.cache.slot_stride;
     const int before = (int)(spot.place & (block - 1));
     const int64_t scale_at = page * j.s.page_stride + (spot.place & (j.cache.page_size - 1)) / block;
+    const bool shared = SHARE && !once;
+    const int first = shared ? wave * 64 : 0, step = shared ? kRopeThreads : 64;  // units
     for (int pass = once ? 1 : 0; pass < 2; pass++)
         for (int c0 = 0; c0 < count; c0 += at_once) {
             const int n = min(at_once, count - c0);
@@ -272,15 +277,16 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
                 if (pass || c0) __syncthreads();
                 turn(spot.place + c0, n);
             }
-            if (keys) __syncthreads();
-            for (int r = r0 + wave; r < r1; r += 4) {
+            if (keys || (shared && pass)) __syncthreads();  // the angles, and the maxima of the first pass
+            for (int r = r0 + (shared ? 0 : wave); r < r1; r += shared ? 1 : 4) {
                 const bool is_v = r >= j.kv_heads;
                 const int h = is_v ? r - j.kv_heads : r, units = is_v ? units_plain : units_rot;
                 uint8_t* scale = (is_v ? j.s.v : j.s.k) + scale_at + h * j.s.head_stride;
-                const int old = before ? min(max((int)*scale - 127, kLeast), kMost) : kLeast;
                 float top = 0.0f;
+                int old;
                 if (pass == 0 || once) {
-                    for (int w0 = 0; w0 < n * units; w0 += 64) {
+                    old = before && c0 == 0 ? min(max((int)*scale - 127, kLeast), kMost) : kLeast;
+                    for (int w0 = first; w0 < n * units; w0 += step) {
                         if (!once || r != r0 + wave) fetch(r, c0, w0, n);
                         held.rotate(cs, rot, half);
                         top = fmaxf(top, held.top());
@@ -288,30 +294,35 @@ __global__ __launch_bounds__(kRopeThreads) void kv8_append_kernel(Kv8Job j) {
 #pragma unroll
                     for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
                     if (!once) {
-                        // the same wave has the row in both passes
-                        if (lane == 0) tops[r - r0] = c0 ? fmaxf(tops[r - r0], top) : top;
+                        if (lane == 0) {
+                            float& t = tops[r - r0][SHARE ? wave : 0];
+                            t = c0 ? fmaxf(t, top) : top;
+                            if (c0 == 0 && (!SHARE || wave == 0)) olds[r - r0] = old;
+                        }
                         continue;
                     }
                 } else {
-                    top = tops[r - r0];
+#pragma unroll
+                    for (int w = 0; w < kTops; w++) top = fmaxf(top, tops[r - r0][w]);
+                    old = olds[r - r0];
                 }
                 const int e = max(exponent_for(top), old);
                 const int slot = (int)j.cache.slot_stride;
                 uint8_t* dst = static_cast<uint8_t*>(is_v ? j.cache.v : j.cache.k) + at + h * (int64_t)j.cache.head_stride;
-                if (c0 == 0) {  // (later, `old` is what is stored here, which is e)
+                if (c0 == 0) {
                     const int words = j.head_dim / 4;
                     if (before && e > old)
-                        for (int w = lane; w < before * words; w += 64) {
+                        for (int w = first + lane; w < before * words; w += step) {
                             uint32_t* x = reinterpret_cast<uint32_t*>(dst - (int64_t)(before - w / words) * slot) + w % words;
                             *x = shifted4(*x, old - e);
                         }
-                    if (lane == 0) *scale = (uint8_t)(e + 127);
+                    if (first + lane == 0) *scale = (uint8_t)(e + 127);
                 }
                 dst += (int64_t)c0 * slot;
                 if (once) {
                     held.put(dst, slot, e);
                 } else {
-                    for (int w0 = 0; w0 < n * units; w0 += 64) {
+                    for (int w0 = first; w0 < n * units; w0 += step) {
                         fetch(r, c0, w0, n);
                         held.rotate(cs, rot, half);
                         held.put(dst, slot, e);
@@ -340,20 +351,32 @@ hipError_t launch_kv8_append(const RopeJob& job, const Scales& s, int type, hipS
     j.q_groups = j.q_per ? (j.x_heads + j.q_per - 1) / j.q_per : 1;
     const int64_t q_work = j.x_heads ? (j.tokens + j.q_tokens - 1) / j.q_tokens * j.q_groups : 0;
     // Keys and values: a row a wave where blocks are few, up to 8 where cosines of a block's
-    // tokens would be worked out by many workgroups.
+    // tokens would be worked out by many workgroups.  Where that leaves most of the chip idle, and by
+    // the hint a wave does not hold a row, a row is all waves' and up to all of a workgroup (11
+    // prompts of up to 180, 4 KV heads of 128 by blocks of 64: 14 us against 26; where it does not, the
+    // angles worked out again cost more: prompts of 4,500 tokens 41 against 26).
     const int64_t blocks = std::min<int64_t>(j.tokens, j.tokens / s.block + 2 * (int64_t)j.batch.batch);
     const int rows = 2 * j.kv_heads;
-    const int64_t wanted = std::max<int64_t>((rows + kMostRows - 1) / kMostRows, std::min<int64_t>((rows + 3) / 4, 2048 / blocks));
+    const int most = j.batch.max_q > 0 ? std::min(j.batch.max_q, s.block) : s.block;
+    const bool share = blocks * ((rows + 3) / 4) < 256 && (int64_t)most * (j.head_dim / n) > 256;
+    const int64_t wanted = std::max<int64_t>((rows + kMostRows - 1) / kMostRows,
+                                             share ? std::min<int64_t>(rows, 512 / blocks)
+                                                   : std::min<int64_t>((rows + 3) / 4, 2048 / blocks));
     j.rows_per = (int)((rows + wanted - 1) / wanted);
     j.kv_groups = (rows + j.rows_per - 1) / j.rows_per;
     j.kv_work = blocks * j.kv_groups;
     const dim3 grid((unsigned)(j.kv_work + q_work));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (n == 8) hipLaunchKernelGGL((kv8_append_kernel<T, 8>), grid, dim3(kRopeThreads), 0, stream, j);
+        auto launch = [&](auto n_of) {
+            constexpr int N = decltype(n_of)::value;
+            if (share) hipLaunchKernelGGL((kv8_append_kernel<T, N, true>), grid, dim3(kRopeThreads), 0, stream, j);
+            else hipLaunchKernelGGL((kv8_append_kernel<T, N, false>), grid, dim3(kRopeThreads), 0, stream, j);
+        };
+        if (n == 8) launch(std::integral_constant<int, 8>{});
         if constexpr (sizeof(T) == 4)
-            if (n == 4) hipLaunchKernelGGL((kv8_append_kernel<T, 4>), grid, dim3(kRopeThreads), 0, stream, j);
-        if (n == 1) hipLaunchKernelGGL((kv8_append_kernel<T, 1>), grid, dim3(kRopeThreads), 0, stream, j);
+            if (n == 4) launch(std::integral_constant<int, 4>{});
+        if (n == 1) launch(std::integral_constant<int, 1>{});
         return hipGetLastError();
     });
 }
