@@ -8,8 +8,8 @@
 // atomic additions of whole numbers, whose order changes nothing: the same lists every time.
 //
 // 32 sequences of 64 places on 1400 pages: 3.3 and 5.9 us; 256 of 256 on 40000: 3.6 and 7.9; 1000
-// and 4096 pages closed up 9.8 and 12.7.  Copies are memory's: 4096 pages of 8 layers, 1.05 GB,
-// 222 us (4.7 TB/s).
+// and 4096 pages closed up 9.9 and 12.4.  Copies are memory's: 4096 pages of 8 layers, 1.05 GB,
+// 204 us (5.1 TB/s; 222 where a workgroup finds its place by dividing one index).
 #include <algorithm>
 
 #include "vtq_device.h"
@@ -434,11 +434,8 @@ struct CopyJob : PagesCopy {
     int elem;
     int row_chunks;  // of 16 bytes, of a head's row
     int units;       // of a copy: layers x 2
-    int unit_rows;   // units to an XCD
     int share;       // XCDs to a unit, where units are few
     int pieces;      // workgroups to a unit
-    int turns;       // of an XCD, for its share of them
-    int64_t work;
 };
 
 // (as the runtime's uint4 the four would be put in LDS, by numbers from the dispatch packet,
@@ -449,20 +446,15 @@ constexpr int kPiece = 4 * kThreads;  // chunks to a workgroup, in flight at onc
 // A workgroup takes up to 16 KB of a copy's keys or values of a layer.  Pages lie anywhere, and
 // address translation is what a short list of copies waits for: workgroups go to the 8 XCDs
 // in turn, and a layer's keys (or values) stay on one of them, or on some where layers are few
-// (240 pages of 256 KB on one layer, with the lists: 56 us against 137).
+// (240 pages of 256 KB on one layer, with the lists: 55 us against 137).
 __global__ __launch_bounds__(kThreads) void copy_kernel(CopyJob j) {
     const int tid = threadIdx.x;
     const int64_t n = j.count ? min(max((int64_t)*j.count, (int64_t)0), j.max_copies) : j.max_copies;
     const vtq_kv_cache& c = j.cache;
-    for (int64_t i = blockIdx.x; i < j.work; i += gridDim.x) {
-        int64_t at = i >> 3;
-        const int xcd = (int)(i & 7), of = j.share > 1 ? xcd / j.units : 0;
-        const int unit = j.share > 1 ? xcd % j.units : (int)(at % j.unit_rows) * 8 + xcd;
-        at /= j.unit_rows;
-        const int piece = (int)(at % j.turns) * j.share + of;
-        const int64_t copy = at / j.turns;
-        if (copy >= n) return;
-        if (unit >= j.units || of >= j.share || piece >= j.pieces) continue;
+    const int xcd = (int)(blockIdx.x & 7), of = j.share > 1 ? xcd / j.units : 0;
+    const int unit = j.share > 1 ? xcd % j.units : (int)blockIdx.x;
+    if (unit >= j.units || of >= j.share) return;
+    for (int64_t copy = blockIdx.z; copy < n; copy += gridDim.z) {
         const int32_t from = j.copies[3 * copy], to = j.copies[3 * copy + 1];
         const int slots = min(max(j.copies[3 * copy + 2], 0), c.page_size);
         if (!is_page(from, (int64_t)c.n_pages) || !is_page(to, (int64_t)c.n_pages)) continue;
@@ -472,30 +464,32 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(CopyJob j) {
         const char* src = base + from * (int64_t)c.page_stride * j.elem;
         char* dst = base + to * (int64_t)c.page_stride * j.elem;
         const uint32_t of_head = (uint32_t)slots * j.row_chunks, chunks = of_head * c.kv_heads;  // below 2^31
-        const uint32_t first = (uint32_t)piece * kPiece + tid;
-        if (chunks) {
-            // (past the end the last chunk again, which is not stored: every load stands alone)
-            v4u x[4];
-            int64_t where[4];
+        for (int piece = (int)blockIdx.y * j.share + of; piece < j.pieces; piece += (int)gridDim.y * j.share) {
+            const uint32_t first = (uint32_t)piece * kPiece + tid;
+            if ((uint32_t)piece * kPiece < chunks) {
+                // (past the end the last chunk again, which is not stored: every load stands alone)
+                v4u x[4];
+                int64_t where[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint32_t chunk = min(first + k * kThreads, chunks - 1);
-                const uint32_t head = chunk / of_head, rest = chunk - head * of_head;
-                const uint32_t slot = rest / (uint32_t)j.row_chunks;
-                where[k] = (head * (int64_t)c.head_stride + slot * (int64_t)c.slot_stride) * j.elem +
-                           (rest - slot * j.row_chunks) * 16;
-                x[k] = *reinterpret_cast<const v4u*>(src + where[k]);
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t chunk = min(first + k * kThreads, chunks - 1);
+                    const uint32_t head = chunk / of_head, rest = chunk - head * of_head;
+                    const uint32_t slot = rest / (uint32_t)j.row_chunks;
+                    where[k] = (head * (int64_t)c.head_stride + slot * (int64_t)c.slot_stride) * j.elem +
+                               (rest - slot * j.row_chunks) * 16;
+                    x[k] = *reinterpret_cast<const v4u*>(src + where[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (first + k * kThreads < chunks) *reinterpret_cast<v4u*>(dst + where[k]) = x[k];
             }
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (first + k * kThreads < chunks) *reinterpret_cast<v4u*>(dst + where[k]) = x[k];
-        }
-        if (piece == 0 && j.scales.k) {
-            uint8_t* scale = (is_v ? j.scales.v : j.scales.k) + layer * j.scale_layer_stride;
-            const int blocks = (slots + j.scales.block - 1) / j.scales.block;
-            for (int k = tid; k < blocks * c.kv_heads; k += kThreads) {
-                uint8_t* s = scale + (k / blocks) * j.scales.head_stride + k % blocks;
-                s[to * j.scales.page_stride] = s[from * j.scales.page_stride];
+            if (piece == 0 && j.scales.k) {
+                uint8_t* scale = (is_v ? j.scales.v : j.scales.k) + layer * j.scale_layer_stride;
+                const int blocks = (slots + j.scales.block - 1) / j.scales.block;
+                for (int k = tid; k < blocks * c.kv_heads; k += kThreads) {
+                    uint8_t* s = scale + (k / blocks) * j.scales.head_stride + k % blocks;
+                    s[to * j.scales.page_stride] = s[from * j.scales.page_stride];
+                }
             }
         }
     }
@@ -591,13 +585,13 @@ hipError_t launch_pages_copy(const PagesCopy& a, hipStream_t stream) {
     j.elem = a.cache.type == VTQ_TYPE_E4M3 ? 1 : (int)type_bytes(a.cache.type);
     j.row_chunks = a.cache.head_dim * j.elem / 16;
     j.units = a.layers * 2;
-    j.unit_rows = (j.units + 7) / 8;
     j.pieces = (int)(((int64_t)a.cache.kv_heads * a.cache.page_size * j.row_chunks + kPiece - 1) / kPiece);
     j.share = j.units <= 4 ? 8 / j.units : 1;
-    j.turns = (j.pieces + j.share - 1) / j.share;
-    j.work = 8 * a.max_copies * j.turns * j.unit_rows;
-    const int64_t groups = std::min<int64_t>(j.work, 1 << 16);
-    hipLaunchKernelGGL(copy_kernel, dim3((unsigned)groups), dim3(kThreads), 0, stream, j);
+    // units (in eights: XCDs in turn), pieces, copies; the last two in strides where there are many
+    const unsigned x = (unsigned)(j.units + 7) / 8 * 8;
+    const unsigned y = (unsigned)std::min<int64_t>((j.pieces + j.share - 1) / j.share, std::max<int64_t>(1, 65536 / x));
+    const unsigned z = (unsigned)std::min<int64_t>(a.max_copies, std::max<int64_t>(1, 131072 / ((int64_t)x * y)));
+    hipLaunchKernelGGL(copy_kernel, dim3(x, y, std::min(z, 65535u)), dim3(kThreads), 0, stream, j);
     return hipGetLastError();
 }
 
