@@ -42,6 +42,8 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
+constexpr float kLargestBf16 = 3.3895313892515355e38f;  // 2^128 - 2^120
+
 struct Job8 : Job {
     Scales s;
     int block_shift;
@@ -209,10 +211,12 @@ struct Compute8 {
                 float rest = x[e];
 #pragma unroll
                 for (int i = 0; i < PQ; i++) {
-                    const __bf16 part = (__bf16)rest;
+                    // a finite number that would round to an infinity leaves its rest to the other parts, as
+                    // many bits as they hold; an infinity's own rest would be no number: the first has it all
+                    const bool finite = fabsf(rest) < INFINITY;
+                    const __bf16 part = (__bf16)(finite ? __builtin_amdgcn_fmed3f(rest, -kLargestBf16, kLargestBf16) : rest);
                     give(i, e, part);
-                    // an infinity's remainder would be no number: the first part has it all
-                    rest = fabsf(rest) < INFINITY ? rest - (float)part : 0.0f;
+                    rest = finite ? rest - (float)part : 0.0f;
                 }
             }
         }
