@@ -369,8 +369,10 @@ int vtq_kv8_append_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv
  * products as the numbers they stand for.  BF16 and F16 queries multiply as they
  * are, F32 ones as the exact sum of three bf16 parts; weights are rounded to one
  * (BF16), two (F16) and three (F32) bf16 parts: off by 2^-8, 2^-16 and 2^-24 of
- * themselves at most.  Heads of more than 128 elements count four times in the
- * limit of workgroups. */
+ * themselves at most.  (Parts of a query or a weight below 2^-126 may be lost.)  A mean of
+ * values is never lost to a sum past f32's range; where a block among the keys at hand has a scale
+ * above 2^80, values below 2^-77 are off by up to that much.  Heads of more than 128 elements
+ * count four times in the limit of workgroups. */
 size_t vtq_kv8_attention_workspace(const vtq_kv8_cache *cache, const vtq_kv_batch *batch, int type, size_t tokens,
                                    size_t heads);
 int vtq_kv8_attention_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv_batch *batch, int type,

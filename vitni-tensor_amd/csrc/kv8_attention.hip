@@ -82,7 +82,15 @@ struct Runs {
     int first;  // in 16 keys
     int low, high;      // bytes from the head's start, -1: outside the cache
     int scales;         // bytes: the keys' scale, the values' 16 bits above
+    int down;           // the values' are this much lower: 0 or kDown, the same in every lane
 };
+
+// Values above 2^80 may add up past f32's end though their mean does not: weights of up to 2^8 times 2^30
+// keys times 448 x 2^119 are 2^166.  From the first 1024 keys on that have such a scale, a wave takes
+// all values 2^-kDown as large as they count, and its sums so far too.  Powers of two change no bits, so
+// that rows that do not see such a block are what they are without it; only values below 2^-77, whose
+// scale would be none of a bf16, are off, by 2^-77 at most.
+constexpr int kLargeScale = 127 + 80;
 
 template <int DK, int DV>
 struct Loader8 {
@@ -127,8 +135,8 @@ struct Loader8 {
             v_off[i] = at_chunk(row, TV::v_chunk(row, lane % TV::kChunks), v_bytes);
         }
     }
-    // Holds the runs from `key`'s on.
-    __device__ __forceinline__ void hold(Runs& p, int key) const {
+    // Holds the runs from `key`'s on; whether their values are lower now than those before.
+    __device__ __forceinline__ bool hold(Runs& p, int key) const {
         const int lane = threadIdx.x & 63;
         p.first = key >> 4;
         const int at = min(p.first + lane, (p.keys - 1) >> 4) * 16;
@@ -138,10 +146,15 @@ struct Loader8 {
         p.low = (int)(uint32_t)byte;
         p.high = (int)(byte >> 32);
         const int64_t scale = there ? (int64_t)page * scale_page + (slot >> block_shift) : 0;
-        p.scales = there ? min(max((int)k_scale[scale], 10), 246) | min(max((int)v_scale[scale], 10), 246) << 16 : 127 * 0x10001;
+        const int of_keys = there ? min(max((int)k_scale[scale], 10), 246) : 127;
+        const int of_values = there ? min(max((int)v_scale[scale], 10), 246) : 127;
+        const bool lower = !p.down && __ballot(of_values > kLargeScale);
+        p.down = lower ? kDown : p.down;
+        p.scales = of_keys | max(of_values - p.down, 1) << 16;
         // waited for here: left to its use, the wait would stand in every tile, and be one for
         // all loads to LDS in flight as well
         asm volatile("" : "+v"(p.low), "+v"(p.high), "+v"(p.scales));
+        return lower;
     }
     // the lane of `key`'s 16 keys (those past the end have any)
     __device__ __forceinline__ int lane_of(const Runs& p, int key) const { return ((key >> 4) - p.first) & 63; }
@@ -175,6 +188,10 @@ struct Loader8 {
         for (int i = 0; i < TV::kLoads; i++) load_to_lds<16>(rv, v_off[i], v_lds + 1024u * i);
     }
 };
+
+__device__ __forceinline__ float lower_scale(float x) {
+    return __int_as_float(max(__float_as_int(x) - (kDown << 23), 1 << 23));
+}
 
 // ------------------------------------------------ one tile of 32 keys
 
@@ -213,8 +230,9 @@ struct Compute8 {
                 for (int i = 0; i < PQ; i++) {
                     // a finite number that would round to an infinity leaves its rest to the other parts, as
                     // many bits as they hold; an infinity's own rest would be no number: the first has it all
-                    const bool finite = fabsf(rest) < INFINITY;
-                    const __bf16 part = (__bf16)(finite ? __builtin_amdgcn_fmed3f(rest, -kLargestBf16, kLargestBf16) : rest);
+                    const bool finite = i || fabsf(rest) < INFINITY;
+                    const float near = i ? rest : __builtin_amdgcn_fmed3f(rest, -kLargestBf16, kLargestBf16);
+                    const __bf16 part = (__bf16)(finite ? near : rest);
                     give(i, e, part);
                     rest = finite ? rest - (float)part : 0.0f;
                 }
@@ -305,9 +323,6 @@ struct Compute8 {
 #pragma unroll
             for (int i = 0; i < 2; i++) r.x[b][i] = values_at(from, b, i);
     }
-    __device__ __forceinline__ static bool near_end(TileScales sc) {  // scales above 2^95; scalar as integers
-        return max(__float_as_int(sc.v0), __float_as_int(sc.v1)) > (222 << 23);
-    }
     __device__ __forceinline__ static float key_scale(TileScales sc) { return threadIdx.x & 16 ? sc.k1 : sc.k0; }
     // scores of 32 keys: register 4i + e is key 8i + 4h + e, row lane & 31
     __device__ __forceinline__ static v16f scores(const uint8_t* k, const Query& q, TileScales sc) {
@@ -376,19 +391,11 @@ struct Compute8 {
     }
 
     // m follows the maximum only once it is 8 powers of two behind: weights up to 256
-    // cost nothing, and rows rarely rescale.  Beside values near f32's end (raise) m is 24 powers
-    // above the maximum, so that sums of them do not pass it.
-    __device__ __forceinline__ static bool moved(float top, float m, bool raise, float c) {
-        return (top - m) * c > (raise ? 0.0f : 8.0f);
-    }
-    // Whether some row's does; top as it is to be.
-    __device__ __forceinline__ static bool moves(float& top, float m, bool raise, float c) {
-        if (raise) top += fminf(24.0f / c, 1e38f);
-        return __ballot(moved(top, m, raise, c)) != 0;
-    }
+    // cost nothing, and rows rarely rescale.
+    __device__ __forceinline__ static bool moved(float top, float m, float c) { return (top - m) * c > 8.0f; }
     // Scores of N tiles to weights, with the row's maximum and sum.
     template <int N>
-    __device__ __forceinline__ static void softmax(State<DV>& st, Weights (&w)[N], v16f (&s)[N], bool raise, float c) {
+    __device__ __forceinline__ static void softmax(State<DV>& st, Weights (&w)[N], v16f (&s)[N], float c) {
         float top = s[0][0];
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -397,8 +404,8 @@ struct Compute8 {
         const float2 both = halves(top);
         top = fmaxf(both.x, both.y);
         const float before = st.m;
-        if (moves(top, before, raise, c)) {
-            const bool mine = moved(top, before, raise, c);  // each row for itself
+        if (__ballot(moved(top, before, c))) {
+            const bool mine = moved(top, before, c);  // each row for itself
             const float shrink = mine ? __builtin_amdgcn_exp2f((before - top) * c) : 1.0f;
             st.m = mine ? top : before;
             st.l *= shrink;
@@ -480,7 +487,7 @@ struct Compute8 {
         scores(s, k0, k1, q, s0, s1);
         read_values(v1, v + TV::kBytes);
         Weights w[2];
-        softmax<2>(st, w, s, near_end(s0) || near_end(s1), c);
+        softmax<2>(st, w, s, c);
         add_values(st, v0, w[0], s0);
         add_values(st, v1, w[1], s1);
     }
@@ -498,7 +505,7 @@ struct Compute8 {
                 if (key + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[0][r] = -INFINITY;
         }
         Weights w[1];
-        softmax<1>(st, w, s, near_end(sc), c);
+        softmax<1>(st, w, s, c);
         Values x;
         read_values(x, v);
         const bool nans = edge && low < there && !all_numbers(v);
@@ -616,14 +623,14 @@ struct Few8 {
     __device__ __forceinline__ static float sum(float l) {
         return of_groups(l, [](float a, float b) { return a + b; });
     }
-    __device__ __forceinline__ static void softmax(Rows& st, Weights& w, v4f (&s)[2], bool raise, float c) {
+    __device__ __forceinline__ static void softmax(Rows& st, Weights& w, v4f (&s)[2], float c) {
         float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
         for (int r = 1; r < 4; r++) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
         top = of_groups(top, [](float a, float b) { return fmaxf(a, b); });
         const float before = st.m;
-        if (X::moves(top, before, raise, c)) {
-            const bool mine = X::moved(top, before, raise, c);
+        if (__ballot(X::moved(top, before, c))) {
+            const bool mine = X::moved(top, before, c);
             const float shrink = mine ? __builtin_amdgcn_exp2f((before - top) * c) : 1.0f;
             st.m = mine ? top : before;
             st.l *= shrink;
@@ -676,7 +683,7 @@ struct Few8 {
                     if (key + key_of(t, group(), r) >= limit) s[t][r] = -INFINITY;
         }
         Weights w;
-        softmax(st, w, s, X::near_end(sc), c);
+        softmax(st, w, s, c);
         const uint32_t from = values_from(v);
         const float scale = value_scale(sc);
         v2i x[DV / 16];
@@ -820,7 +827,14 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
         auto clear = [&](auto& st) {
             st.m = -INFINITY;
             st.l = 0.0f;
+            runs.down = 0;
             for (auto& o : st.o) o = std::remove_reference_t<decltype(o)>{};
+        };
+        auto hold = [&](auto& st, int key) {
+            const bool lower = from.hold(runs, key);
+            if (lower)
+                for (auto& o : st.o) o *= kToDown;
+            return lower;
         };
         // the query's loads are waited for before the loops, as those of hold()
         auto wait_for = [&](auto& q) {
@@ -829,7 +843,7 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
         };
         if (shared) {
             typename X::Query q;
-            State<DV> st;
+            typename X::Rows st;
             X::load_query(q, q_row, valid, hd);
             clear(st);
             // the prefix's keys, where they are this workgroup's too (never beside 16 rows), then its own
@@ -843,7 +857,7 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                 const int least = of_prefix ? stop : low, most = !of_prefix ? high : __ballot(valid) ? stop : 0;
                 if (inside) runs.list = of_prefix ? a.batch.prefix_pages : own_list;
                 runs.keys = stop;  // past the last row's sight nothing is read
-                from.hold(runs, begin);
+                hold(st, begin);
                 wait_for(q);
                 // stages of two tiles (K, then V), S - 1 of them ahead; a wave loads 16 of the 64 keys
                 constexpr int kStage = 2 * Cfg::kTile, S = Cfg::kLds / kStage;
@@ -853,8 +867,6 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                 // those in flight stays the same.
                 auto load_stage = [&](int m, int to) {
                     const int key = begin + 64 * m;
-                    // (what is held begins at the tiles at hand, whose scales are read from it too)
-                    if ((min(key + 64, runs.keys) - 1) / 16 - runs.first >= 64) from.hold(runs, begin + 64 * n);
                     const uint32_t stage = lds0 + (uint32_t)(to * kStage);
                     from.load16(runs, key + 16 * wave, stage + 16 * wave * TK::kRow,
                                 stage + 2 * TK::kBytes + 16 * wave * TV::kRow);
@@ -869,7 +881,11 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
-                    load_stage(n + S - 1, at == 0 ? S - 1 : at - 1);
+                    // (what is held begins at the tiles at hand, whose scales are read from it too; the first
+                    // stages ahead are held from `begin` on)
+                    const int ahead = n + S - 1;
+                    if ((min(begin + 64 * ahead + 64, runs.keys) - 1) / 16 - runs.first >= 64) hold(st, begin + 64 * n);
+                    load_stage(ahead, at == 0 ? S - 1 : at - 1);
                     here0 = from.scales(runs, begin + 64 * n), here1 = from.scales(runs, begin + 64 * n + 32);
                     const uint8_t* k = lds + at * kStage;
                     at = at + 1 == S ? 0 : at + 1;
@@ -899,11 +915,12 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                 asm volatile("" ::: "memory");
             }
             st.l = X::sum(st.l);
+            if (runs.down) st.l = -st.l;
             const int first_row = r0 + wave * 32;
             X::each(st, [&](int late_row, int chunk, float4 o) {
                 const int row = first_row + late_row, d = DV * part + 4 * chunk;
                 if (row < n_rows && d < hd)
-                    put_row<Q, 0>(j, out_split, t0 + row / G, kv_head * G + row % G, d, o, st.m, st.l);
+                    put_row<Q, 0, true>(j, out_split, t0 + row / G, kv_head * G + row % G, d, o, st.m, st.l);
             });
             continue;
         }
@@ -914,7 +931,7 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
             Y::load_query(q, q_row, valid, hd);
             clear(st);
             runs.keys = end;  // past the last row's sight nothing is read
-            if (tiles > 0) from.hold(runs, k0);
+            if (tiles > 0) hold(st, k0);
             wait_for(q);
             if (wave < tiles) {
                 // a wave's two stages of a tile
@@ -922,7 +939,6 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                 const uint32_t to = lds0 + (uint32_t)wave * 2 * Cfg::kTile;
                 auto load = [&](int n, int at) {
                     const int key = k0 + 32 * n;
-                    if ((min(key + 32, runs.keys) - 1) / 16 - runs.first >= 64) from.hold(runs, key);
                     const uint32_t stage = to + (uint32_t)(at * Cfg::kTile);
                     from.load16(runs, key, stage, stage + TK::kBytes);
                     from.load16(runs, key + 16, stage + 16 * TK::kRow, stage + TK::kBytes + 16 * TV::kRow);
@@ -939,12 +955,18 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
                     Y::tile(st, q, k, k + TK::kBytes, here, n >= whole, k0 + 32 * n, limit, low, runs.keys, j.c);
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     here = next;
+                    const int key = k0 + 32 * (n + 2 * W);  // (the first two tiles are held from k0 on)
+                    if ((min(key + 32, runs.keys) - 1) / 16 - runs.first >= 64 && hold(st, key)) {
+                        here.v0 = lower_scale(here.v0);
+                        here.v1 = lower_scale(here.v1);
+                    }
                     next = load(n + 2 * W, at);
                 }
                 wait_vmcnt<0>();
                 asm volatile("" ::: "memory");
             }
             st.l = Y::sum(st.l);
+            if (runs.down) st.l = -st.l;
             // each wave's part of the rows in its own part of LDS
             float* mine = reinterpret_cast<float*>(lds + wave * 2 * Cfg::kTile);
             asm volatile("" ::: "memory");
@@ -960,8 +982,9 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
             const int rr = e / (DV / 4), c = e % (DV / 4), d = DV * part + 4 * c;
             if (d >= hd) continue;
             float m = -INFINITY;
+            bool down = false;  // some wave's are held lower: the others' are brought to it
 #pragma unroll
-            for (int w = 0; w < W; w++) m = fmaxf(m, wave_ml[w][rr].x);
+            for (int w = 0; w < W; w++) m = fmaxf(m, wave_ml[w][rr].x), down |= lowered<true>(wave_ml[w][rr].y);
             const float base = m == -INFINITY ? 0.0f : m;
             float l = 0.0f;
             float4 o = make_float4(0, 0, 0, 0);
@@ -969,12 +992,13 @@ __global__ __launch_bounds__((kWaves8 * 64), (Config8<Q, DK, DV>::kPerCu)) void 
             for (int w = 0; w < W; w++) {
                 const float2 ml = wave_ml[w][rr];
                 const float f = __builtin_amdgcn_exp2f((ml.x - base) * j.c);
-                const float4 x = *reinterpret_cast<const float4*>(
+                float4 x = *reinterpret_cast<const float4*>(
                     reinterpret_cast<const float*>(lds + w * 2 * Cfg::kTile) + rr * DV + 4 * (c ^ (rr & 15)));
-                l = fmaf(ml.y, f, l);
+                scale4(x, down && !lowered<true>(ml.y) ? kToDown : 1.0f);
+                l = fmaf(fabsf(ml.y), f, l);
                 o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
             }
-            put_row<Q, 0>(j, out_split, t0 + (r0 + rr) / G, kv_head * G + (r0 + rr) % G, d, o, m, l);
+            put_row<Q, 0, true>(j, out_split, t0 + (r0 + rr) / G, kv_head * G + (r0 + rr) % G, d, o, m, down ? -l : l);
         }
         __syncthreads();
     }
@@ -994,7 +1018,7 @@ hipError_t launch_of(const Job8& j, hipStream_t stream) {
         return hipGetLastError();
     };
     if (hipError_t e = few ? launch(kv8_attention_kernel<Q, DK, DV, 16>) : launch(kv8_attention_kernel<Q, DK, DV, 32>)) return e;
-    return launch_join<Q, DK, 0>(j, stream);
+    return launch_join<Q, DK, 0, true>(j, stream);
 }
 
 }  // namespace
