@@ -51,6 +51,11 @@ inline TileCost attention_cost(int type, int cache_type, int head_dim) {
             type == VTQ_TYPE_F32 ? 3.6 * d / 128 : d > 128 ? 2.4 : 0.18 + 0.0025 * d};
 }
 
+// A part of the rows on its way through memory and the join, us.
+inline double part_cost(int64_t tokens, int heads, int head_dim) {
+    return 0.08 + 2.3e-6 * (double)(tokens * heads * head_dim);
+}
+
 // The arguments are what the checks let through: tokens, heads and batch above 0.
 inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batch& batch, const TileCost& cost,
                                     int64_t tokens, int heads) {
@@ -74,7 +79,7 @@ inline AttentionPlan plan_attention(const vtq_kv_cache& cache, const vtq_kv_batc
     const int grain = slow ? 32 : 128;
     p.own_grain = p.shared_own ? grain : 128;
     auto least_keys = [&](int64_t keys) {
-        const double part = 0.08 + 2.3e-6 * (double)(tokens * heads * cache.head_dim);
+        const double part = part_cost(tokens, heads, cache.head_dim);
         return (1 + (int64_t)std::sqrt(32.0 * keys * part / cost.tile) / grain) * grain;
     };
     if (batch.prefix_len) {
@@ -138,11 +143,35 @@ inline int per_xcd(int64_t units, int rows) {
     const int last = (int)(units % 8), share = xcds_of(last);
     return (int)(units / 8 * rows + (last ? (rows + share - 1) / share : 0));
 }
-// Whether the sequences' own workgroups take the prefix too: prompts that fill the chip behind a
-// prefix that a L2 holds.  Their rows then leave once, not as two parts in f32 to be joined (12 prompts
-// of up to 218 tokens, 32 heads on 8 of 96, behind 161 keys: 39 us against 66).
-inline bool kv8_prefix_inside(const vtq_kv_batch& batch, const AttentionPlan& without) {
-    return batch.prefix_len > 0 && batch.prefix_len <= 4096 && without.shared_own && without.own_splits == 1;
+// Whether the sequences' own workgroups take the prefix too: their rows then leave once, not as two parts
+// in f32 to be joined, but each walks all of the prefix, which rows of all sequences packed would in
+// fewer, and fuller, workgroups.  `with` and `without` are the plans with prefix workgroups and of the
+// own keys alone; the estimate, in us, is what walks the most keys or, above a workgroup a CU, all
+// walks, and what a part of the rows costs (plan_attention's least_keys).  Measured inside / outside (bf16,
+// 32 heads on 8 of 128): 12 prompts of up to 218 behind 161 keys, of 96, 41 / 70; 64 drafts of 9
+// behind 300 31 / 41, behind 1000 55 / 48 and taken outside; one of 60 behind 1000 35 / 19 and behind 4096
+// 96 / 24, outside.  Beyond 4096 keys the parts are the least of it (40 x 100, 64 heads, 8000:
+// 1324 / 1230).
+inline bool kv8_prefix_inside(const vtq_kv_cache& part, const vtq_kv_batch& batch, const TileCost& cost, int64_t tokens,
+                              int heads, bool joined, const AttentionPlan& without, const AttentionPlan& with) {
+    if (!batch.prefix_len || !without.shared_own || without.own_splits != 1) return false;
+    // Rows that are joined anyway (heads of more than 128 elements) save workgroups only: 10 and 62 prompts
+    // of 64, f16, 8 heads on 4 of 256, behind 64 keys 23.3 / 22.7 and 84 / 76, behind 200 31 / 27 and 115 / 91.
+    if (batch.prefix_len > (joined ? 64 : 4096)) return false;
+    const double rows = (double)tokens * without.group, tiles = (double)without.own_rows * batch.batch;
+    // One long sequence among short ones: most of the others' tiles have no rows, and the rest few (63
+    // tokens of 900 keys beside a chunk of 512 behind 300 204 / 172, behind 1000 287 / 181).
+    if (128 * tiles > 5 * rows) return false;
+    const double packed = std::ceil(rows / 128), filled = std::min(tiles, rows / 128 + batch.batch);
+    const int64_t most = (int64_t)batch.max_pages << without.page_shift;
+    const double own = (batch.max_len ? std::min<int64_t>(batch.max_len, most) : most) / 32.0;
+    const double prefix = batch.prefix_len / 32.0, range = std::min(prefix, with.prefix_chunk / 32.0);
+    // a lone workgroup takes longer to a tile than one of several on a CU do
+    auto walk = [&](double longest, double all) { return cost.tile * std::max(1.28 * longest, all * part.kv_heads / 256); };
+    const double in = walk(prefix + own, filled * (prefix + own)) + 3;  // (the second page list's latency)
+    const double out = walk(std::max(range, own), packed * prefix + filled * own) + 2 +
+                       (with.prefix_splits + with.own_splits) * part_cost(tokens, heads, part.head_dim);
+    return in <= out;
 }
 inline AttentionPlan plan_kv8_attention(const vtq_kv_cache& cache, const vtq_kv_batch& batch, int type, int64_t tokens,
                                         int heads, bool* inside = nullptr) {
@@ -153,9 +182,10 @@ inline AttentionPlan plan_kv8_attention(const vtq_kv_cache& cache, const vtq_kv_
     vtq_kv_batch own = batch;
     own.prefix_len = 0;
     const TileCost cost = kv8_attention_cost(type, cache.head_dim);
-    AttentionPlan p = plan_attention(part, own, cost, tokens, heads * parts);
-    const bool in = kv8_prefix_inside(batch, p);
-    if (!in && batch.prefix_len) p = plan_attention(part, batch, cost, tokens, heads * parts);
+    AttentionPlan p = plan_attention(part, batch, cost, tokens, heads * parts);
+    const AttentionPlan without = plan_attention(part, own, cost, tokens, heads * parts);
+    const bool in = kv8_prefix_inside(part, batch, cost, tokens, heads * parts, parts > 1, without, p);
+    if (in) p = without;
     if (inside) *inside = in;
     // y may be q: no part writes rows that the other still reads, so they are joined even if alone
     if (parts > 1 && p.prefix_splits + p.own_splits == 1) p.own_splits = 2;
