@@ -388,7 +388,9 @@ int vtq_kv8_attention_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq
 /* The best continuations of beams.  groups x beams rows of `vocab` logits (rows ld
  * apart), each with the sum so far of its beam, score[row] (f32).  A candidate is a
  * token of a row, worth score + logit - ln sum exp(logits of the row), worked out in
- * f64.  The n_out greatest of a group come out in falling order, equal ones by falling
+ * f64 with the logarithm right to 2^-32: rows whose sums are equal but for the order of their
+ * logits, or a constant in them, may come out up to 2^-31 apart, and in either order.  Those of
+ * a row, and of rows of the same logits, are in the order that follows.  The n_out greatest of a group come out in falling order, equal ones by falling
  * logit and then by rising (beam, token): out_score (f32), out_token and out_parent
  * (the row, counted over all groups), each groups x n_out.  A row whose score or sum
  * is not finite (a NaN or +infinity among the logits, or -infinity alone) has all its
