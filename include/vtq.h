@@ -369,10 +369,10 @@ int vtq_kv8_append_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv
  * products as the numbers they stand for.  BF16 and F16 queries multiply as they
  * are, F32 ones as the exact sum of three bf16 parts; weights are rounded to one
  * (BF16), two (F16) and three (F32) bf16 parts: off by 2^-8, 2^-16 and 2^-24 of
- * themselves at most.  (Parts of a query or a weight below 2^-126 may be lost.)  A mean of
- * values is never lost to a sum past f32's range; where a block among the keys at hand has a scale
- * above 2^80, values below 2^-77 are off by up to that much.  Heads of more than 128 elements
- * count four times in the limit of workgroups. */
+ * themselves at most.  (Parts of a query or a weight below 2^-126 may be lost.)  A mean
+ * of values is never lost to a sum past f32's range; where a block among the keys at
+ * hand has a scale above 2^80, values below 2^-77 are off by up to that much.  Heads of
+ * more than 128 elements count four times in the limit of workgroups. */
 size_t vtq_kv8_attention_workspace(const vtq_kv8_cache *cache, const vtq_kv_batch *batch, int type, size_t tokens,
                                    size_t heads);
 int vtq_kv8_attention_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq_kv_batch *batch, int type,
@@ -388,10 +388,11 @@ int vtq_kv8_attention_device(vtq_ctx *ctx, const vtq_kv8_cache *cache, const vtq
 /* The best continuations of beams.  groups x beams rows of `vocab` logits (rows ld
  * apart), each with the sum so far of its beam, score[row] (f32).  A candidate is a
  * token of a row, worth score + logit - ln sum exp(logits of the row), worked out in
- * f64 with the logarithm right to 2^-32: rows whose sums are equal but for the order of their
- * logits, or a constant in them, may come out up to 2^-31 apart, and in either order.  Those of
- * a row, and of rows of the same logits, are in the order that follows.  The n_out greatest of a group come out in falling order, equal ones by falling
- * logit and then by rising (beam, token): out_score (f32), out_token and out_parent
+ * f64 with the logarithm right to 2^-32: candidates of rows that differ in the order of
+ * their logits or by a constant, and are equal otherwise, may come out up to 2^-31 apart,
+ * and in either order.  Those of a row, and of rows of the same logits, are in the order
+ * that follows.  The n_out greatest of a group come out in falling order, equal ones by
+ * falling logit and then by rising (beam, token): out_score (f32), out_token and out_parent
  * (the row, counted over all groups), each groups x n_out.  A row whose score or sum
  * is not finite (a NaN or +infinity among the logits, or -infinity alone) has all its
  * candidates at -infinity, equal ones.  done (NULL: none) marks rows that ended: such a

@@ -87,7 +87,7 @@ def test_without_queries_without_rotation_and_other_orders(ctx):
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("head_dim,rot,layout,page", [(128, 128, HALF, 64), (64, 32, INTER, 16), (48, 10, HALF, 32)])
 def test_the_longest_sequence_is_only_a_hint(ctx, name, head_dim, rot, layout, page):
-    # by tokens of a sequence a wave holds one unit of a row at a time or four; every hint gives the same cache
+    # by tokens of a sequence a row of a block is one wave's or all waves'; every hint gives the same cache
     seen = []
     for max_q in (0, 1, 3, 100, 100000):
         p = Paged8([1, 70, 5, 33], [30, 90, 5, 40], 7, 3, head_dim, page, page, seed=4)

@@ -7,9 +7,11 @@
 // itself.  Free pages are taken lowest first and in the order of sequences, and counts change by
 // atomic additions of whole numbers, whose order changes nothing: the same lists every time.
 //
-// 32 sequences of 64 places on 1400 pages: 3.3 and 5.9 us; 256 of 256 on 40000: 3.6 and 7.9; 1000
-// and 4096 pages closed up 9.9 and 12.4.  Copies are memory's: 4096 pages of 8 layers, 1.05 GB,
-// 204 us (5.1 TB/s; 222 where a workgroup finds its place by dividing one index).
+// Kernel times beside the copies that they are for: 32 sequences of 64 places on 1400 pages 3.3 and
+// 5.8 us; 256 of 256 on 40000 3.6 and 7.3; 1000 and 4096 pages closed up 9.7 and 12.1, as the copies
+// before have taken the caches (7.3 and 8.6 without them, 6.9 and 7.0 in a graph).  Copies are
+// memory's: 4096 pages of 8 layers, 1.05 GB, 204 us (5.1 TB/s; 222 where a workgroup finds its place by
+// dividing one index).
 #include <algorithm>
 
 #include "vtq_device.h"
@@ -338,9 +340,10 @@ __global__ __launch_bounds__(kThreads) void compact_apply_kernel(CompactJob j) {
 }
 
 // All of it in one launch where pages are few: every workgroup makes a bit to each page in use
-// for itself, and finds ranks, and pages of a rank, by counting bits.  One launch / three, us: 1000
-// pages in 960 places 7.2 / 8.9, 4096 in 65536 7.2 / 9.6; 4096 in 2^20, where the search in
-// bits costs more than launches, 20.8 / 11.0, and 8192 in 65536 10.8 / 10.
+// for itself, and finds ranks, and pages of a rank, by counting bits.  One launch / three, us, both in
+// a graph of calls alone: 256 pages in 200 places 5.7 / 6.9, 1000 in 960 6.8 / 8.7, 4096 in 5120 7.0 / 9.5
+// and in 65536 7.0 / 9.3 (eager 7.4 / 12.4 throughout); 4096 in 2^20, where the search in bits costs more
+// than launches, 20.8 / 11.0, and 8192 in 65536 10.8 / 10.
 constexpr int kMaskWords = 64, kMaskPages = 64 * kMaskWords, kFewEntries = 1 << 16;
 
 struct PageBits {

@@ -23,11 +23,13 @@
 // spilled in every loop: 26 sequences of 7 behind 8099 keys, f16, 565 us against 100.)
 //
 // Measured (8 KV heads of 128, groups of 4, bf16; 16-bit keys in brackets): 128 sequences behind
-// 32768 keys with up to 1024 of their own 111 and 6 to join (148); the prefix alone 101 (97), 700
-// TFLOP/s at 2.05 GHz, the same with one workgroup a CU and with two: vector instructions, of
-// which a SIMD starts one every 4.3 cycles, 180 to a tile beside its 16 products (without the
-// softmax 15 us less, without the conversions 7).  The own keys alone 41 (88), 4.9 TB/s; 8
-// sequences of 32000 87 (160).
+// 32768 keys with up to 1024 of their own 111 and 6 to join (145); the prefix alone 99 (98), 700
+// TFLOP/s at 2.05 GHz, the same with one workgroup a CU and with two.  There a SIMD's vector
+// instructions, 210 to a tile beside its 16 products and one started every 4.4 cycles, take 68 %
+// of its cycles and its products 35 %: they hardly overlap.  Its two waves wait for memory or LDS
+// in a quarter of theirs, and for the other's turn in another.  (Without the softmax 15 us
+// less, without the conversions 7.)  The own keys alone 41 (88), 4.9 TB/s; 8 sequences of
+// 32000 88 (160).
 #include <type_traits>
 
 #include "vtq_attention_rows.h"
@@ -377,8 +379,10 @@ struct Compute8 {
         Weights w;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            // As many parts as the query has: off by 2^-8 (bf16), 2^-16 (f16) or 2^-24 (f32) of each
-            // at most.  The sum is of the unrounded ones, in f32.
+            // Off by 2^-8 (bf16), 2^-16 (f16) or 2^-24 (f32) of each at most; the sum is of the
+            // unrounded ones, in f32.  In bf16 that leaves y 1.8e-3 off 64 bits, 1.6e-3 of which are
+            // its own rounding (128 behind 32768 keys, in the norm); a second part would take half as
+            // many products again.
             float rest = p[r];
 #pragma unroll
             for (int i = 0; i < P; i++) {
